@@ -26,8 +26,7 @@ DEV = "cuda"
 DTYPES = {"f16": torch.float16, "bf16": torch.bfloat16}
 HEADS = [(8, 2, 64), (28, 4, 128), (40, 8, 128), (32, 8, 128), (64, 8, 128), (16, 8, 256)]     # (Hq, Hkv, D)
 GROUP = 64                   # channels that share a scale and an offset
-LIMIT = 65504.0              # values beyond, and infinities, are stored as this; NaN as 0
-MAX_SCALE = 8728.0           # the largest scale whose 15 steps stay within fp16
+LIMIT = 65024.0              # values beyond, and infinities, are stored as this; NaN as 0 (offset + 15 scales then stay within fp16)
 MAX_LOGITS = 2.2e8           # of one layer of the plain form, padded
 MAX_NEW = 4 * 8192 * 8 * 128  # channels of keys that an append brings, all layers
 MAX_BYTES = 2.5e8            # of the 4-bit caches of all layers
@@ -156,7 +155,7 @@ def _quantise(x):
     """Codes [..., D], scales and offsets [..., D / 64] (float32 numbers that fp16 holds) of values [..., D]."""
     x = torch.nan_to_num(x.float(), nan=0.0, posinf=LIMIT, neginf=-LIMIT).clamp(-LIMIT, LIMIT).unflatten(-1, (-1, GROUP))
     m = x.amin(-1, keepdim=True).half().float()
-    s = ((x.amax(-1, keepdim=True) - m) / 15.0).clamp(0.0, MAX_SCALE).half().float()
+    s = ((x.amax(-1, keepdim=True) - m) / 15.0).clamp(min=0.0).half().float()
     c = torch.where(s > 0, torch.round((x - m) / s), torch.zeros_like(x)).clamp(0.0, 15.0)
     return c.flatten(-2), s.squeeze(-1), m.squeeze(-1)
 
@@ -476,9 +475,9 @@ def _exact_quantised(x):
     out = torch.empty(x.shape, dtype=torch.float64, device=x.device)
     for g in range(0, x.size(-1), 64):
         part = x[..., g: g + 64].double()
-        part = torch.where(torch.isnan(part), torch.zeros_like(part), part).clamp(-65504, 65504)
+        part = torch.where(torch.isnan(part), torch.zeros_like(part), part).clamp(-65024, 65024)
         low = part.min(-1, keepdim=True).values.half().double()
-        step = ((part.max(-1, keepdim=True).values - low) / 15).clamp(0, 8728).half().double()
+        step = ((part.max(-1, keepdim=True).values - low) / 15).clamp(min=0).half().double()
         code = ((part - low) / step.clamp(min=1e-30)).round().clamp(0, 15) * (step > 0)
         out[..., g: g + 64] = low + step * code
     return out
