@@ -26,6 +26,9 @@
  *                            (locations :173-181, model.rotary_emb + float cast :191-193)
  *   hw_rope_append ......... apply_rotary_pos_emb on the new keys + the per-worker cache update,
  *                            python/hogwild/attention.py:84-90, :313-318, :148-158; and merge_caches, :251-257
+ *   hw_copy_to_blocks_q4, hw_read_blocks_q4, hw_paged_sdpa_q4, hw_varlen_paged_sdpa_q4 ... no counterpart: the paged operators with
+ *                            caches in 4 bits
+ *   hw_fork_blocks, hw_free_blocks, hw_reserve_blocks, hw_compact_blocks, hw_copy_pages ... no counterpart: the pages of paged caches
  *   hw_build_inputs_dev, hw_advance_lengths, hw_problem.len_dev, hw_append.len_dev ... no counterpart: the same steps
  *                            with the segment lengths in device memory, so that a decode step captured as a HIP graph
  *                            can be replayed while the segments grow
@@ -299,6 +302,89 @@ typedef struct hw_copy_blocks {
 } hw_copy_blocks;
 
 int hw_copy_to_blocks(const hw_copy_blocks* c, void* stream);
+
+/*
+ * Paged caches in 4 bits.  A value is offset + scale * code, code in 0 .. 15, with a scale and an offset in fp16 for every token, kv
+ * head and group of 64 channels: 9/16 of a byte for every channel.  E == Ev in {64, 128, 256}; block_size is a multiple of 8.
+ *   key_cache, value_cache   [num_blocks, Hkv, block_size, HW_Q4_ROW_BYTES(E)] bytes, 16-byte aligned.  Eight consecutive tokens of a
+ *       block and kv head lie together, 8 * HW_Q4_ROW_BYTES(E) bytes: the codes, 4 * E bytes, then for every group of 64 channels the
+ *       eight tokens' scales and their eight offsets.  Codes of keys: [8 tokens][E / 8 words of 32 bits], word w of a token the channels
+ *       64 * (r / 2) + 16 * (w / (E / 32)) + 8 * (r % 2) + 0 .. 7, r = w % (E / 32); of values: [E words], word c the eight tokens of
+ *       channel c.  Nibble i (from the low end) of a word is element 2 * i for i < 4 and 2 * i - 7 for the others.
+ * Stored are, of the values x of a group, offset = fp16(min x), scale = fp16(max((max x - offset) / 15, 0)), code =
+ * round((x - offset) / scale) within 0 .. 15 (0 with scale 0), computed in fp32, ties to the even number.  Values beyond +-65024 and
+ * infinities count as +-65024, NaN as 0: what a cache holds is finite, whatever came in, so that a token that a query does not
+ * see cannot reach its result.
+ */
+#define HW_Q4_ROW_BYTES(D) ((D) / 16 * 9)
+
+/* hw_copy_to_blocks into such caches (E and Ev are channels).  The tokens of an eight that are not appended keep their codes, so two
+   sequences that append at a time must not share the blocks that they write (hw_reserve_blocks sees to that). */
+int hw_copy_to_blocks_q4(const hw_copy_blocks* c, void* stream);
+
+/* The other way: key_states and value_states are written, packed [B, Hkv, S_new, E] in `dtype` (the strides are not looked at), with
+   the values at positions seq_lengths[b] + t; zeros where a position is negative or behind the table, or its block outside the cache. */
+int hw_read_blocks_q4(const hw_copy_blocks* c, void* stream);
+
+/* hw_paged_sdpa and hw_varlen_paged_sdpa over such caches: the same problem, limits and results (also lse), queries and output in
+   16 bits.  The logits are products of the queries with the codes themselves, in fp32; values are rounded to fp16 (by less than 2^-11
+   of themselves), weights too.  row_blocks: 0, 1 or 2 (1 at E == 256). */
+int hw_paged_q4_validate(const hw_paged_problem* p);
+int hw_paged_q4_plan_debug(const hw_paged_problem* p, int num_cus, hw_paged_plan* plan);   /* host only */
+int hw_paged_q4_workspace_bytes(const hw_paged_problem* p, size_t* bytes);
+int hw_paged_sdpa_q4(const hw_paged_problem* p, void* stream);
+int hw_varlen_paged_sdpa_q4(const hw_paged_problem* p, void* stream);
+
+/* ------------------------------------------------------------------------------------------------------------
+ * The pages (blocks) of a pool: which sequences name them, and copies of them.  All of it is worked out on the device, so the
+ * operators can be captured in a graph; results depend on no order of execution.
+ *   block_table  [W, max_blocks]  int32   row w names the pages of sequence w; entries outside 0 .. num_blocks - 1 name none (-1 is written)
+ *   seq_lengths  [W]              int32   tokens of the sequences (hw_compact_blocks does not look at them)
+ *   ref_counts   [num_blocks]     int32   how many entries name a page; 0 = free
+ *   caches       HOST array of n_caches device pointers: tensors of num_blocks pages each (keys and values of every layer, 4-bit
+ *                caches as well), page_bytes[i] consecutive bytes a page.  hw_fork_blocks and hw_free_blocks do not look at them.
+ *   workspace    hw_pool_workspace_bytes() bytes of device memory, 4-byte aligned; hw_reserve_blocks and hw_compact_blocks only
+ * W <= 4096, block_size * max_blocks <= 2^30, pages below 2 GiB.
+ */
+typedef struct hw_pool {
+    int32_t W, max_blocks, num_blocks, block_size;
+    int32_t* block_table;
+    int32_t* seq_lengths;
+    int32_t* ref_counts;
+    void* const* caches;
+    const size_t* page_bytes;
+    int32_t n_caches;
+    void* workspace;
+    size_t workspace_bytes;
+} hw_pool;
+
+int hw_pool_workspace_bytes(const hw_pool* p, size_t* bytes);
+
+/* Sequence w becomes what sequence parents[w] (device int32 [W]) is: its pages, shared, and its length; all sequences at once.  Itself: it
+   stays as it is.  A number outside 0 .. W - 1: it gives its pages back and has length 0.  Pages without tokens (entries from
+   ceil(length / block_size) on) are not passed on. */
+int hw_fork_blocks(const hw_pool* p, const int32_t* parents, void* stream);
+/* The sequences with finished[w] != 0 (device, one byte each) give their pages back and have length 0. */
+int hw_free_blocks(const hw_pool* p, const uint8_t* finished, void* stream);
+
+/*
+ * Room for n_new[w] (device int32 [W]) more tokens of every sequence, whose lengths grow by that.  A sequence wants the pages that its row
+ * lacks for positions length .. length + n_new - 1, and a copy of the page of its next token where that holds tokens already and is
+ * named by others too -- all but the last of several sequences that ask for that page.  The wants of the sequences in their
+ * order, of one by position, get the free pages in ascending order.  From the first sequence on whose wants the free pages do
+ * not cover, no sequence that wants a page or is to write a shared one gets any: all or nothing for each.  positions[w] (device
+ * int32 [W], written) = the first new token's position; for a sequence that gets nothing, asks for none or would outgrow its row,
+ * block_size * max_blocks, which the appends leave out, and its length stays.
+ */
+int hw_reserve_blocks(const hw_pool* p, const int32_t* n_new, int32_t* positions, void* stream);
+
+/* The pages that sequences name (ref_counts > 0) become the first ones of the pool: those behind as many places as there are of them
+   move, in ascending order, to the free pages before.  used[0] (device int32) = how many there are. */
+int hw_compact_blocks(const hw_pool* p, int32_t* used, void* stream);
+
+/* Pages src[i] -> dst[i] (HOST arrays) of every tensor.  A page that is written is named once and is no source (HW_ERR_SHAPE). */
+int hw_copy_pages(void* const* caches, const size_t* page_bytes, int n_caches, int num_blocks, const int32_t* src, const int32_t* dst, int n,
+                  void* stream);
 
 /* ------------------------------------------------------------------------------------------------------------
  * Caller-side steps of a decode step (the reference does them in Python, python/hogwild/attention.py:137-204,251-257).

@@ -30,6 +30,9 @@ EXPORTS = [
     "hw_paged_sdpa_stages", "hw_copy_to_blocks", "hw_build_inputs", "hw_rope_append",
     "hw_build_inputs_dev", "hw_advance_lengths", "hw_fused_attention_static", "hw_sdpa_workspace_bytes",
     "hw_merge_segments",
+    "hw_copy_to_blocks_q4", "hw_read_blocks_q4", "hw_paged_q4_validate", "hw_paged_q4_plan_debug", "hw_paged_q4_workspace_bytes",
+    "hw_paged_sdpa_q4", "hw_varlen_paged_sdpa_q4",
+    "hw_pool_workspace_bytes", "hw_fork_blocks", "hw_free_blocks", "hw_reserve_blocks", "hw_compact_blocks", "hw_copy_pages",
 ]
 
 
@@ -95,6 +98,15 @@ class HwCopyBlocks(C.Structure):
     ]
 
 
+class HwPool(C.Structure):
+    _fields_ = [
+        ("W", C.c_int32), ("max_blocks", C.c_int32), ("num_blocks", C.c_int32), ("block_size", C.c_int32),
+        ("block_table", C.c_void_p), ("seq_lengths", C.c_void_p), ("ref_counts", C.c_void_p),
+        ("caches", C.POINTER(C.c_void_p)), ("page_bytes", C.POINTER(C.c_size_t)), ("n_caches", C.c_int32),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
 class HwAppend(C.Structure):
     _fields_ = [
         ("dtype", C.c_int32), ("cs_dtype", C.c_int32), ("mode", C.c_int32),
@@ -155,6 +167,19 @@ def _load() -> C.CDLL:
     lib.hw_build_inputs_dev.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.POINTER(C.c_int32), C.c_void_p, C.c_float,
                                         C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p]
     lib.hw_advance_lengths.argtypes = [C.c_void_p, C.POINTER(C.c_int32), C.c_int, C.c_void_p]
+    lib.hw_copy_to_blocks_q4.argtypes = [C.POINTER(HwCopyBlocks), C.c_void_p]
+    lib.hw_read_blocks_q4.argtypes = [C.POINTER(HwCopyBlocks), C.c_void_p]
+    lib.hw_paged_q4_validate.argtypes = [C.POINTER(HwPagedProblem)]
+    lib.hw_paged_q4_plan_debug.argtypes = [C.POINTER(HwPagedProblem), C.c_int, C.POINTER(HwPagedPlan)]
+    lib.hw_paged_q4_workspace_bytes.argtypes = [C.POINTER(HwPagedProblem), C.POINTER(C.c_size_t)]
+    lib.hw_paged_sdpa_q4.argtypes = [C.POINTER(HwPagedProblem), C.c_void_p]
+    lib.hw_varlen_paged_sdpa_q4.argtypes = [C.POINTER(HwPagedProblem), C.c_void_p]
+    lib.hw_pool_workspace_bytes.argtypes = [C.POINTER(HwPool), C.POINTER(C.c_size_t)]
+    lib.hw_fork_blocks.argtypes = [C.POINTER(HwPool), C.c_void_p, C.c_void_p]
+    lib.hw_free_blocks.argtypes = [C.POINTER(HwPool), C.c_void_p, C.c_void_p]
+    lib.hw_reserve_blocks.argtypes = [C.POINTER(HwPool), C.c_void_p, C.c_void_p, C.c_void_p]
+    lib.hw_compact_blocks.argtypes = [C.POINTER(HwPool), C.c_void_p, C.c_void_p]
+    lib.hw_copy_pages.argtypes = [C.POINTER(C.c_void_p), C.POINTER(C.c_size_t), C.c_int, C.c_int, C.POINTER(C.c_int32), C.POINTER(C.c_int32), C.c_int, C.c_void_p]
     return lib
 
 
@@ -350,19 +375,36 @@ def plan(lens: Sequence[int], *, W: int, S: int, Hq: int, Hkv: int, Ev: int, num
     return out
 
 
+def q4_row_bytes(head_dim: int) -> int:
+    """Bytes of one token's codes, scales and offsets in a 4-bit cache (HW_Q4_ROW_BYTES)."""
+    return head_dim // 16 * 9
+
+
+def check_q4_caches(key_cache: torch.Tensor, value_cache: torch.Tensor, head_dim: int) -> None:
+    if key_cache.dtype != torch.uint8 or value_cache.dtype != torch.uint8:
+        raise ValueError("4-bit caches must be uint8")
+    if head_dim not in (64, 128, 256):
+        raise HogwildError(-4, "4-bit caches")
+    if key_cache.size(3) != q4_row_bytes(head_dim) or value_cache.size(3) != q4_row_bytes(head_dim):
+        raise ValueError(f"4-bit caches of head dimension {head_dim} have rows of {q4_row_bytes(head_dim)} bytes")
+    if key_cache.size(2) % 8 != 0:
+        raise ValueError("the block size of a 4-bit cache must be a multiple of 8")
+
+
 class PagedProblem:
     """One call of the paged attention operators (hw_paged_sdpa, or hw_varlen_paged_sdpa when cu_seqlens_q is given).
 
     fixed length:    q [F, W, Hq, S, E], locations [F, W, S], fragment_lengths [F], out [W, Hq, S, Ev], lse [W, Hq, S]
     variable length: q [F, T, Hq, E], locations [F, T], fragment_lengths [F, W], cu_seqlens_q [W+1], out [T, Hq, Ev],
                      lse [T, Hq]
-    key_cache / value_cache [num_blocks, Hkv, block_size, E|Ev], block_table int32 [W, max_blocks].
+    key_cache / value_cache [num_blocks, Hkv, block_size, E|Ev], block_table int32 [W, max_blocks]; with q4 = True uint8
+    [num_blocks, Hkv, block_size, q4_row_bytes(E)] (hw_paged_sdpa_q4, hw_varlen_paged_sdpa_q4).
     """
 
     def __init__(self, *, q: torch.Tensor, locations: torch.Tensor, fragment_lengths: torch.Tensor,
                  key_cache: torch.Tensor, value_cache: torch.Tensor, block_table: torch.Tensor, scale: float,
                  out: torch.Tensor, cu_seqlens_q: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
-                 splits: int = 0, row_blocks: int = 0):
+                 splits: int = 0, row_blocks: int = 0, q4: bool = False):
         varlen = cu_seqlens_q is not None
         if out.dtype not in _DTYPE_CODE:
             raise HogwildError(-2, "PagedProblem")
@@ -370,6 +412,9 @@ class PagedProblem:
             raise ValueError("key_cache / value_cache must be [num_blocks, Hkv, block_size, E|Ev]")
         NB, Hkv, BS, E = key_cache.shape
         Ev = value_cache.size(3)
+        if q4:
+            E = Ev = q.size(-1)
+            check_q4_caches(key_cache, value_cache, E)
         if block_table.dim() != 2:
             raise ValueError("block_table must be [W, max_blocks]")
         W = block_table.size(0)
@@ -402,7 +447,7 @@ class PagedProblem:
         for t in (locations, fragment_lengths, block_table) + ((cu_seqlens_q,) if varlen else ()):
             if t.dtype != torch.int32:
                 raise ValueError("locations, fragment_lengths, block_table and cu_seqlens_q must be int32")
-        for t in (q, key_cache, value_cache):
+        for t in (q,) if q4 else (q, key_cache, value_cache):
             if t.dtype != out.dtype:
                 raise ValueError("queries and caches must have the dtype of the output")
         for t in tensors:
@@ -430,12 +475,17 @@ class PagedProblem:
         p.row_blocks = int(row_blocks)
         self.p = p
         self.varlen = varlen
+        self.q4 = q4
         self._ws = None
 
     def workspace_bytes(self) -> int:
         n = C.c_size_t(0)
         with torch.cuda.device(self.device):
-            check(lib.hw_paged_workspace_bytes(C.byref(self.p), C.byref(n)), "hw_paged_workspace_bytes")
+            if self.q4:
+                check(lib.hw_paged_q4_validate(C.byref(self.p)), "hw_paged_q4_validate")
+                check(lib.hw_paged_q4_workspace_bytes(C.byref(self.p), C.byref(n)), "hw_paged_q4_workspace_bytes")
+            else:
+                check(lib.hw_paged_workspace_bytes(C.byref(self.p), C.byref(n)), "hw_paged_workspace_bytes")
         return n.value
 
     def set_workspace(self, ws: Optional[torch.Tensor] = None) -> None:
@@ -451,15 +501,20 @@ class PagedProblem:
         with torch.cuda.device(self.device):
             stream = torch.cuda.current_stream(self.device).cuda_stream
             if stages != 3:
+                if self.q4:
+                    raise ValueError("separate stages exist for caches in 16 and 32 bits only")
                 check(lib.hw_paged_sdpa_stages(C.byref(self.p), C.c_void_p(stream), stages), "hw_paged_sdpa_stages")
                 return
-            fn = lib.hw_varlen_paged_sdpa if self.varlen else lib.hw_paged_sdpa
+            if self.q4:
+                fn = lib.hw_varlen_paged_sdpa_q4 if self.varlen else lib.hw_paged_sdpa_q4
+            else:
+                fn = lib.hw_varlen_paged_sdpa if self.varlen else lib.hw_paged_sdpa
             check(fn(C.byref(self.p), C.c_void_p(stream)), fn.__name__)
 
 
 def paged_plan(*, W: int, Hq: int, Hkv: int, Ev: int, block_size: int, max_blocks: int, num_cus: int, S: int = 0,
-               total_q: Optional[int] = None, splits: int = 0, dtype: int = HW_BF16, row_blocks: int = 0) -> HwPagedPlan:
-    """Host-only plan of the paged operators (no GPU needed); total_q selects the variable-length operator."""
+               total_q: Optional[int] = None, splits: int = 0, dtype: int = HW_BF16, row_blocks: int = 0, q4: bool = False) -> HwPagedPlan:
+    """Host-only plan of the paged operators (no GPU needed); total_q selects the variable-length operator, q4 caches in 4 bits."""
     p = HwPagedProblem()
     p.dtype = dtype
     p.F, p.W, p.Hq, p.Hkv, p.E, p.Ev, p.S = 1, W, Hq, Hkv, Ev, Ev, S
@@ -470,24 +525,29 @@ def paged_plan(*, W: int, Hq: int, Hkv: int, Ev: int, block_size: int, max_block
     p.splits = splits
     p.row_blocks = row_blocks
     out = HwPagedPlan()
-    check(lib.hw_paged_plan_debug(C.byref(p), num_cus, C.byref(out)), "hw_paged_plan_debug")
+    fn = lib.hw_paged_q4_plan_debug if q4 else lib.hw_paged_plan_debug
+    check(fn(C.byref(p), num_cus, C.byref(out)), fn.__name__)
     return out
 
 
 def copy_to_blocks(key_states: torch.Tensor, value_states: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
-                   block_table: torch.Tensor, seq_lengths: torch.Tensor) -> None:
+                   block_table: torch.Tensor, seq_lengths: torch.Tensor, q4: bool = False) -> None:
     """Append key_states / value_states [B, Hkv, S_new, E|Ev] (any strides with a contiguous last dimension) to the
-    paged caches at positions seq_lengths[b] + t."""
+    paged caches at positions seq_lengths[b] + t; with q4 to caches in 4 bits."""
     if key_states.dim() != 4 or value_states.dim() != 4 or key_states.shape[:3] != value_states.shape[:3]:
         raise ValueError("key_states / value_states must be [B, Hkv, S_new, E|Ev]")
     B, Hkv, S_new, E = key_states.shape
     Ev = value_states.size(3)
-    if key_cache.dim() != 4 or value_cache.dim() != 4 or key_cache.size(1) != Hkv or key_cache.size(3) != E \
-            or value_cache.size(3) != Ev or key_cache.shape[:3] != value_cache.shape[:3]:
+    if key_cache.dim() != 4 or value_cache.dim() != 4 or key_cache.size(1) != Hkv or key_cache.shape[:3] != value_cache.shape[:3] \
+            or (not q4 and (key_cache.size(3) != E or value_cache.size(3) != Ev)):
         raise ValueError("caches must be [num_blocks, Hkv, block_size, E|Ev]")
     if key_states.dtype not in _DTYPE_CODE:
         raise HogwildError(-2, "copy_to_blocks")
-    for t in (value_states, key_cache, value_cache):
+    if q4:
+        if E != Ev:
+            raise ValueError("4-bit caches have one head dimension for keys and values")
+        check_q4_caches(key_cache, value_cache, E)
+    for t in (value_states,) if q4 else (value_states, key_cache, value_cache):
         if t.dtype != key_states.dtype:
             raise ValueError("states and caches must share one dtype")
     if tuple(seq_lengths.shape) != (B,) or block_table.dim() != 2 or block_table.size(0) != B:
@@ -513,7 +573,134 @@ def copy_to_blocks(key_states: torch.Tensor, value_states: torch.Tensor, key_cac
     c.block_table, c.seq_lengths = block_table.data_ptr(), seq_lengths.data_ptr()
     with torch.cuda.device(key_cache.device):
         stream = torch.cuda.current_stream(key_cache.device).cuda_stream
-        check(lib.hw_copy_to_blocks(C.byref(c), C.c_void_p(stream)), "hw_copy_to_blocks")
+        fn = lib.hw_copy_to_blocks_q4 if q4 else lib.hw_copy_to_blocks
+        check(fn(C.byref(c), C.c_void_p(stream)), fn.__name__)
+
+
+def read_blocks_q4(key_states: torch.Tensor, value_states: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                   block_table: torch.Tensor, seq_lengths: torch.Tensor) -> None:
+    """Write the values of a 4-bit cache at positions seq_lengths[b] + t into key_states / value_states [B, Hkv, n, D]."""
+    if key_states.dim() != 4 or key_states.shape != value_states.shape or not key_states.is_contiguous() or not value_states.is_contiguous():
+        raise ValueError("key_states / value_states must be contiguous [B, Hkv, n, D]")
+    if key_states.dtype not in _DTYPE_CODE or value_states.dtype != key_states.dtype:
+        raise HogwildError(-2, "read_blocks_q4")
+    B, Hkv, n, D = key_states.shape
+    if key_cache.dim() != 4 or key_cache.shape != value_cache.shape or key_cache.size(1) != Hkv or not key_cache.is_contiguous() or not value_cache.is_contiguous():
+        raise ValueError("caches must be contiguous [num_blocks, Hkv, block_size, row bytes]")
+    check_q4_caches(key_cache, value_cache, D)
+    if tuple(seq_lengths.shape) != (B,) or block_table.dim() != 2 or block_table.size(0) != B:
+        raise ValueError("block_table must be [B, max_blocks], seq_lengths [B]")
+    for t in (block_table, seq_lengths):
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise ValueError("block_table and seq_lengths must be contiguous int32")
+    for t in (key_states, value_states, value_cache, block_table, seq_lengths):
+        if t.device != key_cache.device:
+            raise ValueError("all tensors must live on the caches' device")
+    c = HwCopyBlocks()
+    c.dtype = _DTYPE_CODE[key_states.dtype]
+    c.B, c.Hkv, c.S_new, c.E, c.Ev = B, Hkv, n, D, D
+    c.block_size, c.max_blocks, c.num_blocks = key_cache.size(2), block_table.size(1), key_cache.size(0)
+    c.key_states, c.value_states = key_states.data_ptr(), value_states.data_ptr()
+    c.key_cache, c.value_cache = key_cache.data_ptr(), value_cache.data_ptr()
+    c.block_table, c.seq_lengths = block_table.data_ptr(), seq_lengths.data_ptr()
+    with torch.cuda.device(key_cache.device):
+        stream = torch.cuda.current_stream(key_cache.device).cuda_stream
+        check(lib.hw_read_blocks_q4(C.byref(c), C.c_void_p(stream)), "hw_read_blocks_q4")
+
+
+class _Pool:
+    """hw_pool of a block table [W, max_blocks], the sequences' lengths [W], the pages' counts [num_blocks] and the caches."""
+
+    def __init__(self, block_table: torch.Tensor, seq_lengths: Optional[torch.Tensor], ref_counts: torch.Tensor, block_size: int = 1,
+                 caches: Sequence[torch.Tensor] = ()):
+        if block_table.dim() != 2 or ref_counts.dim() != 1 or block_table.numel() == 0 or ref_counts.numel() == 0:
+            raise ValueError("block_table must be [W, max_blocks], ref_counts [num_blocks]")
+        if seq_lengths is not None and tuple(seq_lengths.shape) != (block_table.size(0),):
+            raise ValueError("seq_lengths must be [W]")
+        if int(block_size) < 1:
+            raise ValueError("block_size must be positive")
+        self.device = block_table.device
+        self.vectors = [t for t in (block_table, seq_lengths, ref_counts) if t is not None]
+        self.check_ints(*self.vectors)
+        p = HwPool()
+        p.W, p.max_blocks, p.num_blocks, p.block_size = block_table.size(0), block_table.size(1), ref_counts.numel(), int(block_size)
+        p.block_table, p.ref_counts = block_table.data_ptr(), ref_counts.data_ptr()
+        p.seq_lengths = seq_lengths.data_ptr() if seq_lengths is not None else None
+        self._ptr, self._bytes = _pages_of(caches, p.num_blocks, self.device)
+        p.caches, p.page_bytes, p.n_caches = C.cast(self._ptr, C.POINTER(C.c_void_p)), C.cast(self._bytes, C.POINTER(C.c_size_t)), len(caches)
+        self.p = p
+
+    def check_ints(self, *tensors: torch.Tensor) -> None:
+        for t in tensors:
+            if t.dtype != torch.int32 or not t.is_contiguous() or t.device != self.device:
+                raise ValueError("the tables of a pool must be contiguous int32 on one device")
+
+    def run(self, fn, *args, workspace: bool = False) -> None:
+        with torch.cuda.device(self.device):
+            if workspace:
+                n = C.c_size_t(0)
+                check(lib.hw_pool_workspace_bytes(C.byref(self.p), C.byref(n)), "hw_pool_workspace_bytes")
+                ws = torch.empty(n.value, dtype=torch.uint8, device=self.device)
+                self.p.workspace, self.p.workspace_bytes = ws.data_ptr(), n.value
+            stream = torch.cuda.current_stream(self.device).cuda_stream
+            check(fn(C.byref(self.p), *args, C.c_void_p(stream)), fn.__name__)
+
+
+def _pages_of(caches: Sequence[torch.Tensor], num_blocks: int, device):
+    for i, t in enumerate(caches):
+        if t.dim() < 1 or t.size(0) != num_blocks or not t.is_contiguous() or t.numel() == 0 or t.device != device:
+            raise ValueError(f"cache {i} must be contiguous [num_blocks, ...] with {num_blocks} blocks on the pool's device")
+    n = max(1, len(caches))
+    return ((C.c_void_p * n)(*[t.data_ptr() for t in caches]),
+            (C.c_size_t * n)(*[t.numel() // num_blocks * t.element_size() for t in caches]))
+
+
+def fork_blocks(block_table, seq_lengths, ref_counts, parents, block_size: int) -> None:
+    pool = _Pool(block_table, seq_lengths, ref_counts, block_size)
+    if tuple(parents.shape) != (block_table.size(0),):
+        raise ValueError("parents must be [W]")
+    pool.check_ints(parents)
+    pool.run(lib.hw_fork_blocks, parents.data_ptr())
+
+
+def free_blocks(block_table, seq_lengths, ref_counts, finished) -> None:
+    pool = _Pool(block_table, seq_lengths, ref_counts)
+    if tuple(finished.shape) != (block_table.size(0),) or finished.dtype not in (torch.bool, torch.uint8) or not finished.is_contiguous() \
+            or finished.device != pool.device:
+        raise ValueError("finished must be contiguous bool [W]")
+    pool.run(lib.hw_free_blocks, finished.data_ptr())
+
+
+def reserve_blocks(block_table, seq_lengths, ref_counts, n_new, positions, caches, block_size: int) -> None:
+    pool = _Pool(block_table, seq_lengths, ref_counts, block_size, caches)
+    if tuple(n_new.shape) != (block_table.size(0),) or tuple(positions.shape) != (block_table.size(0),):
+        raise ValueError("n_new and positions must be [W]")
+    pool.check_ints(n_new, positions)
+    pool.run(lib.hw_reserve_blocks, n_new.data_ptr(), positions.data_ptr(), workspace=True)
+
+
+def compact_blocks(block_table, ref_counts, caches, used) -> None:
+    pool = _Pool(block_table, None, ref_counts, 1, caches)
+    if used.numel() != 1:
+        raise ValueError("used must be one number")
+    pool.check_ints(used)
+    pool.run(lib.hw_compact_blocks, used.data_ptr(), workspace=True)
+
+
+def copy_blocks(caches: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int]) -> None:
+    if len(caches) == 0 or caches[0].dim() < 1:
+        raise ValueError("copy_blocks needs caches [num_blocks, ...]")
+    if len(src) != len(dst):
+        raise ValueError("one destination for every source block")
+    nb, device = caches[0].size(0), caches[0].device
+    if any(not 0 <= int(x) < nb for x in list(src) + list(dst)):
+        raise ValueError(f"blocks outside 0..{nb - 1}")
+    ptr, nbytes = _pages_of(caches, nb, device)
+    n = len(src)
+    with torch.cuda.device(device):
+        stream = torch.cuda.current_stream(device).cuda_stream
+        check(lib.hw_copy_pages(ptr, nbytes, len(caches), nb, (C.c_int32 * max(1, n))(*[int(x) for x in src]),
+                                (C.c_int32 * max(1, n))(*[int(x) for x in dst]), n, C.c_void_p(stream)), "hw_copy_pages")
 
 
 def build_inputs(pos_end: Sequence[Sequence[int]], S: int, inv_freq: Optional[torch.Tensor], *, attention_scaling: float = 1.0,

@@ -9,7 +9,7 @@ C entry points are called through ctypes.
 from __future__ import annotations
 
 import os
-from typing import Iterable, List, Optional
+from typing import Iterable, List, Optional, Sequence, Tuple
 
 import torch
 
@@ -159,3 +159,127 @@ def copy_to_blocks(key_states: torch.Tensor, value_states: torch.Tensor, key_cac
         torch.ops.libhogatt.copy_to_blocks(key_states, value_states, key_cache, value_cache, block_table, seq_lengths)
         return
     _lib.copy_to_blocks(key_states, value_states, key_cache, value_cache, block_table, seq_lengths)
+
+
+# ---- paged caches in 4 bits (no counterpart in the reference) ---------------------------------------------------------------------
+
+def q4_cache(num_blocks: int, num_kv_heads: int, block_size: int, head_dim: int, device="cuda") -> torch.Tensor:
+    """A paged cache in 4 bits, for keys or for values: uint8 [num_blocks, Hkv, block_size, 9 * head_dim / 16].  A value is
+    offset + scale * code, with a scale and an offset in fp16 for every token, kv head and group of 64 channels (the layout stands in
+    include/hogwild_hip.h)."""
+    if head_dim not in (64, 128, 256) or block_size < 8 or block_size % 8 != 0:
+        raise ValueError("4-bit caches exist for head dimensions 64, 128 and 256 and block sizes that are multiples of 8")
+    return torch.zeros((num_blocks, num_kv_heads, block_size, _lib.q4_row_bytes(head_dim)), dtype=torch.uint8, device=device)
+
+
+def copy_to_blocks_q4(key_states: torch.Tensor, value_states: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                      block_table: torch.Tensor, seq_lengths: torch.Tensor) -> None:
+    """copy_to_blocks into caches in 4 bits: the new rows [B,Hkv,S_new,D] are quantised on the way.  Values beyond +-65024 count as
+    +-65024 and NaN as 0, so that a cache holds finite values only."""
+    if HAVE_TORCH_OPS:
+        torch.ops.libhogatt.copy_to_blocks_q4(key_states, value_states, key_cache, value_cache, block_table, seq_lengths)
+        return
+    _lib.copy_to_blocks(key_states, value_states, key_cache, value_cache, block_table, seq_lengths, q4=True)
+
+
+def read_blocks_q4(key_cache: torch.Tensor, value_cache: torch.Tensor, block_table: torch.Tensor, seq_lengths: torch.Tensor, n: int, *,
+                   dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The keys and values [B,Hkv,n,D] that a cache in 4 bits holds at positions seq_lengths[b] + t, t < n (float32: exactly); zeros
+    where there are none (a position behind the table, a block outside the cache)."""
+    shape = (block_table.size(0), key_cache.size(1), int(n), key_cache.size(3) // 9 * 16)
+    k, v = torch.empty(shape, dtype=dtype, device=key_cache.device), torch.empty(shape, dtype=dtype, device=key_cache.device)
+    if HAVE_TORCH_OPS:
+        torch.ops.libhogatt.read_blocks_q4(k, v, key_cache, value_cache, block_table, seq_lengths)
+    else:
+        _lib.read_blocks_q4(k, v, key_cache, value_cache, block_table, seq_lengths)
+    return k, v
+
+
+def hogwild_paged_sdpa_q4(queries: torch.Tensor, locations: torch.Tensor, fragment_lengths: torch.Tensor, key_cache: torch.Tensor,
+                          value_cache: torch.Tensor, block_table: torch.Tensor, scale: float, out=None,
+                          lse: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """hogwild_paged_sdpa over caches in 4 bits: queries [F,W,Hq,S,D] and output [W,Hq,S,D] in float16 or bfloat16."""
+    if out is None:
+        out = torch.empty((queries.size(1), queries.size(2), queries.size(3), queries.size(4)), dtype=queries.dtype, device=queries.device)
+    if HAVE_TORCH_OPS and lse is None:
+        torch.ops.libhogatt.hogwild_paged_sdpa_q4(out, scale, locations, queries.contiguous(), fragment_lengths, key_cache, value_cache,
+                                                  block_table)
+        return out
+    _lib.PagedProblem(q=queries.contiguous(), locations=locations, fragment_lengths=fragment_lengths, key_cache=key_cache,
+                      value_cache=value_cache, block_table=block_table, scale=scale, out=out, lse=lse, q4=True).run()
+    return out
+
+
+def hogwild_varlen_paged_sdpa_q4(queries: torch.Tensor, locations: torch.Tensor, fragment_lengths: torch.Tensor,
+                                 key_cache: torch.Tensor, value_cache: torch.Tensor, block_table: torch.Tensor,
+                                 cu_seqlens_q: torch.Tensor, cu_seqlens_k: Optional[torch.Tensor], scale: float, out=None,
+                                 lse: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """hogwild_varlen_paged_sdpa over caches in 4 bits: packed queries [F,total_q,Hq,D] in float16 or bfloat16.  Query tokens that belong
+    to no sequence get zeros."""
+    if out is None:
+        out = torch.empty((queries.size(1), queries.size(2), queries.size(3)), dtype=queries.dtype, device=queries.device)
+    if HAVE_TORCH_OPS and lse is None:
+        torch.ops.libhogatt.hogwild_varlen_paged_sdpa_q4(out, scale, locations, queries.contiguous(), fragment_lengths, key_cache,
+                                                         value_cache, block_table, cu_seqlens_q,
+                                                         cu_seqlens_k if cu_seqlens_k is not None else cu_seqlens_q)
+        return out
+    _lib.PagedProblem(q=queries.contiguous(), locations=locations, fragment_lengths=fragment_lengths, key_cache=key_cache,
+                      value_cache=value_cache, block_table=block_table, scale=scale, out=out, cu_seqlens_q=cu_seqlens_q,
+                      lse=lse, q4=True).run()
+    return out
+
+
+# ---- the pages of paged caches (no counterpart in the reference) --------------------------------------------------------------------
+# A pool: block_table int32 [W, max_blocks], seq_lengths int32 [W], ref_counts int32 [num_blocks] (how many rows name a page; 0 = free)
+# and `caches`, tensors [num_blocks, ...] of any type (keys and values of every layer).  Everything is worked out on the device.
+
+def fork_blocks(block_table: torch.Tensor, seq_lengths: torch.Tensor, ref_counts: torch.Tensor, parents: torch.Tensor, block_size: int) -> None:
+    """Sequence w becomes what sequence parents[w] (int32 [W]) is, all at once: its pages, shared, and its length.  Itself: it stays as it
+    is; a number that is no sequence: it gives its pages back and has length 0."""
+    if HAVE_TORCH_OPS:
+        torch.ops.libhogatt.fork_blocks(block_table, seq_lengths, ref_counts, parents, block_size)
+        return
+    _lib.fork_blocks(block_table, seq_lengths, ref_counts, parents, block_size)
+
+
+def free_blocks(block_table: torch.Tensor, seq_lengths: torch.Tensor, ref_counts: torch.Tensor, finished: torch.Tensor) -> None:
+    """The sequences with finished[w] (bool [W]) give their pages back and have length 0."""
+    if HAVE_TORCH_OPS:
+        torch.ops.libhogatt.free_blocks(block_table, seq_lengths, ref_counts, finished)
+        return
+    _lib.free_blocks(block_table, seq_lengths, ref_counts, finished)
+
+
+def reserve_blocks(block_table: torch.Tensor, seq_lengths: torch.Tensor, ref_counts: torch.Tensor, n_new: torch.Tensor,
+                   caches: Sequence[torch.Tensor], block_size: int, positions: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Pages for n_new[w] (int32 [W]) more tokens of every sequence: those its row lacks, and a copy (in all `caches`) of a shared page
+    that is about to be written.  Returns positions [W], where the new tokens go (the lengths so far); a sequence that gets
+    nothing has block_size * max_blocks there, which the appends leave out, and keeps its length (see hw_reserve_blocks)."""
+    if positions is None:
+        positions = torch.empty_like(seq_lengths)
+    if HAVE_TORCH_OPS:
+        torch.ops.libhogatt.reserve_blocks(block_table, seq_lengths, ref_counts, n_new, positions, list(caches), block_size)
+    else:
+        _lib.reserve_blocks(block_table, seq_lengths, ref_counts, n_new, positions, list(caches), block_size)
+    return positions
+
+
+def compact_blocks(block_table: torch.Tensor, ref_counts: torch.Tensor, caches: Sequence[torch.Tensor],
+                   used: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The pages in use become the first ones of the pool, in all `caches`, table and counts.  Returns their number, int32 [1] on the
+    device."""
+    if used is None:
+        used = torch.empty(1, dtype=torch.int32, device=ref_counts.device)
+    if HAVE_TORCH_OPS:
+        torch.ops.libhogatt.compact_blocks(block_table, ref_counts, list(caches), used)
+    else:
+        _lib.compact_blocks(block_table, ref_counts, list(caches), used)
+    return used
+
+
+def copy_blocks(caches: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int]) -> None:
+    """Pages src[i] -> dst[i] (host numbers) of every tensor of `caches`.  A page that is written is named once, and not as a source."""
+    if HAVE_TORCH_OPS and len(caches) > 0 and caches[0].is_cuda:
+        torch.ops.libhogatt.copy_blocks(list(caches), src, dst)
+        return
+    _lib.copy_blocks(list(caches), src, dst)

@@ -12,6 +12,9 @@ library: the objects a model's attention layer talks to during a Hogwild! decode
                       rotary tables (:164-196) is one `hw_build_inputs` launch.
   merge_caches ...... attention.py:251-257: re-rotate a segment by the target's length and append it, all layers in one
                       launch.
+  PagedCache ........ sequences in pages of one pool, in 16, 32 or 4 bits, for the paged operators (src/binding.cu:110-215 has the
+                      operators; who holds which page is left to the caller there): reserving, forking, freeing and compacting
+                      pages on the device.
 
 Everything numeric runs in the HIP library; there is no torch fallback.
 """
@@ -23,6 +26,7 @@ from typing import Any, Dict, List, Optional, Sequence
 import torch
 
 from . import _lib
+from . import attention as _ops
 from .attention import HAVE_TORCH_OPS
 
 if HAVE_TORCH_OPS:
@@ -390,3 +394,83 @@ def merge_caches(target: SegmentCache, source: SegmentCache, model=None, *, inv_
         _lib.rope_append(source.k[layer][:, :m, :].unsqueeze(0), source.v[layer][:, :m, :].unsqueeze(0), [target.k[layer]], [target.v[layer]],
                          [target.lengths[layer]], cosines=cos, sines=sin, mode=mode)
         target.lengths[layer] += m
+
+
+class PagedCache:
+    """`max_seqs` sequences in the pages of one pool, for all layers of a model: keys[layer] / values[layer] are the caches of the paged
+    operators, [num_blocks, Hkv, block_size, D] in `dtype` or, with bits = 4, caches in 4 bits.  Block table, lengths and the pages'
+    counts live in device memory and are worked on there, so a step (reserve, then update and attend of every layer) can be
+    captured in a graph and replayed while the sequences grow.
+
+        cache.reserve(S)                                 # room for S tokens of every sequence (or a number for each, int32 [max_seqs])
+        for layer in ...:
+            cache.update(k, v, layer)                    # [max_seqs, Hkv, S, D], keys rotated
+            out = cache.attend(q, layer, scale)          # [max_seqs, Hq, S, D], queries rotated; new tokens see each other causally
+        cache.fork(parents)                              # sequence w goes on as sequence parents[w]; pages are shared until they are written
+        cache.free(finished); cache.compact()            # pages in use to the front of the pool
+
+    A sequence that `reserve` has nothing for (the pool or its row of the table is full, or it asked for no tokens) is left out of the
+    step: its states are not written, its output is 0 and its length stays; `granted()` says which ones took part."""
+
+    def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, num_blocks: int, max_seqs: int, *, block_size: int = 16,
+                 max_blocks: Optional[int] = None, bits: int = 16, dtype=torch.bfloat16, device="cuda"):
+        if bits not in (4, 16, 32) or (bits != 4 and torch.empty((), dtype=dtype).element_size() * 8 != bits):
+            raise ValueError(f"bits must be 4, or the size of {dtype}")
+        self.bits, self.block_size, self.dtype = bits, int(block_size), dtype
+        max_blocks = int(num_blocks if max_blocks is None else max_blocks)
+
+        def one():
+            if bits == 4:
+                return _ops.q4_cache(num_blocks, num_kv_heads, block_size, head_dim, device=device)
+            return torch.zeros((num_blocks, num_kv_heads, block_size, head_dim), dtype=dtype, device=device)
+
+        self.keys, self.values = [one() for _ in range(num_layers)], [one() for _ in range(num_layers)]
+        ints = dict(dtype=torch.int32, device=device)
+        self.block_table = torch.full((max_seqs, max_blocks), -1, **ints)
+        self.seq_lengths, self.ref_counts = torch.zeros(max_seqs, **ints), torch.zeros(num_blocks, **ints)
+        self.positions = torch.zeros(max_seqs, **ints)
+        self.used = torch.zeros(1, **ints)
+        self._longest = torch.full((1,), max_blocks * self.block_size, **ints)
+        self._locations: Dict[int, torch.Tensor] = {}
+
+    @property
+    def caches(self) -> List[torch.Tensor]:
+        return self.keys + self.values
+
+    def reserve(self, n_new) -> torch.Tensor:
+        """Positions [max_seqs] of the first new token of every sequence (see attention.reserve_blocks)."""
+        if not isinstance(n_new, torch.Tensor):
+            n_new = torch.full_like(self.seq_lengths, int(n_new))
+        self._locations = {}
+        return _ops.reserve_blocks(self.block_table, self.seq_lengths, self.ref_counts, n_new, self.caches, self.block_size, self.positions)
+
+    def granted(self) -> torch.Tensor:
+        """Which sequences got room in the last reserve, bool [max_seqs] on the device."""
+        return self.positions < self._longest
+
+    def update(self, key_states: torch.Tensor, value_states: torch.Tensor, layer_idx: int) -> None:
+        append = _ops.copy_to_blocks_q4 if self.bits == 4 else _ops.copy_to_blocks
+        append(key_states, value_states, self.keys[layer_idx], self.values[layer_idx], self.block_table, self.positions)
+
+    def attend(self, queries: torch.Tensor, layer_idx: int, scale: float) -> torch.Tensor:
+        S = queries.size(2)
+        loc = self._locations.get(S)
+        if loc is None:          # (the same for all layers of a step)
+            steps = torch.arange(S, dtype=torch.int32, device=self.positions.device)
+            loc = torch.where(self.granted()[:, None], self.positions[:, None] + steps[None, :], -1).unsqueeze(0).contiguous()
+            self._locations[S] = loc
+        sdpa = _ops.hogwild_paged_sdpa_q4 if self.bits == 4 else _ops.hogwild_paged_sdpa
+        return sdpa(queries.unsqueeze(0), loc, self._longest, self.keys[layer_idx], self.values[layer_idx], self.block_table, scale)
+
+    def fork(self, parents: torch.Tensor) -> None:
+        _ops.fork_blocks(self.block_table, self.seq_lengths, self.ref_counts, parents, self.block_size)
+
+    def free(self, finished: torch.Tensor) -> None:
+        _ops.free_blocks(self.block_table, self.seq_lengths, self.ref_counts, finished)
+
+    def compact(self) -> torch.Tensor:
+        """The number of pages in use, int32 [1] on the device: they are now pages 0 .. used - 1."""
+        return _ops.compact_blocks(self.block_table, self.ref_counts, self.caches, self.used)
+
+    def copy_blocks(self, src: Sequence[int], dst: Sequence[int]) -> None:
+        _ops.copy_blocks(self.caches, src, dst)

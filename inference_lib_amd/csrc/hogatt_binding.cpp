@@ -282,10 +282,19 @@ void hogwild_fused_lse(at::Tensor& out, at::Tensor& rq, at::Tensor& lse, double 
 
 // ---- paged operators -------------------------------------------------------------------------------------------
 
+// Caches in 4 bits: uint8 [num_blocks, Hkv, block_size, HW_Q4_ROW_BYTES(D)].
+void check_q4_caches(const at::Tensor& key_cache, const at::Tensor& value_cache, int64_t D) {
+    TORCH_CHECK(key_cache.scalar_type() == at::kByte && value_cache.scalar_type() == at::kByte, "libhogatt: 4-bit caches must be uint8");
+    TORCH_CHECK(D == 64 || D == 128 || D == 256, "libhogatt: 4-bit caches exist for head dimensions 64, 128 and 256, got ", D);
+    TORCH_CHECK(key_cache.size(3) == HW_Q4_ROW_BYTES(D) && value_cache.size(3) == HW_Q4_ROW_BYTES(D), "libhogatt: 4-bit caches of head dimension ", D,
+                " have rows of ", HW_Q4_ROW_BYTES(D), " bytes, got ", key_cache.size(3), " and ", value_cache.size(3));
+    TORCH_CHECK(key_cache.size(2) % 8 == 0, "libhogatt: the block size of a 4-bit cache must be a multiple of 8, got ", key_cache.size(2));
+}
+
 // Checks shared by the two paged attention operators; fills everything of hw_paged_problem except the query layout.
 void unpack_paged(hw_paged_problem& p, at::Tensor& out, double scale, const at::Tensor& locations, const at::Tensor& queries,
                   const at::Tensor& fragment_lengths, const at::Tensor& key_cache, const at::Tensor& value_cache,
-                  const at::Tensor& block_table) {
+                  const at::Tensor& block_table, bool q4 = false) {
     TORCH_CHECK(key_cache.dim() == 4 && value_cache.dim() == 4, "libhogatt: caches must be [num_blocks, Hkv, block_size, D]");
     TORCH_CHECK(key_cache.size(0) == value_cache.size(0) && key_cache.size(1) == value_cache.size(1) && key_cache.size(2) == value_cache.size(2),
                 "libhogatt: key_cache and value_cache differ in blocks, heads or block size");
@@ -295,16 +304,21 @@ void unpack_paged(hw_paged_problem& p, at::Tensor& out, double scale, const at::
     TORCH_CHECK(fragment_lengths.scalar_type() == at::kInt && fragment_lengths.is_contiguous(), "libhogatt: fragment_lengths must be contiguous int32");
     TORCH_CHECK(out.is_contiguous() && queries.is_contiguous() && key_cache.is_contiguous() && value_cache.is_contiguous(),
                 "libhogatt: output, queries and caches must be contiguous");
-    TORCH_CHECK(queries.scalar_type() == out.scalar_type() && key_cache.scalar_type() == out.scalar_type() && value_cache.scalar_type() == out.scalar_type(),
-                "libhogatt: queries and caches must have the dtype of the output");
+    if (q4) {
+        TORCH_CHECK(queries.scalar_type() == out.scalar_type(), "libhogatt: queries and output must have the same dtype");
+        check_q4_caches(key_cache, value_cache, queries.size(-1));
+    } else {
+        TORCH_CHECK(queries.scalar_type() == out.scalar_type() && key_cache.scalar_type() == out.scalar_type() && value_cache.scalar_type() == out.scalar_type(),
+                    "libhogatt: queries and caches must have the dtype of the output");
+    }
     for (const at::Tensor* t : {&locations, &queries, &fragment_lengths, &key_cache, &value_cache, &block_table})
         TORCH_CHECK(t->device() == out.device(), "libhogatt: all tensors must live on the output's device");
     p.dtype = dtype_code(out);
     p.F = (int32_t)locations.size(0);
     p.W = (int32_t)block_table.size(0);
     p.Hkv = (int32_t)key_cache.size(1);
-    p.E = (int32_t)key_cache.size(3);
-    p.Ev = (int32_t)value_cache.size(3);
+    p.E = (int32_t)(q4 ? queries.size(-1) : key_cache.size(3));
+    p.Ev = (int32_t)(q4 ? queries.size(-1) : value_cache.size(3));
     p.block_size = (int32_t)key_cache.size(2);
     p.max_blocks = (int32_t)block_table.size(1);
     p.num_blocks = (int32_t)key_cache.size(0);
@@ -318,25 +332,32 @@ void unpack_paged(hw_paged_problem& p, at::Tensor& out, double scale, const at::
     p.block_table = block_table.const_data_ptr<int32_t>();
 }
 
-void run_paged(hw_paged_problem& p, const at::Tensor& out, bool varlen) {
+void run_paged(hw_paged_problem& p, const at::Tensor& out, bool varlen, bool q4 = false) {
     c10::hip::HIPGuardMasqueradingAsCUDA guard(out.device());
     size_t bytes = 0;
-    check_status(hw_paged_workspace_bytes(&p, &bytes), "hw_paged_workspace_bytes");
+    if (q4) {
+        check_status(hw_paged_q4_validate(&p), "hw_paged_q4_validate");
+        check_status(hw_paged_q4_workspace_bytes(&p, &bytes), "hw_paged_q4_workspace_bytes");
+    } else {
+        check_status(hw_paged_workspace_bytes(&p, &bytes), "hw_paged_workspace_bytes");
+    }
     at::Tensor workspace = at::empty({(int64_t)(bytes > 0 ? bytes : 256)}, out.options().dtype(at::kByte));
     p.workspace = workspace.data_ptr();
     p.workspace_bytes = bytes;
     hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(out.device().index()).stream();
-    if (varlen)
+    if (q4)
+        check_status(varlen ? hw_varlen_paged_sdpa_q4(&p, stream) : hw_paged_sdpa_q4(&p, stream), varlen ? "hw_varlen_paged_sdpa_q4" : "hw_paged_sdpa_q4");
+    else if (varlen)
         check_status(hw_varlen_paged_sdpa(&p, stream), "hw_varlen_paged_sdpa");
     else
         check_status(hw_paged_sdpa(&p, stream), "hw_paged_sdpa");
 }
 
-void hogwild_paged_sdpa(at::Tensor& out, double scale, const at::Tensor& locations, const at::Tensor& queries,
-                        const at::Tensor& fragment_lengths, const at::Tensor& key_cache, const at::Tensor& value_cache,
-                        const at::Tensor& block_table) {
+template <bool Q4>
+void paged_sdpa(at::Tensor& out, double scale, const at::Tensor& locations, const at::Tensor& queries, const at::Tensor& fragment_lengths,
+                const at::Tensor& key_cache, const at::Tensor& value_cache, const at::Tensor& block_table) {
     hw_paged_problem p{};
-    unpack_paged(p, out, scale, locations, queries, fragment_lengths, key_cache, value_cache, block_table);
+    unpack_paged(p, out, scale, locations, queries, fragment_lengths, key_cache, value_cache, block_table, Q4);
     TORCH_CHECK(out.dim() == 4 && out.size(0) == p.W && out.size(3) == p.Ev, "libhogatt: output must be [W, Hq, S, Ev] with one block-table row per worker");
     p.Hq = (int32_t)out.size(1);
     p.S = (int32_t)out.size(2);
@@ -344,14 +365,15 @@ void hogwild_paged_sdpa(at::Tensor& out, double scale, const at::Tensor& locatio
                 "libhogatt: queries must be [F, W, Hq, S, E]");
     TORCH_CHECK(locations.dim() == 3 && locations.size(1) == p.W && locations.size(2) == p.S, "libhogatt: locations must be [F, W, S]");
     TORCH_CHECK(fragment_lengths.dim() == 1 && fragment_lengths.size(0) == p.F, "libhogatt: fragment_lengths must be [F]");
-    run_paged(p, out, false);
+    run_paged(p, out, false, Q4);
 }
 
-void hogwild_varlen_paged_sdpa(at::Tensor& out, double scale, const at::Tensor& locations, const at::Tensor& queries,
-                               const at::Tensor& fragment_lengths, const at::Tensor& key_cache, const at::Tensor& value_cache,
-                               const at::Tensor& block_table, const at::Tensor& cu_seqlens_q, const at::Tensor& cu_seqlens_k) {
+template <bool Q4>
+void varlen_paged_sdpa(at::Tensor& out, double scale, const at::Tensor& locations, const at::Tensor& queries,
+                       const at::Tensor& fragment_lengths, const at::Tensor& key_cache, const at::Tensor& value_cache,
+                       const at::Tensor& block_table, const at::Tensor& cu_seqlens_q, const at::Tensor& cu_seqlens_k) {
     hw_paged_problem p{};
-    unpack_paged(p, out, scale, locations, queries, fragment_lengths, key_cache, value_cache, block_table);
+    unpack_paged(p, out, scale, locations, queries, fragment_lengths, key_cache, value_cache, block_table, Q4);
     TORCH_CHECK(out.dim() == 3 && out.size(2) == p.Ev, "libhogatt: output must be [total_q, Hq, Ev]");
     p.total_q = (int32_t)out.size(0);
     p.Hq = (int32_t)out.size(1);
@@ -365,10 +387,11 @@ void hogwild_varlen_paged_sdpa(at::Tensor& out, double scale, const at::Tensor& 
                 "libhogatt: cu_seqlens_q must be contiguous int32 [W + 1] on the output's device");
     (void)cu_seqlens_k;   // carried in the reference's Shape but never read by its kernel (src/kernels/kernel_v21.cuh:658-899)
     p.cu_seqlens_q = cu_seqlens_q.const_data_ptr<int32_t>();
-    run_paged(p, out, true);
+    run_paged(p, out, true, Q4);
 }
 
-void copy_to_blocks(const at::Tensor& key_states, const at::Tensor& value_states, at::Tensor& key_cache, at::Tensor& value_cache,
+template <bool Q4>
+void append_blocks(const at::Tensor& key_states, const at::Tensor& value_states, at::Tensor& key_cache, at::Tensor& value_cache,
                     const at::Tensor& block_table, const at::Tensor& seq_lengths) {
     TORCH_CHECK(key_states.dim() == 4 && value_states.dim() == 4, "libhogatt: key_states / value_states must be [B, Hkv, S_new, D]");
     TORCH_CHECK(key_states.size(0) == value_states.size(0) && key_states.size(1) == value_states.size(1) && key_states.size(2) == value_states.size(2),
@@ -376,10 +399,16 @@ void copy_to_blocks(const at::Tensor& key_states, const at::Tensor& value_states
     TORCH_CHECK(key_cache.dim() == 4 && value_cache.dim() == 4 && key_cache.is_contiguous() && value_cache.is_contiguous(),
                 "libhogatt: caches must be contiguous [num_blocks, Hkv, block_size, D]");
     TORCH_CHECK(key_cache.size(0) == value_cache.size(0) && key_cache.size(1) == key_states.size(1) && value_cache.size(1) == key_states.size(1) &&
-                    key_cache.size(2) == value_cache.size(2) && key_cache.size(3) == key_states.size(3) && value_cache.size(3) == value_states.size(3),
+                    key_cache.size(2) == value_cache.size(2) && (Q4 || (key_cache.size(3) == key_states.size(3) && value_cache.size(3) == value_states.size(3))),
                 "libhogatt: caches do not match the states");
-    TORCH_CHECK(value_states.scalar_type() == key_states.scalar_type() && key_cache.scalar_type() == key_states.scalar_type() &&
-                    value_cache.scalar_type() == key_states.scalar_type(), "libhogatt: states and caches must share one dtype");
+    if (Q4) {
+        TORCH_CHECK(value_states.scalar_type() == key_states.scalar_type(), "libhogatt: key_states and value_states must share one dtype");
+        TORCH_CHECK(value_states.size(3) == key_states.size(3), "libhogatt: 4-bit caches have one head dimension for keys and values");
+        check_q4_caches(key_cache, value_cache, key_states.size(3));
+    } else {
+        TORCH_CHECK(value_states.scalar_type() == key_states.scalar_type() && key_cache.scalar_type() == key_states.scalar_type() &&
+                        value_cache.scalar_type() == key_states.scalar_type(), "libhogatt: states and caches must share one dtype");
+    }
     TORCH_CHECK(block_table.dim() == 2 && block_table.size(0) == key_states.size(0) && block_table.scalar_type() == at::kInt && block_table.is_contiguous(),
                 "libhogatt: block_table must be contiguous int32 [B, max_blocks]");
     TORCH_CHECK(seq_lengths.dim() == 1 && seq_lengths.size(0) == key_states.size(0) && seq_lengths.scalar_type() == at::kInt && seq_lengths.is_contiguous(),
@@ -401,7 +430,149 @@ void copy_to_blocks(const at::Tensor& key_states, const at::Tensor& value_states
     c.block_table = block_table.const_data_ptr<int32_t>(); c.seq_lengths = seq_lengths.const_data_ptr<int32_t>();
     c10::hip::HIPGuardMasqueradingAsCUDA guard(key_cache.device());
     hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(key_cache.device().index()).stream();
-    check_status(hw_copy_to_blocks(&c, stream), "hw_copy_to_blocks");
+    if (Q4)
+        check_status(hw_copy_to_blocks_q4(&c, stream), "hw_copy_to_blocks_q4");
+    else
+        check_status(hw_copy_to_blocks(&c, stream), "hw_copy_to_blocks");
+}
+
+// The values of a 4-bit cache at positions seq_lengths[b] + t into key_states / value_states [B, Hkv, n, D].
+void read_blocks_q4(at::Tensor& key_states, at::Tensor& value_states, const at::Tensor& key_cache, const at::Tensor& value_cache,
+                    const at::Tensor& block_table, const at::Tensor& seq_lengths) {
+    TORCH_CHECK(key_states.dim() == 4 && key_states.sizes() == value_states.sizes() && key_states.is_contiguous() && value_states.is_contiguous() &&
+                    key_states.scalar_type() == value_states.scalar_type(),
+                "libhogatt: key_states / value_states must be contiguous [B, Hkv, n, D] of one dtype");
+    TORCH_CHECK(key_cache.dim() == 4 && key_cache.sizes() == value_cache.sizes() && key_cache.is_contiguous() && value_cache.is_contiguous() &&
+                    key_cache.size(1) == key_states.size(1),
+                "libhogatt: caches must be contiguous [num_blocks, Hkv, block_size, row bytes] with the heads of the states");
+    check_q4_caches(key_cache, value_cache, key_states.size(3));
+    TORCH_CHECK(block_table.dim() == 2 && block_table.size(0) == key_states.size(0) && block_table.scalar_type() == at::kInt && block_table.is_contiguous(),
+                "libhogatt: block_table must be contiguous int32 [B, max_blocks]");
+    TORCH_CHECK(seq_lengths.dim() == 1 && seq_lengths.size(0) == key_states.size(0) && seq_lengths.scalar_type() == at::kInt && seq_lengths.is_contiguous(),
+                "libhogatt: seq_lengths must be contiguous int32 [B]");
+    for (const at::Tensor* t : std::initializer_list<const at::Tensor*>{&key_states, &value_states, &value_cache, &block_table, &seq_lengths})
+        TORCH_CHECK(t->device() == key_cache.device(), "libhogatt: all tensors must live on the caches' device");
+    hw_copy_blocks c{};
+    c.dtype = dtype_code(key_states);
+    c.B = (int32_t)key_states.size(0); c.Hkv = (int32_t)key_states.size(1); c.S_new = (int32_t)key_states.size(2);
+    c.E = c.Ev = (int32_t)key_states.size(3);
+    c.block_size = (int32_t)key_cache.size(2); c.max_blocks = (int32_t)block_table.size(1); c.num_blocks = (int32_t)key_cache.size(0);
+    c.key_states = key_states.data_ptr(); c.value_states = value_states.data_ptr();
+    c.key_cache = const_cast<void*>(key_cache.const_data_ptr()); c.value_cache = const_cast<void*>(value_cache.const_data_ptr());
+    c.block_table = block_table.const_data_ptr<int32_t>(); c.seq_lengths = seq_lengths.const_data_ptr<int32_t>();
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(key_cache.device());
+    hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(key_cache.device().index()).stream();
+    check_status(hw_read_blocks_q4(&c, stream), "hw_read_blocks_q4");
+}
+
+// ---- pages -----------------------------------------------------------------------------------------------------
+
+// The tensors of a pool as pages, and their table: `caches` [num_blocks, ...], contiguous.
+struct Pool {
+    hw_pool p{};
+    std::vector<void*> ptr;
+    std::vector<size_t> bytes;
+    at::Tensor workspace;
+};
+void pool_caches(Pool& u, at::TensorList caches, int64_t num_blocks, const at::Device& device) {
+    for (size_t i = 0; i < caches.size(); ++i) {
+        const at::Tensor& t = caches[i];
+        TORCH_CHECK(t.dim() >= 1 && t.size(0) == num_blocks && t.is_contiguous() && t.numel() > 0 && t.device() == device,
+                    "libhogatt: cache ", i, " must be contiguous [num_blocks, ...] with ", num_blocks, " blocks on the pool's device, got ", t.sizes());
+        u.ptr.push_back(t.data_ptr());
+        u.bytes.push_back((size_t)(t.numel() / num_blocks) * t.element_size());
+    }
+    u.p.caches = u.ptr.data();
+    u.p.page_bytes = u.bytes.data();
+    u.p.n_caches = (int32_t)u.ptr.size();
+}
+void pool_tables(Pool& u, at::Tensor& block_table, const at::Tensor* seq_lengths, at::Tensor& ref_counts, int64_t block_size) {
+    TORCH_CHECK(block_table.dim() == 2 && block_table.scalar_type() == at::kInt && block_table.is_contiguous() && block_table.numel() > 0,
+                "libhogatt: block_table must be contiguous int32 [W, max_blocks]");
+    TORCH_CHECK(ref_counts.dim() == 1 && ref_counts.scalar_type() == at::kInt && ref_counts.is_contiguous() && ref_counts.numel() > 0 && ref_counts.device() == block_table.device(),
+                "libhogatt: ref_counts must be contiguous int32 [num_blocks] on the table's device");
+    TORCH_CHECK(block_table.size(0) < (1ll << 31) && block_table.size(1) < (1ll << 31) && ref_counts.size(0) < (1ll << 31), "libhogatt: the pool is too large");
+    if (seq_lengths != nullptr)
+        TORCH_CHECK(seq_lengths->dim() == 1 && seq_lengths->size(0) == block_table.size(0) && seq_lengths->scalar_type() == at::kInt && seq_lengths->is_contiguous() &&
+                        seq_lengths->device() == block_table.device(),
+                    "libhogatt: seq_lengths must be contiguous int32 [W] on the table's device");
+    TORCH_CHECK(block_size >= 1 && block_size < (1ll << 31), "libhogatt: block_size must be positive");
+    u.p.W = (int32_t)block_table.size(0);
+    u.p.max_blocks = (int32_t)block_table.size(1);
+    u.p.num_blocks = (int32_t)ref_counts.size(0);
+    u.p.block_size = (int32_t)block_size;
+    u.p.block_table = block_table.data_ptr<int32_t>();
+    u.p.seq_lengths = seq_lengths != nullptr ? seq_lengths->data_ptr<int32_t>() : nullptr;
+    u.p.ref_counts = ref_counts.data_ptr<int32_t>();
+}
+void pool_workspace(Pool& u, const at::Tensor& like) {
+    size_t bytes = 0;
+    check_status(hw_pool_workspace_bytes(&u.p, &bytes), "hw_pool_workspace_bytes");
+    u.workspace = at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
+    u.p.workspace = u.workspace.data_ptr();
+    u.p.workspace_bytes = bytes;
+}
+hipStream_t stream_of(const at::Tensor& t) { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream(); }
+
+void fork_blocks(at::Tensor& block_table, at::Tensor& seq_lengths, at::Tensor& ref_counts, const at::Tensor& parents, int64_t block_size) {
+    Pool u;
+    pool_tables(u, block_table, &seq_lengths, ref_counts, block_size);
+    TORCH_CHECK(parents.dim() == 1 && parents.size(0) == u.p.W && parents.scalar_type() == at::kInt && parents.is_contiguous() && parents.device() == block_table.device(),
+                "libhogatt: parents must be contiguous int32 [W] on the table's device");
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(block_table.device());
+    check_status(hw_fork_blocks(&u.p, parents.const_data_ptr<int32_t>(), stream_of(block_table)), "hw_fork_blocks");
+}
+
+void free_blocks(at::Tensor& block_table, at::Tensor& seq_lengths, at::Tensor& ref_counts, const at::Tensor& finished) {
+    Pool u;
+    pool_tables(u, block_table, &seq_lengths, ref_counts, 1);
+    TORCH_CHECK(finished.dim() == 1 && finished.size(0) == u.p.W && (finished.scalar_type() == at::kBool || finished.scalar_type() == at::kByte) && finished.is_contiguous() &&
+                    finished.device() == block_table.device(),
+                "libhogatt: finished must be contiguous bool [W] on the table's device");
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(block_table.device());
+    check_status(hw_free_blocks(&u.p, reinterpret_cast<const uint8_t*>(finished.const_data_ptr()), stream_of(block_table)), "hw_free_blocks");
+}
+
+void reserve_blocks(at::Tensor& block_table, at::Tensor& seq_lengths, at::Tensor& ref_counts, const at::Tensor& n_new, at::Tensor& positions,
+                    at::TensorList caches, int64_t block_size) {
+    Pool u;
+    pool_tables(u, block_table, &seq_lengths, ref_counts, block_size);
+    pool_caches(u, caches, u.p.num_blocks, block_table.device());
+    for (const at::Tensor* t : std::initializer_list<const at::Tensor*>{&n_new, &positions})
+        TORCH_CHECK(t->dim() == 1 && t->size(0) == u.p.W && t->scalar_type() == at::kInt && t->is_contiguous() && t->device() == block_table.device(),
+                    "libhogatt: n_new and positions must be contiguous int32 [W] on the table's device");
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(block_table.device());
+    pool_workspace(u, block_table);
+    check_status(hw_reserve_blocks(&u.p, n_new.const_data_ptr<int32_t>(), positions.data_ptr<int32_t>(), stream_of(block_table)), "hw_reserve_blocks");
+}
+
+void compact_blocks(at::Tensor& block_table, at::Tensor& ref_counts, at::TensorList caches, at::Tensor& used) {
+    Pool u;
+    pool_tables(u, block_table, nullptr, ref_counts, 1);
+    pool_caches(u, caches, u.p.num_blocks, block_table.device());
+    TORCH_CHECK(used.numel() == 1 && used.scalar_type() == at::kInt && used.device() == block_table.device(), "libhogatt: used must be one int32 on the table's device");
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(block_table.device());
+    pool_workspace(u, block_table);
+    check_status(hw_compact_blocks(&u.p, used.data_ptr<int32_t>(), stream_of(block_table)), "hw_compact_blocks");
+}
+
+void copy_blocks(at::TensorList caches, at::IntArrayRef src, at::IntArrayRef dst) {
+    TORCH_CHECK(!caches.empty() && caches[0].dim() >= 1, "libhogatt: copy_blocks needs caches [num_blocks, ...]");
+    TORCH_CHECK(src.size() == dst.size(), "libhogatt: one destination for every source block, got ", src.size(), " and ", dst.size());
+    const int64_t num_blocks = caches[0].size(0);
+    Pool u;
+    pool_caches(u, caches, num_blocks, caches[0].device());
+    std::vector<int32_t> s(src.size()), d(dst.size());
+    for (size_t i = 0; i < src.size(); ++i) {
+        TORCH_CHECK(src[i] >= 0 && src[i] < num_blocks && dst[i] >= 0 && dst[i] < num_blocks, "libhogatt: blocks ", src[i], " -> ", dst[i], " outside 0..", num_blocks - 1);
+        s[i] = (int32_t)src[i];
+        d[i] = (int32_t)dst[i];
+    }
+    TORCH_CHECK(num_blocks < (1ll << 31) && (int64_t)src.size() <= num_blocks, "libhogatt: more pairs than blocks");
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(caches[0].device());
+    const int status = hw_copy_pages(u.ptr.data(), u.bytes.data(), (int)u.ptr.size(), (int)num_blocks, s.data(), d.data(), (int)s.size(), stream_of(caches[0]));
+    TORCH_CHECK(status != HW_ERR_SHAPE, "libhogatt: a block that is written may be named once only, and not as a source");
+    check_status(status, "hw_copy_pages");
 }
 
 // ---- segments ----------------------------------------------------------------------------------------------------
@@ -604,6 +775,21 @@ TORCH_LIBRARY(libhogatt, m) {
           "Tensor block_table, Tensor seq_lengths) -> ()", tags);
     m.def("hogwild_varlen_paged_sdpa(Tensor(a!) output, float scale, Tensor locations, Tensor queries, "
           "Tensor fragment_lengths, Tensor key_cache, Tensor value_cache, Tensor block_table, Tensor cu_seqlens_q, Tensor cu_seqlens_k) -> ()", tags);
+    // additions: caches in 4 bits, and the pages of paged caches
+    m.def("copy_to_blocks_q4(Tensor key_states, Tensor value_states, Tensor(a!) key_cache, Tensor(b!) value_cache, "
+          "Tensor block_table, Tensor seq_lengths) -> ()", tags);
+    m.def("read_blocks_q4(Tensor(a!) key_states, Tensor(b!) value_states, Tensor key_cache, Tensor value_cache, "
+          "Tensor block_table, Tensor seq_lengths) -> ()", tags);
+    m.def("hogwild_paged_sdpa_q4(Tensor(a!) output, float scale, Tensor locations, Tensor queries, "
+          "Tensor fragment_lengths, Tensor key_cache, Tensor value_cache, Tensor block_table) -> ()", tags);
+    m.def("hogwild_varlen_paged_sdpa_q4(Tensor(a!) output, float scale, Tensor locations, Tensor queries, "
+          "Tensor fragment_lengths, Tensor key_cache, Tensor value_cache, Tensor block_table, Tensor cu_seqlens_q, Tensor cu_seqlens_k) -> ()", tags);
+    m.def("fork_blocks(Tensor(a!) block_table, Tensor(b!) seq_lengths, Tensor(c!) ref_counts, Tensor parents, int block_size) -> ()", tags);
+    m.def("free_blocks(Tensor(a!) block_table, Tensor(b!) seq_lengths, Tensor(c!) ref_counts, Tensor finished) -> ()", tags);
+    m.def("reserve_blocks(Tensor(a!) block_table, Tensor(b!) seq_lengths, Tensor(c!) ref_counts, Tensor n_new, Tensor(d!) positions, "
+          "Tensor(e!)[] caches, int block_size) -> ()", tags);
+    m.def("compact_blocks(Tensor(a!) block_table, Tensor(b!) ref_counts, Tensor(c!)[] caches, Tensor(d!) used) -> ()", tags);
+    m.def("copy_blocks(Tensor(a!)[] caches, int[] src, int[] dst) -> ()", tags);
     // addition: merge_caches (python/hogwild/attention.py:251-257) for all layers of a segment
     m.def("merge_segments(Tensor(a!)[] k_dst, Tensor(b!)[] v_dst, int[] dst_len, Tensor[] k_src, Tensor[] v_src, int[] n, Tensor inv_freq, "
           "float scaling, int position, ScalarType table_dtype, int mode) -> bool", tags);
@@ -625,9 +811,18 @@ TORCH_LIBRARY_IMPL(libhogatt, CUDA, m) {
     m.impl("hogwild_sdpa_lse", hogwild_sdpa_lse);
     m.impl("hogwild_fused_lse", hogwild_fused_lse);
     m.impl("hogwild_fused_devlen", hogwild_fused_devlen);
-    m.impl("hogwild_paged_sdpa", hogwild_paged_sdpa);
-    m.impl("copy_to_blocks", copy_to_blocks);
-    m.impl("hogwild_varlen_paged_sdpa", hogwild_varlen_paged_sdpa);
+    m.impl("hogwild_paged_sdpa", paged_sdpa<false>);
+    m.impl("copy_to_blocks", append_blocks<false>);
+    m.impl("hogwild_varlen_paged_sdpa", varlen_paged_sdpa<false>);
+    m.impl("hogwild_paged_sdpa_q4", paged_sdpa<true>);
+    m.impl("copy_to_blocks_q4", append_blocks<true>);
+    m.impl("hogwild_varlen_paged_sdpa_q4", varlen_paged_sdpa<true>);
+    m.impl("read_blocks_q4", read_blocks_q4);
+    m.impl("fork_blocks", fork_blocks);
+    m.impl("free_blocks", free_blocks);
+    m.impl("reserve_blocks", reserve_blocks);
+    m.impl("compact_blocks", compact_blocks);
+    m.impl("copy_blocks", copy_blocks);
     m.impl("merge_segments", merge_segments);
     m.impl("rope_append", rope_append);
     m.impl("segment_views", segment_views);

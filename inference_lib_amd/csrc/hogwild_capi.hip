@@ -4,9 +4,11 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <cstring>
+#include <new>
 
 #include "../../include/hogwild_hip.h"
 #include "hogwild_kernels.h"
@@ -203,6 +205,35 @@ int run(const hw_problem* p, void* stream_, int fused, int stages = HW_STAGE_ATT
 // ---------------------------------------------------------------------------------------------------------
 // paged variants
 // ---------------------------------------------------------------------------------------------------------
+// What a paged launch is told about its tensors and sizes, whatever it does with them; the row groups are those of the unplanned launches.
+void paged_header(const hw_paged_problem* p, const hw_paged_plan& plan, hw::PagedHeader& ph) {
+    const bool varlen = p->cu_seqlens_q != nullptr;
+    std::memset(&ph, 0, sizeof(ph));
+    ph.q = p->q;
+    ph.loc = p->locations;
+    ph.frag_len = p->fragment_lengths;
+    ph.kcache = p->key_cache;
+    ph.vcache = p->value_cache;
+    ph.block_table = p->block_table;
+    ph.cu_q = p->cu_seqlens_q;
+    ph.F = p->F; ph.W = p->W; ph.Hq = p->Hq; ph.Hkv = p->Hkv;
+    ph.LW = varlen ? p->total_q : p->W;
+    ph.LS = varlen ? 1 : p->S;
+    ph.R = plan.rows;
+    ph.block_size = p->block_size; ph.max_blocks = p->max_blocks; ph.num_blocks = p->num_blocks;
+    ph.nsplit = plan.splits;
+    ph.nitems = plan.row_groups;
+    ph.nrg = varlen ? 1 : plan.row_groups / p->W;
+    ph.nwg = plan.workgroups;
+    ph.sc = (float)((double)p->scale * 1.4426950408889634074);
+    ph.magic_gq = magic_of(p->Hq / p->Hkv);
+    ph.magic_ls = magic_of(ph.LS);
+    ph.magic_bs = magic_of(p->block_size);
+    ph.magic_nsplit = magic_of(ph.nsplit);
+    ph.magic_nitems = magic_of(ph.nitems);
+    ph.magic_nrg = magic_of(ph.nrg);
+}
+
 int paged_run(const hw_paged_problem* p, void* stream_, int stages) {
     int st = paged_validate(p);
     if (st != HW_OK) return st;
@@ -216,45 +247,25 @@ int paged_run(const hw_paged_problem* p, void* stream_, int stages) {
     if (p->workspace == nullptr || p->workspace_bytes < plan.workspace_bytes || !aligned16(p->workspace)) return HW_ERR_WORKSPACE;
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     const bool varlen = p->cu_seqlens_q != nullptr;
-    auto magic = [](int d) { return magic_of(d); };
 
     hw::PagedHeader ph;
-    std::memset(&ph, 0, sizeof(ph));
-    ph.q = p->q;
-    ph.loc = p->locations;
-    ph.frag_len = p->fragment_lengths;
-    ph.kcache = p->key_cache;
-    ph.vcache = p->value_cache;
-    ph.block_table = p->block_table;
-    ph.cu_q = p->cu_seqlens_q;
+    paged_header(p, plan, ph);
     // partial sums by (split, row), or -- planned on the device -- by workgroup slot, then the merge's row table
     const bool planned = plan.device_planned != 0;
     const size_t prows = planned ? (size_t)plan.row_groups * hw::PLAN_SLOT_ROWS : (size_t)plan.splits * plan.rows;
     ph.part_o = reinterpret_cast<float*>(p->workspace);
     ph.part_ml = ph.part_o + (size_t)p->Hkv * prows * p->Ev;
     int* row_tab = reinterpret_cast<int*>(ph.part_ml + (size_t)p->Hkv * prows * 2);
-    ph.F = p->F; ph.W = p->W; ph.Hq = p->Hq; ph.Hkv = p->Hkv;
-    ph.LW = varlen ? p->total_q : p->W;
-    ph.LS = varlen ? 1 : p->S;
-    ph.R = plan.rows;
-    ph.block_size = p->block_size; ph.max_blocks = p->max_blocks; ph.num_blocks = p->num_blocks;
-    ph.nsplit = plan.splits;
-    ph.nitems = plan.row_groups;
-    ph.nrg = planned ? (cus / p->Hkv > 0 ? cus / p->Hkv : 1) : varlen ? 1 : plan.row_groups / p->W;
-    ph.nwg = plan.workgroups;
+    if (planned) {
+        ph.nrg = cus / p->Hkv > 0 ? cus / p->Hkv : 1;
+        ph.magic_nrg = magic_of(ph.nrg);
+    }
     // (with the stages on their own, and in a workspace sized for hw_paged_plan only, the partials are laid out by it)
     const bool shared = stages == (HW_STAGE_ATTENTION | HW_STAGE_MERGE) && paged_shared(p, plan) && paged_shares_save(p, plan, cus) >= 0 && p->workspace_bytes >= paged_call_bytes(p, plan);
     ph.flags = ((plan.workgroups % 8 == 0) ? hw::PH_XCD_REMAP : 0) | (shared ? hw::PH_SHARED : 0) | (planned ? hw::PH_PLANNED : 0) | (paged_keep_in_l2(p, plan) ? hw::PH_KEEP : 0);
     if ((unsigned long long)p->num_blocks * p->Hkv * p->block_size * p->E * elem_size(p->dtype) < 0xffff0000ull) ph.flags |= hw::PH_SMALL;
     if (planned) ph.flags |= (p->W + plan.rows / hw::PLAN_SLOT_ROWS) << hw::PH_GROUPS_SHIFT;
     if (shared) ph.flags |= paged_shares_save(p, plan, cus) << hw::PH_SAVED_SHIFT;
-    ph.sc = (float)((double)p->scale * 1.4426950408889634074);
-    ph.magic_gq = magic(p->Hq / p->Hkv);
-    ph.magic_ls = magic(ph.LS);
-    ph.magic_bs = magic(p->block_size);
-    ph.magic_nsplit = magic(ph.nsplit);
-    ph.magic_nitems = magic(ph.nitems);
-    ph.magic_nrg = magic(ph.nrg);
 
     hipError_t e = hipSuccess;
     if (stages & HW_STAGE_ATTENTION) {
@@ -277,30 +288,229 @@ int paged_run(const hw_paged_problem* p, void* stream_, int stages) {
     ma.pslots = planned ? plan.row_groups : shared ? plan.row_groups * plan.splits : 0;
     ma.slot_rows = shared ? plan.rows / p->W : 0;
     ma.guess = shared ? plan.splits : 0;
-    ma.magic_rows = magic(shared ? ma.slot_rows : 1);
+    ma.magic_rows = magic_of(shared ? ma.slot_rows : 1);
     if (planned) ma.wgs_per_head = 8;       // a row's slots are device data: the merge shape that suits a handful of them
     e = hw::launch_merge(ma, p->dtype, p->Ev, stream);
     return (int)e;
 }
 
-int copy_blocks_run(const hw_copy_blocks* c, void* stream) {
-    if (c == nullptr) return HW_ERR_NULL;
-    if (c->dtype != HW_F32 && c->dtype != HW_F16 && c->dtype != HW_BF16) return HW_ERR_DTYPE;
-    if (c->B < 0 || c->Hkv < 1 || c->S_new < 0 || c->E < 1 || c->Ev < 1) return HW_ERR_SHAPE;
-    if (c->block_size < 1 || c->max_blocks < 1 || c->num_blocks < 1) return HW_ERR_SHAPE;
-    if ((long long)c->num_blocks * c->Hkv * c->block_size >= (1ll << 31)) return HW_ERR_SHAPE;
-    if (c->B == 0 || c->S_new == 0) return HW_OK;
+// The paged operators over caches in 4 bits.
+int paged_q4_run(const hw_paged_problem* p, void* stream_, int stages) {
+    int st = paged_q4_validate(p);
+    if (st != HW_OK) return st;
+    int cus = 0;
+    st = device_cus(&cus);
+    if (st != HW_OK) return st;
+    hw_paged_plan plan;
+    st = paged_q4_plan(p, cus, &plan);
+    if (st != HW_OK) return st;
+    if (plan.rows == 0) return HW_OK;       // no query tokens
+    if (p->workspace == nullptr || p->workspace_bytes < plan.workspace_bytes || !aligned16(p->workspace)) return HW_ERR_WORKSPACE;
+    hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+    hw::PagedHeader ph;
+    paged_header(p, plan, ph);
+    ph.magic_bs = magic_of(p->block_size / 8);
+    ph.part_o = reinterpret_cast<float*>(p->workspace);
+    ph.part_ml = ph.part_o + (size_t)p->Hkv * plan.splits * plan.rows * p->Ev;
+    ph.flags = plan.workgroups % 8 == 0 ? hw::PH_XCD_REMAP : 0;
+    hipError_t e = hipSuccess;
+    if (stages & HW_STAGE_ATTENTION) {
+        e = hw::launch_paged_q4(ph, p->dtype, p->E, plan.row_blocks, stream);
+        if (e != hipSuccess) return (int)e;
+    }
+    if (!(stages & HW_STAGE_MERGE)) return (int)e;
+    hw::MergeArgs ma;
+    std::memset(&ma, 0, sizeof(ma));
+    ma.part_o = ph.part_o;
+    ma.part_ml = ph.part_ml;
+    ma.out = p->out;
+    ma.lse = p->lse;
+    ma.W = ph.LW; ma.Hq = p->Hq; ma.Hkv = p->Hkv; ma.S = ph.LS; ma.R = ma.rows = plan.rows;
+    ma.wgs_per_head = plan.splits;
+    ma.xcd_local = (p->cu_seqlens_q == nullptr && plan.workgroups % 8 == 0 && p->Hkv % 8 == 0) ? 1 : 0;
+    ma.magic_rows = magic_of(1);
+    return (int)hw::launch_merge(ma, p->dtype, p->Ev, stream);
+}
+
+// What the operators on blocks of a cache have in common; false with *st = HW_OK: nothing to do.
+bool copy_blocks_args(const hw_copy_blocks* c, bool q4, hw::CopyBlocksArgs* a, int* st) {
+    *st = HW_OK;
+    auto refuse = [&](int s) { *st = s; return false; };
+    if (c == nullptr) return refuse(HW_ERR_NULL);
+    if (c->dtype != HW_F32 && c->dtype != HW_F16 && c->dtype != HW_BF16) return refuse(HW_ERR_DTYPE);
+    if (c->B < 0 || c->Hkv < 1 || c->S_new < 0 || c->E < 1 || c->Ev < 1) return refuse(HW_ERR_SHAPE);
+    if (c->block_size < 1 || c->max_blocks < 1 || c->num_blocks < 1) return refuse(HW_ERR_SHAPE);
+    if ((long long)c->num_blocks * c->Hkv * c->block_size >= (1ll << 31)) return refuse(HW_ERR_SHAPE);
+    if (q4) {
+        if (c->block_size % 8 != 0) return refuse(HW_ERR_SHAPE);
+        if ((long long)c->block_size * c->max_blocks > (1ll << 30) || c->S_new > (1 << 28) || c->B > 65535 || c->Hkv > 65535) return refuse(HW_ERR_SHAPE);
+        if (c->E != c->Ev || (c->E != 64 && c->E != 128 && c->E != 256)) return refuse(HW_ERR_UNSUPPORTED);
+    }
+    if (c->B == 0 || c->S_new == 0) return false;
     if (c->key_states == nullptr || c->value_states == nullptr || c->key_cache == nullptr || c->value_cache == nullptr ||
         c->block_table == nullptr || c->seq_lengths == nullptr)
-        return HW_ERR_NULL;
+        return refuse(HW_ERR_NULL);
+    if (q4 && (!aligned16(c->key_cache) || !aligned16(c->value_cache))) return refuse(HW_ERR_ALIGN);
+    a->key_states = c->key_states; a->value_states = c->value_states;
+    a->kcache = c->key_cache; a->vcache = c->value_cache;
+    a->block_table = c->block_table; a->seq_lengths = c->seq_lengths;
+    a->ks_b = c->ks_b; a->ks_h = c->ks_h; a->ks_s = c->ks_s; a->vs_b = c->vs_b; a->vs_h = c->vs_h; a->vs_s = c->vs_s;
+    a->B = c->B; a->Hkv = c->Hkv; a->S_new = c->S_new; a->E = c->E; a->Ev = c->Ev;
+    a->block_size = c->block_size; a->max_blocks = c->max_blocks; a->num_blocks = c->num_blocks;
+    return true;
+}
+
+int copy_blocks_run(const hw_copy_blocks* c, void* stream) {
     hw::CopyBlocksArgs a;
-    a.key_states = c->key_states; a.value_states = c->value_states;
-    a.kcache = c->key_cache; a.vcache = c->value_cache;
-    a.block_table = c->block_table; a.seq_lengths = c->seq_lengths;
-    a.ks_b = c->ks_b; a.ks_h = c->ks_h; a.ks_s = c->ks_s; a.vs_b = c->vs_b; a.vs_h = c->vs_h; a.vs_s = c->vs_s;
-    a.B = c->B; a.Hkv = c->Hkv; a.S_new = c->S_new; a.E = c->E; a.Ev = c->Ev;
-    a.block_size = c->block_size; a.max_blocks = c->max_blocks; a.num_blocks = c->num_blocks;
+    int st;
+    if (!copy_blocks_args(c, false, &a, &st)) return st;
     return (int)hw::launch_copy_to_blocks(a, c->dtype, reinterpret_cast<hipStream_t>(stream));
+}
+
+int append_q4_run(const hw_copy_blocks* c, void* stream) {
+    hw::CopyBlocksArgs a;
+    int st;
+    if (!copy_blocks_args(c, true, &a, &st)) return st;
+    return (int)hw::launch_append_q4(a, c->dtype, reinterpret_cast<hipStream_t>(stream));
+}
+
+int read_q4_run(const hw_copy_blocks* c, void* stream) {
+    hw::CopyBlocksArgs a;
+    int st;
+    if (!copy_blocks_args(c, true, &a, &st)) return st;
+    if (!aligned16(c->key_states) || !aligned16(c->value_states)) return HW_ERR_ALIGN;
+    return (int)hw::launch_read_q4(a, c->dtype, reinterpret_cast<hipStream_t>(stream));
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// the pages of a pool
+// ---------------------------------------------------------------------------------------------------------
+// What every operator on a pool needs; `lengths`, `tensors`: the sequences' lengths and the caches themselves too.
+int pool_args(const hw_pool* p, bool lengths, bool tensors, hw::PoolArgs* a) {
+    if (p == nullptr) return HW_ERR_NULL;
+    if (p->W < 1 || p->max_blocks < 1 || p->num_blocks < 1 || p->block_size < 1) return HW_ERR_SHAPE;
+    if (p->W > hw::POOL_MAX_ROWS) return HW_ERR_UNSUPPORTED;
+    if ((long long)p->block_size * p->max_blocks > (1ll << 30) || (long long)p->W * p->max_blocks > (1ll << 29)) return HW_ERR_SHAPE;
+    if (p->num_blocks > (1 << 28)) return HW_ERR_SHAPE;
+    if (p->block_table == nullptr || (lengths && p->seq_lengths == nullptr) || p->ref_counts == nullptr) return HW_ERR_NULL;
+    if (tensors) {
+        if (p->n_caches < 0) return HW_ERR_SHAPE;
+        if (p->n_caches > 0 && (p->caches == nullptr || p->page_bytes == nullptr)) return HW_ERR_NULL;
+        for (int i = 0; i < p->n_caches; ++i) {
+            if (p->caches[i] == nullptr) return HW_ERR_NULL;
+            if (p->page_bytes[i] < 1 || p->page_bytes[i] > 0x7fffffffu) return HW_ERR_SHAPE;
+        }
+    }
+    a->table = p->block_table;
+    a->lengths = p->seq_lengths;
+    a->refs = p->ref_counts;
+    a->W = p->W; a->max_blocks = p->max_blocks; a->num_blocks = p->num_blocks; a->block_size = p->block_size;
+    return HW_OK;
+}
+
+size_t pool_bytes(const hw_pool* p) {       // header, a number for every page, the pairs
+    return ((size_t)hw::POOL_WS_HEADER + (size_t)p->num_blocks + 2 * ((size_t)p->num_blocks / 2 + (size_t)p->W + 1)) * sizeof(int);
+}
+
+// Copies the pages that `a` names (its pairs are filled in already) in all tensors, as many launches as their table takes.
+int copy_tensors(hw::PageCopyArgs& a, void* const* caches, const size_t* page_bytes, int n, int most_pairs, hipStream_t stream) {
+    for (int i = 0; i < n || i == 0; i += hw::POOL_MAX_TENSORS) {
+        a.n_tensors = n - i < hw::POOL_MAX_TENSORS ? n - i : hw::POOL_MAX_TENSORS;
+        for (int t = 0; t < a.n_tensors; ++t) {
+            a.ptr[t] = caches[i + t];
+            a.bytes[t] = (unsigned)page_bytes[i + t];
+        }
+        if (a.n_tensors == 0 && a.to == nullptr) return HW_OK;
+        const hipError_t e = hw::launch_copy_pages(a, most_pairs, stream);
+        if (e != hipSuccess) return (int)e;
+        a.to = nullptr;                     // (the table is renamed once)
+    }
+    return HW_OK;
+}
+
+int fork_run(const hw_pool* p, const void* who, bool free_rows, void* stream) {
+    hw::PoolArgs a;
+    const int st = pool_args(p, true, false, &a);
+    if (st != HW_OK) return st;
+    if (who == nullptr) return HW_ERR_NULL;
+    return (int)hw::launch_fork(a, who, free_rows, reinterpret_cast<hipStream_t>(stream));
+}
+
+int reserve_run(const hw_pool* p, const int32_t* n_new, int32_t* positions, void* stream_) {
+    hw::PoolArgs a;
+    const int st = pool_args(p, true, true, &a);
+    if (st != HW_OK) return st;
+    if (n_new == nullptr || positions == nullptr) return HW_ERR_NULL;
+    if (p->workspace == nullptr || p->workspace_bytes < pool_bytes(p)) return HW_ERR_WORKSPACE;
+    hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+    int* ws = reinterpret_cast<int*>(p->workspace);
+    const hipError_t e = hw::launch_reserve(a, n_new, positions, ws, stream);
+    if (e != hipSuccess) return (int)e;
+    hw::PageCopyArgs c;
+    std::memset(&c, 0, sizeof(c));
+    c.num_blocks = p->num_blocks;
+    c.dev_pairs = ws + hw::POOL_WS_HEADER + p->num_blocks;
+    c.dev_pairs_n = ws;
+    return copy_tensors(c, p->caches, p->page_bytes, p->n_caches, p->W, stream);
+}
+
+int compact_run(const hw_pool* p, int32_t* used, void* stream_) {
+    hw::PoolArgs a;
+    const int st = pool_args(p, false, true, &a);
+    if (st != HW_OK) return st;
+    if (used == nullptr) return HW_ERR_NULL;
+    if (p->workspace == nullptr || p->workspace_bytes < pool_bytes(p)) return HW_ERR_WORKSPACE;
+    hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+    int* ws = reinterpret_cast<int*>(p->workspace);
+    const hipError_t e = hw::launch_compact(a, used, ws, stream);
+    if (e != hipSuccess) return (int)e;
+    hw::PageCopyArgs c;
+    std::memset(&c, 0, sizeof(c));
+    c.num_blocks = p->num_blocks;
+    c.to = ws + hw::POOL_WS_HEADER;
+    c.dev_pairs = c.to + p->num_blocks;
+    c.dev_pairs_n = ws;
+    c.table = p->block_table;
+    c.table_entries = (size_t)p->W * p->max_blocks;
+    return copy_tensors(c, p->caches, p->page_bytes, p->n_caches, p->num_blocks / 2 + 1, stream);
+}
+
+int copy_pages_run(void* const* caches, const size_t* page_bytes, int n_caches, int num_blocks, const int32_t* src, const int32_t* dst, int n, void* stream_) {
+    if (n < 0 || n_caches < 0 || num_blocks < 1 || n > num_blocks) return HW_ERR_SHAPE;
+    if (n == 0 || n_caches == 0) return HW_OK;
+    if (caches == nullptr || page_bytes == nullptr || src == nullptr || dst == nullptr) return HW_ERR_NULL;
+    for (int i = 0; i < n_caches; ++i) {
+        if (caches[i] == nullptr) return HW_ERR_NULL;
+        if (page_bytes[i] < 1 || page_bytes[i] > 0x7fffffffu) return HW_ERR_SHAPE;
+    }
+    // a page that is written is written once and not read: the pairs run side by side
+    int32_t* to = new (std::nothrow) int32_t[(size_t)n];
+    if (to == nullptr) return HW_ERR_WORKSPACE;
+    int st = HW_OK;
+    for (int i = 0; i < n; ++i) {
+        to[i] = dst[i];
+        if (src[i] < 0 || src[i] >= num_blocks || dst[i] < 0 || dst[i] >= num_blocks) st = HW_ERR_SHAPE;
+    }
+    std::sort(to, to + n);
+    for (int i = 1; i < n; ++i)
+        if (to[i] == to[i - 1]) st = HW_ERR_SHAPE;
+    for (int i = 0; i < n && st == HW_OK; ++i)
+        if (std::binary_search(to, to + n, src[i])) st = HW_ERR_SHAPE;
+    delete[] to;
+    if (st != HW_OK) return st;
+    hw::PageCopyArgs c;
+    std::memset(&c, 0, sizeof(c));
+    c.num_blocks = num_blocks;
+    for (int i = 0; i < n; i += hw::POOL_MAX_PAIRS) {
+        c.n_pairs = n - i < hw::POOL_MAX_PAIRS ? n - i : hw::POOL_MAX_PAIRS;
+        for (int k = 0; k < c.n_pairs; ++k) {
+            c.pairs[2 * k] = src[i + k];
+            c.pairs[2 * k + 1] = dst[i + k];
+        }
+        st = copy_tensors(c, caches, page_bytes, n_caches, c.n_pairs, reinterpret_cast<hipStream_t>(stream_));
+        if (st != HW_OK) return st;
+    }
+    return HW_OK;
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -597,6 +807,58 @@ int hw_paged_sdpa_stages(const hw_paged_problem* p, void* stream, int stages) {
 }
 
 int hw_copy_to_blocks(const hw_copy_blocks* c, void* stream) { return copy_blocks_run(c, stream); }
+
+int hw_copy_to_blocks_q4(const hw_copy_blocks* c, void* stream) { return append_q4_run(c, stream); }
+
+int hw_read_blocks_q4(const hw_copy_blocks* c, void* stream) { return read_q4_run(c, stream); }
+
+int hw_paged_q4_validate(const hw_paged_problem* p) { return paged_q4_validate(p); }
+
+int hw_paged_q4_plan_debug(const hw_paged_problem* p, int num_cus, hw_paged_plan* plan) {
+    if (p == nullptr || plan == nullptr) return HW_ERR_NULL;
+    return paged_q4_plan(p, num_cus, plan);
+}
+
+int hw_paged_q4_workspace_bytes(const hw_paged_problem* p, size_t* bytes) {
+    if (p == nullptr || bytes == nullptr) return HW_ERR_NULL;
+    int cus = 0;
+    int st = device_cus(&cus);
+    if (st != HW_OK) return st;
+    hw_paged_plan plan;
+    st = paged_q4_plan(p, cus, &plan);
+    if (st != HW_OK) return st;
+    *bytes = plan.workspace_bytes;
+    return HW_OK;
+}
+
+int hw_paged_sdpa_q4(const hw_paged_problem* p, void* stream) {
+    if (p != nullptr && p->cu_seqlens_q != nullptr) return HW_ERR_SHAPE;
+    return paged_q4_run(p, stream, HW_STAGE_ATTENTION | HW_STAGE_MERGE);
+}
+
+int hw_varlen_paged_sdpa_q4(const hw_paged_problem* p, void* stream) {
+    if (p != nullptr && p->cu_seqlens_q == nullptr) return HW_ERR_NULL;
+    return paged_q4_run(p, stream, HW_STAGE_ATTENTION | HW_STAGE_MERGE);
+}
+
+int hw_pool_workspace_bytes(const hw_pool* p, size_t* bytes) {
+    if (p == nullptr || bytes == nullptr) return HW_ERR_NULL;
+    if (p->W < 1 || p->num_blocks < 1) return HW_ERR_SHAPE;
+    *bytes = pool_bytes(p);
+    return HW_OK;
+}
+
+int hw_fork_blocks(const hw_pool* p, const int32_t* parents, void* stream) { return fork_run(p, parents, false, stream); }
+
+int hw_free_blocks(const hw_pool* p, const uint8_t* finished, void* stream) { return fork_run(p, finished, true, stream); }
+
+int hw_reserve_blocks(const hw_pool* p, const int32_t* n_new, int32_t* positions, void* stream) { return reserve_run(p, n_new, positions, stream); }
+
+int hw_compact_blocks(const hw_pool* p, int32_t* used, void* stream) { return compact_run(p, used, stream); }
+
+int hw_copy_pages(void* const* caches, const size_t* page_bytes, int n_caches, int num_blocks, const int32_t* src, const int32_t* dst, int n, void* stream) {
+    return copy_pages_run(caches, page_bytes, n_caches, num_blocks, src, dst, n, stream);
+}
 
 int hw_build_inputs(int32_t* locations, float* cosines, float* sines, const int32_t* pos_end, const float* inv_freq,
                     float attention_scaling, int round_dtype, int F, int W, int S, int RotE, void* stream) {

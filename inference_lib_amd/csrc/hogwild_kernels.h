@@ -148,6 +148,43 @@ hipError_t launch_paged_attention(const PagedHeader& ph, int dtype, int E, int r
 hipError_t launch_paged_attention_wide(const PagedHeader& ph, int dtype, int E, hipStream_t stream);   // 128 rows per workgroup
 hipError_t launch_copy_to_blocks(const CopyBlocksArgs& ca, int dtype, hipStream_t stream);
 
+// ---- paged caches in 4 bits (hogwild_q4.hip): E == Ev, block_size a multiple of 8 ----
+hipError_t launch_append_q4(const CopyBlocksArgs& ca, int dtype, hipStream_t stream);
+// key_states / value_states are written: contiguous [B, Hkv, S_new, E], positions seq_lengths[b] + t
+hipError_t launch_read_q4(const CopyBlocksArgs& ca, int dtype, hipStream_t stream);
+// kcache / vcache hold octets, magic_bs divides by block_size / 8
+hipError_t launch_paged_q4(const PagedHeader& ph, int dtype, int E, int rb, hipStream_t stream);
+
+// ---- the pages of a pool (hogwild_pages.hip) ----
+constexpr int POOL_MAX_ROWS = 4096;     // sequences of a pool: their wants are summed up by one workgroup
+constexpr int POOL_WS_HEADER = 16;      // ints of the workspace in front of its lists
+constexpr int POOL_MAX_TENSORS = 96;    // tensors per copy launch: their table travels in the kernel arguments
+constexpr int POOL_MAX_PAIRS = 256;     // pairs per copy launch that come from the host, for the same reason
+
+struct PoolArgs {
+    int* table;            // [W, max_blocks]
+    int* lengths;          // [W]
+    int* refs;             // [num_blocks]
+    int W, max_blocks, num_blocks, block_size;
+};
+struct PageCopyArgs {
+    void* ptr[POOL_MAX_TENSORS];
+    unsigned bytes[POOL_MAX_TENSORS];     // of a page
+    int n_tensors, num_blocks;
+    const int* dev_pairs;                 // {from, to} by pair, and their number behind dev_pairs_n; null: the host's below
+    const int* dev_pairs_n;
+    int n_pairs;
+    int pairs[2 * POOL_MAX_PAIRS];
+    int* table;                           // with `to`: entries from dev_pairs_n[1] on are renamed
+    size_t table_entries;
+    const int* to;
+};
+static_assert(sizeof(PageCopyArgs) <= 4096, "kernel arguments");
+hipError_t launch_fork(const PoolArgs& a, const void* who, bool free_rows, hipStream_t stream);
+hipError_t launch_reserve(const PoolArgs& a, const int* n_new, int* positions, int* ws, hipStream_t stream);
+hipError_t launch_compact(const PoolArgs& a, int* used, int* ws, hipStream_t stream);
+hipError_t launch_copy_pages(const PageCopyArgs& a, int most_pairs, hipStream_t stream);
+
 // ---- caller-side steps: input builder and fused key rotation + append ----
 constexpr int MAX_POS_ENTRIES = 768;    // (fragment, worker) pairs per build_inputs launch
 constexpr int MAX_APPEND_WORKERS = 64;  // workers per rope_append launch

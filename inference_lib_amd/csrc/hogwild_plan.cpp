@@ -729,5 +729,60 @@ int paged_plan(const hw_paged_problem* p, int num_cus, hw_paged_plan* plan) {
     return HW_OK;
 }
 
+int paged_q4_validate(const hw_paged_problem* p) {
+    if (p == nullptr) return HW_ERR_NULL;
+    if (p->dtype == HW_F32) return HW_ERR_UNSUPPORTED;                  // the weights of the values are rounded to 16 bits
+    if (p->block_size % 8 != 0) return HW_ERR_SHAPE;                     // eight tokens lie together
+    return paged_validate(p);
+}
+
+// Workgroups of four waves with 16 query rows (32 from 17 rows a sequence on), each wave a stripe of the sequence's 32-token tiles.
+int paged_q4_plan(const hw_paged_problem* p, int num_cus, hw_paged_plan* plan) {
+    if (plan == nullptr) return HW_ERR_NULL;
+    if (num_cus < 1) return HW_ERR_SHAPE;
+    std::memset(plan, 0, sizeof(*plan));
+    const bool varlen = p->cu_seqlens_q != nullptr;
+    if (p->W < 1 || p->Hq < 1 || p->Hkv < 1 || p->Ev < 1 || p->Hq % p->Hkv != 0) return HW_ERR_SHAPE;
+    if (varlen ? p->total_q < 0 : (p->S < 1 || p->S >= (1 << 12))) return HW_ERR_SHAPE;
+    if (p->block_size < 8 || p->block_size >= (1 << 12) || p->block_size % 8 != 0 || p->max_blocks < 1) return HW_ERR_SHAPE;
+    if ((long long)p->block_size * p->max_blocks > (1ll << 20)) return HW_ERR_SHAPE;
+    const int gq = p->Hq / p->Hkv;
+    const long long tokens = varlen ? p->total_q : (long long)p->W * p->S;
+    if (gq >= (1 << 12) || tokens * gq >= (1 << 20) || p->W >= (1 << 20)) return HW_ERR_SHAPE;
+    plan->rows = (int)(tokens * gq);
+    const long long rows_per_worker = varlen ? (tokens * gq + p->W - 1) / p->W : (long long)p->S * gq;
+    plan->row_blocks = rows_per_worker <= 16 ? 1 : 2;
+    if (p->row_blocks == 1 || p->row_blocks == 2) plan->row_blocks = p->row_blocks;
+    if (p->E > 128) plan->row_blocks = 1;       // (two blocks of 256-wide rows do not fit the registers)
+    const int rpw = 16 * plan->row_blocks;
+    long long items = varlen ? p->W + tokens * gq / rpw : (long long)p->W * (((long long)p->S * gq + rpw - 1) / rpw);
+    if (items < 1) items = 1;
+    plan->row_groups = (int)items;
+    long long splits = p->splits;
+    if (splits <= 0) {
+        const long long tiles = ((long long)p->block_size * p->max_blocks + hw::TILE - 1) / hw::TILE;
+        const long long pairs = (long long)p->Hkv * items, room = 2ll * num_cus;
+        splits = pairs < room ? room / pairs : 1;
+        splits = std::min(splits, (tiles + hw::NWAVES - 1) / hw::NWAVES);
+    }
+    if (splits > 64) splits = 64;
+    if (splits < 1) splits = 1;
+    plan->splits = (int)splits;
+    const long long wgs = (long long)p->Hkv * items * splits;
+    if (wgs >= (1 << 20)) return HW_ERR_SHAPE;
+    plan->workgroups = (int)wgs;
+    const unsigned long long octets = (unsigned long long)(p->block_size / 8) * p->max_blocks + 8;
+    if (!magic_exact((unsigned long long)splits, (unsigned long long)wgs) ||
+        !magic_exact((unsigned long long)items, (unsigned long long)p->Hkv * items) ||
+        !magic_exact((unsigned long long)(varlen ? 1 : items / p->W), (unsigned long long)items) ||
+        !magic_exact((unsigned long long)gq, (unsigned long long)tokens * gq + 32) ||
+        !magic_exact((unsigned long long)(varlen ? 1 : p->S), (unsigned long long)tokens + 32) ||
+        !magic_exact((unsigned long long)(p->block_size / 8), octets))
+        return HW_ERR_SHAPE;
+    plan->workspace_bytes = (size_t)p->Hkv * plan->splits * (size_t)(plan->rows > 0 ? plan->rows : 1) * ((size_t)p->Ev + 2) * sizeof(float);
+    plan->workspace_bytes = (plan->workspace_bytes + 255) & ~(size_t)255;
+    return HW_OK;
+}
+
 }  // namespace host
 }  // namespace hw
