@@ -328,7 +328,7 @@ int hw_read_blocks_q4(const hw_copy_blocks* c, void* stream);
 
 /* hw_paged_sdpa and hw_varlen_paged_sdpa over such caches: the same problem, limits and results (also lse), queries and output in
    16 bits.  The logits are products of the queries with the codes themselves, in fp32; values are rounded to fp16 (by less than 2^-11
-   of themselves), weights too.  row_blocks: 0, 1 or 2 (1 at E == 256). */
+   of themselves), bf16 results' weights too.  row_blocks: 0, 1 or 2 (1 at E == 256). */
 int hw_paged_q4_validate(const hw_paged_problem* p);
 int hw_paged_q4_plan_debug(const hw_paged_problem* p, int num_cus, hw_paged_plan* plan);   /* host only */
 int hw_paged_q4_workspace_bytes(const hw_paged_problem* p, size_t* bytes);

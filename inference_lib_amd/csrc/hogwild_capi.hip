@@ -295,7 +295,7 @@ int paged_run(const hw_paged_problem* p, void* stream_, int stages) {
 }
 
 // The paged operators over caches in 4 bits.
-int paged_q4_run(const hw_paged_problem* p, void* stream_, int stages) {
+int paged_q4_run(const hw_paged_problem* p, void* stream_) {
     int st = paged_q4_validate(p);
     if (st != HW_OK) return st;
     int cus = 0;
@@ -311,14 +311,14 @@ int paged_q4_run(const hw_paged_problem* p, void* stream_, int stages) {
     paged_header(p, plan, ph);
     ph.magic_bs = magic_of(p->block_size / 8);
     ph.part_o = reinterpret_cast<float*>(p->workspace);
-    ph.part_ml = ph.part_o + (size_t)p->Hkv * plan.splits * plan.rows * p->Ev;
-    ph.flags = plan.workgroups % 8 == 0 ? hw::PH_XCD_REMAP : 0;
-    hipError_t e = hipSuccess;
-    if (stages & HW_STAGE_ATTENTION) {
-        e = hw::launch_paged_q4(ph, p->dtype, p->E, plan.row_blocks, stream);
-        if (e != hipSuccess) return (int)e;
-    }
-    if (!(stages & HW_STAGE_MERGE)) return (int)e;
+    const size_t prows = (size_t)plan.splits * plan.rows;
+    ph.part_ml = ph.part_o + (size_t)p->Hkv * prows * p->Ev;
+    const bool shared = plan.splits > 1 && paged_shared(p, plan) && paged_q4_shares_save(p, plan, cus) >= 0 && p->workspace_bytes >= paged_call_bytes(p, plan);
+    const bool direct = plan.splits == 1;
+    ph.flags = (plan.workgroups % 8 == 0 ? hw::PH_XCD_REMAP : 0) | (shared ? hw::PH_SHARED | paged_q4_shares_save(p, plan, cus) << hw::PH_SAVED_SHIFT : 0) |
+               (direct ? hw::PH_DIRECT : 0);
+    const hipError_t e = hw::launch_paged_q4(ph, p->out, p->lse, p->dtype, p->E, plan.row_blocks, stream);
+    if (e != hipSuccess || direct) return (int)e;
     hw::MergeArgs ma;
     std::memset(&ma, 0, sizeof(ma));
     ma.part_o = ph.part_o;
@@ -328,7 +328,13 @@ int paged_q4_run(const hw_paged_problem* p, void* stream_, int stages) {
     ma.W = ph.LW; ma.Hq = p->Hq; ma.Hkv = p->Hkv; ma.S = ph.LS; ma.R = ma.rows = plan.rows;
     ma.wgs_per_head = plan.splits;
     ma.xcd_local = (p->cu_seqlens_q == nullptr && plan.workgroups % 8 == 0 && p->Hkv % 8 == 0) ? 1 : 0;
-    ma.magic_rows = magic_of(1);
+    if (shared) {
+        ma.row_tab = reinterpret_cast<int*>(ph.part_ml + (size_t)p->Hkv * prows * 2);
+        ma.pslots = plan.row_groups * plan.splits;
+        ma.slot_rows = plan.rows / p->W;
+        ma.guess = plan.splits;
+    }
+    ma.magic_rows = magic_of(shared ? ma.slot_rows : 1);
     return (int)hw::launch_merge(ma, p->dtype, p->Ev, stream);
 }
 
@@ -827,18 +833,18 @@ int hw_paged_q4_workspace_bytes(const hw_paged_problem* p, size_t* bytes) {
     hw_paged_plan plan;
     st = paged_q4_plan(p, cus, &plan);
     if (st != HW_OK) return st;
-    *bytes = plan.workspace_bytes;
+    *bytes = paged_call_bytes(p, plan);
     return HW_OK;
 }
 
 int hw_paged_sdpa_q4(const hw_paged_problem* p, void* stream) {
     if (p != nullptr && p->cu_seqlens_q != nullptr) return HW_ERR_SHAPE;
-    return paged_q4_run(p, stream, HW_STAGE_ATTENTION | HW_STAGE_MERGE);
+    return paged_q4_run(p, stream);
 }
 
 int hw_varlen_paged_sdpa_q4(const hw_paged_problem* p, void* stream) {
     if (p != nullptr && p->cu_seqlens_q == nullptr) return HW_ERR_NULL;
-    return paged_q4_run(p, stream, HW_STAGE_ATTENTION | HW_STAGE_MERGE);
+    return paged_q4_run(p, stream);
 }
 
 int hw_pool_workspace_bytes(const hw_pool* p, size_t* bytes) {

@@ -835,6 +835,74 @@ __device__ __forceinline__ PagedItem paged_item(const PagedDevHeader& ph, int it
 }
 
 
+// The workgroups of a kv head shared out by the lengths of the sequences (fixed-length operator, one row group per sequence; the lengths
+// are device data, so every wave works the shares out for itself).  nsplit workgroups for each sequence whatever its length left the
+// launch waiting for those of the longest: append and attention of five sequences of 296 to 10 543 tokens (40/8 heads, D = 128, bf16)
+// 31.7 -> 22.3 us, eight of 210 to 9000 at 32/8 37 -> 24, four of 300 to 11 000 at 16/8 and D = 256 41 -> 28.6, five of 844 to 5868 23.8 -> 22.2.
+// The shares are the smallest bound on the tiles of a workgroup (in steps of the four waves) at which the sequences' workgroups
+// are no more than there are, found by trying one bound in every lane.  Working that out and requesting the queries again takes 0.9 us,
+// a step of the four waves 1.1 to 1.2 (fit over 63 decode steps of 2 to 12 sequences, all head layouts): nsplit each wherever the longest
+// sequence needs two steps at most, or no more than it would need with even shares (more workgroups than CUs: paged_shares_save).  The
+// lengths are read ahead of the queries, which are requested for equal shares, as are the partial sums in the merge.
+// A sequence with fewer workgroups has fewer tiles that are a wave's first, whose largest weight the storage type holds exactly: 1.04 to
+// 1.09 times the error against float64 (seven ragged steps x 6 seeds, bf16 and fp16).  The reference of the exponentials therefore follows
+// the tiles of such a sequence (compute_tile's FOLLOW): 0.96 to 1.00 times the error of equal shares.
+struct PagedShare {
+    int w, split, ns, slot0;      // sequence, which of its ns workgroups, the first one's slot
+    bool found;                   // false: a slot that is left over
+};
+// (loc0, len0: the first location of sequence min(lane, W - 1) and the first fragment's length, requested ahead of what the workgroup
+// needs besides, so that this is worked out while the rest is on its way)
+__device__ __forceinline__ PagedShare paged_share(const PagedDevHeader& ph, int item, int split, int lane, int loc0, int len0) {
+    const int cap = ph.block_size * ph.max_blocks, T = ph.LW * ph.LS, w = min(lane, ph.W - 1);
+    // lane = sequence: the tiles that its workgroups go through
+    auto tiles_to = [&](int most, int len) { return (max(min(min(len, cap), most < cap ? most + 1 : cap), 0) + TILE - 1) / TILE; };
+    int most = loc0;
+    for (int s = 1; s < ph.LS; ++s) most = max(most, ph.loc[w * ph.LS + s]);
+    int tiles = tiles_to(most, len0);
+    for (int f = 1; f < ph.F; ++f) {
+        most = -1;
+        for (int s = 0; s < ph.LS; ++s) most = max(most, ph.loc[f * T + w * ph.LS + s]);
+        tiles += tiles_to(most, ph.frag_len[f]);
+    }
+    if (lane >= ph.W) tiles = 0;
+    // (nothing here depends on the order of the sequences: a sequence's share, and so its result, is the same wherever it is listed)
+    const PagedShare equal = {item, split, ph.nsplit, item * ph.nsplit, true};
+    const int slots = ph.W * ph.nsplit, slot = item * ph.nsplit + split;
+    // whether the longest sequence's workgroups would have more than `most_tiles` tiles each with equal shares
+    auto more_than = [&](int most_tiles) { return __ballot(tiles > ph.nsplit * most_tiles) != 0; };
+    // (on their own: sequences of one length and short steps leave here, 0.1 us sooner than behind the sum)
+    if (__ballot(lane < ph.W && tiles != __builtin_amdgcn_readlane(tiles, 0)) == 0 || !more_than(2 * NWAVES)) return equal;
+    const int saved = NWAVES * (ph.flags >> PH_SAVED_SHIFT);   // (in tiles, like the bounds)
+    const int all = __builtin_amdgcn_readlane(wave_scan_inclusive(tiles), 63);
+    const int least = max(1, (int)((float)all * __builtin_amdgcn_rcpf((float)(NWAVES * slots))));          // steps with even shares, less what is left over
+    int even = NWAVES * (least + (least * NWAVES * slots < all ? 1 : 0));
+    // (with many sequences the search is long; what half a workgroup of each leaves over is estimated instead)
+    if (saved > 0) even = (int)((float)all * __builtin_amdgcn_rcpf((float)(slots - (ph.W >> 1)))) + saved;
+    if (!more_than(even)) return equal;
+    // lane = a bound on the tiles of a workgroup, multiples of the four waves: does every sequence get its workgroups?
+    const float mine = (float)tiles;
+    const int bound = NWAVES * (least + lane * (1 + (least >> 5)));
+    const float per = __builtin_amdgcn_rcpf((float)bound);
+    auto groups = [&](float t, float per_group) { return max(1, (int)__builtin_ceilf(t * per_group - 0.01f)); };
+    int need = 0;
+    for (int sq = 0; sq < ph.W; ++sq) need += groups(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), sq)), per);
+    const unsigned long long fits = __ballot(need <= slots);
+    const int fit = fits != 0 ? __builtin_ctzll(fits) : 0;
+    if (fits == 0 || !more_than(__builtin_amdgcn_readlane(bound, fit))) return equal;
+    const float best = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(per), fit));
+    const int n = lane < ph.W ? groups(mine, best) : 0;
+    const int slot0 = wave_scan_inclusive(n) - n;
+    const unsigned long long owner = __ballot(slot >= slot0 && slot < slot0 + n);
+    PagedShare r;
+    r.found = owner != 0;
+    r.w = r.found ? __builtin_ctzll(owner) : 0;
+    r.slot0 = __builtin_amdgcn_readlane(slot0, r.w);
+    r.split = slot - r.slot0;
+    r.ns = __builtin_amdgcn_readlane(n, r.w);
+    return r;
+}
+
 // row r (0..R) of a kv head -> (worker*S + token, q head, flat q row index)
 struct RowMap {
     int ws;

@@ -131,6 +131,7 @@ constexpr int PH_GROUPS_SHIFT = 8;   // from this bit on, planned: the most row 
 // merge's row table right behind part_ml.
 constexpr int PH_SHARED = 8;
 constexpr int PH_SAVED_SHIFT = 8;    // from this bit on, shared: steps that other than equal shares have to save (paged_shares_save); > 0: more workgroups than CUs
+constexpr int PH_DIRECT = 32;      // one workgroup sees all of a row's tiles: it writes the results (read by launch_paged_q4 only)
 constexpr int PH_SMALL = 16;       // the K cache is less than 4 GB: one buffer descriptor reaches all of it (read by launch_paged_attention only)
 
 struct CopyBlocksArgs {
@@ -153,7 +154,8 @@ hipError_t launch_append_q4(const CopyBlocksArgs& ca, int dtype, hipStream_t str
 // key_states / value_states are written: contiguous [B, Hkv, S_new, E], positions seq_lengths[b] + t
 hipError_t launch_read_q4(const CopyBlocksArgs& ca, int dtype, hipStream_t stream);
 // kcache / vcache hold octets, magic_bs divides by block_size / 8
-hipError_t launch_paged_q4(const PagedHeader& ph, int dtype, int E, int rb, hipStream_t stream);
+// (out, lse (or NULL): written with PH_DIRECT)
+hipError_t launch_paged_q4(const PagedHeader& ph, void* out, float* lse, int dtype, int E, int rb, hipStream_t stream);
 
 // ---- the pages of a pool (hogwild_pages.hip) ----
 constexpr int POOL_MAX_ROWS = 4096;     // sequences of a pool: their wants are summed up by one workgroup

@@ -736,6 +736,14 @@ int paged_q4_validate(const hw_paged_problem* p) {
     return paged_validate(p);
 }
 
+// Workgroups of the 4-bit kernels that a CU holds at once.
+static int q4_resident(const hw_paged_problem* p) { return p->Ev == 256 ? 1 : 2; }
+
+// As paged_shares_save: launches of up to as many workgroups as the chip holds run at once.
+int paged_q4_shares_save(const hw_paged_problem* p, const hw_paged_plan& plan, int num_cus) {
+    return p->Ev == 256 && plan.workgroups <= num_cus ? 0 : -1;
+}
+
 // Workgroups of four waves with 16 query rows (32 from 17 rows a sequence on), each wave a stripe of the sequence's 32-token tiles.
 int paged_q4_plan(const hw_paged_problem* p, int num_cus, hw_paged_plan* plan) {
     if (plan == nullptr) return HW_ERR_NULL;
@@ -753,7 +761,7 @@ int paged_q4_plan(const hw_paged_problem* p, int num_cus, hw_paged_plan* plan) {
     const long long rows_per_worker = varlen ? (tokens * gq + p->W - 1) / p->W : (long long)p->S * gq;
     plan->row_blocks = rows_per_worker <= 16 ? 1 : 2;
     if (p->row_blocks == 1 || p->row_blocks == 2) plan->row_blocks = p->row_blocks;
-    if (p->E > 128) plan->row_blocks = 1;       // (two blocks of 256-wide rows do not fit the registers)
+    if (p->Ev > 128) plan->row_blocks = 1;      // (two blocks of 256-wide rows do not fit the registers)
     const int rpw = 16 * plan->row_blocks;
     long long items = varlen ? p->W + tokens * gq / rpw : (long long)p->W * (((long long)p->S * gq + rpw - 1) / rpw);
     if (items < 1) items = 1;
@@ -761,8 +769,9 @@ int paged_q4_plan(const hw_paged_problem* p, int num_cus, hw_paged_plan* plan) {
     long long splits = p->splits;
     if (splits <= 0) {
         const long long tiles = ((long long)p->block_size * p->max_blocks + hw::TILE - 1) / hw::TILE;
-        const long long pairs = (long long)p->Hkv * items, room = 2ll * num_cus;
-        splits = pairs < room ? room / pairs : 1;
+        const long long pairs = (long long)p->Hkv * items, room = (long long)q4_resident(p) * num_cus;
+        // as many as the chip holds at once; up to one and a half times that many are halved, which fills the last round
+        splits = 2 * pairs <= room ? room / pairs : 2 * pairs <= 3 * room ? 2 : 1;
         splits = std::min(splits, (tiles + hw::NWAVES - 1) / hw::NWAVES);
     }
     if (splits > 64) splits = 64;

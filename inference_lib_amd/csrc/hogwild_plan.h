@@ -87,6 +87,7 @@ int paged_shares_save(const hw_paged_problem* p, const hw_paged_plan& plan, int 
 // The same for caches in 4 bits.
 int paged_q4_validate(const hw_paged_problem* p);
 int paged_q4_plan(const hw_paged_problem* p, int num_cus, hw_paged_plan* plan);
+int paged_q4_shares_save(const hw_paged_problem* p, const hw_paged_plan& plan, int num_cus);
 // Whether the tiles of a paged launch are to stay in the L2 (hogwild_plan.cpp).
 bool paged_keep_in_l2(const hw_paged_problem* p, const hw_paged_plan& plan);
 

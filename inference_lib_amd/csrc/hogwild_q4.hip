@@ -45,7 +45,28 @@ __device__ __forceinline__ u32 h2_bits(f16x2 x) { return __builtin_bit_cast(u32,
 __device__ __forceinline__ f16x2 h2_of(u32 x) { return __builtin_bit_cast(f16x2, x); }
 __device__ __forceinline__ float h_lo(u32 x) { return (float)h2_of(x)[0]; }
 __device__ __forceinline__ float h_hi(u32 x) { return (float)h2_of(x)[1]; }
-__device__ __forceinline__ u32x4 load16(unsigned long long p) { return __builtin_nontemporal_load(reinterpret_cast<const HW_GLOBAL u32x4*>(p)); }
+
+// What the decoding of a tile keeps in registers throughout (as literals the masks cost an instruction more a pair: an instruction
+// with three operands takes none), and a block of zeros for products to begin with.
+struct Q4Consts {
+    u32 lo, hi, magic, one;
+    f32x4 zero;
+    __device__ __forceinline__ explicit Q4Consts(int lane) : lo(Q4_LO), hi(Q4_HI), magic(Q4_MAGIC), one(lane < 16 ? 0x3c003c00u : 0u), zero{0.f, 0.f, 0.f, 0.f} {
+        asm volatile("" : "+v"(lo), "+v"(hi), "+v"(one), "+s"(magic));
+    }
+};
+
+// Four registers of element pairs (0,1) (2,3) (4,5) (6,7) from a word: exactly the codes.
+__device__ __forceinline__ u32x4 q4_codes(u32 w, const Q4Consts& k) {
+    const f16x2 m1024 = {(_Float16)-1024.f, (_Float16)-1024.f}, inv = {(_Float16)0.0625f, (_Float16)0.0625f}, m64 = {(_Float16)-64.f, (_Float16)-64.f};
+    const u32 w8 = w >> 8;
+    u32x4 r;
+    r[0] = h2_bits(h2_of((w & k.lo) | k.magic) + m1024);
+    r[1] = h2_bits(__builtin_elementwise_fma(h2_of((w & k.hi) | k.magic), inv, m64));
+    r[2] = h2_bits(h2_of((w8 & k.lo) | k.magic) + m1024);
+    r[3] = h2_bits(__builtin_elementwise_fma(h2_of((w8 & k.hi) | k.magic), inv, m64));
+    return r;
+}
 
 // ------------------------------------------------------------------------------------------------
 // append and read
@@ -235,64 +256,101 @@ __global__ __launch_bounds__(256) void read_q4_kernel(const CopyBlocksArgs a, in
 // ------------------------------------------------------------------------------------------------
 // attention
 // ------------------------------------------------------------------------------------------------
-// The bytes of one 32-token tile (four octets) that a lane holds: of the keys the rows of two tokens, one from each 16-token block of
+// What a lane holds of one 32-token tile (four octets) in flight.  Of the keys the rows of two tokens, one from each 16-token block of
 // the product K Q^T (block b, row m of it: token 8 (m / 4) + 4 b + m % 4, so that lane quarter q finds the logits of octet q in its
-// accumulators), the parameters of octet q's keys, and of the values octet q of D / 16 neighbouring channels and their parameters.
+// accumulators); of the values octet q of D / 16 neighbouring channels; and its share of the parameters: the sixteen lanes of quarter
+// q hold those of octet q between them (at D = 64 the keys' and the values' in one word a lane).  They go through the wave's own
+// piece of LDS when the tile is multiplied, where every lane reads those it needs: loaded by every lane for itself they took 24 registers
+// a tile instead of 2, and with them the second tile in flight.
 template <int D>
 struct Q4Tile {
     typedef Q4<D> G;
+    static constexpr int NP = D <= 128 ? 1 : 2;          // parameter words of a lane: keys, and values (D > 64)
     u32 k[2][G::WPQ];
-    u32x4 ks[G::NG], km[G::NG];      // scales and offsets of the octet's eight keys
     u32 v[G::NOC];
-    u32x4 vs, vm;
+    u32 kp[NP], vp[NP];
+};
+template <int D>
+struct Q4Params {                                        // a wave's parameters in LDS
+    static constexpr int OCTET = D == 64 ? 64 : Q4<D>::NG * 32;          // bytes between octets
+    static constexpr int VALUES = D == 64 ? 32 : 4 * Q4<D>::NG * 32;     // where those of the values begin
+    static constexpr int BYTES = 256 * Q4<D>::NG;
 };
 
 template <int W>
 __device__ __forceinline__ void load_words(u32 (&dst)[W], unsigned long long p) {
-    if constexpr (W == 2) {
-        const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const HW_GLOBAL u32x2*>(p));
+    if constexpr (W == 1) {
+        dst[0] = *reinterpret_cast<const HW_GLOBAL u32*>(p);
+    } else if constexpr (W == 2) {
+        const u32x2 x = *reinterpret_cast<const HW_GLOBAL u32x2*>(p);
         dst[0] = x.x;
         dst[1] = x.y;
     } else {
 #pragma unroll
         for (int j = 0; j < W / 4; ++j) {
-            const u32x4 x = load16(p + 16 * j);
+            const u32x4 x = *reinterpret_cast<const HW_GLOBAL u32x4*>(p + 16 * j);
 #pragma unroll
             for (int d = 0; d < 4; ++d) dst[4 * j + d] = x[d];
         }
     }
 }
 
-// Four registers of element pairs (0,1) (2,3) (4,5) (6,7) from a word, exactly the codes.
-__device__ __forceinline__ u32x4 q4_codes(u32 w) {
-    const f16x2 m1024 = {(_Float16)-1024.f, (_Float16)-1024.f}, inv = {(_Float16)0.0625f, (_Float16)0.0625f}, m64 = {(_Float16)-64.f, (_Float16)-64.f};
+// The element pairs of a word in 5 instructions instead of the 9 of q4_codes: 2^-24 times the codes, the second and the fourth pair 16
+// times that.  Bits 0..7 of a half are a subnormal number, which the matrix instructions take as it is.
+__device__ __forceinline__ u32x4 q4_tiny(u32 w, const Q4Consts& k) {
     const u32 w8 = w >> 8;
-    u32x4 r;
-    r[0] = h2_bits(h2_of((w & Q4_LO) | Q4_MAGIC) + m1024);
-    r[1] = h2_bits(__builtin_elementwise_fma(h2_of((w & Q4_HI) | Q4_MAGIC), inv, m64));
-    r[2] = h2_bits(h2_of((w8 & Q4_LO) | Q4_MAGIC) + m1024);
-    r[3] = h2_bits(__builtin_elementwise_fma(h2_of((w8 & Q4_HI) | Q4_MAGIC), inv, m64));
-    return r;
+    return u32x4{w & k.lo, w & k.hi, w8 & k.lo, w8 & k.hi};
 }
 
 // The queries of a lane's row as B operands, and what the logits need of them: the products run on the bare codes, which fp16 holds
 // exactly, against the queries times a power of two of their row's own (so bf16 queries lose nothing to fp16's range):
 //   scale * q . k = sum_g s_g (sum_{e in g} q_e c_e) + m_g (sum_{e in g} q_e)
-template <int D, int RB>
-struct Q4Queries {
-    u32x4 b[RB][D / 32];
-    float sum[RB][Q4<D>::NG];        // sum of the group's queries, times the row's power of two
-    float sc[RB];                    // scale * log2(e) over the power of two
+// Sums of a wave.  The logits come out of a tile relative to the reference of the exponentials, in the units of the products (seed =
+// minus the reference in them): the first of the additions that form a logit takes it along.
+template <int RB, int NOC>
+struct Q4State {
+    f32x4 o[RB][NOC];
+    float m[RB], l[RB];              // reference (base-2 units, NEG_BIG: none yet), this lane's part of the sum of the weights
+    u32 seed[RB];                    // two fp16 numbers, their sum is what it stands for
+    float above[RB], unit[RB];   // minus the reference, the logit beyond which it moves, and 1 in base-2 units, in those units
 };
 
-template <class DT, int D, int RB>
-__device__ __forceinline__ void q4_queries(Q4Queries<D, RB>& qq, int rb, unsigned long long row, int q, float sc) {
+// More than 128 channels and rows of 16 together (QLDS): the operands lie in LDS, made ready by one wave for each 16 rows and read by
+// the four for every tile, instead of in 32 registers of every wave, which then are too few for two waves on a SIMD.
+template <int D>
+struct Q4Block {                     // of 16 rows
+    u32x4 b[D / 32];                 // (against q4_tiny: the second and fourth pair over 16)
+    u32 sum;                         // lane quarter g: the sum of group g's queries in the units of the products, as two fp16 numbers
+    float sc;                        // scale * log2(e) over those units
+};
+template <int D, int RB, bool QLDS>
+struct Q4Queries {
+    u32x4 b[QLDS ? 1 : RB][QLDS ? 1 : D / 32];
+    u32x2 row[RB];                   // Q4Block's sum and sc (as two arrays the optimizer put them into memory)
+    __device__ __forceinline__ u32 sum(int rb) const { return row[rb].x; }
+    __device__ __forceinline__ float sc(int rb) const { return __uint_as_float(row[rb].y); }
+};
+
+// A number as the sum of two fp16 ones, 2^-22 of itself exact, the second times `up` (beyond what fp16 counts in: 2^-25 / up).
+__device__ __forceinline__ u32 q4_pair(float x, float up) {
+    const u32 hi = Elem<F16>::pack2(x, 0.f);
+    return hi | Elem<F16>::pack2(0.f, (x - h_lo(hi)) * up);
+}
+// The sum of a row's queries is small in the products' units (2^-11 or so where its largest counts for much): its second half is kept
+// this much larger and meets offsets that much smaller.
+constexpr float Q4_LOW = 256.f;
+// Logits stay within 49000 of the products' units; the reference may lie 2^7 below them, which for queries (or a scale) next to nothing
+// is more of those units than fp16 counts.  Such logits are alike, whatever is taken off them.
+__device__ __forceinline__ u32 q4_seed(float x) { return q4_pair(fminf(fmaxf(x, -6.0e4f), 6.0e4f), 1.f); }
+
+template <class DT, int D>
+__device__ __forceinline__ void q4_queries(Q4Block<D>& qq, const u32x4 (&raw)[D / 32], float sc, int q) {
     typedef Q4<D> G;
     float x[G::WPQ][8];
     float top = 0.f;
 #pragma unroll
     for (int r = 0; r < G::WPQ; ++r) {
-        Chunk<DT>::unpack(*reinterpret_cast<const HW_GLOBAL u32x4*>(row + (64 * (r >> 1) + 16 * q + 8 * (r & 1)) * 2), x[r]);
+        Chunk<DT>::unpack(raw[r], x[r]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) top = fmaxf(top, __builtin_fabsf(x[r][e]));
     }
@@ -300,90 +358,103 @@ __device__ __forceinline__ void q4_queries(Q4Queries<D, RB>& qq, int rb, unsigne
     // 2^f brings the largest of the row into [2^13, 2^14)
     const int f = min(max(14 - __builtin_amdgcn_frexp_expf(top), -90), 90);
     const float up = __builtin_ldexpf(1.f, f);
-#pragma unroll
-    for (int g = 0; g < G::NG; ++g) {
-        float t = 0.f;
-#pragma unroll
-        for (int r = 2 * g; r < 2 * g + 2; ++r)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x[r][e] *= up;
-                t += x[r][e];
-            }
-        qq.sum[rb][g] = quarter_sum(t);
-    }
+    const float up16 = up * 0.0625f;
 #pragma unroll
     for (int r = 0; r < G::WPQ; ++r)
 #pragma unroll
-        for (int d = 0; d < 4; ++d) qq.b[rb][r][d] = Elem<F16>::pack2(x[r][2 * d], x[r][2 * d + 1]);
-    qq.sc[rb] = sc * __builtin_ldexpf(1.f, -f);
+        for (int d = 0; d < 4; ++d) qq.b[r][d] = Elem<F16>::pack2(x[r][2 * d] * (d & 1 ? up16 : up), x[r][2 * d + 1] * (d & 1 ? up16 : up));
+    // their sums, as products with a key of ones: every row of the result holds them
+    const u32x4 ones = {0x3c003c00u, 0x4c004c00u, 0x3c003c00u, 0x4c004c00u};     // 1, and 16 for the pairs over 16
+    float sum = 0.f;
+#pragma unroll
+    for (int g = 0; g < G::NG; ++g) {
+        f32x4 t = Elem<F16>::mfma(ones, qq.b[2 * g], f32x4{0.f, 0.f, 0.f, 0.f});
+        t = Elem<F16>::mfma(ones, qq.b[2 * g + 1], t);
+        sum = q == g ? t[0] * 0x1p-24f : sum;
+    }
+    qq.sum = q4_pair(sum, Q4_LOW);
+    qq.sc = fmaxf(sc * __builtin_ldexpf(1.f, 24 - f), 1e-36f);      // (its inverse has to be finite; such logits are 0)
+}
+
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f32x4 mfma_f16_k16(u32x2 a, u32x2 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
 }
 
 constexpr float Q4_BELOW = 7.f, Q4_ABOVE = 15.f;   // weights are 2^7 where the reference is taken and stay below 2^15
 
-// One tile against the rows of the workgroup.  MASKED: some row does not see all of it, or some of its tokens nobody sees (their bytes
-// may be anything: the parameters of such values are cleared, their logits replaced).
-template <int D, int RB, bool MASKED>
-__device__ __forceinline__ void q4_compute(const Q4Tile<D>& t, const Q4Queries<D, RB>& qq, const int (&lim)[RB], int maxlim,
-                                           WaveState<RB, Q4<D>::NOC>& st, int t0, int q) {
+// (as one instruction each: fmaxf has every operand quieted first)
+__device__ __forceinline__ float max3_nn(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+__device__ __forceinline__ float max8(const float (&x)[8]) {
+    return max_nn(max3_nn(max3_nn(max3_nn(x[0], x[1], x[2]), x[3], x[4]), x[5], x[6]), x[7]);
+}
+
+// One tile against the rows of the workgroup.  `partial` (uniform): some row does not see all of it, or some of its tokens nobody sees
+// (their bytes may be anything: the parameters of such values are cleared, their logits replaced).  SPLIT (fp16 results): the weights as the sum of
+// two fp16 numbers, 2^-22 of themselves exact; with one the result is 1.5 times as far from the exact one as its own rounding makes it.
+template <int D, int RB, bool SPLIT, bool QLDS>
+__device__ __forceinline__ void q4_compute(bool partial, const Q4Tile<D>& t, char* par, const Q4Queries<D, RB, QLDS>& qq, const u32x4* q_lds, const int (&lim)[RB], int maxlim,
+                                           Q4State<RB, Q4<D>::NOC>& st, const Q4Consts& cs, int t0, int n, int q, int lane) {
     typedef Q4<D> G;
-    float p[RB][8];
+    typedef Q4Params<D> P;
+    // (the wave's own piece of LDS: its operations complete in order, so no barrier)
+    if constexpr (Q4Tile<D>::NP == 1) {
+        *reinterpret_cast<u32*>(par + lane * 4) = t.kp[0];
+        if constexpr (D > 64) *reinterpret_cast<u32*>(par + P::VALUES + lane * 4) = t.vp[0];
+    } else {
+        *reinterpret_cast<u32x2*>(par + lane * 8) = u32x2{t.kp[0], t.kp[1]};
+        *reinterpret_cast<u32x2*>(par + P::VALUES + lane * 8) = u32x2{t.vp[0], t.vp[1]};
+    }
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+    const char* kpar = par + q * P::OCTET;
+    f32x4 acc[G::NG][2][RB];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int g = 0; g < G::NG; ++g)
 #pragma unroll
-        for (int g = 0; g < G::NG; ++g) {
-            const u32x4 a0 = q4_codes(t.k[b][2 * g]), a1 = q4_codes(t.k[b][2 * g + 1]);
+        for (int b = 0; b < 2; ++b) {
+            const u32x4 a0 = q4_tiny(t.k[b][2 * g], cs), a1 = q4_tiny(t.k[b][2 * g + 1], cs);
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
-                f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-                acc = Elem<F16>::mfma(a0, qq.b[rb][2 * g], acc);
-                acc = Elem<F16>::mfma(a1, qq.b[rb][2 * g + 1], acc);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const u32 s2 = t.ks[g][2 * b + (r >> 1)], m2 = t.km[g][2 * b + (r >> 1)];
-                    const float s = r & 1 ? h_hi(s2) : h_lo(s2), m = r & 1 ? h_hi(m2) : h_lo(m2);
-                    float& x = p[rb][4 * b + r];
-                    x = g == 0 ? m * qq.sum[rb][0] : __builtin_fmaf(m, qq.sum[rb][g], x);
-                    x = __builtin_fmaf(s, acc[r], x);
-                }
+                const u32x4 b0 = QLDS ? q_lds[(rb * G::WPQ + 2 * g) * 64 + lane] : qq.b[QLDS ? 0 : rb][QLDS ? 0 : 2 * g];
+                const u32x4 b1 = QLDS ? q_lds[(rb * G::WPQ + 2 * g + 1) * 64 + lane] : qq.b[QLDS ? 0 : rb][QLDS ? 0 : 2 * g + 1];
+                acc[g][b][rb] = Elem<F16>::mfma(a0, b0, cs.zero);
+                acc[g][b][rb] = Elem<F16>::mfma(a1, b1, acc[g][b][rb]);
             }
         }
+    // the offsets' part: lane quarter g multiplies those of group g (others by zero) with both halves of the sum of its queries
+    const char* mpar = par + (n >> 2) * P::OCTET + (q < G::NG ? q : 0) * 32 + 16 + (n & 3) * 2;
+    f32x4 off[2][RB];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        const _Float16 m = *reinterpret_cast<const _Float16*>(mpar + 8 * b);
+        const u32 mo = h2_bits(f16x2{m, m} * f16x2{(_Float16)1.f, (_Float16)(1.f / Q4_LOW)});
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) off[b][rb] = mfma_f16_k16(u32x2{mo, cs.one}, u32x2{qq.sum(rb), st.seed[rb]}, cs.zero);
     }
-    u32x4 pw[RB];
+    float p[RB][8];
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-        float top = NEG_BIG;
+    for (int g = 0; g < G::NG; ++g) {
+        const u32x4 ks = *reinterpret_cast<const u32x4*>(kpar + 32 * g);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            p[rb][i] *= qq.sc[rb];
-            if constexpr (MASKED) p[rb][i] = t0 + 8 * q + i < lim[rb] ? p[rb][i] : NEG_BIG;
-            top = fmaxf(top, p[rb][i]);
-        }
-        // the reference moves only when a weight would leave the range that fp16 holds well
-        if (__ballot(top > st.m[rb] + Q4_ABOVE) != 0 || st.fresh) {
-            const float all = quarter_max(top);
-            const float ref = all > st.m[rb] + Q4_ABOVE ? all - Q4_BELOW : st.m[rb];
-            const float w = fast_exp2(st.m[rb] - ref);
-            st.m[rb] = ref;
-            st.l[rb] *= w;
+        for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
-            for (int c = 0; c < G::NOC; ++c) st.o[rb][c] *= w;
-        }
-        float l = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            float e = fast_exp2(p[rb][i] - st.m[rb]);
-            if constexpr (MASKED) e = t0 + 8 * q + i < lim[rb] ? e : 0.f;      // (a row that has seen nothing yet: reference and logits are NEG_BIG)
-            p[rb][i] = e;
-            l += e;
-        }
-        st.l[rb] += l;
-#pragma unroll
-        for (int d = 0; d < 4; ++d) pw[rb][d] = Elem<F16>::pack2(p[rb][2 * d], p[rb][2 * d + 1]);
+            for (int i = 0; i < 8; ++i) {
+                const float s = i & 1 ? h_hi(ks[i >> 1]) : h_lo(ks[i >> 1]);
+                p[rb][i] = __builtin_fmaf(s, acc[g][i >> 2][rb][i & 3], g == 0 ? off[i >> 2][rb][i & 3] : p[rb][i]);
+            }
     }
-    st.fresh = false;
-    u32x4 vs = t.vs, vm = t.vm;
-    if constexpr (MASKED) {
+    const char* vpar = par + P::VALUES + q * P::OCTET + ((n * G::NOC) >> 6) * 32;
+    u32x4 vs = *reinterpret_cast<const u32x4*>(vpar), vm = *reinterpret_cast<const u32x4*>(vpar + 16);
+    if (partial) {
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) p[rb][i] = t0 + 8 * q + i < lim[rb] ? p[rb][i] : -__builtin_inff();
         const int seen = maxlim - t0 - 8 * q;
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
@@ -392,21 +463,75 @@ __device__ __forceinline__ void q4_compute(const Q4Tile<D>& t, const Q4Queries<D
             vm[d] &= keep;
         }
     }
+    // the reference moves only when a weight would leave the range that fp16 holds well
+    float top[RB];
+    bool beyond = false;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        top[rb] = max8(p[rb]);
+        beyond |= top[rb] > st.above[rb];
+    }
+    if (__ballot(beyond) != 0) {
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            const float all = quarter_max(top[rb]);
+            const bool have = st.m[rb] > NEG_BIG, move = all > st.above[rb];      // (of one row alike in all of its lanes)
+            const float was = h_lo(st.seed[rb]) + h_hi(st.seed[rb]);
+            const u32 seed = move ? q4_seed(was - (all - Q4_BELOW * st.unit[rb])) : st.seed[rb];
+            const float is = h_lo(seed) + h_hi(seed), up = was - is;
+            const float w = have ? fast_exp2(-up * qq.sc(rb)) : 1.f;
+            st.m[rb] = move ? -is * qq.sc(rb) : st.m[rb];
+            st.seed[rb] = seed;
+            st.above[rb] = move || have ? Q4_ABOVE * st.unit[rb] : -3.0e38f;
+            st.l[rb] *= w;
+#pragma unroll
+            for (int c = 0; c < G::NOC; ++c) st.o[rb][c] *= w;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) p[rb][i] -= up;
+        }
+    }
+    u32x4 pw[RB], pl[SPLIT ? RB : 1];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[rb][i] = fast_exp2(p[rb][i] * qq.sc(rb));
+        st.l[rb] += ((p[rb][0] + p[rb][1]) + (p[rb][2] + p[rb][3])) + ((p[rb][4] + p[rb][5]) + (p[rb][6] + p[rb][7]));
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            pw[rb][d] = Elem<F16>::pack2(p[rb][2 * d], p[rb][2 * d + 1]);
+            if constexpr (SPLIT) pl[rb][d] = Elem<F16>::pack2(p[rb][2 * d] - h_lo(pw[rb][d]), p[rb][2 * d + 1] - h_hi(pw[rb][d]));
+        }
+    }
 #pragma unroll
     for (int c = 0; c < G::NOC; ++c) {
-        u32x4 a = q4_codes(t.v[c]);
+        if (c % 2 == 0) __builtin_amdgcn_sched_barrier(0);
+        u32x4 a = q4_codes(t.v[c], cs);
 #pragma unroll
         for (int d = 0; d < 4; ++d) a[d] = h2_bits(__builtin_elementwise_fma(h2_of(a[d]), h2_of(vs[d]), h2_of(vm[d])));
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) st.o[rb][c] = Elem<F16>::mfma(a, pw[rb], st.o[rb][c]);
+        for (int rb = 0; rb < RB; ++rb) {
+            st.o[rb][c] = Elem<F16>::mfma(a, pw[rb], st.o[rb][c]);
+            if constexpr (SPLIT) st.o[rb][c] = Elem<F16>::mfma(a, pl[rb], st.o[rb][c]);
+        }
     }
+}
+
+// Where the results go that need no merge.
+struct Q4Out {
+    HW_GLOBAL char* out;
+    HW_GLOBAL float* lse;
+};
+// Row r (query token * GQ + head in group) of a kv head, in rows of the result.
+__device__ __forceinline__ size_t q4_out_row(const PagedDevHeader& ph, int r, int hkv) {
+    const int GQ = ph.Hq / ph.Hkv, ws = fast_div(r, ph.magic_gq), w = fast_div(ws, ph.magic_ls);
+    return ((size_t)w * ph.Hq + hkv * GQ + (r - ws * GQ)) * ph.LS + (ws - w * ph.LS);
 }
 
 // Rows of the partial sums, and of what a workgroup of four waves hands over: as in store_partials, with the output channel of
 // accumulator c, row i being i * D / 16 + c.
-template <int D, int RB>
-__device__ __forceinline__ void q4_store(WaveState<RB, D / 16>& st, Exchange<RB * 16, D>& ex, int wv, int n, int q, int lane, HW_GLOBAL float* part_o,
-                                         HW_GLOBAL float* part_ml, size_t part, int nrows) {
+template <class DT, int D, int RB>
+__device__ __forceinline__ void q4_store(Q4State<RB, D / 16>& st, Exchange<RB * 16, D>& ex, int wv, int n, int q, int lane, const PagedDevHeader& ph,
+                                         size_t part, int nrows, const Q4Out& out, int r0, int hkv) {
     constexpr int NOC = D / 16, NSLOT = RB * NOC, SPW = NSLOT / NWAVES;
     static_assert(NSLOT % NWAVES == 0 && (NOC % SPW == 0), "a wave's share lies within one row block");
 #pragma unroll
@@ -440,27 +565,47 @@ __device__ __forceinline__ void q4_store(WaveState<RB, D / 16>& st, Exchange<RB 
 #pragma unroll
         for (int i = 0; i < 4; ++i) run[i][j] = acc[i];
     }
-    HW_GLOBAL float* dst = part_o + (part + row) * D;
+    if (ph.flags & PH_DIRECT) {              // (the sums are all there are)
+        const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
+        const size_t orow = q4_out_row(ph, r0 + row, hkv);
+        typedef typename Elem<DT>::store_t store_t;
+        HW_GLOBAL store_t* dst = reinterpret_cast<HW_GLOBAL store_t*>(out.out) + orow * D;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < SPW; ++j) dst[(4 * q + i) * NOC + c0 + j] = Elem<DT>::from_float(run[i][j] * inv);
+        if (out.lse != nullptr && q == 0 && c0 == 0) out.lse[orow] = lsum > 0.f ? (mm + __builtin_amdgcn_logf(lsum)) * 0.69314718055994530942f : -__builtin_inff();
+        return;
+    }
+    HW_GLOBAL float* dst = ph.part_o + (part + row) * D;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < SPW; ++j) dst[(4 * q + i) * NOC + c0 + j] = run[i][j];
-    if (q == 0 && c0 == 0) *reinterpret_cast<HW_GLOBAL f32x2*>(part_ml + (part + row) * 2) = f32x2{mm, lsum};
+    if (q == 0 && c0 == 0) *reinterpret_cast<HW_GLOBAL f32x2*>(ph.part_ml + (part + row) * 2) = f32x2{mm, lsum};
 }
 
 // A workgroup = one kv head x up to 16 RB query rows of one sequence x every nsplit-th stripe of its 32-token tiles (four waves, each
-// takes every (4 nsplit)-th tile).  Nothing goes through LDS but the waves' partial sums: a tile is loaded straight into the
-// operands' lanes, one tile ahead of the one being multiplied, its table entries one further.
-template <class DT, int D, int RB, int MINW>
-__global__ __launch_bounds__(NTHREADS, MINW) void paged_q4_kernel(const PagedHeader args) {
+// takes every (4 nsplit)-th tile).  A tile is loaded straight into the operands' lanes, AH tiles ahead of the one being multiplied; the
+// first ones are requested as soon as the rows' bounds are known, and the queries are made ready behind them.
+template <class DT, int D, int RB, int MINW, int AH>
+__global__ __launch_bounds__(NTHREADS, MINW) void paged_q4_kernel(const PagedHeader args, const Q4Out out) {
     typedef Q4<D> G;
     constexpr int ROWS = RB * 16;
+    constexpr bool SPLIT = std::is_same<DT, F16>::value;
+    constexpr bool QLDS = RB * D > 128;
+    constexpr int QB = QLDS ? 1 : RB;       // row blocks whose queries a wave makes ready
+    __shared__ __attribute__((aligned(16))) u32x4 q_lds[QLDS ? RB * G::WPQ * 64 : 1];
+    __shared__ u32 q_sums[QLDS ? RB : 1][64];
+    __shared__ u32 q_sc[QLDS ? RB : 1][16];
     __shared__ __attribute__((aligned(16))) Exchange<ROWS, D> ex;
+    __shared__ __attribute__((aligned(16))) char par_lds[NWAVES][Q4Params<D>::BYTES];
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, q = lane >> 4;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     PagedHeaderBits hb;
     paged_header_request(hb);
-    WaveState<RB, G::NOC> st;
+    const Q4Consts cs(lane);
+    Q4State<RB, G::NOC> st;
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
         st.m[rb] = NEG_BIG;
@@ -468,14 +613,16 @@ __global__ __launch_bounds__(NTHREADS, MINW) void paged_q4_kernel(const PagedHea
 #pragma unroll
         for (int c = 0; c < G::NOC; ++c) st.o[rb][c] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    st.fresh = true;
     const PagedDevHeader ph = paged_header_wait(hb);
 
     int bid = blockIdx.x;
     if (ph.flags & PH_XCD_REMAP) bid = (bid & 7) * (ph.nwg >> 3) + (bid >> 3);
     const int hi = fast_div(bid, ph.magic_nsplit);
     const int hkv = fast_div(hi, ph.magic_nitems);
-    const int item = hi - hkv * ph.nitems, split = bid - hi * ph.nsplit;
+    int item = hi - hkv * ph.nitems, split = bid - hi * ph.nsplit;
+    int ns = ph.nsplit;                     // workgroups that share the sequence's tiles
+    const int wg_slot = item * ns + split;
+    const bool shared = (ph.flags & PH_SHARED) != 0;
     const int GQ = ph.Hq / ph.Hkv, T = ph.LW * ph.LS;
     const int cap = ph.block_size * ph.max_blocks, per = ph.block_size >> 3;
     const size_t slot = (size_t)(hkv * ph.nsplit + split) * ph.R;
@@ -483,100 +630,189 @@ __global__ __launch_bounds__(NTHREADS, MINW) void paged_q4_kernel(const PagedHea
         // query tokens in front of the first sequence's and behind the last one's: nothing is seen
         const int from = min(max(ph.cu_q[ph.W], 0), T) * GQ, front = min(max(ph.cu_q[0], 0), T) * GQ;
         for (int r = tid; r < front + (ph.R - from); r += NTHREADS) {
-            const size_t row = slot + (r < front ? r : from + r - front);
+            const int at = r < front ? r : from + r - front;
+            if (ph.flags & PH_DIRECT) {
+                const size_t orow = q4_out_row(ph, at, hkv);
+                for (int e = 0; e < D; ++e) reinterpret_cast<HW_GLOBAL unsigned short*>(out.out)[orow * D + e] = 0;
+                if (out.lse != nullptr) out.lse[orow] = -__builtin_inff();
+                continue;
+            }
+            const size_t row = slot + at;
             for (int e = 0; e < D; ++e) ph.part_o[row * D + e] = 0.f;
             *reinterpret_cast<HW_GLOBAL f32x2*>(ph.part_ml + row * 2) = f32x2{NEG_BIG, 0.f};
         }
     }
-    const PagedItem it = paged_item<ROWS>(ph, item, lane, GQ);
-    if (!it.found) return;                  // the grid is sized for the worst case; uniform over the workgroup
-    const int r0 = it.qs * GQ + it.rg * ROWS, rend = it.qe * GQ;
-    if (r0 >= rend) return;
-    const int NW = ph.nsplit * NWAVES, gw = split * NWAVES + wv;
-    const HW_GLOBAL int* btw = ph.block_table + (size_t)it.w * ph.max_blocks;
+    const int last_octet = (cap >> 3) - 1;
     const unsigned long long kbase = reinterpret_cast<unsigned long long>(ph.kcache), vbase = reinterpret_cast<unsigned long long>(ph.vcache);
+    int seq = 0, r0 = 0, rend = 0;          // sequence; first row (token * GQ + head in group), end of the sequence's rows
+    int NW = 0, gw = 0;                     // waves that share the tiles of this (kv head, row group); this one
+    const HW_GLOBAL int* btw = nullptr;
+    auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+    auto take = [&](int w, int row_group, int qs, int qe) {
+        seq = uniform(w);
+        r0 = uniform(qs * GQ + row_group * ROWS);
+        rend = uniform(qe * GQ);
+        NW = ns * NWAVES;
+        gw = split * NWAVES + wv;
+        btw = ph.block_table + (size_t)seq * ph.max_blocks;
+    };
+    auto octet_of = [&](int t) { return min(t * 4 + q, last_octet); };
+    auto entry = [&](int t) { return btw[fast_div(octet_of(t), ph.magic_bs)]; };     // of the octet of this lane's quarter
+    // (its octet, in octets from the start of the caches; what the table says is clamped into them)
+    auto place = [&](int t, int e) {
+        const int o = octet_of(t);
+        return (min(max(e, 0), ph.num_blocks - 1) * ph.Hkv + hkv) * per + (o - fast_div(o, ph.magic_bs) * per);
+    };
+    // one batch of independent loads: the table entries of the first tiles, the rows' bounds and queries
+    int e[AH + 1], flen = 0, loc[RB];
+    u32x4 raw[QB][G::WPQ];
+    auto fetch = [&](int f) {
+#pragma unroll
+        for (int i = 0; i <= AH; ++i) e[i] = entry(gw + i * NW);
+        flen = ph.frag_len[ph.cu_q != nullptr ? f * ph.W + seq : f];
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) loc[rb] = ph.loc[(size_t)f * T + fast_div(min(r0 + rb * 16 + n, rend - 1), ph.magic_gq)];
+#pragma unroll
+        for (int i = 0; i < QB; ++i) {
+            const int rb = QLDS ? min(wv, RB - 1) : i;
+            const int rc = min(r0 + rb * 16 + n, rend - 1), ws = fast_div(rc, ph.magic_gq), gq = rc - ws * GQ;
+            const int w = fast_div(ws, ph.magic_ls), s = ws - w * ph.LS;
+            const HW_GLOBAL char* row = ph.q + ((((size_t)f * ph.LW + w) * ph.Hq + hkv * GQ + gq) * ph.LS + s) * (D * 2);
+#pragma unroll
+            for (int r = 0; r < G::WPQ; ++r) raw[i][r] = *reinterpret_cast<const HW_GLOBAL u32x4*>(row + (64 * (r >> 1) + 16 * q + 8 * (r & 1)) * 2);
+        }
+    };
+    {
+        const PagedItem it = paged_item<ROWS>(ph, item, lane, GQ);
+        if (!it.found) return;              // the grid is sized for the worst case; uniform over the workgroup
+        take(it.w, it.rg, it.qs, it.qe);
+    }
+    if (r0 >= rend) return;                 // uniform over the workgroup
+    int loc0 = 0, len0 = 0, first_slot = 0;
+    if (shared) {
+        loc0 = ph.loc[min(lane, ph.W - 1) * ph.LS];
+        len0 = ph.frag_len[0];
+    }
+    // (what is requested holds for equal sequences: only where the share turns out another is it requested again)
+    for (bool again = shared;; again = false) {
+        fetch(0);
+        if (!again) break;
+        const PagedShare sh = paged_share(ph, item, split, lane, loc0, len0);
+        if (!sh.found) return;              // uniform over the workgroup
+        first_slot = sh.slot0;
+        if (sh.w == item && sh.split == split && sh.ns == ns) break;
+        item = uniform(sh.w);
+        split = uniform(sh.split);
+        ns = uniform(sh.ns);
+        take(item, 0, item * ph.LS, item * ph.LS + ph.LS);
+    }
 
     for (int f = 0; f < ph.F; ++f) {
-        const int flen = ph.frag_len[ph.cu_q != nullptr ? f * ph.W + it.w : f];
-        Q4Queries<D, RB> qq;
+        if (f > 0) fetch(f);
         int lim[RB], maxlim = 0, minlim = 0x7fffffff;
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
-            const int r = r0 + rb * 16 + n, rc = min(r, rend - 1);
-            const int ws = fast_div(rc, ph.magic_gq), gq = rc - ws * GQ;
-            const int w = fast_div(ws, ph.magic_ls), s = ws - w * ph.LS;
-            const int loc = ph.loc[(size_t)f * T + ws];
-            const size_t qrow = (((size_t)f * ph.LW + w) * ph.Hq + hkv * GQ + gq) * ph.LS + s;
-            q4_queries<DT, D, RB>(qq, rb, reinterpret_cast<unsigned long long>(ph.q) + qrow * (D * 2), q, ph.sc);
-            const int seen = max(0, min(min(flen, cap), loc < cap ? loc + 1 : cap));
-            lim[rb] = seen;
-            maxlim = max(maxlim, seen);
-            minlim = min(minlim, seen);      // (rows that pad the block repeat the last one)
+            lim[rb] = max(0, min(min(flen, cap), loc[rb] < cap ? loc[rb] + 1 : cap));
+            maxlim = max(maxlim, lim[rb]);
+            minlim = min(minlim, lim[rb]);       // (rows that pad the block repeat the last one)
         }
         maxlim = __builtin_amdgcn_readfirstlane(row_max16(maxlim));
         minlim = __builtin_amdgcn_readfirstlane(row_min16(minlim));
         const int tiles = (maxlim + TILE - 1) / TILE;
-        if (gw >= tiles) continue;          // (no barrier before the end)
-        const int last = (maxlim - 1) >> 3;    // octets behind it are read as this one, and masked
+        if (!QLDS && gw >= tiles) continue;      // (no barrier before the end)
+        const int idle = __builtin_amdgcn_readfirstlane(place(gw, e[0]));   // a tile that does not exist: this octet again, four times
 
-        auto octet_of = [&](int t) { return min(t * 4 + q, last); };
-        auto entry = [&](int t) { return btw[fast_div(octet_of(t), ph.magic_bs)]; };
-        auto request = [&](Q4Tile<D>& tr, int t, int e) {
-            const int o = octet_of(t);
-            const int blk = min(max(e, 0), ph.num_blocks - 1);
-            const int rid = (blk * ph.Hkv + hkv) * per + (o - fast_div(o, ph.magic_bs) * per);
+        auto request = [&](Q4Tile<D>& tr, int t, int entry_t) {
+            int rid = place(t, entry_t);
+            rid = t < tiles ? rid : idle;
             const int krid = __shfl(rid, (n >> 2) << 4, 64);
             const unsigned long long krow = kbase + (unsigned long long)(unsigned)krid * G::OCT + (n & 3) * G::KROW + q * (G::WPQ * 4);
+            const unsigned long long oct = (unsigned long long)(unsigned)rid * G::OCT;
             load_words(tr.k[0], krow);
             load_words(tr.k[1], krow + 4 * G::KROW);
-            const unsigned long long kp = kbase + (unsigned long long)(unsigned)rid * G::OCT + G::PAR;
-#pragma unroll
-            for (int g = 0; g < G::NG; ++g) {
-                tr.ks[g] = load16(kp + 32 * g);
-                tr.km[g] = load16(kp + 32 * g + 16);
+            if constexpr (D == 64) {
+                load_words(tr.kp, (n < 8 ? kbase : vbase) + oct + G::PAR + (n & 7) * 4);
+            } else {
+                load_words(tr.kp, kbase + oct + G::PAR + n * (4 * Q4Tile<D>::NP));
+                load_words(tr.vp, vbase + oct + G::PAR + n * (4 * Q4Tile<D>::NP));
             }
-            const unsigned long long vp = vbase + (unsigned long long)(unsigned)rid * G::OCT;
-            load_words(tr.v, vp + n * (G::NOC * 4));
-            const unsigned long long vpp = vp + G::PAR + ((n * G::NOC) >> 6) * 32;
-            tr.vs = load16(vpp);
-            tr.vm = load16(vpp + 16);
+            load_words(tr.v, vbase + oct + n * (G::NOC * 4));
         };
-        auto compute = [&](const Q4Tile<D>& tr, int t) {
-            if ((t + 1) * TILE <= minlim) q4_compute<D, RB, false>(tr, qq, lim, maxlim, st, t * TILE, q);
-            else q4_compute<D, RB, true>(tr, qq, lim, maxlim, st, t * TILE, q);
-        };
-        Q4Tile<D> ta, tb;
-        int e0 = entry(gw), e1 = entry(gw + NW);
-        request(ta, gw, e0);
-        for (int t = gw; t < tiles; t += 2 * NW) {
-            e0 = entry(t + 2 * NW);
-            request(tb, t + NW, e1);
-            compute(ta, t);
-            if (t + NW >= tiles) break;
-            e1 = entry(t + 3 * NW);
-            request(ta, t + 2 * NW, e0);
-            compute(tb, t + NW);
+        Q4Tile<D> tr[AH + 1];
+#pragma unroll
+        for (int i = 0; i < AH; ++i) request(tr[i], gw + i * NW, e[i]);
+        Q4Queries<D, RB, QLDS> qq;
+        if constexpr (QLDS) {
+            lds_barrier();                       // the fragment before is done with them
+            if (wv < RB) {
+                Q4Block<D> blk;
+                q4_queries<DT, D>(blk, raw[0], ph.sc, q);
+#pragma unroll
+                for (int r = 0; r < G::WPQ; ++r) q_lds[(wv * G::WPQ + r) * 64 + lane] = blk.b[r];
+                q_sums[wv][lane] = blk.sum;
+                if (q == 0) q_sc[wv][n] = __builtin_bit_cast(u32, blk.sc);
+            }
+            lds_barrier();
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+                qq.row[rb] = u32x2{q_sums[rb][lane], q_sc[rb][n]};
+            }
+        } else {
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+                Q4Block<D> blk;
+                q4_queries<DT, D>(blk, raw[QLDS ? 0 : rb], ph.sc, q);
+#pragma unroll
+                for (int r = 0; r < G::WPQ; ++r) qq.b[QLDS ? 0 : rb][QLDS ? 0 : r] = blk.b[r];
+                qq.row[rb] = u32x2{blk.sum, __builtin_bit_cast(u32, blk.sc)};
+            }
+        }
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            // (a fragment's products have units of their own; the reference goes on)
+            st.unit[rb] = 1.f / qq.sc(rb);
+            st.seed[rb] = st.m[rb] == NEG_BIG ? 0u : q4_seed(-st.m[rb] * st.unit[rb]);
+            st.above[rb] = st.m[rb] == NEG_BIG ? -3.0e38f : Q4_ABOVE * st.unit[rb];
+        }
+        int next = e[AH];
+        for (int t = gw; t < tiles; t += (AH + 1) * NW) {
+#pragma unroll
+            for (int u = 0; u <= AH; ++u) {
+                const int tu = t + u * NW;
+                if (u > 0 && tu >= tiles) break;
+                const int ahead = next;
+                next = entry(tu + (AH + 1) * NW);
+                request(tr[(u + AH) % (AH + 1)], tu + AH * NW, ahead);
+                q4_compute<D, RB, SPLIT, QLDS>((tu + 1) * TILE > minlim, tr[u], par_lds[wv], qq, q_lds, lim, maxlim, st, cs, tu * TILE, n, q, lane);
+            }
         }
     }
-    q4_store<D, RB>(st, ex, wv, n, q, lane, ph.part_o, ph.part_ml, slot + r0, min(ROWS, rend - r0));
+    q4_store<DT, D, RB>(st, ex, wv, n, q, lane, ph, shared ? (size_t)(hkv * ph.nitems * ph.nsplit + wg_slot) * (ph.LS * GQ) : slot + r0,
+                        min(ROWS, rend - r0), out, r0, hkv);
+    // where the merge finds the rows' partial sums
+    if (shared && split == 0 && tid < rend - r0) {
+        HW_GLOBAL int* row_tab = reinterpret_cast<HW_GLOBAL int*>(ph.part_ml + (size_t)ph.Hkv * ph.nsplit * ph.R * 2) + ((size_t)hkv * ph.R + r0) * 2;
+        row_tab[2 * tid] = first_slot | (ns << 16);
+        row_tab[2 * tid + 1] = tid;
+    }
 }
 
 // ------------------------------------------------------------------------------------------------
 // launchers
 // ------------------------------------------------------------------------------------------------
 template <class DT>
-static hipError_t launch_q4_dt(const PagedHeader& ph, int E, int rb, hipStream_t stream) {
+static hipError_t launch_q4_dt(const PagedHeader& ph, const Q4Out& out, int E, int rb, hipStream_t stream) {
     const dim3 grid(ph.nwg), threads(NTHREADS);
     if (E == 64) {
-        if (rb == 1) hipLaunchKernelGGL((paged_q4_kernel<DT, 64, 1, 3>), grid, threads, 0, stream, ph);
-        else if (rb == 2) hipLaunchKernelGGL((paged_q4_kernel<DT, 64, 2, 2>), grid, threads, 0, stream, ph);
+        if (rb == 1) hipLaunchKernelGGL((paged_q4_kernel<DT, 64, 1, 3, 2>), grid, threads, 0, stream, ph, out);
+        else if (rb == 2) hipLaunchKernelGGL((paged_q4_kernel<DT, 64, 2, 2, 2>), grid, threads, 0, stream, ph, out);
         else return hipErrorInvalidValue;
     } else if (E == 128) {
-        if (rb == 1) hipLaunchKernelGGL((paged_q4_kernel<DT, 128, 1, 2>), grid, threads, 0, stream, ph);
-        else if (rb == 2) hipLaunchKernelGGL((paged_q4_kernel<DT, 128, 2, 1>), grid, threads, 0, stream, ph);
+        if (rb == 1) hipLaunchKernelGGL((paged_q4_kernel<DT, 128, 1, 2, 1>), grid, threads, 0, stream, ph, out);
+        else if (rb == 2) hipLaunchKernelGGL((paged_q4_kernel<DT, 128, 2, 2, 1>), grid, threads, 0, stream, ph, out);
         else return hipErrorInvalidValue;
     } else if (E == 256) {
-        if (rb == 1) hipLaunchKernelGGL((paged_q4_kernel<DT, 256, 1, 1>), grid, threads, 0, stream, ph);
+        if (rb == 1) hipLaunchKernelGGL((paged_q4_kernel<DT, 256, 1, 1, 1>), grid, threads, 0, stream, ph, out);
         else return hipErrorInvalidValue;
     } else {
         return hipErrorInvalidValue;
@@ -584,8 +820,9 @@ static hipError_t launch_q4_dt(const PagedHeader& ph, int E, int rb, hipStream_t
     return hipGetLastError();
 }
 
-hipError_t launch_paged_q4(const PagedHeader& ph, int dtype, int E, int rb, hipStream_t stream) {
-    return dtype == 1 ? launch_q4_dt<F16>(ph, E, rb, stream) : launch_q4_dt<BF16>(ph, E, rb, stream);
+hipError_t launch_paged_q4(const PagedHeader& ph, void* out, float* lse, int dtype, int E, int rb, hipStream_t stream) {
+    const Q4Out o = {(HW_GLOBAL char*)out, (HW_GLOBAL float*)lse};
+    return dtype == 1 ? launch_q4_dt<F16>(ph, o, E, rb, stream) : launch_q4_dt<BF16>(ph, o, E, rb, stream);
 }
 
 // The octets that S_new tokens from any position on may touch, and the grid that takes them.

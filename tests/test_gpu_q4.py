@@ -4,8 +4,8 @@ the values that the cache holds, in float64.
 What the attention may be off by, from its arithmetic: weights and values are rounded to fp16 on the way into the product (2^-11
 of each, half a step), the sum of the weights is not; the logits carry the rounding of fp32 sums of D products and of the additions of
 the groups (their terms come to scale * sum |q| (|offset| + 15 scale) at most, each rounding is 2^-24 of that, and there are fewer than
-D + 8 of them); the result is rounded to its type.  So |out - exact| <= (2 * 2^-11 + 2 * logit error) * sum p |v| + half a step of |out|,
-with 10 % for the products of those, and lse by the logit error."""
+D + 8 of them) and of the sum of the queries as two fp16 numbers (2^-22 of it and of the largest query, 8 * 2^-24 together); the result is
+rounded to its type.  So |out - exact| <= (2 * 2^-11 + 2 * logit error) * sum p |v| + half a step of |out|, with 10 % for the products of those, and lse by the logit error."""
 import numpy as np
 import pytest
 import torch
@@ -171,7 +171,7 @@ def exact(q, lims, k, v, params, scale):
     with np.errstate(divide="ignore"):
         lse = (np.log(total) + top)[..., 0]
     p = p / np.where(total > 0, total, 1)
-    err = np.where(seen[None], size, 0).max(-1, initial=0.0)[..., None] * (D + 8) * 2.0 ** -24 + 2.0 ** -22    # of a logit (and of the exponential)
+    err = np.where(seen[None], size, 0).max(-1, initial=0.0)[..., None] * (D + 16) * 2.0 ** -24 + 2.0 ** -22    # of a logit (and of the exponential)
     vs = np.tile(vv, (1, F, 1))
     out, mass = np.matmul(p, vs), np.matmul(p, np.abs(vs))
     return out, lse, 1.1 * (2 * 2.0 ** -11 + 2 * err) * mass + 2.0 ** -24, err[..., 0] + np.abs(np.where(np.isfinite(lse), lse, 0)) * 2.0 ** -22
@@ -357,6 +357,8 @@ PACKED = [
     dict(lens=[64, 33, 500], q=[30, 33, 1], Hq=8, Hkv=4, D=64, block=8, F=2),
     dict(lens=[130, 1], q=[17, 1], Hq=16, Hkv=8, D=256, block=32, F=1),
     dict(lens=[600], q=[300], Hq=10, Hkv=2, D=128, block=64, F=1),
+    dict(lens=[200, 333, 90, 64], q=[100, 7, 90, 33], Hq=16, Hkv=4, D=64, block=8, F=1),
+    dict(lens=[50, 700], q=[40, 45], Hq=8, Hkv=2, D=128, block=24, F=2),
 ]
 
 
@@ -397,6 +399,36 @@ def test_packed_queries(dtype, i):
         assert (np.abs(np64(lse[a:b]).T - want_lse) <= may_lse).all()
     if behind:
         assert (out[-behind:] == 0).all() and torch.isneginf(lse[-behind:]).all()
+
+
+@gpu
+@pytest.mark.parametrize("W,Hq,Hkv,D,row_blocks,splits", [(70, 8, 2, 64, 0, 0), (3, 10, 2, 128, 2, 3), (3, 10, 2, 128, 1, 1), (4, 8, 8, 64, 2, 1), (300, 16, 2, 128, 0, 0), (5, 6, 2, 256, 0, 1), (3, 8, 1, 256, 1, 2)])
+def test_packed_queries_however_they_are_dealt(W, Hq, Hkv, D, row_blocks, splits):
+    """More than 64 and more than 256 sequences, and rows and splits of a workgroup that the caller fixes (one split writes the results itself)."""
+    from inference_lib_amd import _lib
+    rng = np.random.default_rng(W + splits)
+    lens = [int(x) for x in rng.integers(1, 150, W)]
+    qt = [int(min(n, x)) for n, x in zip(lens, rng.integers(0, 40 if W < 100 else 12, W))]
+    qt[0] = min(lens[0], 33)
+    block = 16
+    table, P = pool(rng, lens, block)
+    kc, vc = random_cache(rng, P, Hkv, block, D, True, "bf16"), random_cache(rng, P, Hkv, block, D, False, "bf16")
+    T = sum(qt)
+    q = torch.tensor(rng.standard_normal((1, T, Hq, D))).to(torch.bfloat16)
+    cu = np.concatenate([[0], np.cumsum(qt)])
+    loc = np.concatenate([np.arange(n - m, n) for n, m in zip(lens, qt)])[None]
+    out, lse = torch.full((T, Hq, D), float("nan"), dtype=torch.bfloat16, device="cuda"), torch.empty((T, Hq), device="cuda")
+    _lib.PagedProblem(q=q.cuda(), locations=ints(loc), fragment_lengths=ints([lens]), key_cache=torch.tensor(kc).cuda(), value_cache=torch.tensor(vc).cuda(),
+                      block_table=ints(table), scale=0.1, out=out, lse=lse, cu_seqlens_q=ints(cu), row_blocks=row_blocks, splits=splits, q4=True).run()
+    kd, vd, pd = Q.dense(kc, D, True), Q.dense(vc, D, False), params_of(kc, D)
+    for w in range(W):
+        a, b = cu[w], cu[w + 1]
+        if a < b:
+            k, v, p = (gather_sequence(x, table[w], lens[w]) for x in (kd, vd, pd))
+            qw = np64(q)[:, a:b].transpose(0, 2, 1, 3)
+            want, want_lse, may, may_lse = exact(qw, loc[:, a:b] + 1, k, v, p, 0.1)
+            close(out[a:b].transpose(0, 1), want, may, "bf16", f"{w}")
+            assert (np.abs(np64(lse[a:b]).T - want_lse) <= may_lse).all()
 
 
 @gpu
