@@ -31,6 +31,7 @@ constexpr float Q4_LIMIT = 65024.f;
 template <int D>
 struct Q4 {
     static constexpr int OCT = 9 * D / 2;        // bytes of an octet
+    static constexpr int UNIT = D == 64 ? 5 : D == 128 ? 6 : 7;   // an octet is 9 << UNIT bytes
     static constexpr int PAR = 4 * D;            // where its scales and offsets begin
     static constexpr int NG = D / 64;            // groups
     static constexpr int KROW = D / 2;           // bytes of a key's codes
@@ -295,6 +296,10 @@ __device__ __forceinline__ void load_words(u32 (&dst)[W], unsigned long long p) 
     }
 }
 
+// The first lane of every sixteen for all of them; and each lane's value one lane down.
+__device__ __forceinline__ unsigned q4_first(unsigned v) { return (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x150, 0xf, 0xf, true); }
+__device__ __forceinline__ unsigned q4_next(unsigned v) { return (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x12F, 0xf, 0xf, true); }
+
 // The element pairs of a word in 5 instructions instead of the 9 of q4_codes: 2^-24 times the codes, the second and the fourth pair 16
 // times that.  Bits 0..7 of a half are a subnormal number, which the matrix instructions take as it is.
 __device__ __forceinline__ u32x4 q4_tiny(u32 w, const Q4Consts& k) {
@@ -477,12 +482,13 @@ __device__ __forceinline__ void q4_compute(bool partial, const Q4Tile<D>& t, cha
             const float all = quarter_max(top[rb]);
             const bool have = st.m[rb] > NEG_BIG, move = all > st.above[rb];      // (of one row alike in all of its lanes)
             const float was = h_lo(st.seed[rb]) + h_hi(st.seed[rb]);
-            const u32 seed = move ? q4_seed(was - (all - Q4_BELOW * st.unit[rb])) : st.seed[rb];
+            const u32 moved = q4_seed(was - (all - Q4_BELOW * st.unit[rb])), seed = move ? moved : st.seed[rb];
             const float is = h_lo(seed) + h_hi(seed), up = was - is;
-            const float w = have ? fast_exp2(-up * qq.sc(rb)) : 1.f;
-            st.m[rb] = move ? -is * qq.sc(rb) : st.m[rb];
+            const float shrink = fast_exp2(-up * qq.sc(rb)), w = have ? shrink : 1.f;
+            const float m = -is * qq.sc(rb), above = Q4_ABOVE * st.unit[rb];
+            st.m[rb] = move ? m : st.m[rb];
             st.seed[rb] = seed;
-            st.above[rb] = move || have ? Q4_ABOVE * st.unit[rb] : -3.0e38f;
+            st.above[rb] = move | have ? above : -3.0e38f;
             st.l[rb] *= w;
 #pragma unroll
             for (int c = 0; c < G::NOC; ++c) st.o[rb][c] *= w;
@@ -586,9 +592,9 @@ __device__ __forceinline__ void q4_store(Q4State<RB, D / 16>& st, Exchange<RB * 
 }
 
 // A workgroup = one kv head x up to 16 RB query rows of one sequence x every nsplit-th stripe of its 32-token tiles (four waves, each
-// takes every (4 nsplit)-th tile).  A tile is loaded straight into the operands' lanes, AH tiles ahead of the one being multiplied; the
+// takes every (4 nsplit)-th tile).  A tile is loaded straight into the operands' lanes, one ahead of the one being multiplied; the
 // first ones are requested as soon as the rows' bounds are known, and the queries are made ready behind them.
-template <class DT, int D, int RB, int MINW, int AH>
+template <class DT, int D, int RB, int MINW>
 __global__ __launch_bounds__(NTHREADS, MINW) void paged_q4_kernel(const PagedHeader args, const Q4Out out) {
     typedef Q4<D> G;
     constexpr int ROWS = RB * 16;
@@ -643,7 +649,11 @@ __global__ __launch_bounds__(NTHREADS, MINW) void paged_q4_kernel(const PagedHea
         }
     }
     const int last_octet = (cap >> 3) - 1;
+    // what of an octet this lane loads
     const unsigned long long kbase = reinterpret_cast<unsigned long long>(ph.kcache), vbase = reinterpret_cast<unsigned long long>(ph.vcache);
+    const unsigned long long klane = kbase + (n & 3) * G::KROW + q * (G::WPQ * 4), vlane = vbase + n * (G::NOC * 4);
+    const unsigned long long kplane = D == 64 ? (n < 8 ? kbase : vbase) + G::PAR + (n & 7) * 4 : kbase + G::PAR + n * (4 * Q4Tile<D>::NP);
+    const unsigned long long vplane = vbase + G::PAR + n * (4 * Q4Tile<D>::NP);
     int seq = 0, r0 = 0, rend = 0;          // sequence; first row (token * GQ + head in group), end of the sequence's rows
     int NW = 0, gw = 0;                     // waves that share the tiles of this (kv head, row group); this one
     const HW_GLOBAL int* btw = nullptr;
@@ -656,19 +666,20 @@ __global__ __launch_bounds__(NTHREADS, MINW) void paged_q4_kernel(const PagedHea
         gw = split * NWAVES + wv;
         btw = ph.block_table + (size_t)seq * ph.max_blocks;
     };
+    // A tile's octets are worked out for sixteen tiles of the wave at once, lane n of quarter q for octet q of the n-th, and handed
+    // out from there (q4_first, q4_next): table entry, division and products by lane and tile were a sixth of a tile's instructions.
     auto octet_of = [&](int t) { return min(t * 4 + q, last_octet); };
-    auto entry = [&](int t) { return btw[fast_div(octet_of(t), ph.magic_bs)]; };     // of the octet of this lane's quarter
-    // (its octet, in octets from the start of the caches; what the table says is clamped into them)
+    auto entry = [&](int t) { return btw[fast_div(octet_of(t), ph.magic_bs)]; };
+    // where it starts in the caches, in D / 2 bytes (what the table says is clamped into them; there are less than 2^28 octets)
     auto place = [&](int t, int e) {
         const int o = octet_of(t);
-        return (min(max(e, 0), ph.num_blocks - 1) * ph.Hkv + hkv) * per + (o - fast_div(o, ph.magic_bs) * per);
+        return 9u * (unsigned)((min(max(e, 0), ph.num_blocks - 1) * ph.Hkv + hkv) * per + (o - fast_div(o, ph.magic_bs) * per));
     };
     // one batch of independent loads: the table entries of the first tiles, the rows' bounds and queries
-    int e[AH + 1], flen = 0, loc[RB];
+    int e = 0, flen = 0, loc[RB];
     u32x4 raw[QB][G::WPQ];
     auto fetch = [&](int f) {
-#pragma unroll
-        for (int i = 0; i <= AH; ++i) e[i] = entry(gw + i * NW);
+        e = entry(gw + n * NW);
         flen = ph.frag_len[ph.cu_q != nullptr ? f * ph.W + seq : f];
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) loc[rb] = ph.loc[(size_t)f * T + fast_div(min(r0 + rb * 16 + n, rend - 1), ph.magic_gq)];
@@ -720,27 +731,22 @@ __global__ __launch_bounds__(NTHREADS, MINW) void paged_q4_kernel(const PagedHea
         minlim = __builtin_amdgcn_readfirstlane(row_min16(minlim));
         const int tiles = (maxlim + TILE - 1) / TILE;
         if (!QLDS && gw >= tiles) continue;      // (no barrier before the end)
-        const int idle = __builtin_amdgcn_readfirstlane(place(gw, e[0]));   // a tile that does not exist: this octet again, four times
-
-        auto request = [&](Q4Tile<D>& tr, int t, int entry_t) {
-            int rid = place(t, entry_t);
-            rid = t < tiles ? rid : idle;
-            const int krid = __shfl(rid, (n >> 2) << 4, 64);
-            const unsigned long long krow = kbase + (unsigned long long)(unsigned)krid * G::OCT + (n & 3) * G::KROW + q * (G::WPQ * 4);
-            const unsigned long long oct = (unsigned long long)(unsigned)rid * G::OCT;
+        int ahead = entry(gw + (16 + n) * NW);       // of the sixteen tiles after these
+        unsigned at = place(gw + n * NW, e);
+        const unsigned idle = uniform(at);           // a tile that does not exist: this octet again, four times
+        at = gw + n * NW < tiles ? at : idle;
+        auto request = [&](Q4Tile<D>& tr) {
+            const unsigned rid = q4_first(at), krid = __shfl(rid, (n >> 2) << 4, 64);
+            at = q4_next(at);
+            const unsigned long long krow = klane + ((unsigned long long)krid << G::UNIT), oct = (unsigned long long)rid << G::UNIT;
             load_words(tr.k[0], krow);
             load_words(tr.k[1], krow + 4 * G::KROW);
-            if constexpr (D == 64) {
-                load_words(tr.kp, (n < 8 ? kbase : vbase) + oct + G::PAR + (n & 7) * 4);
-            } else {
-                load_words(tr.kp, kbase + oct + G::PAR + n * (4 * Q4Tile<D>::NP));
-                load_words(tr.vp, vbase + oct + G::PAR + n * (4 * Q4Tile<D>::NP));
-            }
-            load_words(tr.v, vbase + oct + n * (G::NOC * 4));
+            load_words(tr.kp, kplane + oct);
+            if constexpr (D > 64) load_words(tr.vp, vplane + oct);
+            load_words(tr.v, vlane + oct);
         };
-        Q4Tile<D> tr[AH + 1];
-#pragma unroll
-        for (int i = 0; i < AH; ++i) request(tr[i], gw + i * NW, e[i]);
+        Q4Tile<D> tr[2];
+        request(tr[0]);
         Q4Queries<D, RB, QLDS> qq;
         if constexpr (QLDS) {
             lds_barrier();                       // the fragment before is done with them
@@ -774,18 +780,22 @@ __global__ __launch_bounds__(NTHREADS, MINW) void paged_q4_kernel(const PagedHea
             st.seed[rb] = st.m[rb] == NEG_BIG ? 0u : q4_seed(-st.m[rb] * st.unit[rb]);
             st.above[rb] = st.m[rb] == NEG_BIG ? -3.0e38f : Q4_ABOVE * st.unit[rb];
         }
-        int next = e[AH];
-        for (int t = gw; t < tiles; t += (AH + 1) * NW) {
+        for (int t = gw, i = 1; gw < tiles;) {
 #pragma unroll
-            for (int u = 0; u <= AH; ++u) {
-                const int tu = t + u * NW;
-                if (u > 0 && tu >= tiles) break;
-                const int ahead = next;
-                next = entry(tu + (AH + 1) * NW);
-                request(tr[(u + AH) % (AH + 1)], tu + AH * NW, ahead);
-                q4_compute<D, RB, SPLIT, QLDS>((tu + 1) * TILE > minlim, tr[u], par_lds[wv], qq, q_lds, lim, maxlim, st, cs, tu * TILE, n, q, lane);
+            for (int u = 0; u < 2; ++u, ++i) {
+                if (u == 1 && (i & 15) == 0) {
+                    const int tn = t + (1 + n) * NW;
+                    at = place(tn, ahead);
+                    at = tn < tiles ? at : idle;
+                    ahead = entry(tn + 16 * NW);
+                }
+                request(tr[u ^ 1]);
+                q4_compute<D, RB, SPLIT, QLDS>((t + 1) * TILE > minlim, tr[u], par_lds[wv], qq, q_lds, lim, maxlim, st, cs, t * TILE, n, q, lane);
+                t += NW;
+                if (t >= tiles) goto tiles_done;
             }
         }
+    tiles_done:;
     }
     q4_store<DT, D, RB>(st, ex, wv, n, q, lane, ph, shared ? (size_t)(hkv * ph.nitems * ph.nsplit + wg_slot) * (ph.LS * GQ) : slot + r0,
                         min(ROWS, rend - r0), out, r0, hkv);
@@ -804,15 +814,15 @@ template <class DT>
 static hipError_t launch_q4_dt(const PagedHeader& ph, const Q4Out& out, int E, int rb, hipStream_t stream) {
     const dim3 grid(ph.nwg), threads(NTHREADS);
     if (E == 64) {
-        if (rb == 1) hipLaunchKernelGGL((paged_q4_kernel<DT, 64, 1, 3, 2>), grid, threads, 0, stream, ph, out);
-        else if (rb == 2) hipLaunchKernelGGL((paged_q4_kernel<DT, 64, 2, 2, 2>), grid, threads, 0, stream, ph, out);
+        if (rb == 1) hipLaunchKernelGGL((paged_q4_kernel<DT, 64, 1, 3>), grid, threads, 0, stream, ph, out);
+        else if (rb == 2) hipLaunchKernelGGL((paged_q4_kernel<DT, 64, 2, 2>), grid, threads, 0, stream, ph, out);
         else return hipErrorInvalidValue;
     } else if (E == 128) {
-        if (rb == 1) hipLaunchKernelGGL((paged_q4_kernel<DT, 128, 1, 2, 1>), grid, threads, 0, stream, ph, out);
-        else if (rb == 2) hipLaunchKernelGGL((paged_q4_kernel<DT, 128, 2, 2, 1>), grid, threads, 0, stream, ph, out);
+        if (rb == 1) hipLaunchKernelGGL((paged_q4_kernel<DT, 128, 1, 2>), grid, threads, 0, stream, ph, out);
+        else if (rb == 2) hipLaunchKernelGGL((paged_q4_kernel<DT, 128, 2, 2>), grid, threads, 0, stream, ph, out);
         else return hipErrorInvalidValue;
     } else if (E == 256) {
-        if (rb == 1) hipLaunchKernelGGL((paged_q4_kernel<DT, 256, 1, 1, 1>), grid, threads, 0, stream, ph, out);
+        if (rb == 1) hipLaunchKernelGGL((paged_q4_kernel<DT, 256, 1, 1>), grid, threads, 0, stream, ph, out);
         else return hipErrorInvalidValue;
     } else {
         return hipErrorInvalidValue;
