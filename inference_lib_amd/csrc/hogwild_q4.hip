@@ -72,73 +72,99 @@ __device__ __forceinline__ u32x4 q4_codes(u32 w, const Q4Consts& k) {
 // ------------------------------------------------------------------------------------------------
 // append and read
 // ------------------------------------------------------------------------------------------------
-// Reductions over the eight lanes of a token (lane % 8), by data-parallel-primitive moves.
+// Of values that are no NaN, as one instruction each (fmaxf has every operand quieted first).
+__device__ __forceinline__ float max3_nn(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+__device__ __forceinline__ float min3_nn(float a, float b, float c) {
+    float r;
+    asm("v_min3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+__device__ __forceinline__ float max8(const float (&x)[8]) {
+    return max_nn(max3_nn(max3_nn(max3_nn(x[0], x[1], x[2]), x[3], x[4]), x[5], x[6]), x[7]);
+}
+__device__ __forceinline__ float min8(const float (&x)[8]) {
+    return min3_nn(min3_nn(min3_nn(min3_nn(x[0], x[1], x[2]), x[3], x[4]), x[5], x[6]), x[7], x[7]);
+}
+// Over the eight lanes of a token (lane % 8), by data-parallel-primitive moves.
+template <int CTRL>
+__device__ __forceinline__ float lane_dpp(float v) { return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true)); }
 __device__ __forceinline__ float oct_min(float v) {
-    v = fminf(v, __int_as_float(row_dpp<0xB1>(__float_as_int(v))));
-    v = fminf(v, __int_as_float(row_dpp<0x4E>(__float_as_int(v))));
-    return fminf(v, __int_as_float(row_dpp<0x141>(__float_as_int(v))));
+    v = min3_nn(v, v, lane_dpp<0xB1>(v));
+    v = min3_nn(v, v, lane_dpp<0x4E>(v));
+    return min3_nn(v, v, lane_dpp<0x141>(v));
 }
 __device__ __forceinline__ float oct_max(float v) {
-    v = fmaxf(v, __int_as_float(row_dpp<0xB1>(__float_as_int(v))));
-    v = fmaxf(v, __int_as_float(row_dpp<0x4E>(__float_as_int(v))));
-    return fmaxf(v, __int_as_float(row_dpp<0x141>(__float_as_int(v))));
+    v = max_nn(v, lane_dpp<0xB1>(v));
+    v = max_nn(v, lane_dpp<0x4E>(v));
+    return max_nn(v, lane_dpp<0x141>(v));
 }
 
 // nibble position of element i (0..7) of a word
 __device__ __forceinline__ constexpr int q4_shift(int i) { return 4 * ((i >> 1) + ((i & 1) << 2)); }
 
-// Transposes the 8 x 8 nibbles that the lanes with one lane % 8 hold (lane / 8 = row i, one word each, its element j in nibble
-// position j of the plain order 0..7): afterwards lane row i holds element i of rows 0..7.  Three rounds of exchanges with the lane
-// 8, 16 and 32 away.
-__device__ __forceinline__ u32 q4_transpose(u32 w, int lane) {
+// Transposes the 8 x 8 nibbles of the lanes with one lane % 8 (lane row = lane / 8, one word each): afterwards lane row i holds element
+// i of rows 0..7, row r as element r.  Three rounds: bit k of the lane row changes places with that of the element, which stand in a
+// word's places in the order of q4_shift (bit 0 of the element is 16 bits, bit 1 is 4, bit 2 is 8).  A lane takes from its partner
+// the nibbles that `from` names, moved by the distance one way or (by a rotation, as the others are not taken) the other.
+struct Q4Transpose {
+    u32 from[3], turn[3];
+    __device__ __forceinline__ explicit Q4Transpose(int lane) {
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
-        const u32 mask = k == 0 ? 0x0F0F0F0Fu : k == 1 ? 0x00FF00FFu : 0x0000FFFFu;
-        const int sh = 4 << k;
-        const u32 other = (u32)__shfl_xor((int)w, 8 << k, 64);
-        w = (lane >> (3 + k)) & 1 ? ((other >> sh) & mask) | (w & ~mask) : (w & mask) | ((other & mask) << sh);
+        for (int k = 0; k < 3; ++k) {
+            const u32 low = k == 0 ? 0x0000FFFFu : k == 1 ? 0x0F0F0F0Fu : 0x00FF00FFu;
+            const int sh = k == 0 ? 16 : 4 * k;
+            const bool up = (lane >> (3 + k)) & 1;
+            from[k] = up ? low : ~low;
+            turn[k] = up ? sh : 32 - sh;
+        }
     }
-    return w;
-}
-// plain nibble order <-> the cache's (even elements below, odd ones above)
-__device__ __forceinline__ u32 q4_spread(u32 w) {       // element i at q4_shift(i)
-    u32 r = 0;
+    __device__ __forceinline__ u32 operator()(u32 w) const {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r |= ((w >> (4 * i)) & 15u) << q4_shift(i);
-    return r;
-}
-__device__ __forceinline__ u32 q4_gather(u32 w) {
-    u32 r = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r |= ((w >> q4_shift(i)) & 15u) << (4 * i);
-    return r;
+        for (int k = 0; k < 3; ++k) {
+            const u32 other = k == 0 ? (u32)row_dpp<0x128>((int)w) : (u32)__shfl_xor((int)w, 8 << k, 64);     // (half a row of sixteen on)
+            w = (__builtin_amdgcn_alignbit(other, other, turn[k]) & from[k]) | (w & ~from[k]);
+        }
+        return w;
+    }
+};
+
+// x / y to the nearest, as the division gives it, from r = 1 / y to the nearest: the remainder of the first quotient is exact and what it
+// adds is, but for less than 2^-22 of a last place, and quotients by numbers of 11 bits stay 2^-12 of a last place away from
+// the middle between two.  (Eight divisions a lane were a third of the append's instructions.)
+__device__ __forceinline__ float q4_divide(float x, float y, float r) {
+    const float q = x * r;
+    return __builtin_fmaf(__builtin_fmaf(-q, y, x), r, q);
 }
 
-// Where the octet `o` of sequence b lies, in octets from the cache's start; -1: nowhere (outside the table or the cache).
-__device__ __forceinline__ long long q4_octet(const CopyBlocksArgs& a, int b, int h, int o) {
+// Where the octet `o` of sequence b lies, in octets from the cache's start, and whether it lies anywhere (in the table and the cache; if
+// not: at the start).
+__device__ __forceinline__ long long q4_octet(const CopyBlocksArgs& a, int b, int h, int o, bool& there) {
     const int per = a.block_size >> 3;
-    const int bi = o / per;
-    if (bi >= a.max_blocks) return -1;
-    const int blk = a.block_table[(size_t)b * a.max_blocks + bi];
-    if (blk < 0 || blk >= a.num_blocks) return -1;
-    return ((long long)blk * a.Hkv + h) * per + (o - bi * per);
+    const int bi = max(o, 0) / per;
+    const int blk = a.block_table[(size_t)b * a.max_blocks + min(bi, a.max_blocks - 1)];
+    there = o >= 0 && bi < a.max_blocks && blk >= 0 && blk < a.num_blocks;
+    return there ? ((long long)blk * a.Hkv + h) * per + (o - bi * per) : 0;
 }
 
-// One wave = one octet x one group of 64 channels of one (sequence, kv head), of the keys or of the values: lane = (token of the
+// One wave = one octet x one group of 64 channels of one (sequence, kv head), of the keys and of the values: lane = (token of the
 // octet, eight channels).  The lane's channels are one word of a key row as they are; for the values the words are transposed over
-// the lanes of the eight tokens.  Tokens of the octet that are not being appended keep their codes: the only writer of an octet is
-// one wave, and what it does not replace it reads first (a decode step's append reads and writes 9 D / 2 bytes a head besides
-// the token's own 2 D).  grid = (octets * groups * 2 / 4 waves, kv head, sequence).
+// the lanes of the eight tokens.  Tokens of the octet that are not being appended keep their codes: the only writer of an octet's group
+// is one wave, and what it does not replace it reads first (a decode step's append reads and writes 9 D / 2 bytes a head besides
+// the token's own 2 D).  Both tensors' rows and the table entry are requested together.  grid = (octets * groups / 4 waves, kv head,
+// sequence).
 template <class DT, int D, bool VEC>
 __global__ __launch_bounds__(256) void append_q4_kernel(const CopyBlocksArgs a, int octets) {
     typedef typename Elem<DT>::store_t store_t;
     typedef Q4<D> G;
+    constexpr int CH = Chunk<DT>::CH;
     const int lane = threadIdx.x & 63;
     const int item = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 4 + (int)(threadIdx.x >> 6));
     const int h = blockIdx.y, b = blockIdx.z;
-    const int oi = item / (2 * G::NG), part = item - oi * (2 * G::NG);
-    const bool keys = part < G::NG;
-    const int g = keys ? part : part - G::NG;
+    const int oi = item / G::NG, g = item % G::NG;
     if (oi >= octets) return;
     const int first = a.seq_lengths[b];
     const int o = (first >> 3) + oi;                     // (floor: of a negative position the part from 0 on is appended, as by copy_to_blocks)
@@ -146,67 +172,80 @@ __global__ __launch_bounds__(256) void append_q4_kernel(const CopyBlocksArgs a, 
     const int t = o * 8 + i - first;                     // new token of this lane
     const bool mine = t >= 0 && t < a.S_new;
     if (o < 0 || o * 8 >= first + a.S_new) return;       // uniform
-    const long long at = q4_octet(a, b, h, o);
-    if (at < 0) return;                                  // uniform
-    char* oct = reinterpret_cast<char*>(keys ? a.kcache : a.vcache) + at * G::OCT;
 
-    float x[8];
-    {
-        const store_t* src = reinterpret_cast<const store_t*>(keys ? a.key_states : a.value_states) +
-                             ((long long)b * (keys ? a.ks_b : a.vs_b) + (long long)h * (keys ? a.ks_h : a.vs_h) +
-                              (long long)(mine ? t : 0) * (keys ? a.ks_s : a.vs_s) + 64 * g + 8 * c);
+    float x[2][8];
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+        const store_t* src = reinterpret_cast<const store_t*>(kv == 0 ? a.key_states : a.value_states) +
+                             ((long long)b * (kv == 0 ? a.ks_b : a.vs_b) + (long long)h * (kv == 0 ? a.ks_h : a.vs_h) +
+                              (long long)(mine ? t : 0) * (kv == 0 ? a.ks_s : a.vs_s) + 64 * g + 8 * c);
         if constexpr (VEC) {
-            constexpr int CH = Chunk<DT>::CH;
 #pragma unroll
             for (int k = 0; k < 8 / CH; ++k) {
                 float y[CH];
                 Chunk<DT>::unpack(*reinterpret_cast<const u32x4*>(src + k * CH), y);
 #pragma unroll
-                for (int e = 0; e < CH; ++e) x[k * CH + e] = y[e];
+                for (int e = 0; e < CH; ++e) x[kv][k * CH + e] = y[e];
             }
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = Elem<DT>::to_float(src[e]);
+            for (int e = 0; e < 8; ++e) x[kv][e] = Elem<DT>::to_float(src[e]);
         }
     }
-    float lo = Q4_LIMIT, hi = -Q4_LIMIT;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        x[e] = x[e] != x[e] ? 0.f : fminf(fmaxf(x[e], -Q4_LIMIT), Q4_LIMIT);
-        lo = fminf(lo, x[e]);
-        hi = fmaxf(hi, x[e]);
-    }
-    lo = oct_min(lo);
-    hi = oct_max(hi);
-    const _Float16 mh = (_Float16)lo;
-    const float m = (float)mh;
-    const _Float16 sh = (_Float16)fmaxf((hi - m) / 15.f, 0.f);
-    const float s = (float)sh;
-    u32 w = 0;                                           // plain nibble order
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float code = s > 0.f ? fminf(fmaxf(__builtin_rintf((x[e] - m) / s), 0.f), 15.f) : 0.f;
-        w |= (u32)code << (4 * e);
-    }
+    bool there;
+    const long long at = q4_octet(a, b, h, o, there) * G::OCT;
     const u32 tokens = 0xffu & (u32)(((1 << min(max(first + a.S_new - o * 8, 0), 8)) - 1) & ~((1 << min(max(first - o * 8, 0), 8)) - 1));   // the octet's new tokens
-    if (keys) {
-        // channels 64 g + 8 c .. + 7: quarter c / 2, word (quarter) * WPQ + 2 g + c % 2
-        if (mine) *reinterpret_cast<u32*>(oct + i * G::KROW + ((c >> 1) * G::WPQ + 2 * g + (c & 1)) * 4) = q4_spread(w);
-    } else {
-        w = q4_transpose(w, lane);                       // now: channel 64 g + 8 c + i, its eight tokens
-        u32* dst = reinterpret_cast<u32*>(oct) + 64 * g + 8 * c + i;
-        if (tokens != 0xffu) {
-            u32 keep = 0;
+    const Q4Transpose transpose(lane);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) keep |= (tokens >> e) & 1 ? 0u : 15u << (4 * e);
-            w = (q4_gather(*dst) & keep) | (w & ~keep);
+    for (int kv = 0; kv < 2; ++kv) {
+        float lo = min8(x[kv]), hi = max8(x[kv]), zero = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) zero = __builtin_fmaf(x[kv][e], 0.f, zero);
+        // (NaN and what is beyond the limit are rare, and three instructions an element)
+        if (__ballot(!(zero == 0.f) || lo < -Q4_LIMIT || hi > Q4_LIMIT) != 0) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float y = x[kv][e];
+                x[kv][e] = y != y ? 0.f : __builtin_amdgcn_fmed3f(y, -Q4_LIMIT, Q4_LIMIT);
+            }
+            lo = min8(x[kv]);
+            hi = max8(x[kv]);
         }
-        *dst = q4_spread(w);
-    }
-    if (mine && c == 0) {
-        _Float16* par = reinterpret_cast<_Float16*>(oct + G::PAR + 32 * g) + i;
-        par[0] = sh;
-        par[8] = mh;
+        lo = oct_min(lo);
+        hi = oct_max(hi);
+        const _Float16 mh = (_Float16)lo;
+        const float m = (float)mh;
+        const _Float16 sh = (_Float16)fmaxf(q4_divide(hi - m, 15.f, 1.f / 15.f), 0.f);
+        const float s = (float)sh, r = 1.f / (s > 0.f ? s : 1.f);
+        // (codes as the last bits of 2^23 + code; the sum of the words that the 2^23 come to is taken off at the end)
+        u32 w = 0, bias = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float code = __builtin_amdgcn_fmed3f(q4_divide(x[kv][e] - m, s, r), 0.f, 15.f) + 0x1p23f;
+            w += __float_as_uint(code) << q4_shift(e);
+            bias += 0x4B000000u << q4_shift(e);
+        }
+        w = s > 0.f ? w - bias : 0u;
+        char* oct = reinterpret_cast<char*>(kv == 0 ? a.kcache : a.vcache) + at;
+        if (kv == 0) {
+            // channels 64 g + 8 c .. + 7: quarter c / 2, word (quarter) * WPQ + 2 g + c % 2
+            if (there && mine) *reinterpret_cast<u32*>(oct + i * G::KROW + ((c >> 1) * G::WPQ + 2 * g + (c & 1)) * 4) = w;
+        } else {
+            w = transpose(w);                            // now: channel 64 g + 8 c + i, its eight tokens
+            u32* dst = reinterpret_cast<u32*>(oct) + 64 * g + 8 * c + i;
+            if (there && tokens != 0xffu) {
+                u32 keep = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) keep |= (tokens >> e) & 1 ? 0u : 15u << q4_shift(e);
+                w = (*dst & keep) | (w & ~keep);
+            }
+            if (there) *dst = w;
+        }
+        if (there && mine && c == 0) {
+            _Float16* par = reinterpret_cast<_Float16*>(oct + G::PAR + 32 * g) + i;
+            par[0] = sh;
+            par[8] = mh;
+        }
     }
 }
 
@@ -216,42 +255,43 @@ template <class DT, int D>
 __global__ __launch_bounds__(256) void read_q4_kernel(const CopyBlocksArgs a, int octets) {
     typedef typename Elem<DT>::store_t store_t;
     typedef Q4<D> G;
+    constexpr int CH = Chunk<DT>::CH;
     const int lane = threadIdx.x & 63;
     const int item = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 4 + (int)(threadIdx.x >> 6));
     const int h = blockIdx.y, b = blockIdx.z;
-    const int oi = item / (2 * G::NG), part = item - oi * (2 * G::NG);
-    const bool keys = part < G::NG;
-    const int g = keys ? part : part - G::NG;
+    const int oi = item / G::NG, g = item % G::NG;
     if (oi >= octets) return;
     const int first = a.seq_lengths[b];
     const int i = lane >> 3, c = lane & 7;
     const int o = (first >> 3) + oi;                     // (floor, also of negative positions)
     const int t = oi * 8 + i - (first & 7);
-    if (t < 0 || t >= a.S_new) return;
-    const long long at = o < 0 ? -1 : q4_octet(a, b, h, o);
+    bool there;
+    const long long at = q4_octet(a, b, h, o, there) * G::OCT;
+    const char* koct = reinterpret_cast<const char*>(a.kcache) + at;
+    const char* voct = reinterpret_cast<const char*>(a.vcache) + at;
+    const u32 kw = *reinterpret_cast<const u32*>(koct + i * G::KROW + ((c >> 1) * G::WPQ + 2 * g + (c & 1)) * 4);
+    const u32 vw = *reinterpret_cast<const u32*>(voct + (64 * g + 8 * c + i) * 4);
+    const _Float16* kpar = reinterpret_cast<const _Float16*>(koct + G::PAR + 32 * g) + i;
+    const _Float16* vpar = reinterpret_cast<const _Float16*>(voct + G::PAR + 32 * g) + i;
+    const float ks = (float)kpar[0], km = (float)kpar[8], vs = (float)vpar[0], vm = (float)vpar[8];
+    const Q4Transpose transpose(lane);
+    const u32 words[2] = {kw, transpose(vw)};            // (of the values: token i, channels 64 g + 8 c .. + 7)
     const size_t row = ((size_t)b * a.Hkv + h) * a.S_new + t;
-    store_t* dst = reinterpret_cast<store_t*>(const_cast<void*>(keys ? a.key_states : a.value_states)) + row * D + 64 * g + 8 * c;
-    constexpr int CH = Chunk<DT>::CH;
-    float y[8 / CH][CH];
+    if (t < 0 || t >= a.S_new) return;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e / CH][e % CH] = 0.f;
-    if (at >= 0) {
-        const char* oct = reinterpret_cast<const char*>(keys ? a.kcache : a.vcache) + at * G::OCT;
-        const _Float16* par = reinterpret_cast<const _Float16*>(oct + G::PAR + 32 * g) + i;
-        const float s = (float)par[0], m = (float)par[8];
-        if (keys) {
-            const u32 w = *reinterpret_cast<const u32*>(oct + i * G::KROW + ((c >> 1) * G::WPQ + 2 * g + (c & 1)) * 4);
+    for (int kv = 0; kv < 2; ++kv) {
+        const float sc = there ? (kv == 0 ? ks : vs) : 0.f, m = there ? (kv == 0 ? km : vm) : 0.f;
+        const u32 even = words[kv] & 0x0F0F0F0Fu, odd = (words[kv] >> 4) & 0x0F0F0F0Fu;   // bytes: elements 0 4 1 5 and 2 6 3 7
+        float y[8 / CH][CH];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[e / CH][e % CH] = __builtin_fmaf((float)((w >> q4_shift(e)) & 15u), s, m);
-        } else {
-            const u32* src = reinterpret_cast<const u32*>(oct) + 64 * g + 8 * c;
-            const int sh = 4 * ((i >> 1) + ((i & 1) << 2));
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y[e / CH][e % CH] = __builtin_fmaf((float)((src[e] >> sh) & 15u), s, m);
+        for (int e = 0; e < 8; ++e) {
+            const int n = q4_shift(e) / 4;
+            y[e / CH][e % CH] = __builtin_fmaf((float)(((n & 1 ? odd : even) >> (8 * (n >> 1))) & 0xffu), sc, m);
         }
-    }
+        store_t* dst = reinterpret_cast<store_t*>(const_cast<void*>(kv == 0 ? a.key_states : a.value_states)) + row * D + 64 * g + 8 * c;
 #pragma unroll
-    for (int k = 0; k < 8 / CH; ++k) *reinterpret_cast<u32x4*>(dst + k * CH) = Chunk<DT>::pack(y[k]);
+        for (int k = 0; k < 8 / CH; ++k) *reinterpret_cast<u32x4*>(dst + k * CH) = Chunk<DT>::pack(y[k]);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -387,16 +427,6 @@ __device__ __forceinline__ f32x4 mfma_f16_k16(u32x2 a, u32x2 b, f32x4 c) {
 }
 
 constexpr float Q4_BELOW = 7.f, Q4_ABOVE = 15.f;   // weights are 2^7 where the reference is taken and stay below 2^15
-
-// (as one instruction each: fmaxf has every operand quieted first)
-__device__ __forceinline__ float max3_nn(float a, float b, float c) {
-    float r;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-    return r;
-}
-__device__ __forceinline__ float max8(const float (&x)[8]) {
-    return max_nn(max3_nn(max3_nn(max3_nn(x[0], x[1], x[2]), x[3], x[4]), x[5], x[6]), x[7]);
-}
 
 // One tile against the rows of the workgroup.  `partial` (uniform): some row does not see all of it, or some of its tokens nobody sees
 // (their bytes may be anything: the parameters of such values are cleared, their logits replaced).  SPLIT (fp16 results): the weights as the sum of
@@ -838,7 +868,7 @@ hipError_t launch_paged_q4(const PagedHeader& ph, void* out, float* lse, int dty
 // The octets that S_new tokens from any position on may touch, and the grid that takes them.
 static dim3 q4_grid(const CopyBlocksArgs& a, int D, int* octets) {
     *octets = (a.S_new + 14) / 8;
-    return dim3((unsigned)(((long long)*octets * 2 * (D / 64) + 3) / 4), (unsigned)a.Hkv, (unsigned)a.B);
+    return dim3((unsigned)(((long long)*octets * (D / 64) + 3) / 4), (unsigned)a.Hkv, (unsigned)a.B);
 }
 
 template <class DT>
