@@ -154,7 +154,9 @@ __device__ __forceinline__ long long q4_octet(const CopyBlocksArgs& a, int b, in
 // octet, eight channels).  The lane's channels are one word of a key row as they are; for the values the words are transposed over
 // the lanes of the eight tokens.  Tokens of the octet that are not being appended keep their codes: the only writer of an octet's group
 // is one wave, and what it does not replace it reads first (a decode step's append reads and writes 9 D / 2 bytes a head besides
-// the token's own 2 D).  Both tensors' rows and the table entry are requested together.  grid = (octets * groups / 4 waves, kv head,
+// the token's own 2 D).  Both tensors' rows and the table entry are requested together.  The rows are
+// read once and stream past the caches: 4 x 2048 tokens of 8 kv heads, D = 128, bf16 (43 MB) 17.5 us with cached loads, 13.2 without
+// (3.3 TB/s; the arithmetic alone, some 330 instructions a wave, is 8 us).  grid = (octets * groups / 4 waves, kv head,
 // sequence).
 template <class DT, int D, bool VEC>
 __global__ __launch_bounds__(256) void append_q4_kernel(const CopyBlocksArgs a, int octets) {
@@ -183,7 +185,7 @@ __global__ __launch_bounds__(256) void append_q4_kernel(const CopyBlocksArgs a, 
 #pragma unroll
             for (int k = 0; k < 8 / CH; ++k) {
                 float y[CH];
-                Chunk<DT>::unpack(*reinterpret_cast<const u32x4*>(src + k * CH), y);
+                Chunk<DT>::unpack(__builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + k * CH)), y);
 #pragma unroll
                 for (int e = 0; e < CH; ++e) x[kv][k * CH + e] = y[e];
             }
