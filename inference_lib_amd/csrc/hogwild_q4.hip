@@ -349,17 +349,20 @@ __device__ __forceinline__ u32x4 q4_tiny(u32 w, const Q4Consts& k) {
     return u32x4{w & k.lo, w & k.hi, w8 & k.lo, w8 & k.hi};
 }
 
-// The queries of a lane's row as B operands, and what the logits need of them: the products run on the bare codes, which fp16 holds
-// exactly, against the queries times a power of two of their row's own (so bf16 queries lose nothing to fp16's range):
-//   scale * q . k = sum_g s_g (sum_{e in g} q_e c_e) + m_g (sum_{e in g} q_e)
-// Sums of a wave.  The logits come out of a tile relative to the reference of the exponentials, in the units of the products (seed =
-// minus the reference in them): the first of the additions that form a logit takes it along.
+// The logits.  The products run on the bare codes, which fp16 holds exactly, against the queries times a power of two of their row's own
+// (so bf16 queries lose nothing to fp16's range); scales and offsets of the groups g join in fp32:
+//   q . k = sum_g s_g (sum_{e in g} q_e c_e) + m_g (sum_{e in g} q_e)
+// The second part and minus the reference of the exponentials (seed) are one product more for 16 tokens, of the offsets and a one with the
+// sums of the queries and the seed, each as two fp16 numbers: by fp32 instructions it took 16 a tile and row block instead of 2.  What
+// comes out counts in the units of the products; `sc` takes it to base 2.
+//
+// Sums of a wave over its tiles:
 template <int RB, int NOC>
 struct Q4State {
     f32x4 o[RB][NOC];
     float m[RB], l[RB];              // reference (base-2 units, NEG_BIG: none yet), this lane's part of the sum of the weights
-    u32 seed[RB];                    // two fp16 numbers, their sum is what it stands for
-    float above[RB], unit[RB];   // minus the reference, the logit beyond which it moves, and 1 in base-2 units, in those units
+    u32 seed[RB];                    // minus the reference in the products' units: two fp16 numbers, their sum is what it stands for
+    float above[RB], unit[RB];       // in them, too: the logit (less the reference) beyond which that moves, and 1 in base 2
 };
 
 // More than 128 channels and rows of 16 together (QLDS): the operands lie in LDS, made ready by one wave for each 16 rows and read by
@@ -386,8 +389,9 @@ __device__ __forceinline__ u32 q4_pair(float x, float up) {
 // The sum of a row's queries is small in the products' units (2^-11 or so where its largest counts for much): its second half is kept
 // this much larger and meets offsets that much smaller.
 constexpr float Q4_LOW = 256.f;
-// Logits stay within 49000 of the products' units; the reference may lie 2^7 below them, which for queries (or a scale) next to nothing
-// is more of those units than fp16 counts.  Such logits are alike, whatever is taken off them.
+// Logits stay within D 2^14 65024 2^-24 <= 16 256 of the products' units, and 2^7 is 448 of them at most (q4_queries): what lies beyond
+// fp16's range are references of fragments with much larger queries.  44 000 units are more than 2^600 there, so either way one side's
+// weights are nothing.
 __device__ __forceinline__ u32 q4_seed(float x) { return q4_pair(fminf(fmaxf(x, -6.0e4f), 6.0e4f), 1.f); }
 
 template <class DT, int D>
@@ -402,8 +406,8 @@ __device__ __forceinline__ void q4_queries(Q4Block<D>& qq, const u32x4 (&raw)[D 
         for (int e = 0; e < 8; ++e) top = fmaxf(top, __builtin_fabsf(x[r][e]));
     }
     top = quarter_max(top);
-    // 2^f brings the largest of the row into [2^13, 2^14)
-    const int f = min(max(14 - __builtin_amdgcn_frexp_expf(top), -90), 90);
+    // 2^f brings the largest of the row into [2^13, 2^14), or less where a logit of 1 in base 2 would come to more than 64 units
+    const int f = min(max(min(14 - __builtin_amdgcn_frexp_expf(top), 29 + __builtin_amdgcn_frexp_expf(sc)), -113), 90);
     const float up = __builtin_ldexpf(1.f, f);
     const float up16 = up * 0.0625f;
 #pragma unroll
@@ -420,7 +424,7 @@ __device__ __forceinline__ void q4_queries(Q4Block<D>& qq, const u32x4 (&raw)[D 
         sum = q == g ? t[0] * 0x1p-24f : sum;
     }
     qq.sum = q4_pair(sum, Q4_LOW);
-    qq.sc = fmaxf(sc * __builtin_ldexpf(1.f, 24 - f), 1e-36f);      // (its inverse has to be finite; such logits are 0)
+    qq.sc = fmaxf(__builtin_ldexpf(sc, 24 - f), 1e-36f);      // (its inverse has to be finite; such logits are 0)
 }
 
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));

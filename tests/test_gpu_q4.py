@@ -297,6 +297,32 @@ def test_rows_that_see_nothing_or_little():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("D,S", [(64, 1), (128, 8), (256, 1)])
+def test_fragments_whose_queries_differ_by_orders(dtype, D, S):
+    """The reference of the exponentials goes from fragment to fragment, whose products count in units of their own: logits of +-100 beside
+    some of next to nothing, in either order."""
+    from inference_lib_amd.attention import copy_to_blocks_q4, hogwild_paged_sdpa_q4
+    rng = np.random.default_rng(D + S)
+    u = rng.choice([-1.0, 1.0], D)
+    for sign in (1, -1):
+        for sizes in ((4.0, 3e-7), (3e-7, 4.0), (4.0, 0.0), (0.0, 4.0), (4.0, 2e-5)):
+            pos = torch.tensor(3 * u + rng.standard_normal((300, D)))          # keys about 3 u, of 300 tokens
+            k = pos.to(DT[dtype])[None, None].expand(2, 2, 300, D)
+            table, P = pool(rng, [300, 300], 16)
+            kc, vc = (torch.zeros(P, 2, 16, Q.row_bytes(D), dtype=torch.uint8, device="cuda") for _ in range(2))
+            copy_to_blocks_q4(k.cuda().contiguous(), torch.tensor(rng.standard_normal((2, 2, 300, D))).to(DT[dtype]).cuda(), kc, vc, ints(table), ints([0, 0]))
+            q = np.empty((2, 2, 8, S, D))
+            for f in range(2):
+                q[f] = sizes[f] * (sign * u + 0.2 * rng.standard_normal((2, 8, S, D)))
+            locs = np.stack([[[n - S + s for s in range(S)] for n in (300, 170)], [[n - S + s for s in range(S)] for n in (90, 300)]]).astype(np.int32)
+            c = dict(q=torch.tensor(q).to(DT[dtype]), locs=locs, frag=np.array([300, 200], np.int32), kc=kc.cpu().numpy(), vc=vc.cpu().numpy(), table=table)
+            lse = torch.empty((2, 8, S), device="cuda")
+            out = hogwild_paged_sdpa_q4(*gpu_args(c), 0.1, lse=lse)
+            check_fixed(c, dtype, 0.1, out, lse, f"{sign} {sizes}")
+
+
+@gpu
 def test_extreme_values_queries_and_offsets():
     """Values near the ends of fp16, tiny ones, keys far off zero with small differences, queries that fp16 does not hold."""
     from inference_lib_amd.attention import copy_to_blocks_q4, hogwild_paged_sdpa_q4
@@ -429,6 +455,24 @@ def test_packed_queries_however_they_are_dealt(W, Hq, Hkv, D, row_blocks, splits
             want, want_lse, may, may_lse = exact(qw, loc[:, a:b] + 1, k, v, p, 0.1)
             close(out[a:b].transpose(0, 1), want, may, "bf16", f"{w}")
             assert (np.abs(np64(lse[a:b]).T - want_lse) <= may_lse).all()
+
+
+@gpu
+@pytest.mark.parametrize("D,block,dtype", [(64, 8, "bf16"), (128, 24, "f16"), (128, 512, "bf16"), (256, 16, "bf16")])
+def test_one_workgroup_for_long_sequences(D, block, dtype):
+    """Many tiles for every wave, up to one more and one less than a multiple of sixteen; the workgroup writes the results itself."""
+    from inference_lib_amd import _lib
+    rng = np.random.default_rng(D)
+    lens = [5003, 2048, 2049, 4096, 2080, 1]
+    table, P = pool(rng, lens, block)
+    kc, vc = (np.repeat(random_cache(rng, P, 1, block, D, k, dtype), 2, 1) for k in (True, False))
+    q = torch.tensor(rng.standard_normal((1, len(lens), 8, 1, D))).to(DT[dtype])
+    c = dict(q=q, locs=np.array([[[n - 1] for n in lens]], np.int32), frag=np.array([max(lens)], np.int32), kc=kc, vc=vc, table=table)
+    out, lse = torch.full((len(lens), 8, 1, D), float("nan"), dtype=DT[dtype], device="cuda"), torch.empty((len(lens), 8, 1), device="cuda")
+    a = gpu_args(c)
+    _lib.PagedProblem(q=a[0], locations=a[1], fragment_lengths=a[2], key_cache=a[3], value_cache=a[4], block_table=a[5], scale=0.1, out=out, lse=lse, splits=1,
+                      q4=True).run()
+    check_fixed(c, dtype, 0.1, out, lse, f"{D} {block}")
 
 
 @gpu
