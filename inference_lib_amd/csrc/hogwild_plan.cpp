@@ -596,7 +596,7 @@ bool paged_keep_in_l2(const hw_paged_problem* p, const hw_paged_plan& plan) {
 }
 
 // One row group per sequence, and what the waves go through to find a length (F * S locations) is little: a decode step, a draft of a few
-// tokens.  The measurements are at paged_share in hogwild_paged.hip.  (A caller that fixes the split keeps it.)
+// tokens.  The measurements are at paged_share in hogwild_device.h.  (A caller that fixes the split keeps it.)
 bool paged_shared(const hw_paged_problem* p, const hw_paged_plan& plan) {
     return p->cu_seqlens_q == nullptr && p->splits <= 0 && plan.row_blocks != hw::WIDE_ROW_BLOCKS && p->W >= 2 && p->W <= 64 &&
            plan.row_groups == p->W && plan.splits >= 2 && (long long)p->F * p->S <= 8;
@@ -736,15 +736,20 @@ int paged_q4_validate(const hw_paged_problem* p) {
     return paged_validate(p);
 }
 
-// Workgroups of the 4-bit kernels that a CU holds at once.
+// Workgroups of the 4-bit kernels that a CU is given at once.  At head dimension 256 their registers leave room for one (two splits where
+// one fits: ragged decode steps of 4 and 5 sequences at 8 kv heads 16.5 -> 21.4 us).
 static int q4_resident(const hw_paged_problem* p) { return p->Ev == 256 ? 1 : 2; }
 
-// As paged_shares_save: launches of up to as many workgroups as the chip holds run at once.
+// As paged_shares_save, for 256 channels only, where a tile takes long: ragged decode steps of 5 and 4 sequences of 296 to 11 000 tokens
+// at 8 kv heads 24.1 -> 16.5, 20.8 -> 16.5 us.  Below, what the shares cost in every workgroup is more than what they save: the
+// like of them at D = 128 11.4 -> 12.2 and 14.0 -> 14.3, four tokens each 17.2 -> 20.4, at 64 equal.
 int paged_q4_shares_save(const hw_paged_problem* p, const hw_paged_plan& plan, int num_cus) {
     return p->Ev == 256 && plan.workgroups <= num_cus ? 0 : -1;
 }
 
-// Workgroups of four waves with 16 query rows (32 from 17 rows a sequence on), each wave a stripe of the sequence's 32-token tiles.
+// Workgroups of four waves with 16 query rows (32 from 17 rows a sequence on), each wave a stripe of the sequence's 32-token tiles.  What a
+// tile costs whatever the rows (its decoding above all) is as much as 1.6 blocks of 16: 64 packed tokens at 5 rows each 135 (16 rows) ->
+// 115 us (32), 128 at 4 rows 71 -> 61; decode steps of 24 rows 16.9 -> 16.2.
 int paged_q4_plan(const hw_paged_problem* p, int num_cus, hw_paged_plan* plan) {
     if (plan == nullptr) return HW_ERR_NULL;
     if (num_cus < 1) return HW_ERR_SHAPE;
@@ -770,8 +775,14 @@ int paged_q4_plan(const hw_paged_problem* p, int num_cus, hw_paged_plan* plan) {
     if (splits <= 0) {
         const long long tiles = ((long long)p->block_size * p->max_blocks + hw::TILE - 1) / hw::TILE;
         const long long pairs = (long long)p->Hkv * items, room = (long long)q4_resident(p) * num_cus;
-        // as many as the chip holds at once; up to one and a half times that many are halved, which fills the last round
-        splits = 2 * pairs <= room ? room / pairs : 2 * pairs <= 3 * room ? 2 : 1;
+        // As many as the chip holds at once.  More than half of that, up to one and a half times, are cut in three where sequences may
+        // be long, which evens out the last round and ragged lengths: 8 kv heads, D = 128, 36 to 84 sequences, 4 rows each, of 12 000
+        // tokens 114 -> 99, 125 -> 127, 133 -> 136, 156 -> 163, 208 -> 182, 222 -> 214 us, of 500 to 16 000 104 -> 80, 117 -> 96, 115 ->
+        // 109, 149 -> 139, 138 -> 135, 186 -> 165; 32 rows each 123 -> 97 to 213 -> 206.  The same with 2000 tokens each (whole, cut)
+        // 22 / 23, 21 / 26, 23 / 28, 26 / 32, 35 / 35, 36 / 39, with 200 to 3800 29 / 25, 27 / 28, 33 / 31, 33 / 35, 36 / 37, 43 / 42; whole
+        // ones need no merge.
+        const bool lengthy = tiles >= 64 * hw::NWAVES;
+        splits = 2 * pairs <= room ? room / pairs : lengthy && 2 * pairs <= 3 * room ? 3 : 1;
         splits = std::min(splits, (tiles + hw::NWAVES - 1) / hw::NWAVES);
     }
     if (splits > 64) splits = 64;

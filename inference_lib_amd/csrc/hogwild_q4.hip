@@ -1,5 +1,5 @@
 // Paged caches in 4 bits for gfx950 (MI355X, CDNA4, wave64): the append that quantises, the read that gives the values back, and
-// the attention that reads the codes.
+// the attention that reads the codes (each kernel's measurements stand above it).
 //
 // A value is offset + scale * code, code in 0 .. 15, with a scale and an offset (fp16) for every token, kv head and group of 64
 // channels: 9 bits per 2 channels against 32 in 16 bits.  Eight consecutive tokens (an octet) of a kv head lie together, 9 D / 2 bytes:
@@ -252,7 +252,8 @@ __global__ __launch_bounds__(256) void append_q4_kernel(const CopyBlocksArgs a, 
 }
 
 // The values of positions first[b] .. first[b] + n - 1 as [B, Hkv, n, D]; positions outside the table or the cache give zeros.  The
-// waves and lanes of append_q4_kernel, the other way round.
+// waves and lanes of append_q4_kernel, the other way round.  Bound by its writes: 4 x 2048 tokens of 8 kv heads, D = 128, to fp32 16.2 us
+// (76 MB, 4.7 TB/s; stores that stream past the caches 21 us).
 template <class DT, int D>
 __global__ __launch_bounds__(256) void read_q4_kernel(const CopyBlocksArgs a, int octets) {
     typedef typename Elem<DT>::store_t store_t;
@@ -546,7 +547,6 @@ __device__ __forceinline__ void q4_compute(bool partial, const Q4Tile<D>& t, cha
     }
 #pragma unroll
     for (int c = 0; c < G::NOC; ++c) {
-        if (c % 2 == 0) __builtin_amdgcn_sched_barrier(0);
         u32x4 a = q4_codes(t.v[c], cs);
 #pragma unroll
         for (int d = 0; d < 4; ++d) a[d] = h2_bits(__builtin_elementwise_fma(h2_of(a[d]), h2_of(vs[d]), h2_of(vm[d])));
@@ -630,6 +630,21 @@ __device__ __forceinline__ void q4_store(Q4State<RB, D / 16>& st, Exchange<RB * 
 // A workgroup = one kv head x up to 16 RB query rows of one sequence x every nsplit-th stripe of its 32-token tiles (four waves, each
 // takes every (4 nsplit)-th tile).  A tile is loaded straight into the operands' lanes, one ahead of the one being multiplied; the
 // first ones are requested as soon as the rows' bounds are known, and the queries are made ready behind them.
+//
+// What bounds it: with few rows the stream of the codes, 5.5 to 6 TB/s from some thousand tokens on, and about 5 us before and behind it;
+// with 32 rows the vector arithmetic (65 % of the issue slots over a prompt chunk, 80 % while both waves of a SIMD are there; the
+// matrix units 30 %): of some 310 slots a tile 104 are for the values' codes, 40 for the keys', 74 for the softmax of each row block, 64
+// of those for exponentials.  Measured (MI355X, us a layer with the merge, GB/s of what has to be read and TFLOP/s):
+//   4 x 12 528 tokens, one query each, 40/8 heads, D = 128, bf16        18.1   3200
+//   296 to 10 543 tokens, 16/8 heads, D = 256, bf16                     16.5   2460
+//   2052 to 11 111 tokens, four queries each, 64/8, D = 128, f16        18.5   1730   193
+//   1 / 8 / 32 / 64 packed queries on 12 528 each, 40/8, bf16           57     1050   474
+//   1024 queries on 5120, 40/8, bf16                                    137           706
+// One tile ahead is enough: two, or the loop arranged so that nothing waits for the tile in flight at its head, changed nothing (the other
+// wave of the SIMD, or the other SIMDs at D = 256, cover it).  Loads that stay in the caches beat streaming ones everywhere, by up to
+// 12 % (the halves of a line are requested apart, and the row groups of a sequence read the same tiles).  128-row workgroups that decode
+// into LDS for their waves were built: half a barrier's wait a step, 456 against 325 us on the prompt chunk, 134 against 125 packed.  64
+// rows a wave, one wave a SIMD: nothing runs beside the softmax then, 362 against 272 and 168 against 113.
 template <class DT, int D, int RB, int MINW>
 __global__ __launch_bounds__(NTHREADS, MINW) void paged_q4_kernel(const PagedHeader args, const Q4Out out) {
     typedef Q4<D> G;
