@@ -155,8 +155,8 @@ __device__ __forceinline__ long long q4_octet(const CopyBlocksArgs& a, int b, in
 // the lanes of the eight tokens.  Tokens of the octet that are not being appended keep their codes: the only writer of an octet's group
 // is one wave, and what it does not replace it reads first (a decode step's append reads and writes 9 D / 2 bytes a head besides
 // the token's own 2 D).  Both tensors' rows and the table entry are requested together.  The rows are
-// read once and stream past the caches: 4 x 2048 tokens of 8 kv heads, D = 128, bf16 (43 MB) 17.5 us with cached loads, 13.2 without
-// (3.3 TB/s; the arithmetic alone, some 330 instructions a wave, is 8 us).  grid = (octets * groups / 4 waves, kv head,
+// read once and stream past the caches: 4 x 2048 tokens of 8 kv heads, D = 128, bf16 (43 MB) 17.4 us with cached loads, 14.2 without
+// (3.0 TB/s; the arithmetic alone, some 330 instructions a wave, is 8 us).  grid = (octets * groups / 4 waves, kv head,
 // sequence).
 template <class DT, int D, bool VEC>
 __global__ __launch_bounds__(256) void append_q4_kernel(const CopyBlocksArgs a, int octets) {
@@ -252,8 +252,8 @@ __global__ __launch_bounds__(256) void append_q4_kernel(const CopyBlocksArgs a, 
 }
 
 // The values of positions first[b] .. first[b] + n - 1 as [B, Hkv, n, D]; positions outside the table or the cache give zeros.  The
-// waves and lanes of append_q4_kernel, the other way round.  Bound by its writes: 4 x 2048 tokens of 8 kv heads, D = 128, to fp32 16.2 us
-// (76 MB, 4.7 TB/s; stores that stream past the caches 21 us).
+// waves and lanes of append_q4_kernel, the other way round.  Bound by its writes: 4 x 2048 tokens of 8 kv heads, D = 128, to fp32 16.5 us
+// (76 MB, 4.6 TB/s; stores that stream past the caches 21 us).
 template <class DT, int D>
 __global__ __launch_bounds__(256) void read_q4_kernel(const CopyBlocksArgs a, int octets) {
     typedef typename Elem<DT>::store_t store_t;
