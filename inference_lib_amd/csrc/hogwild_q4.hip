@@ -569,62 +569,61 @@ __device__ __forceinline__ size_t q4_out_row(const PagedDevHeader& ph, int r, in
     return ((size_t)w * ph.Hq + hkv * GQ + (r - ws * GQ)) * ph.LS + (ws - w * ph.LS);
 }
 
-// Rows of the partial sums, and of what a workgroup of four waves hands over: as in store_partials, with the output channel of
-// accumulator c, row i being i * D / 16 + c.
+// Rows of the partial sums (or of the result, PH_DIRECT), from what the four waves hand over: accumulator c, row i holds output channel
+// i * D / 16 + c.  A wave takes whole rows, four at a time, sixteen lanes to a row and D / 16 neighbouring channels to a lane, so that what it
+// writes are whole lines (by accumulators as they come a store is 64 pieces of 8 or 16 bytes: 0.5 to 4 % of a call).  In LDS a quarter's
+// lanes change places so that those sixteen meet no bank twice.  What is left of the end is that the 8 MB of 512 workgroups of 32 rows have to
+// reach memory: 2.9 us of a launch without any tiles, whose whole is 8.1 (empty launch 2.2, tables and first tile 1.4, queries 1.4).
 template <class DT, int D, int RB>
 __device__ __forceinline__ void q4_store(Q4State<RB, D / 16>& st, Exchange<RB * 16, D>& ex, int wv, int n, int q, int lane, const PagedDevHeader& ph,
                                          size_t part, int nrows, const Q4Out& out, int r0, int hkv) {
-    constexpr int NOC = D / 16, NSLOT = RB * NOC, SPW = NSLOT / NWAVES;
-    static_assert(NSLOT % NWAVES == 0 && (NOC % SPW == 0), "a wave's share lies within one row block");
+    constexpr int NOC = D / 16, NSLOT = RB * NOC;
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
         const float l = quarter_sum(st.l[rb]);
 #pragma unroll
-        for (int c = 0; c < NOC; ++c) ex.o[wv][rb * NOC + c][lane] = st.o[rb][c];
+        for (int c = 0; c < NOC; ++c) ex.o[wv][rb * NOC + c][q * 16 + (n ^ (4 * q))] = st.o[rb][c];
         if (q == 0) {
             ex.m[rb * 16 + n][wv] = st.m[rb];
             ex.l[rb * 16 + n][wv] = l;
         }
     }
     __syncthreads();
-    const int s0 = wv * SPW, rb = s0 / NOC, c0 = s0 % NOC, row = rb * 16 + n;
-    if (row >= nrows) return;
-    const f32x4 m4 = *reinterpret_cast<const f32x4*>(&ex.m[row][0]);
-    const f32x4 l4 = *reinterpret_cast<const f32x4*>(&ex.l[row][0]);
-    const float mm = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-    float wgt[NWAVES], lsum = 0.f;
+    const int i = lane & 3, from = (lane >> 2) & 3, nn = wv * 4 + (lane >> 4);
+    const int e = (4 * from + i) * NOC;          // the lane's first channel
 #pragma unroll
-    for (int w2 = 0; w2 < NWAVES; ++w2) {
-        wgt[w2] = fast_exp2(m4[w2] - mm);
-        lsum = __builtin_fmaf(l4[w2], wgt[w2], lsum);
+    for (int rb = 0; rb < RB; ++rb) {
+        const int row = rb * 16 + nn;
+        if (row >= nrows) return;
+        const f32x4 m4 = *reinterpret_cast<const f32x4*>(&ex.m[row][0]);
+        const f32x4 l4 = *reinterpret_cast<const f32x4*>(&ex.l[row][0]);
+        const float mm = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        const float* src = reinterpret_cast<const float*>(&ex.o[0][rb * NOC][from * 16 + (nn ^ (4 * from))]) + i;
+        float lsum = 0.f, run[NOC];
+#pragma unroll
+        for (int c = 0; c < NOC; ++c) run[c] = 0.f;
+#pragma unroll
+        for (int w2 = 0; w2 < NWAVES; ++w2) {
+            const float wgt = fast_exp2(m4[w2] - mm);
+            lsum = __builtin_fmaf(l4[w2], wgt, lsum);
+#pragma unroll
+            for (int c = 0; c < NOC; ++c) run[c] = __builtin_fmaf(src[(w2 * NSLOT + c) * 256], wgt, run[c]);
+        }
+        if (ph.flags & PH_DIRECT) {              // (the sums are all there are)
+            const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
+            const size_t orow = q4_out_row(ph, r0 + row, hkv);
+            HW_GLOBAL u32x2* dst = reinterpret_cast<HW_GLOBAL u32x2*>(out.out + (orow * D + e) * 2);
+#pragma unroll
+            for (int c = 0; c < NOC; c += 4)
+                dst[c / 4] = u32x2{Elem<DT>::pack2(run[c] * inv, run[c + 1] * inv), Elem<DT>::pack2(run[c + 2] * inv, run[c + 3] * inv)};
+            if (out.lse != nullptr && e == 0) out.lse[orow] = lsum > 0.f ? (mm + __builtin_amdgcn_logf(lsum)) * 0.69314718055994530942f : -__builtin_inff();
+        } else {
+            HW_GLOBAL f32x4* dst = reinterpret_cast<HW_GLOBAL f32x4*>(ph.part_o + (part + row) * D + e);
+#pragma unroll
+            for (int c = 0; c < NOC; c += 4) dst[c / 4] = f32x4{run[c], run[c + 1], run[c + 2], run[c + 3]};
+            if (e == 0) *reinterpret_cast<HW_GLOBAL f32x2*>(ph.part_ml + (part + row) * 2) = f32x2{mm, lsum};
+        }
     }
-    float run[4][SPW];
-#pragma unroll
-    for (int j = 0; j < SPW; ++j) {
-        f32x4 acc = ex.o[0][s0 + j][lane] * wgt[0];
-#pragma unroll
-        for (int w2 = 1; w2 < NWAVES; ++w2) acc += ex.o[w2][s0 + j][lane] * wgt[w2];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) run[i][j] = acc[i];
-    }
-    if (ph.flags & PH_DIRECT) {              // (the sums are all there are)
-        const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
-        const size_t orow = q4_out_row(ph, r0 + row, hkv);
-        typedef typename Elem<DT>::store_t store_t;
-        HW_GLOBAL store_t* dst = reinterpret_cast<HW_GLOBAL store_t*>(out.out) + orow * D;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < SPW; ++j) dst[(4 * q + i) * NOC + c0 + j] = Elem<DT>::from_float(run[i][j] * inv);
-        if (out.lse != nullptr && q == 0 && c0 == 0) out.lse[orow] = lsum > 0.f ? (mm + __builtin_amdgcn_logf(lsum)) * 0.69314718055994530942f : -__builtin_inff();
-        return;
-    }
-    HW_GLOBAL float* dst = ph.part_o + (part + row) * D;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < SPW; ++j) dst[(4 * q + i) * NOC + c0 + j] = run[i][j];
-    if (q == 0 && c0 == 0) *reinterpret_cast<HW_GLOBAL f32x2*>(ph.part_ml + (part + row) * 2) = f32x2{mm, lsum};
 }
 
 // A workgroup = one kv head x up to 16 RB query rows of one sequence x every nsplit-th stripe of its 32-token tiles (four waves, each
