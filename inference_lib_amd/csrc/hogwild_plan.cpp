@@ -784,6 +784,11 @@ int paged_q4_plan(const hw_paged_problem* p, int num_cus, hw_paged_plan* plan) {
         const bool lengthy = tiles >= 64 * hw::NWAVES;
         splits = 2 * pairs <= room ? room / pairs : lengthy && 2 * pairs <= 3 * room ? 3 : 1;
         splits = std::min(splits, (tiles + hw::NWAVES - 1) / hw::NWAVES);
+        // Short tables stay with one workgroup, which needs no merge (2.5 us in a graph, a launch more on the host): a turn of its four waves
+        // takes 0.55 us at 64 channels, 0.65 at 128, 0.9 with 32 rows, 1.1 at 256.  Split / whole, 2 to 8 sequences: D = 64 768 tokens 6.3 /
+        // 6.0, 1024 6.4 / 7.0; 128 640 tokens 6.9 / 6.8, 768 6.9 / 7.5; with 32 rows 384 8.4 / 8.0, 512 8.5 / 9.0 (D = 64 640 7.7 / 7.2, 768 7.9 / 7.9); 256 384 8.9 / 8.6, 512 8.8 / 9.7.
+        const bool one_row_block = plan->row_blocks == 1;
+        if (tiles <= (p->Ev <= 64 ? (one_row_block ? 24 : 20) : p->Ev <= 128 && one_row_block ? 20 : 12)) splits = 1;
     }
     if (splits > 64) splits = 64;
     if (splits < 1) splits = 1;
