@@ -635,10 +635,10 @@ __device__ __forceinline__ void q4_store(Q4State<RB, D / 16>& st, Exchange<RB * 
 // matrix units 30 %): of some 310 slots a tile 104 are for the values' codes, 40 for the keys', 74 for the softmax of each row block, 64
 // of those for exponentials.  Measured (MI355X, us a layer with the merge, GB/s of what has to be read and TFLOP/s):
 //   4 x 12 528 tokens, one query each, 40/8 heads, D = 128, bf16        18.1   3200
-//   296 to 10 543 tokens, 16/8 heads, D = 256, bf16                     16.5   2460
+//   296 to 10 543 tokens, 16/8 heads, D = 256, bf16                     16.4   2480
 //   2052 to 11 111 tokens, four queries each, 64/8, D = 128, f16        18.5   1730   193
-//   1 / 8 / 32 / 64 packed queries on 12 528 each, 40/8, bf16           57     1050   474
-//   1024 queries on 5120, 40/8, bf16                                    137           706
+//   1 / 8 / 32 / 64 packed queries on 12 528 each, 40/8, bf16           56     1060   480
+//   1024 queries on 5120, 40/8, bf16                                    135           715
 // One tile ahead is enough: two, or the loop arranged so that nothing waits for the tile in flight at its head, changed nothing (the other
 // wave of the SIMD, or the other SIMDs at D = 256, cover it).  Loads that stay in the caches beat streaming ones everywhere, by up to
 // 12 % (the halves of a line are requested apart, and the row groups of a sequence read the same tiles).  128-row workgroups that decode
