@@ -536,6 +536,89 @@ def test_captured_on_another_stream_and_replayed():
 
 
 @gpu
+@pytest.mark.parametrize("dtype,D", [("f16", 64), ("bf16", 128), ("f32", 256)])
+def test_append_of_rows_at_any_address(dtype, D):
+    """Rows one element off a 16-byte border, with strides that are no multiple of one, and heads before tokens."""
+    from inference_lib_amd.attention import copy_to_blocks_q4
+    rng = np.random.default_rng(D)
+    B, Hkv, S, block = 2, 3, 21, 8
+    starts = [3, 40]
+    table, P = pool(rng, [n + S for n in starts], block)
+    x = [torch.randn((B, Hkv, S, D + 5), generator=torch.Generator().manual_seed(k)).to(DT[dtype])[..., 1: D + 1] for k in (0, 1)]
+    ref = {k: rng.integers(0, 256, (P, Hkv, block, Q.row_bytes(D)), dtype=np.uint8) for k in (True, False)}
+    dev = {k: torch.tensor(v).cuda() for k, v in ref.items()}
+    wide = [torch.empty((B, Hkv, S, D + 5), dtype=DT[dtype], device="cuda")[..., 1: D + 1] for _ in range(2)]
+    for w, y in zip(wide, x):
+        w.copy_(y)
+    copy_to_blocks_q4(wide[0], wide[1], dev[True], dev[False], ints(table), ints(starts))
+    for k, y in zip((True, False), x):
+        Q.copy_to_blocks_q4(y.float().numpy(), ref[k], table, np.array(starts), k)
+        assert (dev[k].cpu().numpy() == ref[k]).all(), k
+
+
+def decode_and_packed(rng, dtype):
+    """A decode step whose sequences several workgroups share and a packed batch with tokens before and behind its sequences, on one cache."""
+    lens, qt, front, behind = [2100, 1333, 40], [5, 70, 1], 3, 2
+    D, Hq, Hkv, block = 128, 8, 2, 16
+    table, P = pool(rng, lens, block)
+    kc, vc = (torch.tensor(random_cache(rng, P, Hkv, block, D, x, dtype)).cuda() for x in (True, False))
+    T = front + sum(qt) + behind
+    q1 = torch.tensor(rng.standard_normal((1, len(lens), Hq, 1, D))).to(DT[dtype]).cuda()
+    q2 = torch.tensor(rng.standard_normal((1, T, Hq, D))).to(DT[dtype]).cuda()
+    loc1 = ints([[[n - 1] for n in lens]])
+    loc2 = ints([[0] * front + [p for n, m in zip(lens, qt) for p in range(n - m, n)] + [0] * behind])
+    cu = ints(np.concatenate([[front], front + np.cumsum(qt)]))
+    return dict(q1=q1, q2=q2, loc1=loc1, loc2=loc2, cu=cu, frag1=ints([max(lens)]), frag2=ints([lens]), kc=kc, vc=vc, table=ints(table))
+
+
+def run_both(c, q1, q2):
+    from inference_lib_amd.attention import hogwild_paged_sdpa_q4, hogwild_varlen_paged_sdpa_q4
+    return (hogwild_paged_sdpa_q4(q1, c["loc1"], c["frag1"], c["kc"], c["vc"], c["table"], 0.1),
+            hogwild_varlen_paged_sdpa_q4(q2, c["loc2"], c["frag2"], c["kc"], c["vc"], c["table"], c["cu"], None, 0.1))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_decode_and_packed_in_one_graph(dtype):
+    c = decode_and_packed(np.random.default_rng(21), dtype)
+    q1, q2 = c["q1"].clone(), c["q2"].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run_both(c, q1, q2)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = run_both(c, q1, q2)
+    for r in range(4):
+        q1.copy_(c["q1"] * (r + 1)), q2.copy_(c["q2"] / (r + 1))
+        g.replay()
+        torch.cuda.synchronize()
+        got = [x.clone() for x in out]
+        for a, b in zip(got, run_both(c, q1, q2)):
+            assert torch.equal(a, b), r
+        assert (got[1][:3] == 0).all() and (got[1][-2:] == 0).all()
+
+
+@gpu
+def test_two_streams_at_once():
+    """The same calls on two streams without a wait between them, on inputs of their own."""
+    cs = [decode_and_packed(np.random.default_rng(s), "bf16") for s in (31, 32)]
+    want = [run_both(c, c["q1"], c["q2"]) for c in cs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cs]
+    got = [[], []]
+    for _ in range(10):
+        for c, s, g in zip(cs, streams, got):
+            with torch.cuda.stream(s):
+                g.append(run_both(c, c["q1"], c["q2"]))
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        for pair in g:
+            assert torch.equal(pair[0], w[0]) and torch.equal(pair[1], w[1])
+
+
+@gpu
 def test_offsets_beyond_32_bits():
     """The last page of a cache of more than 4 GiB (keys and values 4.5 GiB each)."""
     from inference_lib_amd.attention import copy_to_blocks_q4, hogwild_paged_sdpa_q4, read_blocks_q4

@@ -78,6 +78,32 @@ def test_plans_cover_the_rows(kw):
         assert pl.row_groups * 16 * pl.row_blocks * kw["W"] >= pl.rows
 
 
+def test_plans_of_random_problems():
+    import random
+    rng = random.Random(5)
+    for _ in range(3000):
+        Hkv = rng.choice([1, 2, 3, 8, 16])
+        kw = dict(W=rng.randint(1, 300), Hq=Hkv * rng.choice([1, 2, 5, 8]), Hkv=Hkv, Ev=rng.choice([64, 128, 256]), block_size=8 * rng.randint(1, 64))
+        kw["max_blocks"] = rng.randint(1, max(1, min(3000, (1 << 20) // kw["block_size"])))
+        if rng.random() < 0.5:
+            kw["S"] = rng.randint(1, 40)
+        else:
+            kw["total_q"] = rng.randint(1, 9000)
+        try:
+            pl = _lib.paged_plan(num_cus=256, q4=True, **kw)
+        except _lib.HogwildError:
+            assert (kw.get("total_q") or kw["W"] * kw["S"]) * kw["Hq"] // Hkv >= 1 << 14      # more workgroups than a launch takes
+            continue
+        rows = (kw.get("total_q") or kw["W"] * kw["S"]) * kw["Hq"] // Hkv
+        tiles = (kw["block_size"] * kw["max_blocks"] + 31) // 32
+        assert pl.rows == rows and pl.row_blocks in (1, 2) and (kw["Ev"] < 256 or pl.row_blocks == 1)
+        assert pl.workgroups == Hkv * pl.row_groups * pl.splits < 1 << 20
+        assert 1 <= pl.splits <= max(1, min(64, (tiles + 3) // 4)) and (tiles > 24 or pl.splits == 1 or tiles > 12)
+        assert pl.workspace_bytes >= Hkv * pl.splits * rows * (kw["Ev"] + 2) * 4
+        groups = kw["W"] * -(-kw["S"] * kw["Hq"] // Hkv // (16 * pl.row_blocks)) if "S" in kw else kw["W"] + rows // (16 * pl.row_blocks)
+        assert pl.row_groups >= min(groups, rows)
+
+
 def pool(**over):
     p = _lib.HwPool()
     p.W, p.max_blocks, p.num_blocks, p.block_size = 2, 3, 8, 16
