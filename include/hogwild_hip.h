@@ -331,7 +331,7 @@ int hw_read_blocks_q4(const hw_copy_blocks* c, void* stream);
    of themselves), bf16 results' weights too.  row_blocks: 0, 1 or 2 (1 at E == 256). */
 int hw_paged_q4_validate(const hw_paged_problem* p);
 int hw_paged_q4_plan_debug(const hw_paged_problem* p, int num_cus, hw_paged_plan* plan);   /* host only */
-int hw_paged_q4_workspace_bytes(const hw_paged_problem* p, size_t* bytes);
+int hw_paged_q4_workspace_bytes(const hw_paged_problem* p, size_t* bytes);   /* 0: none is needed (one split: short tables, or many rows) */
 int hw_paged_sdpa_q4(const hw_paged_problem* p, void* stream);
 int hw_varlen_paged_sdpa_q4(const hw_paged_problem* p, void* stream);
 

@@ -341,8 +341,11 @@ void run_paged(hw_paged_problem& p, const at::Tensor& out, bool varlen, bool q4 
     } else {
         check_status(hw_paged_workspace_bytes(&p, &bytes), "hw_paged_workspace_bytes");
     }
-    at::Tensor workspace = at::empty({(int64_t)(bytes > 0 ? bytes : 256)}, out.options().dtype(at::kByte));
-    p.workspace = workspace.data_ptr();
+    at::Tensor workspace;
+    if (!q4 || bytes > 0) {
+        workspace = at::empty({(int64_t)(bytes > 0 ? bytes : 256)}, out.options().dtype(at::kByte));
+        p.workspace = workspace.data_ptr();
+    }
     p.workspace_bytes = bytes;
     hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(out.device().index()).stream();
     if (q4)

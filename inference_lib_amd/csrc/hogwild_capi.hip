@@ -305,7 +305,8 @@ int paged_q4_run(const hw_paged_problem* p, void* stream_) {
     st = paged_q4_plan(p, cus, &plan);
     if (st != HW_OK) return st;
     if (plan.rows == 0) return HW_OK;       // no query tokens
-    if (p->workspace == nullptr || p->workspace_bytes < plan.workspace_bytes || !aligned16(p->workspace)) return HW_ERR_WORKSPACE;
+    const bool direct = plan.splits == 1;
+    if (!direct && (p->workspace == nullptr || p->workspace_bytes < plan.workspace_bytes || !aligned16(p->workspace))) return HW_ERR_WORKSPACE;
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     hw::PagedHeader ph;
     paged_header(p, plan, ph);
@@ -314,7 +315,6 @@ int paged_q4_run(const hw_paged_problem* p, void* stream_) {
     const size_t prows = (size_t)plan.splits * plan.rows;
     ph.part_ml = ph.part_o + (size_t)p->Hkv * prows * p->Ev;
     const bool shared = plan.splits > 1 && paged_shared(p, plan) && paged_q4_shares_save(p, plan, cus) >= 0 && p->workspace_bytes >= paged_call_bytes(p, plan);
-    const bool direct = plan.splits == 1;
     ph.flags = (plan.workgroups % 8 == 0 ? hw::PH_XCD_REMAP : 0) | (shared ? hw::PH_SHARED | paged_q4_shares_save(p, plan, cus) << hw::PH_SAVED_SHIFT : 0) |
                (direct ? hw::PH_DIRECT : 0);
     const hipError_t e = hw::launch_paged_q4(ph, p->out, p->lse, p->dtype, p->E, plan.row_blocks, stream);
@@ -833,7 +833,7 @@ int hw_paged_q4_workspace_bytes(const hw_paged_problem* p, size_t* bytes) {
     hw_paged_plan plan;
     st = paged_q4_plan(p, cus, &plan);
     if (st != HW_OK) return st;
-    *bytes = paged_call_bytes(p, plan);
+    *bytes = plan.splits == 1 ? 0 : paged_call_bytes(p, plan);      // (one workgroup for a row: it writes the results)
     return HW_OK;
 }
 
