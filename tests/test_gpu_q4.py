@@ -601,6 +601,38 @@ def test_decode_and_packed_in_one_graph(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("D,front,behind,splits", [(64, 0, 700, 0), (128, 333, 5, 0), (128, 40, 200, 2), (256, 1, 90, 3)])
+def test_batches_padded_to_a_fixed_size(D, front, behind, splits):
+    """Many query tokens of no sequence: zeros and lse -inf, and the others as without them."""
+    from inference_lib_amd import _lib
+    rng = np.random.default_rng(front + behind)
+    lens, qt, Hq, Hkv, block = [300, 17, 90], [33, 1, 0], 6, 2, 8
+    table, P = pool(rng, lens, block)
+    kc, vc = (torch.tensor(random_cache(rng, P, Hkv, block, D, x, "bf16")).cuda() for x in (True, False))
+    T = front + sum(qt) + behind
+    q = torch.tensor(rng.standard_normal((1, T, Hq, D))).to(torch.bfloat16).cuda()
+    loc = [p for n, m in zip(lens, qt) for p in range(n - m, n)]
+
+    def call(q, loc, cu):
+        out = torch.full((q.size(1), Hq, D), float("nan"), dtype=torch.bfloat16, device="cuda")
+        lse = torch.full((q.size(1), Hq), float("nan"), device="cuda")
+        _lib.PagedProblem(q=q.contiguous(), locations=ints([loc]), fragment_lengths=ints([lens]), key_cache=kc, value_cache=vc, block_table=ints(table), scale=0.1,
+                          out=out, lse=lse, cu_seqlens_q=ints(cu), splits=splits, q4=True).run()
+        return out, lse
+
+    cu = np.concatenate([[0], np.cumsum(qt)])
+    out, lse = call(q, [5] * front + loc + [7] * behind, cu + front)
+    seen = slice(front, front + sum(qt))
+    for x, none in ((out, 0.0), (lse, -np.inf)):
+        assert (x[:front] == none).all() and (x[T - behind:] == none).all()
+    alone, alone_lse = call(q[:, seen], loc, cu)
+    if splits:
+        assert torch.equal(out[seen], alone) and torch.equal(lse[seen], alone_lse)
+    else:                                            # (another number of workgroups: another order of the sums, and both are rounded)
+        assert (np.abs(np64(out[seen]) - np64(alone)) <= 2 * 2.0 ** -8 * np.abs(np64(alone)) + 1e-3).all() and torch.isfinite(lse[seen]).all()
+
+
+@gpu
 def test_two_streams_at_once():
     """The same calls on two streams without a wait between them, on inputs of their own."""
     cs = [decode_and_packed(np.random.default_rng(s), "bf16") for s in (31, 32)]
