@@ -56,6 +56,7 @@ __global__ __launch_bounds__(512) void fork_kernel(const PoolArgs a, const void*
         a.table[(size_t)w * a.max_blocks + j0 + c] = is;
     }
     if (gridDim.x == 1) {                // (otherwise other workgroups still read them: fork_lengths_kernel)
+        __syncthreads();                 // the pages' numbers make room for the lengths only when every wave has used them
         for (int w0 = 0; w0 < a.W; w0 += nt) {
             const int w = w0 + tid;
             if (w < a.W) held[w] = par[w] >= 0 ? a.lengths[par[w]] : 0;
