@@ -369,8 +369,11 @@ int hw_free_blocks(const hw_pool* p, const uint8_t* finished, void* stream);
 
 /*
  * Room for n_new[w] (device int32 [W]) more tokens of every sequence, whose lengths grow by that.  A sequence wants the pages that its row
- * lacks for positions length .. length + n_new - 1, and a copy of the page of its next token where that holds tokens already and is
- * named by others too -- all but the last of several sequences that ask for that page.  The wants of the sequences in their
+ * lacks for positions length .. length + n_new - 1, and a page of its own for each of them that others name too: a copy of the page of
+ * its next token where that holds tokens of it already -- all but the last of several sequences that ask for that page -- and a free one in
+ * the place of a page that holds none (lengths may be shortened between calls, also of sequences that share pages).  Pages
+ * behind the last new token's, up to the first that others do not name, are given up, so that a batch padded to more tokens than a sequence
+ * asked for writes nobody else's.  The wants of the sequences in their
  * order, of one by position, get the free pages in ascending order.  From the first sequence on whose wants the free pages do
  * not cover, no sequence that wants a page or is to write a shared one gets any: all or nothing for each.  positions[w] (device
  * int32 [W], written) = the first new token's position; for a sequence that gets nothing, asks for none or would outgrow its row,

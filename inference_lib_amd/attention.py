@@ -252,8 +252,8 @@ def free_blocks(block_table: torch.Tensor, seq_lengths: torch.Tensor, ref_counts
 
 def reserve_blocks(block_table: torch.Tensor, seq_lengths: torch.Tensor, ref_counts: torch.Tensor, n_new: torch.Tensor,
                    caches: Sequence[torch.Tensor], block_size: int, positions: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Pages for n_new[w] (int32 [W]) more tokens of every sequence: those its row lacks, and a copy (in all `caches`) of a shared page
-    that is about to be written.  Returns positions [W], where the new tokens go (the lengths so far); a sequence that gets
+    """Pages for n_new[w] (int32 [W]) more tokens of every sequence: those its row lacks, a copy (in all `caches`) of a shared page that is
+    about to be written, and a free one in the place of a shared page behind the sequence's tokens.  Returns positions [W], where the new tokens go (the lengths so far); a sequence that gets
     nothing has block_size * max_blocks there, which the appends leave out, and keeps its length (see hw_reserve_blocks)."""
     if positions is None:
         positions = torch.empty_like(seq_lengths)

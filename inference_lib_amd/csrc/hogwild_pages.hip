@@ -93,16 +93,20 @@ __device__ __forceinline__ int wave_base(int mine, int* lds, int wv, int lane, i
 }
 
 // Pages for n_new[w] more tokens of every sequence w: those that its row lacks from the page of its next token to that of its last
-// one, and, where the page of the next token holds tokens already and other rows name it as well, a copy of it (the last of the
-// rows that are about to write a page keeps it).  The pages that the rows want, row by row and in a row by position, get the free pages
-// in ascending order; the first row whose wants go beyond the free pages gets none, and neither do the rows behind it that want
-// any or keep a shared page.  positions[w] = where the new tokens go, or, for a row that gets nothing or asks for nothing, a position
-// behind the table (which the appends leave out).  Sixteen lanes to a row.
+// one, and one in the place of each of them that other rows name as well.  Where the page of the next token holds tokens of the row already
+// it is copied (the last of the rows that are about to write a page keeps it); the others hold none of its tokens (a length that was
+// shortened), and neither do those behind the last new token, which the row gives up as far as others name them.  The pages that
+// the rows want, row by row and in a row by position, get the free pages in ascending order; the first row whose wants go beyond the free
+// pages gets none, and neither do the rows behind it that want any or keep a shared page.  positions[w] = where the new tokens go, or, for
+// a row that gets nothing or asks for nothing, a position behind the table (which the appends leave out).  Sixteen lanes to a row.
+// Counts are lowered as pages are given up where nothing depends on them any more: at once, or (a row wants a page only because others name it)
+// after all wants are served, from the pages that then stand in the list of the free ones.
 __global__ __launch_bounds__(POOL_THREADS) void reserve_kernel(const PoolArgs a, const int* n_new, int* positions, int* ws) {
     __shared__ int page[POOL_MAX_ROWS];      // the shared page that row w is about to write, or -1
     __shared__ int need[POOL_MAX_ROWS];      // pages wanted; then the wants of all rows up to this one
+    __shared__ int behind[POOL_MAX_ROWS];    // pages behind the last new token that the row gives up
     __shared__ int scan[POOL_WAVES];
-    __shared__ int copies;
+    __shared__ int copies, spare;            // spare: pages are given up that hold no tokens of their row
     int* const list = ws + POOL_WS_HEADER;
     int* const pairs = list + a.num_blocks;
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -114,7 +118,8 @@ __global__ __launch_bounds__(POOL_THREADS) void reserve_kernel(const PoolArgs a,
         for (int d = 1; d < 16; d <<= 1) v += __shfl_xor(v, d, 64);
         return v;
     };
-    if (tid == 0) copies = 0;
+    if (tid == 0) copies = spare = 0;
+    __syncthreads();
     struct Row {
         int len, nn, first, last;
         bool grows;
@@ -130,19 +135,39 @@ __global__ __launch_bounds__(POOL_THREADS) void reserve_kernel(const PoolArgs a,
     };
     for (int w = g16; w < a.W; w += rows) {
         const Row r = row_of(w);
-        int miss = 0, p0 = -1;
+        int miss = 0, p0 = -1, give = 0;
         if (r.grows) {
             const int* row = a.table + (size_t)w * a.max_blocks;
-            for (int j = r.first + l16; j <= r.last; j += 16) miss += valid(row[j]) ? 0 : 1;
-            if (r.len % a.block_size != 0) {
-                p0 = row[r.first];
-                if (!valid(p0) || a.refs[p0] <= 1) p0 = -1;
+            const bool holds = r.len % a.block_size != 0;
+            int e = r.last + 1 + l16 < a.max_blocks ? row[r.last + 1 + l16] : -1;
+            for (int j = r.first + l16; j <= r.last; j += 16) {
+                const int p = row[j];
+                if (!valid(p)) {
+                    ++miss;
+                } else if (a.refs[p] > 1) {
+                    if (holds && j == r.first) {
+                        p0 = p;
+                    } else {
+                        ++miss;
+                        spare = 1;
+                    }
+                }
+            }
+            for (int j = r.last + 1 + l16;;) {
+                const bool shared = valid(e) && a.refs[e] > 1;
+                const int run = __builtin_ctz(~((unsigned)(__ballot(shared) >> (lane & 48)) & 0xffffu));
+                give += run;
+                if (run < 16) break;
+                j += 16;
+                e = j < a.max_blocks ? row[j] : -1;
             }
         }
         miss = sum16(miss);
         if (l16 == 0) {
             page[w] = p0;
             need[w] = miss;
+            behind[w] = give;
+            if (give > 0) spare = 1;
         }
     }
     __syncthreads();
@@ -198,36 +223,73 @@ __global__ __launch_bounds__(POOL_THREADS) void reserve_kernel(const PoolArgs a,
         at += __popcll(bits);
     }
     __syncthreads();
+    const bool later = spare != 0;
+    struct Grant {
+        int before, sofar;
+        bool copy, granted;
+    };
+    auto grant_of = [&](int w, const Row& r) {
+        Grant g;
+        g.sofar = need[w] & (COPY - 1);
+        g.before = w > 0 ? need[w - 1] & (COPY - 1) : 0;
+        g.copy = (need[w] & COPY) != 0;
+        g.granted = r.grows && ((g.sofar == g.before && page[w] < 0) || g.sofar <= n_free);
+        return g;
+    };
+    auto finish = [&](int w, const Row& r, bool granted) {
+        if (l16 == 0) {
+            positions[w] = granted ? r.len : cap;
+            if (granted) a.lengths[w] = r.len + r.nn;
+        }
+    };
     for (int w = g16; w < a.W; w += rows) {
         const Row r = row_of(w);
-        const int sofar = need[w] & (COPY - 1), before = w > 0 ? need[w - 1] & (COPY - 1) : 0;
-        const bool copy = (need[w] & COPY) != 0;
-        const bool granted = r.grows && ((sofar == before && page[w] < 0) || sofar <= n_free);
-        if (granted) {
+        const Grant g = grant_of(w, r);
+        if (g.granted) {
             int* row = a.table + (size_t)w * a.max_blocks;
-            int next = before;
-            for (int j0 = r.first; j0 <= r.last && next < sofar; j0 += 16) {
+            const bool holds = r.len % a.block_size != 0;
+            int next = g.before;
+            for (int j0 = r.first; j0 <= r.last && next < g.sofar; j0 += 16) {
                 const int j = j0 + l16;
-                const bool moved = copy && j == r.first;
-                const bool want = j <= r.last && (moved || !valid(row[min(j, r.last)]));
+                const bool moved = g.copy && j == r.first;
+                const int old = row[min(j, r.last)];
+                const bool want = j <= r.last && (moved || !valid(old) || (later && !(holds && j == r.first) && a.refs[old] > 1));
                 const unsigned bits = (unsigned)(__ballot(want) >> (lane & 48)) & 0xffffu;
                 if (want) {
-                    const int fresh = list[next + __popc(bits & ((1u << l16) - 1))];
+                    int* const slot = list + next + __popc(bits & ((1u << l16) - 1));
+                    const int fresh = *slot;
                     row[j] = fresh;
                     a.refs[fresh] = 1;
+                    if (later) *slot = valid(old) ? -2 - old : -1;
+                    else if (moved) atomicSub(a.refs + old, 1);
                     if (moved) {
-                        atomicSub(a.refs + page[w], 1);
                         const int k = atomicAdd(&copies, 1);
-                        pairs[2 * k] = page[w];
+                        pairs[2 * k] = old;
                         pairs[2 * k + 1] = fresh;
                     }
                 }
                 next += __popc(bits);
             }
         }
-        if (l16 == 0) {
-            positions[w] = granted ? r.len : cap;
-            if (granted) a.lengths[w] = r.len + r.nn;
+        if (!later) finish(w, r, g.granted);
+    }
+    if (later) {
+        __syncthreads();
+        for (int i = tid; i < listed; i += POOL_THREADS) {
+            const int old = -2 - list[i];
+            if (old >= 0) atomicSub(a.refs + old, 1);
+        }
+        for (int w = g16; w < a.W; w += rows) {
+            const Row r = row_of(w);
+            const bool granted = grant_of(w, r).granted;
+            if (granted) {
+                int* row = a.table + (size_t)w * a.max_blocks + r.last + 1;
+                for (int j = l16; j < behind[w]; j += 16) {
+                    atomicSub(a.refs + row[j], 1);
+                    row[j] = -1;
+                }
+            }
+            finish(w, r, granted);
         }
     }
     __syncthreads();

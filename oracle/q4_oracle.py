@@ -144,6 +144,8 @@ def reserve(table: np.ndarray, lengths: np.ndarray, refs: np.ndarray, n_new: Seq
     positions = np.full(W, n * block_size, np.int32)
     copies: List[Tuple[int, int]] = []
     start_refs, start_table = refs.copy(), table.copy()
+    named = lambda w, j: 0 <= start_table[w, j] < P      # noqa: E731
+    shared = lambda w, j: named(w, j) and start_refs[start_table[w, j]] > 1      # noqa: E731
     short = False                               # some sequence's wants were not covered
     taken = 0
     for w in range(W):
@@ -152,24 +154,30 @@ def reserve(table: np.ndarray, lengths: np.ndarray, refs: np.ndarray, n_new: Seq
             continue
         first, last = length // block_size, (length + m - 1) // block_size
         p0 = int(start_table[w, first])
-        shared = length % block_size != 0 and 0 <= p0 < P and start_refs[p0] > 1
+        holds = length % block_size != 0        # the first page holds tokens of this sequence already
         copy = False
-        if shared:
+        if holds and shared(w, first):
             left.setdefault(p0, int(start_refs[p0]) - 1)
             copy = left[p0] > 0
             left[p0] -= 1
-        want = [j for j in range(first, last + 1) if not 0 <= start_table[w, j] < P or (copy and j == first)]
+        want = [j for j in range(first, last + 1) if not named(w, j) or (copy if holds and j == first else shared(w, j))]
         taken += len(want)
         short = short or taken > len(free)
-        if (want or shared) and short:
+        if (want or (holds and shared(w, first))) and short:
             continue
         for k, j in enumerate(want):
             fresh = free[taken - len(want) + k]
+            if named(w, j):
+                refs[start_table[w, j]] -= 1
             refs[fresh] = 1
             if copy and j == first:
-                refs[p0] -= 1
                 copies.append((p0, fresh))
             table[w, j] = fresh
+        for j in range(last + 1, n):            # pages behind the new tokens, as far as others name them as well
+            if not shared(w, j):
+                break
+            refs[start_table[w, j]] -= 1
+            table[w, j] = -1
         positions[w] = length
         lengths[w] = length + m
     return positions, copies
