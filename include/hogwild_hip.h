@@ -420,6 +420,10 @@ int hw_build_inputs_dev(int32_t* locations, float* cosines, float* sines, const 
 /* len_dev[f] += add[f] for f < F <= HW_MAX_LAUNCH_FRAGMENTS (add is a HOST array): the first node of a captured decode step. */
 int hw_advance_lengths(int32_t* len_dev, const int32_t* add, int F, void* stream);
 
+/* *id = a number of its own for the capture that `stream` is in, 0 where it is in none: what a caller computes once for several calls
+   of a step is good for one capture only (a graph that holds a tensor made outside of it reads it when it is gone or out of date). */
+int hw_stream_capture_id(void* stream, unsigned long long* id);
+
 #define HW_ROPE_EAGER 0   /* every product and the sum rounded as an eager tensor expression rounds them: bit-identical to
                              apply_rotary_pos_emb of the reference on the same dtypes */
 #define HW_ROPE_FUSED 1   /* fp32 fused multiply-add, one rounding at the end */

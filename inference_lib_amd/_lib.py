@@ -28,7 +28,7 @@ EXPORTS = [
     "hw_fused_attention", "hw_fused_attention_stages", "hw_sdpa", "hw_rope", "hw_device_cus",
     "hw_paged_validate", "hw_paged_plan_debug", "hw_paged_workspace_bytes", "hw_paged_sdpa", "hw_varlen_paged_sdpa",
     "hw_paged_sdpa_stages", "hw_copy_to_blocks", "hw_build_inputs", "hw_rope_append",
-    "hw_build_inputs_dev", "hw_advance_lengths", "hw_fused_attention_static", "hw_sdpa_workspace_bytes",
+    "hw_build_inputs_dev", "hw_advance_lengths", "hw_stream_capture_id", "hw_fused_attention_static", "hw_sdpa_workspace_bytes",
     "hw_merge_segments",
     "hw_copy_to_blocks_q4", "hw_read_blocks_q4", "hw_paged_q4_validate", "hw_paged_q4_plan_debug", "hw_paged_q4_workspace_bytes",
     "hw_paged_sdpa_q4", "hw_varlen_paged_sdpa_q4",
@@ -167,6 +167,7 @@ def _load() -> C.CDLL:
     lib.hw_build_inputs_dev.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.POINTER(C.c_int32), C.c_void_p, C.c_float,
                                         C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p]
     lib.hw_advance_lengths.argtypes = [C.c_void_p, C.POINTER(C.c_int32), C.c_int, C.c_void_p]
+    lib.hw_stream_capture_id.argtypes = [C.c_void_p, C.POINTER(C.c_ulonglong)]
     lib.hw_copy_to_blocks_q4.argtypes = [C.POINTER(HwCopyBlocks), C.c_void_p]
     lib.hw_read_blocks_q4.argtypes = [C.POINTER(HwCopyBlocks), C.c_void_p]
     lib.hw_paged_q4_validate.argtypes = [C.POINTER(HwPagedProblem)]
@@ -685,6 +686,18 @@ def compact_blocks(block_table, ref_counts, caches, used) -> None:
         raise ValueError("used must be one number")
     pool.check_ints(used)
     pool.run(lib.hw_compact_blocks, used.data_ptr(), workspace=True)
+
+
+def capture_id(device: torch.device) -> int:
+    """A number of its own for the graph capture that the device's current stream is in, 0 outside of any."""
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return capture_id(device)
+    if not torch.cuda.is_current_stream_capturing():
+        return 0
+    n = C.c_ulonglong(0)
+    check(lib.hw_stream_capture_id(C.c_void_p(torch.cuda.current_stream(device).cuda_stream), C.byref(n)), "hw_stream_capture_id")
+    return n.value
 
 
 def copy_blocks(caches: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int]) -> None:

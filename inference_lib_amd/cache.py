@@ -402,7 +402,7 @@ class PagedCache:
     counts live in device memory and are worked on there, so a step (reserve, then update and attend of every layer) can be
     captured in a graph and replayed while the sequences grow.
 
-        cache.reserve(S)                                 # room for S tokens of every sequence (or a number for each, int32 [max_seqs])
+        cache.reserve(S)                                 # room for S tokens of every sequence (or a number up to S for each, int32 [max_seqs])
         for layer in ...:
             cache.update(k, v, layer)                    # [max_seqs, Hkv, S, D], keys rotated
             out = cache.attend(q, layer, scale)          # [max_seqs, Hq, S, D], queries rotated; new tokens see each other causally
@@ -410,7 +410,10 @@ class PagedCache:
         cache.free(finished); cache.compact()            # pages in use to the front of the pool
 
     A sequence that `reserve` has nothing for (the pool or its row of the table is full, or it asked for no tokens) is left out of the
-    step: its states are not written, its output is 0 and its length stays; `granted()` says which ones took part."""
+    step: its states are not written, its output is 0 and its length stays; `granted()` says which ones took part.  Tokens behind those
+    that a sequence asked for get 0 too; no other sequence sees their states.
+
+    Every part of a step may be in a graph of its own or in none."""
 
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, num_blocks: int, max_seqs: int, *, block_size: int = 16,
                  max_blocks: Optional[int] = None, bits: int = 16, dtype=torch.bfloat16, device="cuda"):
@@ -428,10 +431,11 @@ class PagedCache:
         ints = dict(dtype=torch.int32, device=device)
         self.block_table = torch.full((max_seqs, max_blocks), -1, **ints)
         self.seq_lengths, self.ref_counts = torch.zeros(max_seqs, **ints), torch.zeros(num_blocks, **ints)
-        self.positions = torch.zeros(max_seqs, **ints)
+        self.positions = torch.full((max_seqs,), max_blocks * self.block_size, **ints)
         self.used = torch.zeros(1, **ints)
         self._longest = torch.full((1,), max_blocks * self.block_size, **ints)
-        self._locations: Dict[int, torch.Tensor] = {}
+        self._made: Dict[tuple, torch.Tensor] = {}       # locations, by capture and number of tokens
+        self._replayed = False                           # whether a graph holds a reserve
 
     @property
     def caches(self) -> List[torch.Tensor]:
@@ -441,8 +445,24 @@ class PagedCache:
         """Positions [max_seqs] of the first new token of every sequence (see attention.reserve_blocks)."""
         if not isinstance(n_new, torch.Tensor):
             n_new = torch.full_like(self.seq_lengths, int(n_new))
-        self._locations = {}
+        self._made = {}
+        self._replayed |= self._capture() != 0
         return _ops.reserve_blocks(self.block_table, self.seq_lengths, self.ref_counts, n_new, self.caches, self.block_size, self.positions)
+
+    def _capture(self) -> int:
+        return _lib.capture_id(self.positions.device) if self.positions.is_cuda else 0
+
+    def _locations(self, S: int) -> torch.Tensor:
+        """Where the new tokens of this step stand, int32 [1, max_seqs, S], -1 for those that nobody asked for: made once for all layers.  Not
+        kept from outside a capture for what is captured, as the graph would read the tensor of that step for ever, from capture to
+        capture, nor for eager layers once a graph holds a reserve, as a replay moves the positions unseen."""
+        capture = self._capture()
+        loc = self._made.get((capture, S)) if capture != 0 or not self._replayed else None
+        if loc is None:
+            at = self.positions[:, None] + torch.arange(S, dtype=torch.int32, device=self.positions.device)
+            loc = torch.where(at < self.seq_lengths[:, None], at, -1).unsqueeze(0)      # (who got nothing: behind any length)
+            self._made[(capture, S)] = loc
+        return loc
 
     def granted(self) -> torch.Tensor:
         """Which sequences got room in the last reserve, bool [max_seqs] on the device."""
@@ -453,14 +473,8 @@ class PagedCache:
         append(key_states, value_states, self.keys[layer_idx], self.values[layer_idx], self.block_table, self.positions)
 
     def attend(self, queries: torch.Tensor, layer_idx: int, scale: float) -> torch.Tensor:
-        S = queries.size(2)
-        loc = self._locations.get(S)
-        if loc is None:          # (the same for all layers of a step)
-            steps = torch.arange(S, dtype=torch.int32, device=self.positions.device)
-            loc = torch.where(self.granted()[:, None], self.positions[:, None] + steps[None, :], -1).unsqueeze(0).contiguous()
-            self._locations[S] = loc
         sdpa = _ops.hogwild_paged_sdpa_q4 if self.bits == 4 else _ops.hogwild_paged_sdpa
-        return sdpa(queries.unsqueeze(0), loc, self._longest, self.keys[layer_idx], self.values[layer_idx], self.block_table, scale)
+        return sdpa(queries.unsqueeze(0), self._locations(queries.size(2)), self._longest, self.keys[layer_idx], self.values[layer_idx], self.block_table, scale)
 
     def fork(self, parents: torch.Tensor) -> None:
         _ops.fork_blocks(self.block_table, self.seq_lengths, self.ref_counts, parents, self.block_size)

@@ -880,6 +880,15 @@ int hw_build_inputs_dev(int32_t* locations, float* cosines, float* sines, const 
 
 int hw_advance_lengths(int32_t* len_dev, const int32_t* add, int F, void* stream) { return advance_lengths_run(len_dev, add, F, stream); }
 
+int hw_stream_capture_id(void* stream, unsigned long long* id) {
+    if (id == nullptr) return HW_ERR_NULL;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long n = 0;
+    const hipError_t e = hipStreamGetCaptureInfo(reinterpret_cast<hipStream_t>(stream), &status, &n);
+    *id = e == hipSuccess && status == hipStreamCaptureStatusActive ? n : 0;
+    return (int)e;
+}
+
 int hw_merge_segments(const hw_merge_segments_args* a, void* stream) { return merge_segments_run(a, stream); }
 
 int hw_rope_append(const hw_append* a, void* stream) { return rope_append_run(a, stream); }
