@@ -411,16 +411,24 @@ class PagedCache:
 
     A sequence that `reserve` has nothing for (the pool or its row of the table is full, or it asked for no tokens) is left out of the
     step: its states are not written, its output is 0 and its length stays; `granted()` says which ones took part.  Tokens behind those
-    that a sequence asked for get 0 too; no other sequence sees their states.
+    that a sequence asked for get 0 too; no other sequence sees their states.  A sequence has at most max_blocks pages: by default as many as
+    the pool, or as the attention takes (2^20 positions).
 
     Every part of a step may be in a graph of its own or in none."""
+
+    MAX_POSITIONS, MAX_BLOCK_SIZE = 1 << 20, 1 << 12         # of hw_paged_sdpa and hw_paged_sdpa_q4
 
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, num_blocks: int, max_seqs: int, *, block_size: int = 16,
                  max_blocks: Optional[int] = None, bits: int = 16, dtype=torch.bfloat16, device="cuda"):
         if bits not in (4, 16, 32) or (bits != 4 and torch.empty((), dtype=dtype).element_size() * 8 != bits):
             raise ValueError(f"bits must be 4, or the size of {dtype}")
         self.bits, self.block_size, self.dtype = bits, int(block_size), dtype
-        max_blocks = int(num_blocks if max_blocks is None else max_blocks)
+        if not 1 <= self.block_size < self.MAX_BLOCK_SIZE:
+            raise ValueError(f"block_size must be 1 .. {self.MAX_BLOCK_SIZE - 1}")
+        most = self.MAX_POSITIONS // self.block_size
+        max_blocks = min(int(num_blocks), most) if max_blocks is None else int(max_blocks)
+        if not 1 <= max_blocks <= most:
+            raise ValueError(f"max_blocks must be 1 .. {most}: a sequence of {max_blocks} blocks of {self.block_size} is beyond the {self.MAX_POSITIONS} positions that the attention takes, or has none")
 
         def one():
             if bits == 4:

@@ -167,3 +167,32 @@ def test_steps_with_a_part_of_them_in_a_graph(bits, S, inside):
             assert torch.equal(layers(eager, other), layers(captured, other))
         del junk
     assert eager.seq_lengths.tolist() == captured.seq_lengths.tolist()
+
+
+def test_tables_stay_within_what_attention_takes():
+    """A row of a table has at most 2^20 positions (hw_paged_problem): the default table of a larger pool too."""
+    make = lambda n, block, **kw: C.PagedCache(1, 1, 64, n, 2, block_size=block, bits=4, device="cpu", **kw)      # noqa: E731
+    for n, block in ((70000, 16), (4, 16), (131073, 8), (9, 4088)):
+        cache = make(n, block)
+        assert cache.block_table.shape == (2, min(n, (1 << 20) // block))
+        assert int(cache._longest) == cache.block_table.size(1) * block <= 1 << 20
+    assert make(4, 16, max_blocks=65536).block_table.size(1) == 65536          # (a row may be longer than the pool)
+    for kw in (dict(n=4, block=16, max_blocks=65537), dict(n=4, block=16, max_blocks=0), dict(n=4, block=4096), dict(n=4, block=16, max_blocks=-1)):
+        with pytest.raises(ValueError, match="position|block_size"):
+            make(**kw)
+
+
+@gpu
+@pytest.mark.parametrize("bits", [4, 16])
+def test_a_pool_of_more_pages_than_a_row_takes(bits):
+    cache = C.PagedCache(1, 1, 64, 70000, 2, block_size=16, bits=bits)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    k, v, q = (torch.randn((2, h, 20, 64), generator=gen, device="cuda").to(torch.bfloat16) for h in (1, 1, 4))
+    cache.reserve(20)
+    cache.update(k, v, 0)
+    out = cache.attend(q, 0, 0.1)
+    small = C.PagedCache(1, 1, 64, 7, 2, block_size=16, bits=bits)
+    small.reserve(20)
+    small.update(k, v, 0)
+    # (another number of workgroups: another order of sums, both rounded to bf16)
+    assert (out.float() - small.attend(q, 0, 0.1).float()).abs().max() <= 2 * 2.0 ** -8 * float(v.abs().max())
