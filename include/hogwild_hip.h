@@ -377,7 +377,7 @@ int hw_free_blocks(const hw_pool* p, const uint8_t* finished, void* stream);
  * order, of one by position, get the free pages in ascending order.  From the first sequence on whose wants the free pages do
  * not cover, no sequence that wants a page or is to write a shared one gets any: all or nothing for each.  positions[w] (device
  * int32 [W], written) = the first new token's position; for a sequence that gets nothing, asks for none or would outgrow its row,
- * block_size * max_blocks, which the appends leave out, and its length stays.
+ * block_size * max_blocks, which the appends leave out, and its length stays.  positions are not seq_lengths (HW_ERR_SHAPE).
  */
 int hw_reserve_blocks(const hw_pool* p, const int32_t* n_new, int32_t* positions, void* stream);
 

@@ -448,6 +448,9 @@ int reserve_run(const hw_pool* p, const int32_t* n_new, int32_t* positions, void
     if (st != HW_OK) return st;
     if (n_new == nullptr || positions == nullptr) return HW_ERR_NULL;
     if (p->workspace == nullptr || p->workspace_bytes < pool_bytes(p)) return HW_ERR_WORKSPACE;
+    // (the lengths grow: in their place the positions would be lost)
+    const uintptr_t at = reinterpret_cast<uintptr_t>(positions), len = reinterpret_cast<uintptr_t>(p->seq_lengths), bytes = (uintptr_t)p->W * sizeof(int32_t);
+    if (at < len + bytes && len < at + bytes) return HW_ERR_SHAPE;
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     int* ws = reinterpret_cast<int*>(p->workspace);
     const hipError_t e = hw::launch_reserve(a, n_new, positions, ws, stream);

@@ -110,3 +110,12 @@ def test_a_pool_whose_lengths_are_shortened_goes_the_way_of_the_oracle_s(seed, W
             assert int(used) == want
         same((t, l, r, c), (table, lengths, refs, data), (step, kind))
         assert (np.bincount(table[table >= 0], minlength=P) == refs).all()
+
+
+@gpu
+def test_positions_in_the_place_of_the_lengths_are_refused():
+    from inference_lib_amd import attention as A
+    t, l, r = ints([[0, -1]]), ints([3]), ints([1, 0])
+    with pytest.raises(RuntimeError):
+        A.reserve_blocks(t, l, r, ints([1]), [], 8, positions=l)
+    assert l.tolist() == [3] and A.reserve_blocks(t, l, r, ints([1]), [], 8).tolist() == [3] and l.tolist() == [4]
