@@ -16,6 +16,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "hogwild_kernels.h"
 #include "hogwild_device.h"
 
@@ -99,14 +101,14 @@ __device__ __forceinline__ int wave_base(int mine, int* lds, int wv, int lane, i
 // the rows want, row by row and in a row by position, get the free pages in ascending order; the first row whose wants go beyond the free
 // pages gets none, and neither do the rows behind it that want any or keep a shared page.  positions[w] = where the new tokens go, or, for
 // a row that gets nothing or asks for nothing, a position behind the table (which the appends leave out).  Sixteen lanes to a row.
-// Counts are lowered as pages are given up where nothing depends on them any more: at once, or (a row wants a page only because others name it)
-// after all wants are served, from the pages that then stand in the list of the free ones.
+// A count is lowered at once where nothing depends on it any more; where a row wants a page only because others name its own, after
+// all wants are served, by the pages that then stand in the list of the free ones.
 __global__ __launch_bounds__(POOL_THREADS) void reserve_kernel(const PoolArgs a, const int* n_new, int* positions, int* ws) {
     __shared__ int page[POOL_MAX_ROWS];      // the shared page that row w is about to write, or -1
     __shared__ int need[POOL_MAX_ROWS];      // pages wanted; then the wants of all rows up to this one
     __shared__ int behind[POOL_MAX_ROWS];    // pages behind the last new token that the row gives up
     __shared__ int scan[POOL_WAVES];
-    __shared__ int copies, spare;            // spare: pages are given up that hold no tokens of their row
+    __shared__ int copies, spare;            // spare: some row gives up pages that hold no tokens of it
     int* const list = ws + POOL_WS_HEADER;
     int* const pairs = list + a.num_blocks;
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -139,27 +141,26 @@ __global__ __launch_bounds__(POOL_THREADS) void reserve_kernel(const PoolArgs a,
         if (r.grows) {
             const int* row = a.table + (size_t)w * a.max_blocks;
             const bool holds = r.len % a.block_size != 0;
-            int e = r.last + 1 + l16 < a.max_blocks ? row[r.last + 1 + l16] : -1;
-            for (int j = r.first + l16; j <= r.last; j += 16) {
-                const int p = row[j];
-                if (!valid(p)) {
-                    ++miss;
-                } else if (a.refs[p] > 1) {
-                    if (holds && j == r.first) {
-                        p0 = p;
-                    } else {
-                        ++miss;
-                        spare = 1;
-                    }
-                }
+            bool there = false;              // pages without tokens of the row, up to the entry behind the last one
+            for (int j = r.first + l16; j <= min(r.last + 1, a.max_blocks - 1); j += 16) {
+                const bool is = valid(row[j]);
+                miss += j <= r.last && !is ? 1 : 0;
+                there |= is && !(holds && j == r.first);
             }
-            for (int j = r.last + 1 + l16;;) {
-                const bool shared = valid(e) && a.refs[e] > 1;
-                const int run = __builtin_ctz(~((unsigned)(__ballot(shared) >> (lane & 48)) & 0xffffu));
-                give += run;
-                if (run < 16) break;
-                j += 16;
-                e = j < a.max_blocks ? row[j] : -1;
+            if (holds) {
+                p0 = row[r.first];
+                if (!valid(p0) || a.refs[p0] <= 1) p0 = -1;
+            }
+            if (((__ballot(there) >> (lane & 48)) & 0xffffu) != 0) {      // (rows that were filled ahead or shortened): which do others name?
+                auto shared = [&](int j) { return valid(row[j]) && a.refs[row[j]] > 1; };
+                int more = 0, run = 16;
+                for (int j = r.first + l16; j <= r.last; j += 16) more += !(holds && j == r.first) && shared(j) ? 1 : 0;
+                for (int j = r.last + 1 + l16; run == 16; j += 16) {
+                    run = __builtin_ctz(~((unsigned)(__ballot(j < a.max_blocks && shared(j)) >> (lane & 48)) & 0xffffu));
+                    give += run;
+                }
+                miss += more;
+                if (more + give > 0) spare = 1;
             }
         }
         miss = sum16(miss);
@@ -167,10 +168,10 @@ __global__ __launch_bounds__(POOL_THREADS) void reserve_kernel(const PoolArgs a,
             page[w] = p0;
             need[w] = miss;
             behind[w] = give;
-            if (give > 0) spare = 1;
         }
     }
     __syncthreads();
+    const bool later = spare != 0;
     constexpr int COPY = 1 << 30;            // (needs are at most the columns of the table, below 2^30)
     for (int w = g16; w < a.W; w += rows) {
         const int p0 = page[w];
@@ -223,7 +224,6 @@ __global__ __launch_bounds__(POOL_THREADS) void reserve_kernel(const PoolArgs a,
         at += __popcll(bits);
     }
     __syncthreads();
-    const bool later = spare != 0;
     struct Grant {
         int before, sofar;
         bool copy, granted;
@@ -242,38 +242,45 @@ __global__ __launch_bounds__(POOL_THREADS) void reserve_kernel(const PoolArgs a,
             if (granted) a.lengths[w] = r.len + r.nn;
         }
     };
-    for (int w = g16; w < a.W; w += rows) {
-        const Row r = row_of(w);
-        const Grant g = grant_of(w, r);
-        if (g.granted) {
-            int* row = a.table + (size_t)w * a.max_blocks;
-            const bool holds = r.len % a.block_size != 0;
-            int next = g.before;
-            for (int j0 = r.first; j0 <= r.last && next < g.sofar; j0 += 16) {
-                const int j = j0 + l16;
-                const bool moved = g.copy && j == r.first;
-                const int old = row[min(j, r.last)];
-                const bool want = j <= r.last && (moved || !valid(old) || (later && !(holds && j == r.first) && a.refs[old] > 1));
-                const unsigned bits = (unsigned)(__ballot(want) >> (lane & 48)) & 0xffffu;
-                if (want) {
-                    int* const slot = list + next + __popc(bits & ((1u << l16) - 1));
-                    const int fresh = *slot;
-                    row[j] = fresh;
-                    a.refs[fresh] = 1;
-                    if (later) *slot = valid(old) ? -2 - old : -1;
-                    else if (moved) atomicSub(a.refs + old, 1);
-                    if (moved) {
-                        const int k = atomicAdd(&copies, 1);
-                        pairs[2 * k] = old;
-                        pairs[2 * k + 1] = fresh;
+    auto serve = [&](auto wait) {            // wait: counts are lowered behind it
+        constexpr bool WAIT = decltype(wait)::value;
+        for (int w = g16; w < a.W; w += rows) {
+            const Row r = row_of(w);
+            const Grant g = grant_of(w, r);
+            if (g.granted) {
+                int* row = a.table + (size_t)w * a.max_blocks;
+                const bool holds = r.len % a.block_size != 0;
+                int next = g.before;
+                for (int j0 = r.first; j0 <= r.last && next < g.sofar; j0 += 16) {
+                    const int j = j0 + l16;
+                    const bool moved = g.copy && j == r.first;
+                    const int old = row[min(j, r.last)];
+                    bool want = moved || !valid(old);
+                    if constexpr (WAIT) want = want || (!(holds && j == r.first) && a.refs[old] > 1);
+                    want = want && j <= r.last;
+                    const unsigned bits = (unsigned)(__ballot(want) >> (lane & 48)) & 0xffffu;
+                    if (want) {
+                        const int at = next + __popc(bits & ((1u << l16) - 1)), fresh = list[at];
+                        row[j] = fresh;
+                        a.refs[fresh] = 1;
+                        if constexpr (WAIT) list[at] = valid(old) ? -2 - old : -1;
+                        if (moved) {
+                            if constexpr (!WAIT) atomicSub(a.refs + page[w], 1);
+                            const int k = atomicAdd(&copies, 1);
+                            pairs[2 * k] = page[w];
+                            pairs[2 * k + 1] = fresh;
+                        }
                     }
+                    next += __popc(bits);
                 }
-                next += __popc(bits);
             }
+            if constexpr (!WAIT) finish(w, r, g.granted);
         }
-        if (!later) finish(w, r, g.granted);
-    }
-    if (later) {
+    };
+    if (!later) {
+        serve(std::false_type{});
+    } else {
+        serve(std::true_type{});
         __syncthreads();
         for (int i = tid; i < listed; i += POOL_THREADS) {
             const int old = -2 - list[i];
