@@ -636,7 +636,7 @@ __device__ __forceinline__ void q4_store(Q4State<RB, D / 16>& st, Exchange<RB * 
 // of those for exponentials.  Measured (MI355X, us a layer with the merge, GB/s of what has to be read and TFLOP/s):
 //   4 x 12 528 tokens, one query each, 40/8 heads, D = 128, bf16        18.1   3200
 //   296 to 10 543 tokens, 16/8 heads, D = 256, bf16                     16.4   2480
-//   2052 to 11 111 tokens, four queries each, 64/8, D = 128, f16        18.5   1730   193
+//   2052 to 11 111 tokens, four queries each, 64/8, D = 128, f16        18.7   1710   191
 //   1 / 8 / 32 / 64 packed queries on 12 528 each, 40/8, bf16           56     1060   480
 //   1024 queries on 5120, 40/8, bf16                                    135           715
 // One tile ahead is enough: two, or the loop arranged so that nothing waits for the tile in flight at its head, changed nothing (the other
