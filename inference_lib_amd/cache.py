@@ -414,7 +414,8 @@ class PagedCache:
     that a sequence asked for get 0 too; no other sequence sees their states.  A sequence has at most max_blocks pages: by default as many as
     the pool, or as the attention takes (2^20 positions).
 
-    Every part of a step may be in a graph of its own or in none."""
+    Every part of a step may be in a graph of its own or in none.  Between steps `seq_lengths` may be shortened in place (drafts that were rejected):
+    what others still read behind a sequence's tokens it does not write."""
 
     MAX_POSITIONS, MAX_BLOCK_SIZE = 1 << 20, 1 << 12         # of hw_paged_sdpa and hw_paged_sdpa_q4
 
