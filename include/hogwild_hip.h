@@ -29,6 +29,8 @@
  *   hw_copy_to_blocks_q4, hw_read_blocks_q4, hw_paged_sdpa_q4, hw_varlen_paged_sdpa_q4 ... no counterpart: the paged operators with
  *                            caches in 4 bits
  *   hw_fork_blocks, hw_free_blocks, hw_reserve_blocks, hw_compact_blocks, hw_copy_pages ... no counterpart: the pages of paged caches
+ *   hw_window_paged_sdpa, hw_window_varlen_paged_sdpa, hw_trim_blocks ... no counterpart: the paged operators with a sliding window
+ *   hw_packed_slots, hw_copy_to_slots, hw_verify_drafts ... no counterpart: packed batches and drafted tokens of serving steps
  *   hw_build_inputs_dev, hw_advance_lengths, hw_problem.len_dev, hw_append.len_dev ... no counterpart: the same steps
  *                            with the segment lengths in device memory, so that a decode step captured as a HIP graph
  *                            can be replayed while the segments grow
@@ -388,6 +390,119 @@ int hw_compact_blocks(const hw_pool* p, int32_t* used, void* stream);
 /* Pages src[i] -> dst[i] (HOST arrays) of every tensor.  A page that is written is named once and is no source (HW_ERR_SHAPE). */
 int hw_copy_pages(void* const* caches, const size_t* page_bytes, int n_caches, int num_blocks, const int32_t* src, const int32_t* dst, int n,
                   void* stream);
+
+/* ------------------------------------------------------------------------------------------------------------
+ * Attention over paged caches with a sliding window and sinks (the first tokens of a sequence, which stay visible).  The query at position
+ * l of its sequence sees the positions j <= l with l - j < window or j < sinks; at a negative one it sees nothing (out 0, lse -inf).
+ *   key_cache, value_cache, block_table   as in hw_paged_problem; entries that name pages without visible positions are not looked at,
+ *                                         so such pages may have been given back (hw_trim_blocks)
+ * fixed-length operator (cu_seqlens_q == NULL), hw_window_paged_sdpa:
+ *   q [W, Hq, S, D] rotated, locations [W, S], out [W, Hq, S, D], lse [W, Hq, S]
+ * packed variable-length operator (cu_seqlens_q != NULL), hw_window_varlen_paged_sdpa:
+ *   q [total_q, Hq, D], locations [total_q], cu_seqlens_q [W + 1] (device), out [total_q, Hq, D], lse [total_q, Hq]; query tokens
+ *   before cu[0] and from cu[W] on belong to no sequence and get zeros (lse -inf)
+ * What a query does not see reaches its result in no way, infinities and NaN included.  Limits: those of hw_paged_problem; window >= 1,
+ * sinks >= 0; D in {64, 128, 256}, float32 up to 128.
+ */
+typedef struct hw_window_problem {
+    int32_t dtype;
+    int32_t W, Hq, Hkv, D;
+    int32_t S;                 /* query tokens per sequence (fixed-length operator) */
+    int32_t total_q;           /* packed query tokens over all sequences (variable-length operator) */
+    int32_t block_size, max_blocks, num_blocks;
+    int32_t window, sinks;
+    float scale;
+    void* out;
+    float* lse;                /* optional */
+    const void* q;
+    const int32_t* locations;
+    const void* key_cache;
+    const void* value_cache;
+    const int32_t* block_table;
+    const int32_t* cu_seqlens_q;
+    void* workspace;           /* hw_window_workspace_bytes() bytes, 16-byte aligned (NULL if those are 0) */
+    size_t workspace_bytes;
+    int32_t splits;            /* 0 = automatic; otherwise workgroups per (kv head, row group) */
+    int32_t row_blocks;        /* 0 = automatic; 1 or 2 = 16-row MFMA blocks per workgroup */
+} hw_window_problem;
+
+int hw_window_validate(const hw_window_problem* p);
+int hw_window_plan_debug(const hw_window_problem* p, int num_cus, hw_paged_plan* plan);   /* host only */
+int hw_window_workspace_bytes(const hw_window_problem* p, size_t* bytes);                 /* 0: none is needed (one split) */
+int hw_window_paged_sdpa(const hw_window_problem* p, void* stream);
+int hw_window_varlen_paged_sdpa(const hw_window_problem* p, void* stream);
+
+/* The pages of which no token from position seq_lengths[w] on sees anything -- behind the sinks' last page and before the window's
+   first one -- are given back: their entries become -1, their counts are lowered.  Lengths stay.  (A length that is shortened later brings
+   back a window whose pages are gone: drafts are verified first, or `window` is larger by as many tokens.) */
+int hw_trim_blocks(const hw_pool* p, int window, int sinks, void* stream);
+
+/*
+ * Packed batches: the new tokens of W sequences one behind the other, n_new[w] of sequence w from position positions[w] on, in
+ * `total` rows.
+ *   cu_seqlens [W + 1]   where each begins (negative numbers count as 0; what goes beyond `total` rows is cut off)
+ *   locations  [total]   the position of every token in its sequence, -1 where it has no place: behind the last sequence, behind the
+ *                        block table, on a page that is none
+ *   slots      [total]   its row of the caches, page * block_size + position % block_size, -1 likewise
+ * All device int32.  W <= 4096, num_blocks * block_size < 2^31, total < 2^28.
+ */
+typedef struct hw_packed_batch {
+    int32_t W, max_blocks, num_blocks, block_size, total;
+    const int32_t* block_table;    /* [W, max_blocks] */
+    const int32_t* positions;      /* [W] */
+    const int32_t* n_new;          /* [W] */
+    int32_t* cu_seqlens;
+    int32_t* locations;
+    int32_t* slots;
+} hw_packed_batch;
+int hw_packed_slots(const hw_packed_batch* b, void* stream);
+
+/* Rows key_states / value_states [total, Hkv, D] (element strides for the first two dimensions, a contiguous last one) to the rows
+   `slots` of the caches [num_blocks, Hkv, block_size, D].  Rows whose slot is no row of the caches are left out; no slot is named
+   twice. */
+typedef struct hw_copy_slots {
+    int32_t dtype;
+    int32_t total, Hkv, E, Ev;
+    int32_t block_size, num_blocks;
+    const void* key_states;
+    const void* value_states;
+    int64_t ks_t, ks_h, vs_t, vs_h;
+    void* key_cache;
+    void* value_cache;
+    const int32_t* slots;
+} hw_copy_slots;
+int hw_copy_to_slots(const hw_copy_slots* c, void* stream);
+
+/*
+ * Verification of drafted tokens.  Sequence w has n = n_drafts[w] of them (all K without n_drafts; numbers are taken into 0 .. K).  Draft
+ * i, token x, is accepted if those before it are and uniforms[w][i] * q[w][i][x] < p[w][i][x], with p the target's probabilities and q the
+ * ones that the draft was drawn from, NULL for drafts that were certain (1 at x).  accepted[w] = how many.  The next token is drawn
+ * from the weights max(p[w][a] - q[w][a], 0) at the first draft a that is not accepted -- from p[w][a] where they come to nothing -- or from
+ * p[w][n] behind the last one: the first token whose running sum exceeds uniforms[w][K] times the sum of all (for numbers in [0, 1); from
+ * 1 on the last token with a weight).  Sums in float64; negative, infinite and NaN weights count as 0; -1 where there is no weight.
+ * tokens[w] = the accepted drafts, the next token, -1 behind.  A draft that is no token (outside 0 .. V - 1) is not accepted, and q of
+ * a certain one is 0 then.  With seq_lengths, a sequence whose step began at positions[w] keeps its token before the drafts and the accepted
+ * ones: seq_lengths[w] = min(seq_lengths[w], positions[w] + 1 + accepted[w]).
+ */
+typedef struct hw_verify {
+    int32_t dtype;                 /* of the probabilities */
+    int32_t token_bytes;           /* 4 or 8: int32 or int64 tokens */
+    int32_t W, K, V;
+    const void* drafts;            /* [W, K] */
+    const void* target;            /* [W, K + 1, V], element strides tp_w, tp_k, contiguous rows */
+    const void* draft_probs;       /* [W, K, V], dp_w, dp_k, or NULL */
+    int64_t tp_w, tp_k, dp_w, dp_k;
+    const float* uniforms;         /* [W, K + 1] */
+    const int32_t* n_drafts;       /* [W] or NULL */
+    const int32_t* positions;      /* [W], with seq_lengths */
+    int32_t* seq_lengths;          /* [W] or NULL */
+    void* tokens;                  /* [W, K + 1] */
+    int32_t* accepted;             /* [W] */
+    void* workspace;               /* hw_verify_workspace_bytes() bytes, 16-byte aligned */
+    size_t workspace_bytes;
+} hw_verify;
+int hw_verify_workspace_bytes(const hw_verify* v, size_t* bytes);
+int hw_verify_drafts(const hw_verify* v, void* stream);
 
 /* ------------------------------------------------------------------------------------------------------------
  * Caller-side steps of a decode step (the reference does them in Python, python/hogwild/attention.py:137-204,251-257).

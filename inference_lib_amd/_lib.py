@@ -32,6 +32,8 @@ EXPORTS = [
     "hw_merge_segments",
     "hw_copy_to_blocks_q4", "hw_read_blocks_q4", "hw_paged_q4_validate", "hw_paged_q4_plan_debug", "hw_paged_q4_workspace_bytes",
     "hw_paged_sdpa_q4", "hw_varlen_paged_sdpa_q4",
+    "hw_window_validate", "hw_window_plan_debug", "hw_window_workspace_bytes", "hw_window_paged_sdpa", "hw_window_varlen_paged_sdpa",
+    "hw_trim_blocks", "hw_packed_slots", "hw_copy_to_slots", "hw_verify_workspace_bytes", "hw_verify_drafts",
     "hw_pool_workspace_bytes", "hw_fork_blocks", "hw_free_blocks", "hw_reserve_blocks", "hw_compact_blocks", "hw_copy_pages",
 ]
 
@@ -95,6 +97,50 @@ class HwCopyBlocks(C.Structure):
         ("vs_b", C.c_int64), ("vs_h", C.c_int64), ("vs_s", C.c_int64),
         ("key_cache", C.c_void_p), ("value_cache", C.c_void_p),
         ("block_table", C.c_void_p), ("seq_lengths", C.c_void_p),
+    ]
+
+
+class HwWindowProblem(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32),
+        ("W", C.c_int32), ("Hq", C.c_int32), ("Hkv", C.c_int32), ("D", C.c_int32), ("S", C.c_int32), ("total_q", C.c_int32),
+        ("block_size", C.c_int32), ("max_blocks", C.c_int32), ("num_blocks", C.c_int32),
+        ("window", C.c_int32), ("sinks", C.c_int32),
+        ("scale", C.c_float),
+        ("out", C.c_void_p), ("lse", C.c_void_p), ("q", C.c_void_p), ("locations", C.c_void_p),
+        ("key_cache", C.c_void_p), ("value_cache", C.c_void_p), ("block_table", C.c_void_p), ("cu_seqlens_q", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("splits", C.c_int32), ("row_blocks", C.c_int32),
+    ]
+
+
+class HwPackedBatch(C.Structure):
+    _fields_ = [
+        ("W", C.c_int32), ("max_blocks", C.c_int32), ("num_blocks", C.c_int32), ("block_size", C.c_int32), ("total", C.c_int32),
+        ("block_table", C.c_void_p), ("positions", C.c_void_p), ("n_new", C.c_void_p),
+        ("cu_seqlens", C.c_void_p), ("locations", C.c_void_p), ("slots", C.c_void_p),
+    ]
+
+
+class HwCopySlots(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32),
+        ("total", C.c_int32), ("Hkv", C.c_int32), ("E", C.c_int32), ("Ev", C.c_int32), ("block_size", C.c_int32), ("num_blocks", C.c_int32),
+        ("key_states", C.c_void_p), ("value_states", C.c_void_p),
+        ("ks_t", C.c_int64), ("ks_h", C.c_int64), ("vs_t", C.c_int64), ("vs_h", C.c_int64),
+        ("key_cache", C.c_void_p), ("value_cache", C.c_void_p), ("slots", C.c_void_p),
+    ]
+
+
+class HwVerify(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("token_bytes", C.c_int32),
+        ("W", C.c_int32), ("K", C.c_int32), ("V", C.c_int32),
+        ("drafts", C.c_void_p), ("target", C.c_void_p), ("draft_probs", C.c_void_p),
+        ("tp_w", C.c_int64), ("tp_k", C.c_int64), ("dp_w", C.c_int64), ("dp_k", C.c_int64),
+        ("uniforms", C.c_void_p), ("n_drafts", C.c_void_p), ("positions", C.c_void_p), ("seq_lengths", C.c_void_p),
+        ("tokens", C.c_void_p), ("accepted", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
     ]
 
 
@@ -175,6 +221,16 @@ def _load() -> C.CDLL:
     lib.hw_paged_q4_workspace_bytes.argtypes = [C.POINTER(HwPagedProblem), C.POINTER(C.c_size_t)]
     lib.hw_paged_sdpa_q4.argtypes = [C.POINTER(HwPagedProblem), C.c_void_p]
     lib.hw_varlen_paged_sdpa_q4.argtypes = [C.POINTER(HwPagedProblem), C.c_void_p]
+    lib.hw_window_validate.argtypes = [C.POINTER(HwWindowProblem)]
+    lib.hw_window_plan_debug.argtypes = [C.POINTER(HwWindowProblem), C.c_int, C.POINTER(HwPagedPlan)]
+    lib.hw_window_workspace_bytes.argtypes = [C.POINTER(HwWindowProblem), C.POINTER(C.c_size_t)]
+    lib.hw_window_paged_sdpa.argtypes = [C.POINTER(HwWindowProblem), C.c_void_p]
+    lib.hw_window_varlen_paged_sdpa.argtypes = [C.POINTER(HwWindowProblem), C.c_void_p]
+    lib.hw_trim_blocks.argtypes = [C.POINTER(HwPool), C.c_int, C.c_int, C.c_void_p]
+    lib.hw_packed_slots.argtypes = [C.POINTER(HwPackedBatch), C.c_void_p]
+    lib.hw_copy_to_slots.argtypes = [C.POINTER(HwCopySlots), C.c_void_p]
+    lib.hw_verify_workspace_bytes.argtypes = [C.POINTER(HwVerify), C.POINTER(C.c_size_t)]
+    lib.hw_verify_drafts.argtypes = [C.POINTER(HwVerify), C.c_void_p]
     lib.hw_pool_workspace_bytes.argtypes = [C.POINTER(HwPool), C.POINTER(C.c_size_t)]
     lib.hw_fork_blocks.argtypes = [C.POINTER(HwPool), C.c_void_p, C.c_void_p]
     lib.hw_free_blocks.argtypes = [C.POINTER(HwPool), C.c_void_p, C.c_void_p]
@@ -609,6 +665,173 @@ def read_blocks_q4(key_states: torch.Tensor, value_states: torch.Tensor, key_cac
         check(lib.hw_read_blocks_q4(C.byref(c), C.c_void_p(stream)), "hw_read_blocks_q4")
 
 
+class WindowProblem:
+    """hw_window_problem: out and q [W, Hq, S, D], locations [W, S], lse [W, Hq, S], or, with cu_seqlens_q [W + 1], packed: out and q
+    [total_q, Hq, D], locations [total_q], lse [total_q, Hq]."""
+
+    def __init__(self, *, q: torch.Tensor, locations: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, block_table: torch.Tensor,
+                 scale: float, window: int, sinks: int, out: torch.Tensor, cu_seqlens_q: Optional[torch.Tensor] = None,
+                 lse: Optional[torch.Tensor] = None, splits: int = 0, row_blocks: int = 0):
+        varlen = cu_seqlens_q is not None
+        if out.dtype not in _DTYPE_CODE:
+            raise HogwildError(-2, "WindowProblem")
+        if key_cache.dim() != 4 or key_cache.shape != value_cache.shape or block_table.dim() != 2:
+            raise ValueError("caches must be [num_blocks, Hkv, block_size, D], block_table [W, max_blocks]")
+        W = block_table.size(0)
+        if out.dim() != (3 if varlen else 4) or q.shape != out.shape or out.size(-1) != key_cache.size(3):
+            raise ValueError("queries and output must be [W, Hq, S, D], or [total_q, Hq, D] with cu_seqlens_q")
+        if not varlen and out.size(0) != W:
+            raise ValueError("output must be [W, Hq, S, D] with one block-table row per sequence")
+        if tuple(locations.shape) != ((out.size(0),) if varlen else (W, out.size(2))):
+            raise ValueError("locations must be [W, S], or [total_q] with cu_seqlens_q")
+        if varlen and tuple(cu_seqlens_q.shape) != (W + 1,):
+            raise ValueError("cu_seqlens_q must be [W + 1]")
+        if lse is not None and (lse.shape != out.shape[:-1] or lse.dtype != torch.float32):
+            raise ValueError("lse must be float32 [W, Hq, S], or [total_q, Hq] with cu_seqlens_q")
+        if any(t.dtype != torch.int32 for t in (locations, block_table) + ((cu_seqlens_q,) if varlen else ())):
+            raise ValueError("locations, block_table and cu_seqlens_q must be int32")
+        if any(t.dtype != out.dtype for t in (q, key_cache, value_cache)):
+            raise ValueError("queries and caches must have the dtype of the output")
+        if not 1 <= int(window) < 1 << 31 or not 0 <= int(sinks) < 1 << 31:
+            raise ValueError("window must be positive and sinks not negative")
+        tensors = [t for t in (out, q, locations, key_cache, value_cache, block_table, cu_seqlens_q, lse) if t is not None]
+        for t in tensors:
+            if not t.is_contiguous() or t.device != out.device:
+                raise ValueError("all tensors must be contiguous and live on the output's device")
+        self._keep, self.device, self.varlen = tensors, out.device, varlen
+        p = HwWindowProblem()
+        p.dtype = _DTYPE_CODE[out.dtype]
+        p.W, p.Hq, p.Hkv, p.D = W, out.size(1), key_cache.size(1), key_cache.size(3)
+        p.S, p.total_q = (0, out.size(0)) if varlen else (out.size(2), 0)
+        p.block_size, p.max_blocks, p.num_blocks = key_cache.size(2), block_table.size(1), key_cache.size(0)
+        p.window, p.sinks, p.scale = int(window), int(sinks), float(scale)
+        p.out, p.q, p.locations = out.data_ptr(), q.data_ptr(), locations.data_ptr()
+        p.lse = lse.data_ptr() if lse is not None else None
+        p.key_cache, p.value_cache, p.block_table = key_cache.data_ptr(), value_cache.data_ptr(), block_table.data_ptr()
+        p.cu_seqlens_q = cu_seqlens_q.data_ptr() if varlen else None
+        p.splits, p.row_blocks = int(splits), int(row_blocks)
+        self.p = p
+
+    def run(self) -> None:
+        with torch.cuda.device(self.device):
+            n = C.c_size_t(0)
+            check(lib.hw_window_workspace_bytes(C.byref(self.p), C.byref(n)), "hw_window_workspace_bytes")
+            ws = torch.empty(n.value, dtype=torch.uint8, device=self.device) if n.value else None
+            self.p.workspace, self.p.workspace_bytes = ws.data_ptr() if ws is not None else None, n.value
+            fn = lib.hw_window_varlen_paged_sdpa if self.varlen else lib.hw_window_paged_sdpa
+            check(fn(C.byref(self.p), C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)), fn.__name__)
+
+
+def window_plan(*, W: int, Hq: int, Hkv: int, D: int, block_size: int, max_blocks: int, window: int, num_cus: int, sinks: int = 0, S: int = 0,
+                total_q: Optional[int] = None, splits: int = 0, dtype: int = HW_BF16, row_blocks: int = 0) -> HwPagedPlan:
+    """Host-only plan of the operators with a sliding window (no GPU needed); total_q selects the variable-length operator."""
+    p = HwWindowProblem()
+    p.dtype = dtype
+    p.W, p.Hq, p.Hkv, p.D, p.S = W, Hq, Hkv, D, S
+    p.block_size, p.max_blocks, p.num_blocks = block_size, max_blocks, 1
+    p.window, p.sinks, p.scale = window, sinks, 1.0
+    p.out = p.q = p.locations = p.key_cache = p.value_cache = p.block_table = 16       # only tested for being aligned and non-NULL
+    if total_q is not None:
+        p.total_q = total_q
+        p.cu_seqlens_q = 16
+    p.splits, p.row_blocks = splits, row_blocks
+    out = HwPagedPlan()
+    check(lib.hw_window_plan_debug(C.byref(p), num_cus, C.byref(out)), "hw_window_plan_debug")
+    return out
+
+
+def packed_slots(block_table: torch.Tensor, positions: torch.Tensor, n_new: torch.Tensor, total: int, block_size: int, num_blocks: int):
+    """(cu_seqlens [W + 1], locations [total], slots [total]) of a packed batch, int32."""
+    if block_table.dim() != 2 or block_table.numel() == 0 or tuple(positions.shape) != (block_table.size(0),) or positions.shape != n_new.shape:
+        raise ValueError("block_table must be [W, max_blocks], positions and n_new [W]")
+    for t in (block_table, positions, n_new):
+        if t.dtype != torch.int32 or not t.is_contiguous() or t.device != block_table.device:
+            raise ValueError("block_table, positions and n_new must be contiguous int32 on one device")
+    total, block_size, num_blocks = int(total), int(block_size), int(num_blocks)
+    if not 0 <= total < 1 << 28 or not 1 <= block_size < 1 << 31 or not 1 <= num_blocks < 1 << 31:
+        raise ValueError("total must be 0 .. 2^28 - 1, block_size and num_blocks positive")
+    W = block_table.size(0)
+    cu, loc, slots = (torch.empty(n, dtype=torch.int32, device=block_table.device) for n in (W + 1, total, total))
+    b = HwPackedBatch(W, block_table.size(1), num_blocks, block_size, total, block_table.data_ptr(), positions.data_ptr(), n_new.data_ptr(),
+                      cu.data_ptr(), loc.data_ptr(), slots.data_ptr())
+    with torch.cuda.device(block_table.device):
+        check(lib.hw_packed_slots(C.byref(b), C.c_void_p(torch.cuda.current_stream(block_table.device).cuda_stream)), "hw_packed_slots")
+    return cu, loc, slots
+
+
+def copy_to_slots(key_states: torch.Tensor, value_states: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, slots: torch.Tensor) -> None:
+    """Rows [total, Hkv, E|Ev] (any strides with a contiguous last dimension) to the rows `slots` of the paged caches."""
+    if key_states.dim() != 3 or value_states.dim() != 3 or key_states.shape[:2] != value_states.shape[:2]:
+        raise ValueError("key_states / value_states must be [total, Hkv, E|Ev]")
+    T, Hkv, E = key_states.shape
+    Ev = value_states.size(2)
+    if key_cache.dim() != 4 or value_cache.dim() != 4 or key_cache.size(1) != Hkv or key_cache.shape[:3] != value_cache.shape[:3] \
+            or key_cache.size(3) != E or value_cache.size(3) != Ev or not key_cache.is_contiguous() or not value_cache.is_contiguous():
+        raise ValueError("caches must be contiguous [num_blocks, Hkv, block_size, E|Ev] and match the states")
+    if key_states.dtype not in _DTYPE_CODE:
+        raise HogwildError(-2, "copy_to_slots")
+    if any(t.dtype != key_states.dtype for t in (value_states, key_cache, value_cache)):
+        raise ValueError("states and caches must share one dtype")
+    if tuple(slots.shape) != (T,) or slots.dtype != torch.int32 or not slots.is_contiguous():
+        raise ValueError("slots must be contiguous int32 [total]")
+    if any(t.device != key_cache.device for t in (key_states, value_states, value_cache, slots)):
+        raise ValueError("all tensors must live on the caches' device")
+    if (E > 1 and key_states.stride(2) != 1) or (Ev > 1 and value_states.stride(2) != 1):
+        key_states, value_states = key_states.contiguous(), value_states.contiguous()
+    c = HwCopySlots(_DTYPE_CODE[key_states.dtype], T, Hkv, E, Ev, key_cache.size(2), key_cache.size(0), key_states.data_ptr(), value_states.data_ptr(),
+                    key_states.stride(0), key_states.stride(1), value_states.stride(0), value_states.stride(1), key_cache.data_ptr(),
+                    value_cache.data_ptr(), slots.data_ptr())
+    with torch.cuda.device(key_cache.device):
+        check(lib.hw_copy_to_slots(C.byref(c), C.c_void_p(torch.cuda.current_stream(key_cache.device).cuda_stream)), "hw_copy_to_slots")
+
+
+def verify_drafts(drafts: torch.Tensor, target_probs: torch.Tensor, uniforms: torch.Tensor, draft_probs: Optional[torch.Tensor] = None,
+                  n_drafts: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None, seq_lengths: Optional[torch.Tensor] = None):
+    """(tokens [W, K + 1], accepted int32 [W]) of drafts [W, K]; see hw_verify."""
+    if drafts.dim() != 2 or drafts.dtype not in (torch.int32, torch.int64) or not drafts.is_contiguous():
+        raise ValueError("drafts must be contiguous int64 or int32 [W, K]")
+    W, K = drafts.shape
+    if target_probs.dim() != 3 or tuple(target_probs.shape[:2]) != (W, K + 1) or target_probs.size(2) < 1:
+        raise ValueError("target_probs must be [W, K + 1, V]")
+    V = target_probs.size(2)
+    if target_probs.dtype not in _DTYPE_CODE:
+        raise HogwildError(-2, "verify_drafts")
+    if tuple(uniforms.shape) != (W, K + 1) or uniforms.dtype != torch.float32 or not uniforms.is_contiguous():
+        raise ValueError("uniforms must be contiguous float32 [W, K + 1]")
+    if draft_probs is not None and (tuple(draft_probs.shape) != (W, K, V) or draft_probs.dtype != target_probs.dtype):
+        raise ValueError("draft_probs must be [W, K, V] in the dtype of target_probs")
+    if (positions is None) != (seq_lengths is None):
+        raise ValueError("positions and seq_lengths go together")
+    for t in (n_drafts, positions, seq_lengths):
+        if t is not None and (tuple(t.shape) != (W,) or t.dtype != torch.int32 or not t.is_contiguous()):
+            raise ValueError("n_drafts, positions and seq_lengths must be contiguous int32 [W]")
+    device = target_probs.device
+    if any(t is not None and t.device != device for t in (drafts, uniforms, draft_probs, n_drafts, positions, seq_lengths)):
+        raise ValueError("all tensors must live on one device")
+    if V > 1 and target_probs.stride(2) != 1:
+        target_probs = target_probs.contiguous()
+    if draft_probs is not None and V > 1 and draft_probs.stride(2) != 1:
+        draft_probs = draft_probs.contiguous()
+    tokens, accepted = torch.empty((W, K + 1), dtype=drafts.dtype, device=device), torch.empty(W, dtype=torch.int32, device=device)
+    ptr = lambda t: t.data_ptr() if t is not None else None      # noqa: E731
+    v = HwVerify()
+    v.dtype, v.token_bytes = _DTYPE_CODE[target_probs.dtype], drafts.element_size()
+    v.W, v.K, v.V = W, K, V
+    v.drafts, v.target, v.draft_probs = drafts.data_ptr(), target_probs.data_ptr(), ptr(draft_probs) if K else None
+    v.tp_w, v.tp_k = target_probs.stride(0), target_probs.stride(1)
+    if draft_probs is not None:
+        v.dp_w, v.dp_k = draft_probs.stride(0), draft_probs.stride(1)
+    v.uniforms, v.n_drafts, v.positions, v.seq_lengths = uniforms.data_ptr(), ptr(n_drafts), ptr(positions), ptr(seq_lengths)
+    v.tokens, v.accepted = tokens.data_ptr(), accepted.data_ptr()
+    with torch.cuda.device(device):
+        n = C.c_size_t(0)
+        check(lib.hw_verify_workspace_bytes(C.byref(v), C.byref(n)), "hw_verify_workspace_bytes")
+        ws = torch.empty(n.value, dtype=torch.uint8, device=device)
+        v.workspace, v.workspace_bytes = ws.data_ptr(), n.value
+        check(lib.hw_verify_drafts(C.byref(v), C.c_void_p(torch.cuda.current_stream(device).cuda_stream)), "hw_verify_drafts")
+    return tokens, accepted
+
+
 class _Pool:
     """hw_pool of a block table [W, max_blocks], the sequences' lengths [W], the pages' counts [num_blocks] and the caches."""
 
@@ -670,6 +893,12 @@ def free_blocks(block_table, seq_lengths, ref_counts, finished) -> None:
             or finished.device != pool.device:
         raise ValueError("finished must be contiguous bool [W]")
     pool.run(lib.hw_free_blocks, finished.data_ptr())
+
+
+def trim_blocks(block_table, seq_lengths, ref_counts, window: int, sinks: int, block_size: int) -> None:
+    if not 1 <= int(window) < 1 << 31 or not 0 <= int(sinks) < 1 << 31:
+        raise ValueError("window must be positive and sinks not negative")
+    _Pool(block_table, seq_lengths, ref_counts, block_size).run(lib.hw_trim_blocks, int(window), int(sinks))
 
 
 def reserve_blocks(block_table, seq_lengths, ref_counts, n_new, positions, caches, block_size: int) -> None:

@@ -229,6 +229,73 @@ def hogwild_varlen_paged_sdpa_q4(queries: torch.Tensor, locations: torch.Tensor,
     return out
 
 
+# ---- paged caches with a sliding window, packed batches, drafted tokens (no counterpart in the reference) ----------------------------
+
+def _window_sdpa(queries, locations, key_cache, value_cache, block_table, cu_seqlens_q, scale, window, sinks, out, lse):
+    queries = queries.contiguous()
+    if out is None:
+        out = torch.empty_like(queries)
+    if HAVE_TORCH_OPS:
+        torch.ops.libhogatt.window_paged_sdpa(out, lse, scale, locations, queries, key_cache, value_cache, block_table, cu_seqlens_q, window, sinks)
+        return out
+    _lib.WindowProblem(q=queries, locations=locations, key_cache=key_cache, value_cache=value_cache, block_table=block_table, scale=scale,
+                       window=window, sinks=sinks, out=out, cu_seqlens_q=cu_seqlens_q, lse=lse).run()
+    return out
+
+
+def hogwild_paged_sdpa_window(queries: torch.Tensor, locations: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                              block_table: torch.Tensor, scale: float, window: int, sinks: int = 0, out=None,
+                              lse: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of rotated queries [W,Hq,S,D] at positions `locations` (int32 [W,S]) over paged sequences, with a sliding window: the
+    query at position l sees the positions j <= l with l - j < window, and those below `sinks`; at a negative position nothing (output 0,
+    lse -inf).  Pages without visible positions need not be there (trim_blocks).  `lse`: float32 [W,Hq,S]."""
+    return _window_sdpa(queries, locations, key_cache, value_cache, block_table, None, scale, window, sinks, out, lse)
+
+
+def hogwild_varlen_paged_sdpa_window(queries: torch.Tensor, locations: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                                     block_table: torch.Tensor, cu_seqlens_q: torch.Tensor, scale: float, window: int, sinks: int = 0,
+                                     out=None, lse: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The same with packed queries [total_q,Hq,D] at positions [total_q], those of sequence w from cu_seqlens_q[w] on (int32 [W+1]).  Query
+    tokens that belong to no sequence get zeros.  `lse`: float32 [total_q,Hq]."""
+    return _window_sdpa(queries, locations, key_cache, value_cache, block_table, cu_seqlens_q, scale, window, sinks, out, lse)
+
+
+def packed_slots(block_table: torch.Tensor, positions: torch.Tensor, n_new: torch.Tensor, total: int, block_size: int,
+                 num_blocks: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """A packed batch laid out on the device: the new tokens of all sequences one behind the other, n_new[w] (int32 [W]) of sequence w from
+    positions[w] (int32 [W]) on, in `total` rows.  Returns cu_seqlens [W+1], where each sequence begins, and of every row its position and
+    its row of the caches [total] each, all int32.  Both are -1 for tokens that have no place (behind the last sequence or the block table,
+    on no page); what goes beyond `total` rows is cut off."""
+    if HAVE_TORCH_OPS:
+        return torch.ops.libhogatt.packed_slots(block_table, positions, n_new, total, block_size, num_blocks)
+    return _lib.packed_slots(block_table, positions, n_new, total, block_size, num_blocks)
+
+
+def copy_to_slots(key_states: torch.Tensor, value_states: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                  slots: torch.Tensor) -> None:
+    """New K/V rows [total,Hkv,D] of a packed batch to the rows `slots` (int32 [total], from packed_slots) of the paged caches; those at -1
+    are left out.  No slot is named twice."""
+    if HAVE_TORCH_OPS:
+        torch.ops.libhogatt.copy_to_slots(key_states, value_states, key_cache, value_cache, slots)
+        return
+    _lib.copy_to_slots(key_states, value_states, key_cache, value_cache, slots)
+
+
+def verify_drafts(drafts: torch.Tensor, target_probs: torch.Tensor, uniforms: torch.Tensor, draft_probs: Optional[torch.Tensor] = None,
+                  n_drafts: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
+                  seq_lengths: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Which drafted tokens [W,K] (int64 or int32) stand, and the token behind them: drafts are accepted one after the other while
+    uniforms[w,i] * q < p, p = target_probs[w,i,x] and q = draft_probs[w,i,x] (1 without draft_probs); the next token is drawn with
+    uniforms[w,K] from what is left of the target's probabilities at the first draft that is not accepted, max(p - q, 0), or from the
+    target's behind the last one.  n_drafts (int32 [W]): how many drafts a sequence has, K by default.  Returns tokens [W,K+1], the
+    accepted drafts, the next token and -1 behind it, and accepted, int32 [W].  uniforms: float32 [W,K+1], in [0,1).  With positions and
+    seq_lengths (int32 [W]; as reserve_blocks left them for a step of 1 + n_drafts tokens) the lengths are shortened in place to the
+    token before the drafts and the accepted ones.  Rounding and special values: see hw_verify_drafts."""
+    if HAVE_TORCH_OPS:
+        return torch.ops.libhogatt.verify_drafts(drafts, target_probs, uniforms, draft_probs, n_drafts, positions, seq_lengths)
+    return _lib.verify_drafts(drafts, target_probs, uniforms, draft_probs, n_drafts, positions, seq_lengths)
+
+
 # ---- the pages of paged caches (no counterpart in the reference) --------------------------------------------------------------------
 # A pool: block_table int32 [W, max_blocks], seq_lengths int32 [W], ref_counts int32 [num_blocks] (how many rows name a page; 0 = free)
 # and `caches`, tensors [num_blocks, ...] of any type (keys and values of every layer).  Everything is worked out on the device.
@@ -248,6 +315,15 @@ def free_blocks(block_table: torch.Tensor, seq_lengths: torch.Tensor, ref_counts
         torch.ops.libhogatt.free_blocks(block_table, seq_lengths, ref_counts, finished)
         return
     _lib.free_blocks(block_table, seq_lengths, ref_counts, finished)
+
+
+def trim_blocks(block_table: torch.Tensor, seq_lengths: torch.Tensor, ref_counts: torch.Tensor, window: int, sinks: int, block_size: int) -> None:
+    """Pages of which no token from position seq_lengths[w] on sees anything (behind the sinks, before the window) are given back.  A
+    length that is shortened afterwards brings back a window whose pages are gone: verify drafts first."""
+    if HAVE_TORCH_OPS:
+        torch.ops.libhogatt.trim_blocks(block_table, seq_lengths, ref_counts, window, sinks, block_size)
+        return
+    _lib.trim_blocks(block_table, seq_lengths, ref_counts, window, sinks, block_size)
 
 
 def reserve_blocks(block_table: torch.Tensor, seq_lengths: torch.Tensor, ref_counts: torch.Tensor, n_new: torch.Tensor,

@@ -578,6 +578,194 @@ void copy_blocks(at::TensorList caches, at::IntArrayRef src, at::IntArrayRef dst
     check_status(status, "hw_copy_pages");
 }
 
+// ---- serving steps: windows, packed batches, drafts -----------------------------------------------------------
+
+// Both operators with a sliding window: with cu_seqlens_q queries and output are packed, [total_q, Hq, D], otherwise [W, Hq, S, D].
+void window_paged_sdpa(at::Tensor& out, const std::optional<at::Tensor>& lse, double scale, const at::Tensor& locations, const at::Tensor& queries,
+                       const at::Tensor& key_cache, const at::Tensor& value_cache, const at::Tensor& block_table, const std::optional<at::Tensor>& cu_seqlens_q,
+                       int64_t window, int64_t sinks) {
+    const bool varlen = cu_seqlens_q.has_value();
+    TORCH_CHECK(key_cache.dim() == 4 && key_cache.sizes() == value_cache.sizes(), "libhogatt: caches must be [num_blocks, Hkv, block_size, D], keys and values alike");
+    TORCH_CHECK(block_table.dim() == 2 && block_table.scalar_type() == at::kInt && block_table.is_contiguous(), "libhogatt: block_table must be contiguous int32 [W, max_blocks]");
+    TORCH_CHECK(locations.scalar_type() == at::kInt && locations.is_contiguous(), "libhogatt: locations must be contiguous int32");
+    TORCH_CHECK(out.is_contiguous() && queries.is_contiguous() && key_cache.is_contiguous() && value_cache.is_contiguous(),
+                "libhogatt: output, queries and caches must be contiguous");
+    TORCH_CHECK(queries.scalar_type() == out.scalar_type() && key_cache.scalar_type() == out.scalar_type() && value_cache.scalar_type() == out.scalar_type(),
+                "libhogatt: queries and caches must have the dtype of the output");
+    TORCH_CHECK(queries.sizes() == out.sizes() && out.dim() == (varlen ? 3 : 4) && out.size(-1) == key_cache.size(3),
+                "libhogatt: queries and output must be ", varlen ? "[total_q, Hq, D]" : "[W, Hq, S, D]", ", got ", queries.sizes(), " and ", out.sizes());
+    TORCH_CHECK(window >= 1 && window < (1ll << 31) && sinks >= 0 && sinks < (1ll << 31), "libhogatt: window must be positive and sinks not negative, got ", window, " and ", sinks);
+    for (const at::Tensor* t : {&locations, &queries, &key_cache, &value_cache, &block_table})
+        TORCH_CHECK(t->device() == out.device(), "libhogatt: all tensors must live on the output's device");
+    hw_window_problem p{};
+    p.dtype = dtype_code(out);
+    p.W = (int32_t)block_table.size(0);
+    p.Hkv = (int32_t)key_cache.size(1);
+    p.D = (int32_t)key_cache.size(3);
+    if (varlen) {
+        p.total_q = (int32_t)out.size(0);
+        p.Hq = (int32_t)out.size(1);
+        TORCH_CHECK(locations.dim() == 1 && locations.size(0) == p.total_q, "libhogatt: locations must be [total_q]");
+        TORCH_CHECK(cu_seqlens_q->dim() == 1 && cu_seqlens_q->size(0) == p.W + 1 && cu_seqlens_q->scalar_type() == at::kInt && cu_seqlens_q->is_contiguous() &&
+                        cu_seqlens_q->device() == out.device(),
+                    "libhogatt: cu_seqlens_q must be contiguous int32 [W + 1] on the output's device");
+        p.cu_seqlens_q = cu_seqlens_q->const_data_ptr<int32_t>();
+    } else {
+        p.Hq = (int32_t)out.size(1);
+        p.S = (int32_t)out.size(2);
+        TORCH_CHECK(out.size(0) == p.W, "libhogatt: output must be [W, Hq, S, D] with one block-table row per sequence");
+        TORCH_CHECK(locations.dim() == 2 && locations.size(0) == p.W && locations.size(1) == p.S, "libhogatt: locations must be [W, S]");
+    }
+    p.block_size = (int32_t)key_cache.size(2);
+    p.max_blocks = (int32_t)block_table.size(1);
+    p.num_blocks = (int32_t)key_cache.size(0);
+    p.window = (int32_t)window;
+    p.sinks = (int32_t)sinks;
+    p.scale = (float)scale;
+    p.out = out.data_ptr();
+    if (lse.has_value()) {
+        TORCH_CHECK(lse->scalar_type() == at::kFloat && lse->is_contiguous() && lse->device() == out.device() && lse->sizes() == out.sizes().slice(0, out.dim() - 1),
+                    "libhogatt: lse must be contiguous float32 ", varlen ? "[total_q, Hq]" : "[W, Hq, S]");
+        p.lse = lse->data_ptr<float>();
+    }
+    p.q = queries.const_data_ptr();
+    p.locations = locations.const_data_ptr<int32_t>();
+    p.key_cache = key_cache.const_data_ptr();
+    p.value_cache = value_cache.const_data_ptr();
+    p.block_table = block_table.const_data_ptr<int32_t>();
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(out.device());
+    size_t bytes = 0;
+    check_status(hw_window_workspace_bytes(&p, &bytes), "hw_window_workspace_bytes");
+    at::Tensor workspace;
+    if (bytes > 0) {
+        workspace = at::empty({(int64_t)bytes}, out.options().dtype(at::kByte));
+        p.workspace = workspace.data_ptr();
+        p.workspace_bytes = bytes;
+    }
+    if (varlen) check_status(hw_window_varlen_paged_sdpa(&p, stream_of(out)), "hw_window_varlen_paged_sdpa");
+    else check_status(hw_window_paged_sdpa(&p, stream_of(out)), "hw_window_paged_sdpa");
+}
+
+void trim_blocks(at::Tensor& block_table, const at::Tensor& seq_lengths, at::Tensor& ref_counts, int64_t window, int64_t sinks, int64_t block_size) {
+    TORCH_CHECK(window >= 1 && window < (1ll << 31) && sinks >= 0 && sinks < (1ll << 31), "libhogatt: window must be positive and sinks not negative, got ", window, " and ", sinks);
+    Pool u;
+    pool_tables(u, block_table, &seq_lengths, ref_counts, block_size);
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(block_table.device());
+    check_status(hw_trim_blocks(&u.p, (int)window, (int)sinks, stream_of(block_table)), "hw_trim_blocks");
+}
+
+// (cu_seqlens [W + 1], locations [total], slots [total])
+std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_slots(const at::Tensor& block_table, const at::Tensor& positions, const at::Tensor& n_new, int64_t total,
+                                                            int64_t block_size, int64_t num_blocks) {
+    TORCH_CHECK(block_table.dim() == 2 && block_table.scalar_type() == at::kInt && block_table.is_contiguous() && block_table.numel() > 0,
+                "libhogatt: block_table must be contiguous int32 [W, max_blocks]");
+    for (const at::Tensor* t : {&positions, &n_new})
+        TORCH_CHECK(t->dim() == 1 && t->size(0) == block_table.size(0) && t->scalar_type() == at::kInt && t->is_contiguous() && t->device() == block_table.device(),
+                    "libhogatt: positions and n_new must be contiguous int32 [W] on the table's device");
+    TORCH_CHECK(total >= 0 && total < (1ll << 28) && block_size >= 1 && block_size < (1ll << 31) && num_blocks >= 1 && num_blocks < (1ll << 31) &&
+                    block_table.size(0) < (1ll << 31) && block_table.size(1) < (1ll << 31),
+                "libhogatt: packed_slots: total must be 0 .. 2^28 - 1, block_size and num_blocks positive");
+    const int64_t W = block_table.size(0);
+    const at::Tensor cu = at::empty({W + 1}, positions.options()), loc = at::empty({total}, positions.options()), slots = at::empty({total}, positions.options());
+    hw_packed_batch b{};
+    b.W = (int32_t)W; b.max_blocks = (int32_t)block_table.size(1); b.num_blocks = (int32_t)num_blocks; b.block_size = (int32_t)block_size; b.total = (int32_t)total;
+    b.block_table = block_table.const_data_ptr<int32_t>();
+    b.positions = positions.const_data_ptr<int32_t>();
+    b.n_new = n_new.const_data_ptr<int32_t>();
+    b.cu_seqlens = cu.data_ptr<int32_t>();
+    b.locations = loc.data_ptr<int32_t>();
+    b.slots = slots.data_ptr<int32_t>();
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(block_table.device());
+    check_status(hw_packed_slots(&b, stream_of(block_table)), "hw_packed_slots");
+    return {cu, loc, slots};
+}
+
+void copy_to_slots(const at::Tensor& key_states, const at::Tensor& value_states, at::Tensor& key_cache, at::Tensor& value_cache, const at::Tensor& slots) {
+    TORCH_CHECK(key_states.dim() == 3 && value_states.dim() == 3 && key_states.size(0) == value_states.size(0) && key_states.size(1) == value_states.size(1),
+                "libhogatt: key_states / value_states must be [total, Hkv, D]");
+    TORCH_CHECK(key_cache.dim() == 4 && value_cache.dim() == 4 && key_cache.is_contiguous() && value_cache.is_contiguous() && key_cache.size(0) == value_cache.size(0) &&
+                    key_cache.size(2) == value_cache.size(2) && key_cache.size(1) == key_states.size(1) && value_cache.size(1) == key_states.size(1) &&
+                    key_cache.size(3) == key_states.size(2) && value_cache.size(3) == value_states.size(2),
+                "libhogatt: caches must be contiguous [num_blocks, Hkv, block_size, D] and match the states");
+    TORCH_CHECK(value_states.scalar_type() == key_states.scalar_type() && key_cache.scalar_type() == key_states.scalar_type() &&
+                    value_cache.scalar_type() == key_states.scalar_type(), "libhogatt: states and caches must share one dtype");
+    TORCH_CHECK(slots.dim() == 1 && slots.size(0) == key_states.size(0) && slots.scalar_type() == at::kInt && slots.is_contiguous(), "libhogatt: slots must be contiguous int32 [total]");
+    for (const at::Tensor* t : std::initializer_list<const at::Tensor*>{&key_states, &value_states, &value_cache, &slots})
+        TORCH_CHECK(t->device() == key_cache.device(), "libhogatt: all tensors must live on the caches' device");
+    const at::Tensor ks = (key_states.size(2) > 1 && key_states.stride(2) != 1) ? key_states.contiguous() : key_states;
+    const at::Tensor vs = (value_states.size(2) > 1 && value_states.stride(2) != 1) ? value_states.contiguous() : value_states;
+    hw_copy_slots c{};
+    c.dtype = dtype_code(key_states);
+    c.total = (int32_t)ks.size(0); c.Hkv = (int32_t)ks.size(1); c.E = (int32_t)ks.size(2); c.Ev = (int32_t)vs.size(2);
+    c.block_size = (int32_t)key_cache.size(2); c.num_blocks = (int32_t)key_cache.size(0);
+    c.key_states = ks.const_data_ptr(); c.value_states = vs.const_data_ptr();
+    c.ks_t = ks.stride(0); c.ks_h = ks.stride(1); c.vs_t = vs.stride(0); c.vs_h = vs.stride(1);
+    c.key_cache = key_cache.data_ptr(); c.value_cache = value_cache.data_ptr();
+    c.slots = slots.const_data_ptr<int32_t>();
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(key_cache.device());
+    check_status(hw_copy_to_slots(&c, stream_of(key_cache)), "hw_copy_to_slots");
+}
+
+// (tokens [W, K + 1] in the drafts' type, accepted int32 [W]); seq_lengths, where given, are shortened in place
+std::tuple<at::Tensor, at::Tensor> verify_drafts(const at::Tensor& drafts, const at::Tensor& target_probs, const at::Tensor& uniforms,
+                                                 const std::optional<at::Tensor>& draft_probs, const std::optional<at::Tensor>& n_drafts,
+                                                 const std::optional<at::Tensor>& positions, const std::optional<at::Tensor>& seq_lengths) {
+    TORCH_CHECK(drafts.dim() == 2 && (drafts.scalar_type() == at::kLong || drafts.scalar_type() == at::kInt) && drafts.is_contiguous(),
+                "libhogatt: drafts must be contiguous int64 or int32 [W, K]");
+    const int64_t W = drafts.size(0), K = drafts.size(1);
+    TORCH_CHECK(target_probs.dim() == 3 && target_probs.size(0) == W && target_probs.size(1) == K + 1 && target_probs.size(2) >= 1, "libhogatt: target_probs must be [W, K + 1, V]");
+    const int64_t V = target_probs.size(2);
+    TORCH_CHECK(W < (1ll << 31) && K < (1ll << 20) && V < (1ll << 30), "libhogatt: verify_drafts: too large");
+    TORCH_CHECK(uniforms.dim() == 2 && uniforms.size(0) == W && uniforms.size(1) == K + 1 && uniforms.scalar_type() == at::kFloat && uniforms.is_contiguous(),
+                "libhogatt: uniforms must be contiguous float32 [W, K + 1]");
+    const at::Device device = target_probs.device();
+    TORCH_CHECK(drafts.device() == device && uniforms.device() == device, "libhogatt: all tensors must live on one device");
+    auto counts = [&](const std::optional<at::Tensor>& t, const char* what) {
+        TORCH_CHECK(t->dim() == 1 && t->size(0) == W && t->scalar_type() == at::kInt && t->is_contiguous() && t->device() == device, "libhogatt: ", what,
+                    " must be contiguous int32 [W] on the probabilities' device");
+    };
+    hw_verify v{};
+    v.dtype = dtype_code(target_probs);
+    v.token_bytes = drafts.scalar_type() == at::kLong ? 8 : 4;
+    v.W = (int32_t)W; v.K = (int32_t)K; v.V = (int32_t)V;
+    const at::Tensor tp = (V > 1 && target_probs.stride(2) != 1) ? target_probs.contiguous() : target_probs;
+    at::Tensor dp;
+    if (draft_probs.has_value()) {
+        TORCH_CHECK(draft_probs->dim() == 3 && draft_probs->size(0) == W && draft_probs->size(1) == K && draft_probs->size(2) == V &&
+                        draft_probs->scalar_type() == target_probs.scalar_type() && draft_probs->device() == device,
+                    "libhogatt: draft_probs must be [W, K, V] in the dtype and on the device of target_probs");
+        dp = (V > 1 && draft_probs->stride(2) != 1) ? draft_probs->contiguous() : *draft_probs;
+        if (K > 0) v.draft_probs = dp.const_data_ptr();
+        v.dp_w = dp.stride(0); v.dp_k = dp.stride(1);
+    }
+    if (n_drafts.has_value()) {
+        counts(n_drafts, "n_drafts");
+        v.n_drafts = n_drafts->const_data_ptr<int32_t>();
+    }
+    TORCH_CHECK(positions.has_value() == seq_lengths.has_value(), "libhogatt: positions and seq_lengths go together");
+    if (positions.has_value()) {
+        counts(positions, "positions");
+        counts(seq_lengths, "seq_lengths");
+        v.positions = positions->const_data_ptr<int32_t>();
+        v.seq_lengths = seq_lengths->data_ptr<int32_t>();
+    }
+    const at::Tensor tokens = at::empty({W, K + 1}, drafts.options()), accepted = at::empty({W}, uniforms.options().dtype(at::kInt));
+    v.drafts = drafts.const_data_ptr();
+    v.target = tp.const_data_ptr();
+    v.tp_w = tp.stride(0); v.tp_k = tp.stride(1);
+    v.uniforms = uniforms.const_data_ptr<float>();
+    v.tokens = tokens.data_ptr();
+    v.accepted = accepted.data_ptr<int32_t>();
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(device);
+    size_t bytes = 0;
+    check_status(hw_verify_workspace_bytes(&v, &bytes), "hw_verify_workspace_bytes");
+    const at::Tensor workspace = at::empty({(int64_t)bytes}, uniforms.options().dtype(at::kByte));
+    v.workspace = workspace.data_ptr();
+    v.workspace_bytes = bytes;
+    check_status(hw_verify_drafts(&v, stream_of(target_probs)), "hw_verify_drafts");
+    return {tokens, accepted};
+}
+
 // ---- segments ----------------------------------------------------------------------------------------------------
 
 // hw_merge_segments on lists of per-layer buffers [Hkv, cap, E|Ev] (all layers of one form, packed).  Returns false, with
@@ -793,6 +981,14 @@ TORCH_LIBRARY(libhogatt, m) {
           "Tensor(e!)[] caches, int block_size) -> ()", tags);
     m.def("compact_blocks(Tensor(a!) block_table, Tensor(b!) ref_counts, Tensor(c!)[] caches, Tensor(d!) used) -> ()", tags);
     m.def("copy_blocks(Tensor(a!)[] caches, int[] src, int[] dst) -> ()", tags);
+    // additions: paged attention with a sliding window and sinks, packed batches, drafted tokens
+    m.def("window_paged_sdpa(Tensor(a!) output, Tensor(b!)? lse, float scale, Tensor locations, Tensor queries, "
+          "Tensor key_cache, Tensor value_cache, Tensor block_table, Tensor? cu_seqlens_q, int window, int sinks) -> ()", tags);
+    m.def("trim_blocks(Tensor(a!) block_table, Tensor seq_lengths, Tensor(b!) ref_counts, int window, int sinks, int block_size) -> ()", tags);
+    m.def("packed_slots(Tensor block_table, Tensor positions, Tensor n_new, int total, int block_size, int num_blocks) -> (Tensor, Tensor, Tensor)", tags);
+    m.def("copy_to_slots(Tensor key_states, Tensor value_states, Tensor(a!) key_cache, Tensor(b!) value_cache, Tensor slots) -> ()", tags);
+    m.def("verify_drafts(Tensor drafts, Tensor target_probs, Tensor uniforms, Tensor? draft_probs, Tensor? n_drafts, Tensor? positions, "
+          "Tensor(a!)? seq_lengths) -> (Tensor, Tensor)", tags);
     // addition: merge_caches (python/hogwild/attention.py:251-257) for all layers of a segment
     m.def("merge_segments(Tensor(a!)[] k_dst, Tensor(b!)[] v_dst, int[] dst_len, Tensor[] k_src, Tensor[] v_src, int[] n, Tensor inv_freq, "
           "float scaling, int position, ScalarType table_dtype, int mode) -> bool", tags);
@@ -826,6 +1022,11 @@ TORCH_LIBRARY_IMPL(libhogatt, CUDA, m) {
     m.impl("reserve_blocks", reserve_blocks);
     m.impl("compact_blocks", compact_blocks);
     m.impl("copy_blocks", copy_blocks);
+    m.impl("window_paged_sdpa", window_paged_sdpa);
+    m.impl("trim_blocks", trim_blocks);
+    m.impl("packed_slots", packed_slots);
+    m.impl("copy_to_slots", copy_to_slots);
+    m.impl("verify_drafts", verify_drafts);
     m.impl("merge_segments", merge_segments);
     m.impl("rope_append", rope_append);
     m.impl("segment_views", segment_views);

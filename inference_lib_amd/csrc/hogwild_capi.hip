@@ -338,6 +338,112 @@ int paged_q4_run(const hw_paged_problem* p, void* stream_) {
     return (int)hw::launch_merge(ma, p->dtype, p->Ev, stream);
 }
 
+// Paged attention with a sliding window.
+int window_run(const hw_window_problem* p, void* stream_) {
+    int st = window_validate(p);
+    if (st != HW_OK) return st;
+    int cus = 0;
+    st = device_cus(&cus);
+    if (st != HW_OK) return st;
+    hw_paged_plan plan;
+    st = window_plan(p, cus, &plan);
+    if (st != HW_OK) return st;
+    if (plan.rows == 0) return HW_OK;       // no query tokens
+    const bool direct = plan.splits == 1;
+    if (!direct && (p->workspace == nullptr || p->workspace_bytes < plan.workspace_bytes || !aligned16(p->workspace))) return HW_ERR_WORKSPACE;
+    hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+    hw_paged_problem pp;
+    std::memset(&pp, 0, sizeof(pp));
+    pp.dtype = p->dtype;
+    pp.F = 1; pp.W = p->W; pp.Hq = p->Hq; pp.Hkv = p->Hkv; pp.E = pp.Ev = p->D; pp.S = p->S; pp.total_q = p->total_q;
+    pp.block_size = p->block_size; pp.max_blocks = p->max_blocks; pp.num_blocks = p->num_blocks;
+    pp.scale = p->scale;
+    pp.q = p->q; pp.locations = p->locations; pp.key_cache = p->key_cache; pp.value_cache = p->value_cache;
+    pp.block_table = p->block_table; pp.cu_seqlens_q = p->cu_seqlens_q;
+    hw::WindowHeader wh;
+    std::memset(&wh, 0, sizeof(wh));
+    paged_header(&pp, plan, wh.p);
+    wh.p.part_o = reinterpret_cast<float*>(p->workspace);
+    if (!direct) wh.p.part_ml = wh.p.part_o + (size_t)p->Hkv * plan.splits * plan.rows * p->D;
+    wh.p.flags = (plan.workgroups % 8 == 0 ? hw::PH_XCD_REMAP : 0) | (direct ? hw::PH_DIRECT : 0);
+    wh.out = p->out;
+    wh.lse = p->lse;
+    wh.window = p->window;
+    wh.sinks = p->sinks;
+    const hipError_t e = hw::launch_window_attention(wh, p->dtype, p->D, plan.row_blocks, stream);
+    if (e != hipSuccess || direct) return (int)e;
+    hw::MergeArgs ma;
+    std::memset(&ma, 0, sizeof(ma));
+    ma.part_o = wh.p.part_o;
+    ma.part_ml = wh.p.part_ml;
+    ma.out = p->out;
+    ma.lse = p->lse;
+    ma.W = wh.p.LW; ma.Hq = p->Hq; ma.Hkv = p->Hkv; ma.S = wh.p.LS; ma.R = ma.rows = plan.rows;
+    ma.wgs_per_head = plan.splits;
+    ma.xcd_local = (p->cu_seqlens_q == nullptr && plan.workgroups % 8 == 0 && p->Hkv % 8 == 0) ? 1 : 0;
+    ma.magic_rows = magic_of(1);
+    return (int)hw::launch_merge(ma, p->dtype, p->D, stream);
+}
+
+int packed_slots_run(const hw_packed_batch* b, void* stream) {
+    if (b == nullptr) return HW_ERR_NULL;
+    if (b->W < 1 || b->max_blocks < 1 || b->num_blocks < 1 || b->block_size < 1 || b->total < 0 || b->total >= (1 << 28)) return HW_ERR_SHAPE;
+    if (b->W > hw::POOL_MAX_ROWS) return HW_ERR_UNSUPPORTED;
+    if ((long long)b->block_size * b->max_blocks > (1ll << 30) || (long long)b->num_blocks * b->block_size >= (1ll << 31)) return HW_ERR_SHAPE;
+    if (b->block_table == nullptr || b->positions == nullptr || b->n_new == nullptr || b->cu_seqlens == nullptr ||
+        (b->total > 0 && (b->locations == nullptr || b->slots == nullptr)))
+        return HW_ERR_NULL;
+    hw::PackedBatchArgs a;
+    a.table = b->block_table; a.positions = b->positions; a.n_new = b->n_new;
+    a.cu = b->cu_seqlens; a.locations = b->locations; a.slots = b->slots;
+    a.W = b->W; a.max_blocks = b->max_blocks; a.num_blocks = b->num_blocks; a.block_size = b->block_size; a.total = b->total;
+    return (int)hw::launch_packed_slots(a, reinterpret_cast<hipStream_t>(stream));
+}
+
+int copy_slots_run(const hw_copy_slots* c, void* stream) {
+    if (c == nullptr) return HW_ERR_NULL;
+    if (c->dtype != HW_F32 && c->dtype != HW_F16 && c->dtype != HW_BF16) return HW_ERR_DTYPE;
+    if (c->total < 0 || c->Hkv < 1 || c->E < 1 || c->Ev < 1 || c->block_size < 1 || c->num_blocks < 1) return HW_ERR_SHAPE;
+    if ((long long)c->num_blocks * c->Hkv * c->block_size >= (1ll << 31) || (long long)c->Hkv * ((long long)c->E + c->Ev) >= (1ll << 28)) return HW_ERR_SHAPE;
+    if (c->total == 0) return HW_OK;
+    if (c->key_states == nullptr || c->value_states == nullptr || c->key_cache == nullptr || c->value_cache == nullptr || c->slots == nullptr) return HW_ERR_NULL;
+    hw::CopySlotsArgs a;
+    a.key_states = c->key_states; a.value_states = c->value_states; a.kcache = c->key_cache; a.vcache = c->value_cache; a.slots = c->slots;
+    a.ks_t = c->ks_t; a.ks_h = c->ks_h; a.vs_t = c->vs_t; a.vs_h = c->vs_h;
+    a.total = c->total; a.Hkv = c->Hkv; a.E = c->E; a.Ev = c->Ev; a.block_size = c->block_size; a.num_blocks = c->num_blocks;
+    return (int)hw::launch_copy_to_slots(a, c->dtype, reinterpret_cast<hipStream_t>(stream));
+}
+
+int verify_check(const hw_verify* v) {
+    if (v == nullptr) return HW_ERR_NULL;
+    if (v->dtype != HW_F32 && v->dtype != HW_F16 && v->dtype != HW_BF16) return HW_ERR_DTYPE;
+    if (v->token_bytes != 4 && v->token_bytes != 8) return HW_ERR_DTYPE;
+    if (v->W < 0 || v->K < 0 || v->V < 1 || v->K >= (1 << 20) || v->V >= (1 << 30)) return HW_ERR_SHAPE;
+    if ((long long)v->W * ((v->V + hw::VERIFY_CHUNK - 1) / hw::VERIFY_CHUNK) >= (1ll << 31)) return HW_ERR_SHAPE;
+    return HW_OK;
+}
+
+size_t verify_bytes(const hw_verify* v) { return (size_t)v->W * ((v->V + hw::VERIFY_CHUNK - 1) / hw::VERIFY_CHUNK) * 2 * sizeof(double); }
+
+int verify_run(const hw_verify* v, void* stream) {
+    const int st = verify_check(v);
+    if (st != HW_OK) return st;
+    if (v->W == 0) return HW_OK;
+    if (v->target == nullptr || v->uniforms == nullptr || v->tokens == nullptr || v->accepted == nullptr || (v->K > 0 && v->drafts == nullptr) ||
+        (v->seq_lengths != nullptr && v->positions == nullptr))
+        return HW_ERR_NULL;
+    if (v->workspace == nullptr || v->workspace_bytes < verify_bytes(v) || !aligned16(v->workspace)) return HW_ERR_WORKSPACE;
+    hw::VerifyArgs a;
+    a.drafts = v->drafts; a.target = v->target; a.draft_probs = v->draft_probs;
+    a.tp_w = v->tp_w; a.tp_k = v->tp_k; a.dp_w = v->dp_w; a.dp_k = v->dp_k;
+    a.uniforms = v->uniforms; a.n_drafts = v->n_drafts; a.positions = v->positions; a.lengths = v->seq_lengths;
+    a.tokens = v->tokens; a.accepted = v->accepted;
+    a.sums = reinterpret_cast<double*>(v->workspace);
+    a.W = v->W; a.K = v->K; a.V = v->V;
+    a.chunks = (v->V + hw::VERIFY_CHUNK - 1) / hw::VERIFY_CHUNK;
+    return (int)hw::launch_verify(a, v->dtype, v->token_bytes == 8, reinterpret_cast<hipStream_t>(stream));
+}
+
 // What the operators on blocks of a cache have in common; false with *st = HW_OK: nothing to do.
 bool copy_blocks_args(const hw_copy_blocks* c, bool q4, hw::CopyBlocksArgs* a, int* st) {
     *st = HW_OK;
@@ -432,6 +538,14 @@ int copy_tensors(hw::PageCopyArgs& a, void* const* caches, const size_t* page_by
         a.to = nullptr;                     // (the table is renamed once)
     }
     return HW_OK;
+}
+
+int trim_run(const hw_pool* p, int window, int sinks, void* stream) {
+    hw::PoolArgs a;
+    const int st = pool_args(p, true, false, &a);
+    if (st != HW_OK) return st;
+    if (window < 1 || sinks < 0) return HW_ERR_SHAPE;
+    return (int)hw::launch_trim(a, window, sinks, reinterpret_cast<hipStream_t>(stream));
 }
 
 int fork_run(const hw_pool* p, const void* who, bool free_rows, void* stream) {
@@ -849,6 +963,51 @@ int hw_varlen_paged_sdpa_q4(const hw_paged_problem* p, void* stream) {
     if (p != nullptr && p->cu_seqlens_q == nullptr) return HW_ERR_NULL;
     return paged_q4_run(p, stream);
 }
+
+int hw_window_validate(const hw_window_problem* p) { return window_validate(p); }
+
+int hw_window_plan_debug(const hw_window_problem* p, int num_cus, hw_paged_plan* plan) {
+    const int st = window_validate(p);
+    return st != HW_OK ? st : window_plan(p, num_cus, plan);
+}
+
+int hw_window_workspace_bytes(const hw_window_problem* p, size_t* bytes) {
+    if (bytes == nullptr) return HW_ERR_NULL;
+    int st = window_validate(p);
+    if (st != HW_OK) return st;
+    int cus = 0;
+    st = device_cus(&cus);
+    if (st != HW_OK) return st;
+    hw_paged_plan plan;
+    st = window_plan(p, cus, &plan);
+    if (st == HW_OK) *bytes = plan.workspace_bytes;
+    return st;
+}
+
+int hw_window_paged_sdpa(const hw_window_problem* p, void* stream) {
+    if (p != nullptr && p->cu_seqlens_q != nullptr) return HW_ERR_SHAPE;
+    return window_run(p, stream);
+}
+
+int hw_window_varlen_paged_sdpa(const hw_window_problem* p, void* stream) {
+    if (p != nullptr && p->cu_seqlens_q == nullptr) return HW_ERR_NULL;
+    return window_run(p, stream);
+}
+
+int hw_trim_blocks(const hw_pool* p, int window, int sinks, void* stream) { return trim_run(p, window, sinks, stream); }
+
+int hw_packed_slots(const hw_packed_batch* b, void* stream) { return packed_slots_run(b, stream); }
+
+int hw_copy_to_slots(const hw_copy_slots* c, void* stream) { return copy_slots_run(c, stream); }
+
+int hw_verify_workspace_bytes(const hw_verify* v, size_t* bytes) {
+    if (bytes == nullptr) return HW_ERR_NULL;
+    const int st = verify_check(v);
+    if (st == HW_OK) *bytes = verify_bytes(v);
+    return st;
+}
+
+int hw_verify_drafts(const hw_verify* v, void* stream) { return verify_run(v, stream); }
 
 int hw_pool_workspace_bytes(const hw_pool* p, size_t* bytes) {
     if (p == nullptr || bytes == nullptr) return HW_ERR_NULL;

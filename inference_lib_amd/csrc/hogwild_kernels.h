@@ -187,6 +187,58 @@ hipError_t launch_reserve(const PoolArgs& a, const int* n_new, int* positions, i
 hipError_t launch_compact(const PoolArgs& a, int* used, int* ws, hipStream_t stream);
 hipError_t launch_copy_pages(const PageCopyArgs& a, int most_pairs, hipStream_t stream);
 
+hipError_t launch_trim(const PoolArgs& a, int window, int sinks, hipStream_t stream);
+
+// ---- paged attention with a sliding window and sinks (hogwild_window.hip) ----
+// PagedHeader as the other paged launches have it (F = 1, no fragment lengths, flags: PH_XCD_REMAP, PH_DIRECT), and what they lack.
+struct alignas(64) WindowHeader {
+    PagedHeader p;
+    void* out;             // written with PH_DIRECT, and where query tokens belong to no sequence
+    float* lse;            // or null
+    int window, sinks;
+};
+hipError_t launch_window_attention(const WindowHeader& wh, int dtype, int D, int rb, hipStream_t stream);
+
+// ---- packed batches and drafts (hogwild_step.hip) ----
+struct PackedBatchArgs {
+    const int* table;      // [W, max_blocks]
+    const int* positions;  // [W]
+    const int* n_new;      // [W]
+    int* cu;               // [W + 1]
+    int* locations;        // [total]
+    int* slots;            // [total]
+    int W, max_blocks, num_blocks, block_size, total;
+};
+hipError_t launch_packed_slots(const PackedBatchArgs& a, hipStream_t stream);
+
+struct CopySlotsArgs {
+    const void* key_states;    // [total, Hkv, E]   (element strides below, innermost contiguous)
+    const void* value_states;  // [total, Hkv, Ev]
+    void* kcache;
+    void* vcache;
+    const int* slots;          // [total]
+    long long ks_t, ks_h, vs_t, vs_h;
+    int total, Hkv, E, Ev, block_size, num_blocks;
+};
+hipError_t launch_copy_to_slots(const CopySlotsArgs& a, int dtype, hipStream_t stream);
+
+struct VerifyArgs {
+    const void* drafts;        // [W, K]
+    const void* target;        // [W, K + 1, V]
+    const void* draft_probs;   // [W, K, V] or null
+    long long tp_w, tp_k, dp_w, dp_k;
+    const float* uniforms;     // [W, K + 1]
+    const int* n_drafts;       // [W] or null
+    const int* positions;      // [W]
+    int* lengths;              // [W] or null
+    void* tokens;              // [W, K + 1]
+    int* accepted;             // [W]
+    double* sums;              // [W][chunks][2]: of the weights left over and of the target's probabilities
+    int W, K, V, chunks;
+};
+constexpr int VERIFY_CHUNK = 4096;      // probabilities that one workgroup adds up
+hipError_t launch_verify(const VerifyArgs& a, int dtype, bool wide_tokens, hipStream_t stream);
+
 // ---- caller-side steps: input builder and fused key rotation + append ----
 constexpr int MAX_POS_ENTRIES = 768;    // (fragment, worker) pairs per build_inputs launch
 constexpr int MAX_APPEND_WORKERS = 64;  // workers per rope_append launch

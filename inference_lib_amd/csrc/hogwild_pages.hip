@@ -8,6 +8,7 @@
 //   reserve_kernel .... pages for the tokens to come, copies of shared pages that are about to be written
 //   compact_kernel .... which pages move where, so that those in use are the first ones
 //   copy_pages_kernel . the pages themselves, of every tensor of the pool (layers, keys and values) in one launch
+//   trim_kernel ....... pages that have left a sliding window are given back
 //
 // The first three are bound by latency: chains of a few dependent accesses to tables of some kilobytes.  One workgroup works out an
 // allocation, because what one sequence gets depends on what the others took; its scans go over the free pages wave by wave.  The
@@ -389,9 +390,29 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(const PageCopyArgs a) {
     }
 }
 
+// Tokens from position length on see, of the positions before it, those from length - window + 1 on and those below sinks: the pages in
+// between are given back.  One workgroup per row; counts go down in any order.
+__global__ __launch_bounds__(256) void trim_kernel(const PoolArgs a, int window, int sinks) {
+    const int w = blockIdx.x;
+    const int first = (int)min(((long long)sinks + a.block_size - 1) / a.block_size, (long long)a.max_blocks);
+    const int last = (int)min(max((long long)a.lengths[w] - window + 1, 0ll) / a.block_size, (long long)a.max_blocks);
+    int* const row = a.table + (size_t)w * a.max_blocks;
+    for (int j = first + threadIdx.x; j < last; j += 256) {
+        const int page = row[j];
+        if (page < 0 || page >= a.num_blocks) continue;
+        atomicSub(a.refs + page, 1);
+        row[j] = -1;
+    }
+}
+
 // ------------------------------------------------------------------------------------------------
 // launchers
 // ------------------------------------------------------------------------------------------------
+hipError_t launch_trim(const PoolArgs& a, int window, int sinks, hipStream_t stream) {
+    hipLaunchKernelGGL(trim_kernel, dim3(a.W), dim3(256), 0, stream, a, window, sinks);
+    return hipGetLastError();
+}
+
 hipError_t launch_fork(const PoolArgs& a, const void* who, bool free_rows, hipStream_t stream) {
     int cols = 8192 / a.W;
     cols = cols < 1 ? 1 : cols > a.max_blocks ? a.max_blocks : cols;

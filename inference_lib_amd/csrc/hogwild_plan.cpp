@@ -809,5 +809,60 @@ int paged_q4_plan(const hw_paged_problem* p, int num_cus, hw_paged_plan* plan) {
     return HW_OK;
 }
 
+int window_validate(const hw_window_problem* p) {
+    if (p == nullptr) return HW_ERR_NULL;
+    if (p->dtype != HW_F32 && p->dtype != HW_F16 && p->dtype != HW_BF16) return HW_ERR_DTYPE;
+    if (p->W < 1 || p->Hq < 1 || p->Hkv < 1 || p->D < 1 || p->Hq % p->Hkv != 0) return HW_ERR_SHAPE;
+    if (!(p->scale > 0.f) || !std::isfinite(p->scale)) return HW_ERR_SHAPE;
+    if (p->window < 1 || p->sinks < 0) return HW_ERR_SHAPE;
+    const bool varlen = p->cu_seqlens_q != nullptr;
+    if (varlen ? p->total_q < 0 : (p->S < 1 || p->S >= (1 << 12))) return HW_ERR_SHAPE;
+    if (p->block_size < 1 || p->block_size >= (1 << 12) || p->max_blocks < 1 || p->num_blocks < 1) return HW_ERR_SHAPE;
+    if ((long long)p->block_size * p->max_blocks > (1ll << 20)) return HW_ERR_SHAPE;
+    if ((long long)p->num_blocks * p->Hkv * p->block_size >= (1ll << 31)) return HW_ERR_SHAPE;
+    const long long tokens = varlen ? p->total_q : (long long)p->W * p->S;
+    const int gq = p->Hq / p->Hkv;
+    if (gq >= (1 << 12) || tokens * gq >= (1 << 20) || p->W >= (1 << 20)) return HW_ERR_SHAPE;
+    if ((p->out == nullptr || p->q == nullptr || p->locations == nullptr) && tokens > 0) return HW_ERR_NULL;
+    if (p->key_cache == nullptr || p->value_cache == nullptr || p->block_table == nullptr) return HW_ERR_NULL;
+    if (!aligned16(p->out) || !aligned16(p->q) || !aligned16(p->key_cache) || !aligned16(p->value_cache)) return HW_ERR_ALIGN;
+    if (p->splits < 0 || p->row_blocks < 0) return HW_ERR_SHAPE;
+    if (p->D != 64 && p->D != 128 && p->D != 256) return HW_ERR_UNSUPPORTED;
+    if (p->D == 256 && p->dtype == HW_F32) return HW_ERR_UNSUPPORTED;   // two fp32 K tiles per wave exceed the LDS
+    return HW_OK;
+}
+
+int window_plan(const hw_window_problem* p, int num_cus, hw_paged_plan* plan) {
+    if (plan == nullptr) return HW_ERR_NULL;
+    if (num_cus < 1) return HW_ERR_SHAPE;
+    const bool varlen = p->cu_seqlens_q != nullptr;
+    const int gq = p->Hq / p->Hkv;
+    const int tokens = varlen ? p->total_q : p->W * p->S;
+    std::memset(plan, 0, sizeof(*plan));
+    plan->rows = tokens * gq;
+    const bool two = p->dtype != HW_F32 && p->D <= 128;        // two row blocks: what the registers hold
+    const int usual = varlen ? (plan->rows + p->W - 1) / p->W : p->S * gq;      // rows of a sequence, in the mean
+    plan->row_blocks = p->row_blocks != 0 ? p->row_blocks : two && usual > 16 ? 2 : 1;
+    if (plan->row_blocks != 1 && !(plan->row_blocks == 2 && two)) return HW_ERR_UNSUPPORTED;
+    const int rows = 16 * plan->row_blocks;
+    // (packed: one more than there can be, which writes the zeros of tokens that belong to no sequence)
+    plan->row_groups = varlen ? (plan->rows + rows - 1) / rows + p->W : p->W * ((p->S * gq + rows - 1) / rows);
+    // The tiles that a row group usually sees, at most: sinks and a window that moves over its tokens.  Splits of two tiles a wave and more,
+    // as far as there are CUs.
+    const long long cap = ((long long)p->block_size * p->max_blocks + hw::TILE - 1) / hw::TILE;
+    const long long seen = (std::min((long long)p->sinks, 1ll << 20) + hw::TILE - 1) / hw::TILE + (std::min((long long)p->window, 1ll << 20) + rows / gq) / hw::TILE + 2;
+    const long long tiles = std::min(cap, seen);
+    const long long groups = (long long)std::max(plan->row_groups, 1) * p->Hkv;
+    long long splits = p->splits;
+    if (splits == 0) splits = std::max(1ll, std::min((num_cus + groups - 1) / groups, tiles / (2 * hw::NWAVES)));
+    splits = std::min(splits, (long long)HW_MAX_SPLITS);
+    plan->splits = (int)splits;
+    const long long wgs = groups * splits;
+    if (wgs >= (1ll << 31)) return HW_ERR_SHAPE;
+    plan->workgroups = (int)wgs;
+    if (splits > 1) plan->workspace_bytes = ((size_t)p->Hkv * splits * plan->rows * ((size_t)p->D + 2) * sizeof(float) + 255) & ~(size_t)255;
+    return HW_OK;
+}
+
 }  // namespace host
 }  // namespace hw

@@ -1,0 +1,468 @@
+// Attention over paged caches with a sliding window and sinks, for gfx950 (MI355X, CDNA4, wave64).
+//
+//   o_r = sum_j p_j v_j,  p = softmax over { j <= l_r : l_r - j < window or j < sinks } of scale * q_r . k_j
+//
+// for the query rows r (a token and a head of the group that shares a kv head) at positions l_r of one sequence, whose keys and values
+// lie in pages.  A workgroup owns one kv head and up to 16 or 32 rows of one sequence.  Its keys are two stretches of the sequence: the
+// sinks, and the union of the rows' windows.  Both are cut into tiles of 32 tokens at multiples of 32, numbered through (tile_at), and
+// tile k goes to wave k mod (4 * nsplit) of the workgroups that share the rows.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "hogwild_kernels.h"
+#include "hogwild_device.h"
+
+namespace hw {
+
+// The bounds of a lane's rows: row n of row block rb sees the tokens below snk[rb], and from lo[rb] to lim[rb] - 1.
+template <int RB>
+struct Band {
+    int lo[RB], lim[RB], snk[RB];
+    __device__ __forceinline__ bool sees(int rb, int tok) const { return tok < snk[rb] || (tok >= lo[rb] && tok < lim[rb]); }
+};
+
+// Not 0 under SIGNS: one of the two 16-bit elements (the 32-bit one) of the word is infinite or NaN, its exponent all ones.
+template <class DT>
+struct Wild {
+    static constexpr u32 EXP = Elem<DT>::size == 4 ? 0x7f800000u : std::is_same<DT, F16>::value ? 0x7c007c00u : 0x7f807f80u;
+    static constexpr u32 ONE = Elem<DT>::size == 4 ? 0x00800000u : std::is_same<DT, F16>::value ? 0x04000400u : 0x00800080u;
+    static constexpr u32 SIGNS = Elem<DT>::size == 4 ? 0x80000000u : 0x80008000u;
+    static __device__ __forceinline__ u32 of(u32 x) { return (x & EXP) + ONE; }
+};
+
+// One 32-token tile against all rows of the wave: K in the staging slot, V in registers (see compute_tile, whose layouts these are).
+// A row's weight of a token that it does not see is 0, which times an infinite value would be NaN: where the tile holds one, the products
+// with V are taken row by row, from the values that the row sees.  mixed: the rows do not all see the same of its tokens.
+template <class DT, int D, int RB>
+__device__ __forceinline__ void band_tile(const TileRegs<DT, D, D>& t, const u32x4* qreg, const Band<RB>& band, WaveState<RB, D / 16>& st, int t0, int n, int q,
+                                          float sc, const char* kstage, bool mixed) {
+    typedef Geo<DT, D, D> G;
+    constexpr float LAZY_LOG2 = 8.0f;     // how far a row's maximum may exceed the reference of its exponentials before that follows
+    float s[RB][8], mxl[RB];
+    {
+        f32x4 sacc[RB][2];
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb) {
+            u32x4 kop[G::KJ];
+#pragma unroll
+            for (int j = 0; j < G::KJ; ++j) kop[j] = *reinterpret_cast<const u32x4*>(kstage + kstage_offset<G>(tb * 16 + n, 4 * j + q));
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+                f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < G::KJ; ++j) {
+                    if constexpr (G::SZ == 2) acc = Elem<DT>::mfma(kop[j], qreg[rb * G::KJ + j], acc);
+                    else {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+                            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kop[j][c]), __uint_as_float(qreg[rb * G::KJ + j][c]), acc, 0, 0, 0);
+                    }
+                }
+                sacc[rb][tb] = acc;
+            }
+        }
+        bool need = false;
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            float mx = NEG_BIG;
+#pragma unroll
+            for (int idx = 0; idx < 8; ++idx) {
+                s[rb][idx] = band.sees(rb, t0 + slot_token(q, idx)) ? sacc[rb][idx >> 2][idx & 3] : NEG_BIG;
+                mx = fmaxf(mx, s[rb][idx]);
+            }
+            mxl[rb] = mx;
+            need = need || ((mx < -1.0e29f ? NEG_BIG : mx * sc) > st.m[rb] + LAZY_LOG2);
+        }
+        if (__builtin_amdgcn_ballot_w64(need) != 0) {
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+                const float mx = quarter_max(mxl[rb]);
+                const float mxs = mx < -1.0e29f ? NEG_BIG : mx * sc;
+                const float mnew = mxs > st.m[rb] + LAZY_LOG2 ? mxs : st.m[rb];
+                const float alpha = fast_exp2(st.m[rb] - mnew);
+                st.m[rb] = mnew;
+                st.l[rb] *= alpha;
+                if (!st.fresh) {
+#pragma unroll
+                    for (int c = 0; c < G::NOC; ++c) st.o[rb][c] *= alpha;
+                }
+            }
+        }
+        st.fresh = false;
+    }
+    float p[RB][8];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        const float mref = st.m[rb] < -1.0e29f ? 0.f : st.m[rb];      // (a row that has seen nothing yet: its slots give 0)
+        float psum;
+#pragma unroll
+        for (int idx = 0; idx < 8; ++idx) {
+            p[rb][idx] = fast_exp2(__builtin_fmaf(s[rb][idx], sc, -mref));
+            psum = idx == 0 ? p[rb][0] : psum + p[rb][idx];
+        }
+        st.l[rb] += psum;
+    }
+
+    bool by_row = false;
+    if (mixed) {                                                      // uniform over the wave
+        u32 wild = 0;
+#pragma unroll
+        for (int idx = 0; idx < 8; ++idx)
+#pragma unroll
+            for (int d = 0; d < G::VW; ++d) wild |= Wild<DT>::of(t.v[idx][d]);
+        by_row = __builtin_amdgcn_ballot_w64((wild & Wild<DT>::SIGNS) != 0) != 0;
+    }
+
+    auto products = [&](const u32 (&v)[8][G::VW], auto&& add) {       // add(row block, accumulator, MFMA of them)
+        if constexpr (G::SZ == 2) {
+            u32x4 pp[RB];
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb)
+                pp[rb] = u32x4{Elem<DT>::pack2(p[rb][0], p[rb][1]), Elem<DT>::pack2(p[rb][2], p[rb][3]), Elem<DT>::pack2(p[rb][4], p[rb][5]),
+                               Elem<DT>::pack2(p[rb][6], p[rb][7])};
+#pragma unroll
+            for (int d = 0; d < G::VW; ++d) {
+                u32x4 lo, hi;
+                lo.x = __builtin_amdgcn_perm(v[1][d], v[0][d], 0x05040100u);
+                lo.y = __builtin_amdgcn_perm(v[3][d], v[2][d], 0x05040100u);
+                lo.z = __builtin_amdgcn_perm(v[5][d], v[4][d], 0x05040100u);
+                lo.w = __builtin_amdgcn_perm(v[7][d], v[6][d], 0x05040100u);
+                hi.x = __builtin_amdgcn_perm(v[1][d], v[0][d], 0x07060302u);
+                hi.y = __builtin_amdgcn_perm(v[3][d], v[2][d], 0x07060302u);
+                hi.z = __builtin_amdgcn_perm(v[5][d], v[4][d], 0x07060302u);
+                hi.w = __builtin_amdgcn_perm(v[7][d], v[6][d], 0x07060302u);
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) {
+                    add(rb, 2 * d, [&](f32x4 c) { return Elem<DT>::mfma(lo, pp[rb], c); });
+                    add(rb, 2 * d + 1, [&](f32x4 c) { return Elem<DT>::mfma(hi, pp[rb], c); });
+                }
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < G::NOC; ++c)
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb)
+                    add(rb, c, [&](f32x4 x) {
+#pragma unroll
+                        for (int idx = 0; idx < 8; ++idx) x = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[idx][c]), p[rb][idx], x, 0, 0, 0);
+                        return x;
+                    });
+        }
+    };
+    if (!by_row) {
+        products(t.v, [&](int rb, int c, auto&& mfma) { st.o[rb][c] = mfma(st.o[rb][c]); });
+        return;
+    }
+#pragma unroll 1
+    for (int i = 0; i < 16 * RB; ++i) {
+        Band<1> row;
+        row.lo[0] = __builtin_amdgcn_readlane(RB == 1 || i < 16 ? band.lo[0] : band.lo[RB - 1], i & 15);
+        row.lim[0] = __builtin_amdgcn_readlane(RB == 1 || i < 16 ? band.lim[0] : band.lim[RB - 1], i & 15);
+        row.snk[0] = __builtin_amdgcn_readlane(RB == 1 || i < 16 ? band.snk[0] : band.snk[RB - 1], i & 15);
+        u32 v[8][G::VW];
+#pragma unroll
+        for (int idx = 0; idx < 8; ++idx) {
+            const bool seen = row.sees(0, t0 + slot_token(q, idx));
+#pragma unroll
+            for (int d = 0; d < G::VW; ++d) v[idx][d] = seen ? t.v[idx][d] : 0u;
+        }
+        products(v, [&](int rb, int c, auto&& mfma) {
+            const f32x4 x = mfma(f32x4{0.f, 0.f, 0.f, 0.f});
+            if (rb * 16 + n == i) st.o[rb][c] += x;
+        });
+    }
+}
+
+// Which rows a work item stands for.  Packed queries: the row groups of ROWS rows are numbered through the sequences in order; an item behind
+// the last of them is `spare`, of which there is one at least (the grid is sized for more row groups than there can be).
+struct WindowItem {
+    int w, rg, qs, qe;       // sequence, row group in it, its query tokens
+    bool found;
+    int spare, spares;       // not found: the how manieth of how many
+    int first, end;          // and the query tokens that belong to sequences
+};
+template <int ROWS>
+__device__ __forceinline__ WindowItem window_item(const PagedDevHeader& ph, int item, int lane, int GQ) {
+    WindowItem it = {0, 0, 0, 0, false, 0, 1, 0, 0};
+    const int T = ph.LW * ph.LS;
+    if (ph.cu_q == nullptr) {
+        it.w = fast_div(item, ph.magic_nrg);
+        it.rg = item - it.w * ph.nrg;
+        it.qs = it.w * ph.LS;
+        it.qe = it.qs + ph.LS;
+        it.found = true;
+        return it;
+    }
+    auto bound = [&](int x) { return min(max(x, 0), T); };      // a malformed array must not lead outside the buffers
+    int base = 0;
+    for (int c = 0; c < ph.W && !it.found; c += 64) {
+        const int idx = c + lane;
+        const int a0 = bound(ph.cu_q[min(idx, ph.W)]), a1 = bound(ph.cu_q[min(idx + 1, ph.W)]);
+        const int cnt = idx < ph.W ? (max(a1 - a0, 0) * GQ + ROWS - 1) / ROWS : 0;
+        const int inc = wave_scan_inclusive(cnt);
+        const int total = __builtin_amdgcn_readlane(inc, 63);
+        if (item < base + total) {
+            const int l0 = __builtin_ctzll(__ballot(base + inc > item));
+            it.w = c + l0;
+            it.rg = item - base - __builtin_amdgcn_readlane(inc - cnt, l0);
+            it.qs = __builtin_amdgcn_readlane(a0, l0);
+            it.qe = __builtin_amdgcn_readlane(a1, l0);
+            it.found = true;
+        }
+        base += total;
+    }
+    if (!it.found) {
+        it.spare = item - base;
+        it.spares = ph.nitems - base;
+        it.first = bound(ph.cu_q[0]);
+        it.end = bound(ph.cu_q[ph.W]);
+    }
+    return it;
+}
+
+template <class DT, int D, int RB>
+__global__ __launch_bounds__(NTHREADS, 1) void window_kernel(const WindowHeader args) {
+    typedef Geo<DT, D, D> G;
+    typedef typename Elem<DT>::store_t store_t;
+    constexpr int ROWS = RB * 16;
+    typedef hw::Exchange<ROWS, D> Ex;
+    constexpr int SBYTES = NWAVES * G::KSTAGE;
+    __shared__ __attribute__((aligned(16))) char q_lds[ROWS * G::QSTR];
+    union Slot0 {
+        char k[SBYTES];
+        Ex ex;
+    };
+    __shared__ __attribute__((aligned(16))) Slot0 slot0;
+    __shared__ __attribute__((aligned(16))) char slot1[SBYTES];
+
+    const int tid = threadIdx.x;
+    const int lane = tid & 63;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 15;
+    const int q = lane >> 4;
+    char* const kslots[2] = {slot0.k + wv * G::KSTAGE, slot1 + wv * G::KSTAGE};
+
+    PagedHeaderBits hb;
+    paged_header_request(hb);
+    // K transfer i of a wave covers tile rows i * RPL .. i * RPL + RPL - 1; the bank swizzle is applied on the global side
+    constexpr int RPL = 64 / G::CPR;
+    const int lrow = lane / G::CPR, lslot = lane % G::CPR;
+    auto k_chunk = [&](int i) -> unsigned {
+        const int row = i * RPL + lrow;
+        const int key = G::CPR >= 16 ? (row & 15) : ((row >> 1) & (G::CPR - 1));
+        return (unsigned)((lslot ^ key) << 4);
+    };
+    WaveState<RB, G::NOC> st;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        st.m[rb] = NEG_BIG;
+        st.l[rb] = 0.f;
+#pragma unroll
+        for (int c = 0; c < G::NOC; ++c) st.o[rb][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    st.fresh = true;
+    const PagedDevHeader ph = paged_header_wait(hb);
+    const bool direct = (ph.flags & PH_DIRECT) != 0;
+
+    // logical workgroup id = ((kv head * nitems) + item) * nsplit + split; consecutive ids share an XCD
+    int bid = blockIdx.x;
+    if (ph.flags & PH_XCD_REMAP) bid = (bid & 7) * (ph.nwg >> 3) + (bid >> 3);
+    const int hi = bid / ph.nsplit, split = bid - hi * ph.nsplit;
+    const int hkv = hi / ph.nitems, item = hi - hkv * ph.nitems;
+    const int GQ = ph.Hq / ph.Hkv;
+    const int T = ph.LW * ph.LS;
+    const int cap = ph.block_size * ph.max_blocks;
+
+    const WindowItem it = window_item<ROWS>(ph, item, lane, GQ);
+    if (!it.found) {                        // uniform over the workgroup: zeros for query tokens that belong to no sequence
+        const int before = it.first, rest = before + T - it.end;
+        for (int i = it.spare; i < rest; i += it.spares) {
+            const int t = i < before ? i : it.end + i - before;
+            for (int x = tid; x < GQ * D; x += NTHREADS) {
+                const int g = x / D, e = x - g * D;
+                if (direct) {
+                    const size_t orow = (size_t)t * ph.Hq + hkv * GQ + g;
+                    reinterpret_cast<store_t*>(args.out)[orow * D + e] = Elem<DT>::from_float(0.f);
+                    if (e == 0 && args.lse != nullptr) args.lse[orow] = -__builtin_inff();
+                } else {
+                    const size_t prow = (size_t)(hkv * ph.nsplit + split) * ph.R + (size_t)t * GQ + g;
+                    ph.part_o[prow * D + e] = 0.f;
+                    if (e == 0) *reinterpret_cast<HW_GLOBAL f32x2*>(ph.part_ml + prow * 2) = f32x2{NEG_BIG, 0.f};
+                }
+            }
+        }
+        return;
+    }
+    const int r0 = it.qs * GQ + it.rg * ROWS;    // first row (global numbering: token * GQ + head in group)
+    const int rend = it.qe * GQ;
+    if (r0 >= rend) return;                      // uniform over the workgroup
+    const HW_GLOBAL int* btw = ph.block_table + (size_t)it.w * ph.max_blocks;
+
+    DevHeader a;                                 // what QueryRotation / map_row need, in the [LW, Hq, LS] layout
+    a.q = ph.q;
+    a.loc = ph.loc;
+    a.cos = nullptr;
+    a.sin = nullptr;
+    a.rq = nullptr;
+    a.part_o = ph.part_o;
+    a.part_ml = ph.part_ml;
+    a.len_dev = nullptr;
+    a.F = 1; a.W = ph.LW; a.Hq = ph.Hq; a.Hkv = ph.Hkv; a.S = ph.LS; a.R = rend;
+    a.nrg = 1; a.wgs_per_head = ph.nsplit; a.nwg = ph.nwg;
+    a.slot_stride = ph.nsplit; a.flags = KH_PREROTATED; a.sc = ph.sc;
+    a.magic_gq = ph.magic_gq; a.magic_s = ph.magic_ls; a.magic_nrg = 0; a.magic_wg = 0;
+
+    QueryRotation<DT, D, ROWS, G::QSTR, true> qrot;
+    qrot.load(a, 0, hkv, r0, GQ, tid);
+    const int NW = ph.nsplit * NWAVES, gw = split * NWAVES + wv;
+
+    // The bounds of the rows (lane l: row l % ROWS; behind the last row, that row again), and of the workgroup: tokens [0, sink_end)
+    // and [low, high).
+    const int at = ph.loc[fast_div(min(r0 + (lane & (ROWS - 1)), rend - 1), ph.magic_gq)];
+    const int lim1 = max(0, at < cap ? at + 1 : cap);
+    const int lo1 = max(0, at < 0 ? 0 : at - args.window + 1);
+    const int snk1 = min(args.sinks, lim1);
+    Band<RB> band;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        band.lo[rb] = RB == 1 ? lo1 : __shfl(lo1, rb * 16 + n, 64);
+        band.lim[rb] = RB == 1 ? lim1 : __shfl(lim1, rb * 16 + n, 64);
+        band.snk[rb] = RB == 1 ? snk1 : __shfl(snk1, rb * 16 + n, 64);
+    }
+    const bool any = lo1 < lim1;                 // the row's window holds something
+    const int high = wave_max(any ? lim1 : 0);
+    const int low = -wave_max(any ? -lo1 : -0x7fffffff);
+    const int sink_end = wave_max(snk1);
+    const bool alike = __ballot(at != __builtin_amdgcn_readfirstlane(at)) == 0;        // all rows at one position
+    const int all_from = wave_max(lo1), all_to = -wave_max(-lim1);                     // what every row's window holds
+    const int sink_tiles = (sink_end + TILE - 1) / TILE;
+    const int first = high > 0 ? max(low / TILE, sink_tiles) : 0;                    // first tile of the window
+    const int tiles = sink_tiles + (high > 0 ? max((high + TILE - 1) / TILE - first, 0) : 0);
+    auto tile_at = [&](int k) { return k < sink_tiles ? k : k - sink_tiles + first; };
+
+    // block-table entry of the token this lane stands for in tile t
+    auto bt_load = [&](int t) -> int {
+        const int tok = min(t * TILE + (lane & 31), cap - 1);
+        return btw[fast_div(tok, ph.magic_bs)];
+    };
+    auto mixed = [&](int t) { return !alike && !(t * TILE >= all_from && t * TILE + TILE <= all_to); };
+    // The loads of tile t, given its table entries: the same number of instructions whether or not the tile exists.  Tokens that no row
+    // sees are replaced by one of the tile that some row does (there is one in every tile that exists), so that no byte of the cache
+    // that is not seen is read; what a tile that does not exist reads is not used.
+    auto issue_tile = [&](TileRegs<DT, D, D>& tr, char* kslot, int btv, int t) {
+        const int t0 = t * TILE;
+        const int tok_raw = t0 + (lane & 31);
+        const int tok = min(tok_raw, cap - 1);
+        const int bi = fast_div(tok, ph.magic_bs);
+        const int blk = min(max(btv, 0), ph.num_blocks - 1);
+        int rid = (blk * ph.Hkv + hkv) * ph.block_size + (tok - bi * ph.block_size);
+        const int last = t0 + TILE > low && high > 0 ? high : sink_end;
+        const int jstar = min(max(last - 1 - t0, 0), TILE - 1);
+        const int rstar = __builtin_amdgcn_readlane(rid, jstar);
+        rid = tok_raw < sink_end || (tok_raw >= low && tok_raw < high) ? rid : rstar;
+        asm volatile("" ::: "memory");   // the transfers keep their place between the reads of the slot (see load_tile)
+#pragma unroll
+        for (int i = 0; i < G::KL; ++i) {
+            const int r = __shfl(rid, i * RPL + lrow, 64);
+            const HW_GLOBAL char* src = ph.kcache + (unsigned long long)(unsigned)r * G::KROW + k_chunk(i);
+            __builtin_amdgcn_global_load_lds(src, HW_LDS_PTR(kslot + i * 1024), 16, 0, HW_KV_AUX);
+        }
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int idx = 0; idx < 8; ++idx) {
+            const int r = __shfl(rid, slot_token(q, idx), 64);
+            const HW_GLOBAL char* src = ph.vcache + (unsigned long long)(unsigned)r * G::VROW + n * (G::VLD * 4);
+#pragma unroll
+            for (int hh = 0; hh < G::NVL; ++hh) {
+                if constexpr (G::VLD == 4) {
+                    const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const HW_GLOBAL u32x4*>(src + hh * 256));
+                    tr.v[idx][hh * 4 + 0] = x.x;
+                    tr.v[idx][hh * 4 + 1] = x.y;
+                    tr.v[idx][hh * 4 + 2] = x.z;
+                    tr.v[idx][hh * 4 + 3] = x.w;
+                } else {
+                    const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const HW_GLOBAL u32x2*>(src));
+                    tr.v[idx][0] = x.x;
+                    tr.v[idx][1] = x.y;
+                }
+            }
+        }
+    };
+
+    int bt_a = bt_load(tile_at(gw)), bt_b = bt_load(tile_at(gw + NW));
+    TileRegs<DT, D, D> tr[2];
+    issue_tile(tr[0], kslots[0], bt_a, tile_at(gw));
+    qrot.finish(a, q_lds, 0, hkv, r0, GQ, false, tid);
+    lds_barrier();
+    u32x4 qreg[RB * G::KJ];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+        for (int j = 0; j < G::KJ; ++j)
+            qreg[rb * G::KJ + j] = *reinterpret_cast<const u32x4*>(q_lds + (rb * 16 + n) * G::QSTR + (4 * j + q) * 16);
+
+    // Two tiles in flight per wave: request the table entries two tiles ahead, then the next tile, then compute the current one.
+    for (int k = gw; k < tiles; k += 2 * NW) {
+        {
+            const int bt_n = bt_load(tile_at(k + 2 * NW));
+            issue_tile(tr[1], kslots[1], bt_b, tile_at(k + NW));
+            wait_k_landed<G, 1>();
+            band_tile<DT, D, RB>(tr[0], qreg, band, st, tile_at(k) * TILE, n, q, ph.sc, kslots[0], mixed(tile_at(k)));
+            bt_a = bt_n;
+        }
+        {
+            const int bt_n = bt_load(tile_at(k + 3 * NW));
+            issue_tile(tr[0], kslots[0], bt_a, tile_at(k + 2 * NW));
+            wait_k_landed<G, 1>();
+            if (k + NW < tiles) band_tile<DT, D, RB>(tr[1], qreg, band, st, tile_at(k + NW) * TILE, n, q, ph.sc, kslots[1], mixed(tile_at(k + NW)));
+            bt_b = bt_n;
+        }
+    }
+
+    size_t orow[RB];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) orow[rb] = map_row(a, min(r0 + rb * 16 + n, rend - 1), hkv, GQ).qrow;
+    store_partials<DT, D, RB, true>(st, slot0.ex, wv, n, q, tid,
+                                    direct ? reinterpret_cast<HW_GLOBAL float*>(reinterpret_cast<unsigned long long>(args.out)) : ph.part_o,
+                                    direct ? reinterpret_cast<HW_GLOBAL float*>(reinterpret_cast<unsigned long long>(args.lse)) : ph.part_ml,
+                                    (size_t)(hkv * ph.nsplit + split) * ph.R + r0, min(ROWS, rend - r0), direct, orow);
+}
+
+// ------------------------------------------------------------------------------------------------
+// launchers
+// ------------------------------------------------------------------------------------------------
+template <class DT, int D>
+static hipError_t launch_window_d(const WindowHeader& wh, int rb, hipStream_t stream) {
+    if constexpr (Elem<DT>::size == 2 && D <= 128) {
+        if (rb == 2) {
+            hipLaunchKernelGGL((window_kernel<DT, D, 2>), dim3(wh.p.nwg), dim3(NTHREADS), 0, stream, wh);
+            return hipGetLastError();
+        }
+    }
+    if (rb != 1) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((window_kernel<DT, D, 1>), dim3(wh.p.nwg), dim3(NTHREADS), 0, stream, wh);
+    return hipGetLastError();
+}
+
+template <class DT>
+static hipError_t launch_window_dt(const WindowHeader& wh, int D, int rb, hipStream_t stream) {
+    if (D == 256) {
+        if constexpr (Elem<DT>::size == 2) return launch_window_d<DT, 256>(wh, rb, stream);
+        return hipErrorInvalidValue;
+    }
+    if (D == 128) return launch_window_d<DT, 128>(wh, rb, stream);
+    if (D == 64) return launch_window_d<DT, 64>(wh, rb, stream);
+    return hipErrorInvalidValue;
+}
+
+hipError_t launch_window_attention(const WindowHeader& wh, int dtype, int D, int rb, hipStream_t stream) {
+    switch (dtype) {
+        case 0: return launch_window_dt<F32>(wh, D, rb, stream);
+        case 1: return launch_window_dt<F16>(wh, D, rb, stream);
+        default: return launch_window_dt<BF16>(wh, D, rb, stream);
+    }
+}
+
+}  // namespace hw
