@@ -364,14 +364,16 @@ int window_run(const hw_window_problem* p, void* stream_) {
     std::memset(&wh, 0, sizeof(wh));
     paged_header(&pp, plan, wh.p);
     wh.p.part_o = reinterpret_cast<float*>(p->workspace);
-    if (!direct) wh.p.part_ml = wh.p.part_o + (size_t)p->Hkv * plan.splits * plan.rows * p->D;
+    const bool wide = plan.row_blocks == hw::WIDE_ROW_BLOCKS;
+    const size_t prows = wide ? (size_t)2 * plan.splits * 16 * hw::WIDE_ROW_BLOCKS : (size_t)plan.splits * plan.rows;
+    if (!direct) wh.p.part_ml = wh.p.part_o + (size_t)p->Hkv * prows * p->D;
     wh.p.flags = (plan.workgroups % 8 == 0 ? hw::PH_XCD_REMAP : 0) | (direct ? hw::PH_DIRECT : 0);
     wh.out = p->out;
     wh.lse = p->lse;
     wh.window = p->window;
     wh.sinks = p->sinks;
     const hipError_t e = hw::launch_window_attention(wh, p->dtype, p->D, plan.row_blocks, stream);
-    if (e != hipSuccess || direct) return (int)e;
+    if (e != hipSuccess || direct || wide) return (int)e;      // (128-row groups: merged by the launcher)
     hw::MergeArgs ma;
     std::memset(&ma, 0, sizeof(ma));
     ma.part_o = wh.p.part_o;

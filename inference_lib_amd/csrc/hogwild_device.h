@@ -191,6 +191,23 @@ struct TileRegs {
 #define HW_LDS_PTR(p) ((__attribute__((address_space(3))) void*)(p))
 #define HW_GLOBAL __attribute__((address_space(1)))
 
+// One global->LDS transfer with a 64-bit address per lane (rows that no descriptor could bound: the paged cache, queries): lane l brings 16
+// bytes from `src` to LDS byte `lds` + 16 l, or, with DWORD, 4 bytes to `lds` + 4 l; non-temporal unless KEEP.  From inline assembly, as the
+// compiler would wait for it before every LDS read that it cannot prove disjoint: the kernels wait themselves.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+template <bool KEEP, bool DWORD = false>
+__device__ __forceinline__ void lds_transfer_flat(unsigned lds, unsigned long long src) {
+    if constexpr (DWORD) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(src) : "m0", "memory");
+    else if constexpr (KEEP) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "m0", "memory");
+    else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(lds), "v"(src) : "m0", "memory");
+}
+#pragma clang diagnostic pop
+
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+    return __builtin_amdgcn_readfirstlane((unsigned)(size_t)HW_LDS_PTR(p));
+}
+
 // A fragment's K and V slices of one kv head.  K goes through a buffer resource: out-of-range rows read as zero, so
 // its global->LDS transfers need no address clamping and a tile that does not exist costs no memory traffic.  V is
 // read with plain global loads (measured: a tile's rows land ~15 % sooner than through buffer loads), with rows beyond

@@ -832,6 +832,8 @@ int window_validate(const hw_window_problem* p) {
     return HW_OK;
 }
 
+constexpr int WINDOW_ROWS = 16 * hw::WIDE_ROW_BLOCKS;
+
 int window_plan(const hw_window_problem* p, int num_cus, hw_paged_plan* plan) {
     if (plan == nullptr) return HW_ERR_NULL;
     if (num_cus < 1) return HW_ERR_SHAPE;
@@ -842,8 +844,9 @@ int window_plan(const hw_window_problem* p, int num_cus, hw_paged_plan* plan) {
     plan->rows = tokens * gq;
     const bool two = p->dtype != HW_F32 && p->D <= 128;        // two row blocks: what the registers hold
     const int usual = varlen ? (plan->rows + p->W - 1) / p->W : p->S * gq;      // rows of a sequence, in the mean
-    plan->row_blocks = p->row_blocks != 0 ? p->row_blocks : two && usual > 16 ? 2 : 1;
-    if (plan->row_blocks != 1 && !(plan->row_blocks == 2 && two)) return HW_ERR_UNSUPPORTED;
+    plan->row_blocks = p->row_blocks != 0 ? p->row_blocks : p->dtype != HW_F32 && usual > 32 ? hw::WIDE_ROW_BLOCKS : two && usual > 16 ? 2 : 1;
+    const bool wide = plan->row_blocks == hw::WIDE_ROW_BLOCKS && p->dtype != HW_F32;
+    if (plan->row_blocks != 1 && !(plan->row_blocks == 2 && two) && !wide) return HW_ERR_UNSUPPORTED;
     const int rows = 16 * plan->row_blocks;
     // (packed: one more than there can be, which writes the zeros of tokens that belong to no sequence)
     plan->row_groups = varlen ? (plan->rows + rows - 1) / rows + p->W : p->W * ((p->S * gq + rows - 1) / rows);
@@ -854,6 +857,16 @@ int window_plan(const hw_window_problem* p, int num_cus, hw_paged_plan* plan) {
     const long long tiles = std::min(cap, seen);
     const long long groups = (long long)std::max(plan->row_groups, 1) * p->Hkv;
     long long splits = p->splits;
+    if (wide) {
+        // `splits` workgroups of every kv head share its row groups out (window_wide_kernel): one for every CU, as far as each gets eight
+        // tiles.  Two slots of partial sums each.
+        if (splits == 0) splits = std::min((long long)std::max(num_cus / p->Hkv, 1), std::max(1ll, std::max(plan->row_groups, 1) * tiles / 8));
+        plan->splits = (int)std::min(splits, (long long)HW_MAX_SPLITS);
+        if ((long long)plan->splits * p->Hkv * (WINDOW_ROWS * p->D / 1024) >= (1ll << 31)) return HW_ERR_SHAPE;
+        plan->workgroups = plan->splits * p->Hkv;
+        if (plan->splits > 1) plan->workspace_bytes = (size_t)p->Hkv * 2 * plan->splits * WINDOW_ROWS * ((size_t)p->D + 2) * sizeof(float);
+        return HW_OK;
+    }
     if (splits == 0) splits = std::max(1ll, std::min((num_cus + groups - 1) / groups, tiles / (2 * hw::NWAVES)));
     splits = std::min(splits, (long long)HW_MAX_SPLITS);
     plan->splits = (int)splits;

@@ -85,18 +85,6 @@ __device__ __forceinline__ void lds_transfer(const u32x4& desc, unsigned lds, un
 }
 #pragma clang diagnostic pop
 
-// The same with a 64-bit address per lane (rows that no descriptor could bound: the paged cache, queries): lane l brings 16 bytes
-// from `src` to LDS byte `lds` + 16 l, or, with DWORD, 4 bytes to `lds` + 4 l.
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-template <bool KEEP, bool DWORD = false>
-__device__ __forceinline__ void lds_transfer_flat(unsigned lds, unsigned long long src) {
-    if constexpr (DWORD) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(src) : "m0", "memory");
-    else if constexpr (KEEP) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "m0", "memory");
-    else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(lds), "v"(src) : "m0", "memory");
-}
-#pragma clang diagnostic pop
-
 // One wave's share of a tile's transfers: TPW 1 KB pieces of ONE image (the first half of the waves fill K, the second
 // half V), into LDS bytes `slot` + 1024 j.  `tile` = byte offset of the tile in the kv head's slice (OOB_OFFSET for a
 // tile that does not exist: the same number of transfers, no memory traffic, zeros in LDS).
@@ -104,10 +92,6 @@ template <int TPW, bool KEEP>
 __device__ __forceinline__ void wide_request(const u32x4& desc, unsigned slot, unsigned tile, const unsigned* off) {
 #pragma unroll
     for (int j = 0; j < TPW; ++j) lds_transfer<KEEP>(desc, slot + j * 1024, tile + off[j]);
-}
-
-__device__ __forceinline__ unsigned lds_address(const void* p) {
-    return __builtin_amdgcn_readfirstlane((unsigned)(size_t)HW_LDS_PTR(p));
 }
 
 // What the opening of a fragment needs besides its tiles, for the 128 rows of a workgroup: the queries, the cos/sin table rows of

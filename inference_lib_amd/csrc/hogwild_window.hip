@@ -6,6 +6,8 @@
 // lie in pages.  A workgroup owns one kv head and up to 16 or 32 rows of one sequence.  Its keys are two stretches of the sequence: the
 // sinks, and the union of the rows' windows.  Both are cut into tiles of 32 tokens at multiples of 32, numbered through (tile_at), and
 // tile k goes to wave k mod (4 * nsplit) of the workgroups that share the rows.
+//
+// Sequences with more rows (prompt chunks) go through window_wide_kernel: row groups of 128, whose waves share every tile through LDS.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -430,11 +432,535 @@ __global__ __launch_bounds__(NTHREADS, 1) void window_kernel(const WindowHeader 
                                     (size_t)(hkv * ph.nsplit + split) * ph.R + r0, min(ROWS, rend - r0), direct, orow);
 }
 
+// ---- many rows -------------------------------------------------------------------------------------------------------------------
+//
+// Row groups of 128 rows of one sequence (a last one of fewer), numbered through the sequences, `groups` of them for every kv head.  The
+// `n` workgroups of a head share them out evenly, in the order of the rows: workgroup i takes the stretch [i groups / n, (i + 1) groups / n),
+// and a part of a group is that part of its tiles.  So every workgroup has the same to do where the groups see about the same (the bound of a
+// window), whatever their number, and a group is cut only where it lies across the end of a stretch.  A workgroup that sees a whole group
+// writes its result; parts leave partial sums in the workgroup's two slots (its first group's, and its last one's), which
+// window_merge_kernel adds up.
+
+constexpr int WINDOW_ROWS = 128;
+
+__device__ __forceinline__ int window_groups(const PagedDevHeader& ph, int lane, int GQ) {
+    if (ph.cu_q == nullptr) return ph.W * ph.nrg;
+    const int T = ph.LW * ph.LS;
+    int n = 0;
+    for (int c = 0; c < ph.W; c += 64) {
+        const int idx = c + lane;
+        const int a0 = min(max(ph.cu_q[min(idx, ph.W)], 0), T), a1 = min(max(ph.cu_q[min(idx + 1, ph.W)], 0), T);
+        n += __builtin_amdgcn_readlane(wave_scan_inclusive(idx < ph.W ? (max(a1 - a0, 0) * GQ + WINDOW_ROWS - 1) / WINDOW_ROWS : 0), 63);
+    }
+    return n;
+}
+
+// One 32-token tile, K and V images in LDS, against the wave's RB * 16 rows.  MASKED: some row may not see all of it.
+template <class DT, int D, int RB, bool MASKED>
+__device__ __forceinline__ void band_tile_lds(const u32x4* qreg, const Band<RB>& band, WaveState<RB, D / 16>& st, int t0, int n, int q, float sc,
+                                              const char* kstage, const char* vimg, const unsigned* voff, bool mixed) {
+    typedef Geo<DT, D, D> G;
+    constexpr float LAZY_LOG2 = 8.0f;
+    f32x4 sacc[RB][2];
+    {
+        u32x4 kop[2][G::KJ];
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+            for (int j = 0; j < G::KJ; ++j) kop[tb][j] = *reinterpret_cast<const u32x4*>(kstage + kstage_offset<G>(tb * 16 + n, 4 * j + q));
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+                f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < G::KJ; ++j) acc = Elem<DT>::mfma(kop[tb][j], qreg[rb * G::KJ + j], acc);
+                sacc[rb][tb] = acc;
+            }
+    }
+    // the V^T operands, requested here: LDS answers while the exponentials are taken
+    u32x4 vops[G::NOC];
+#pragma unroll
+    for (int c = 0; c < G::NOC; ++c) {
+        const char* vp = vimg + voff[c];
+        const u32x2 a0 = lds_read_tr16(vp), a1 = lds_read_tr16(vp + 16 * G::VROW);
+        vops[c] = u32x4{a0.x, a0.y, a1.x, a1.y};     // tokens slot_token(q, 0..7) of element 16c + n
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    float s[RB][8], mxl[RB];
+    bool need = false;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        float mx = NEG_BIG;
+#pragma unroll
+        for (int idx = 0; idx < 8; ++idx) {
+            s[rb][idx] = sacc[rb][idx >> 2][idx & 3];
+            if constexpr (MASKED) s[rb][idx] = band.sees(rb, t0 + slot_token(q, idx)) ? s[rb][idx] : NEG_BIG;
+            mx = fmaxf(mx, s[rb][idx]);
+        }
+        mxl[rb] = mx;
+        const float mine = MASKED ? (mx < -1.0e29f ? NEG_BIG : mx * sc) : mx * sc;
+        need = need || (mine > st.m[rb] + LAZY_LOG2);
+    }
+    if (__builtin_amdgcn_ballot_w64(need) != 0) {
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            const float mx = quarter_max(mxl[rb]);
+            const float mxs = MASKED ? (mx < -1.0e29f ? NEG_BIG : mx * sc) : mx * sc;
+            const float mnew = mxs > st.m[rb] + LAZY_LOG2 ? mxs : st.m[rb];
+            const float alpha = fast_exp2(st.m[rb] - mnew);
+            st.m[rb] = mnew;
+            st.l[rb] *= alpha;
+            if (!st.fresh) {
+#pragma unroll
+                for (int c = 0; c < G::NOC; ++c) st.o[rb][c] *= alpha;
+            }
+        }
+    }
+    st.fresh = false;
+    u32x4 pp[RB];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        const float mref = MASKED ? (st.m[rb] < -1.0e29f ? 0.f : st.m[rb]) : st.m[rb];
+        float p[8], psum;
+#pragma unroll
+        for (int idx = 0; idx < 8; ++idx) {
+            p[idx] = fast_exp2(__builtin_fmaf(s[rb][idx], sc, -mref));
+            psum = idx == 0 ? p[0] : psum + p[idx];
+        }
+        st.l[rb] += psum;
+        pp[rb] = u32x4{Elem<DT>::pack2(p[0], p[1]), Elem<DT>::pack2(p[2], p[3]), Elem<DT>::pack2(p[4], p[5]), Elem<DT>::pack2(p[6], p[7])};
+    }
+    if constexpr (MASKED) {
+        if (mixed) {                                                  // uniform over the wave (see band_tile)
+            u32 wild = 0;
+#pragma unroll
+            for (int c = 0; c < G::NOC; ++c)
+#pragma unroll
+                for (int d = 0; d < 4; ++d) wild |= Wild<DT>::of(vops[c][d]);
+            if (__builtin_amdgcn_ballot_w64((wild & Wild<DT>::SIGNS) != 0) != 0) {
+#pragma unroll 1
+                for (int i = 0; i < 16 * RB; ++i) {
+                    Band<1> row;
+                    row.lo[0] = __builtin_amdgcn_readlane(RB == 1 || i < 16 ? band.lo[0] : band.lo[RB - 1], i & 15);
+                    row.lim[0] = __builtin_amdgcn_readlane(RB == 1 || i < 16 ? band.lim[0] : band.lim[RB - 1], i & 15);
+                    row.snk[0] = __builtin_amdgcn_readlane(RB == 1 || i < 16 ? band.snk[0] : band.snk[RB - 1], i & 15);
+                    u32x4 seen;
+#pragma unroll
+                    for (int d = 0; d < 4; ++d)
+                        seen[d] = (row.sees(0, t0 + slot_token(q, 2 * d)) ? 0xffffu : 0u) | (row.sees(0, t0 + slot_token(q, 2 * d + 1)) ? 0xffff0000u : 0u);
+#pragma unroll
+                    for (int c = 0; c < G::NOC; ++c) {                // (read again: held in registers through this loop they cost all others)
+                        const char* vp = vimg + voff[c];
+                        const u32x2 a0 = lds_read_tr16(vp), a1 = lds_read_tr16(vp + 16 * G::VROW);
+                        const u32x4 v = u32x4{a0.x, a0.y, a1.x, a1.y} & seen;
+#pragma unroll
+                        for (int rb = 0; rb < RB; ++rb) {
+                            const f32x4 x = Elem<DT>::mfma(v, pp[rb], f32x4{0.f, 0.f, 0.f, 0.f});
+                            if (rb * 16 + n == i) st.o[rb][c] += x;
+                        }
+                    }
+                }
+                return;
+            }
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < G::NOC; ++c)
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) st.o[rb][c] = Elem<DT>::mfma(vops[c], pp[rb], st.o[rb][c]);
+}
+
+// NW waves; NW / PAR of them differ in their rows, and the PAR waves that share their rows take the tiles of a step in turn and add up
+// their sums at the end.  A tile comes into LDS once per workgroup, into a ring of NS slots in steps of PAR tiles with one barrier each (see
+// paged_wide_kernel, whose ring this is).  The sequence's table entries come the same way: every wave brings those of the 32 tokens of the
+// tiles of a step into a small ring of its own, one transfer a step, DP steps before it forms the addresses.  (A window may lie anywhere
+// in a table of any length.)
+template <class DT, int D, int NS, int NW, int PAR>
+__global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHeader args) {
+    typedef Geo<DT, D, D> G;
+    typedef typename Elem<DT>::store_t store_t;
+    constexpr int NT = NW * 64;
+    constexpr int NRW = NW / PAR;                // waves that differ in their rows
+    constexpr int RB = WINDOW_ROWS / 16 / NRW;   // 16-row blocks of a wave when the group has more than 64 rows
+    constexpr int NSTEP = NS / PAR, DP = NSTEP - 1;
+    constexpr int KBYTES = G::KSTAGE, VBYTES = TILE * G::VROW, SLOT = KBYTES + VBYTES;
+    constexpr int TPW = SLOT / 1024 / NW;        // 1 KB transfers of a wave per tile
+    constexpr int TPS = PAR * TPW;
+    constexpr int RPL = 64 / G::CPR;
+    constexpr int ER = 2 * DP + 1;               // steps of table entries in a wave's ring
+    static_assert(G::SZ == 2 && KBYTES == VBYTES && TPW >= 1 && NS % PAR == 0 && DP >= 1 && (PAR == 1 || PAR == 2) && RB == 2, "16-bit types, 32 rows a wave");
+    constexpr int OSTR = D + 4, REGION = 16 * OSTR;        // floats of a wave at the end: 16 rows, or as many accumulators
+    static_assert(G::NOC * 64 * 4 <= REGION && (NW * REGION + NW * 64 * 2) * 4 <= NS * SLOT, "the blocks of all waves fit into the ring");
+    __shared__ int entries[NW][ER][64];
+    __shared__ __attribute__((aligned(16))) char ring[NS * SLOT];
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int rw = wv % NRW, par = wv / NRW;
+    const int n = lane & 15, q = lane >> 4;
+
+    PagedHeaderBits hb;
+    paged_header_request(hb);
+    // this wave's transfers of a tile (see paged_wide_kernel): with an even number the same rows of both images
+    constexpr bool BOTH = TPW % 2 == 0;
+    constexpr int NI = BOTH ? 2 : 1, NP = TPW / NI;
+    static_assert((KBYTES / 1024) % NP == 0 && NW * NP * NI * 1024 == SLOT, "the waves' pieces tile both images");
+    const bool k_wave = BOTH || wv < NW / 2;
+    const int piece0 = (BOTH ? wv : (k_wave ? wv : wv - NW / 2)) * NP;
+    const int lrow = lane / G::CPR, lslot = lane % G::CPR;
+    unsigned chunk[NI][NP];
+    int trow[NP];
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+        const int row = (piece0 + j) * RPL + lrow;
+        const int key = G::CPR >= 16 ? (row & 15) : ((row >> 1) & (G::CPR - 1));
+        const unsigned kchunk = (unsigned)((lslot ^ key) << 4), vchunk = (unsigned)((lslot ^ (2 * vimg_segment_key<G::VROW>(row))) << 4);
+        trow[j] = row;
+        chunk[0][j] = k_wave ? kchunk : vchunk;
+        if constexpr (BOTH) chunk[1][j] = vchunk;
+    }
+    unsigned my_image[NI];
+    my_image[0] = lds_address(ring) + (k_wave ? 0 : KBYTES) + piece0 * 1024;
+    if constexpr (BOTH) my_image[1] = my_image[0] + KBYTES;
+    const unsigned my_entries = __builtin_amdgcn_readfirstlane(lds_address(entries) + wv * ER * 256);
+    unsigned voff[G::NOC];
+    vtr_lane_offsets<G::VROW>(voff, lane);
+    const PagedDevHeader ph = paged_header_wait(hb);
+
+    int bid = blockIdx.x;                        // kv head * nsplit + workgroup of the head; consecutive ids share an XCD
+    if (ph.flags & PH_XCD_REMAP) bid = (bid & 7) * (ph.nwg >> 3) + (bid >> 3);
+    const int N = ph.nsplit;
+    const int hkv = bid / N, me = bid - hkv * N;
+    const int GQ = ph.Hq / ph.Hkv;
+    const int T = ph.LW * ph.LS;
+    const int cap = ph.block_size * ph.max_blocks;
+    const int groups = window_groups(ph, lane, GQ);
+    unsigned long long image[NI];
+    image[0] = reinterpret_cast<unsigned long long>(k_wave ? ph.kcache : ph.vcache);
+    if constexpr (BOTH) image[1] = reinterpret_cast<unsigned long long>(ph.vcache);
+
+    DevHeader a;                                 // what map_row needs, in the [LW, Hq, LS] layout
+    a.Hq = ph.Hq; a.S = ph.LS;
+    a.magic_gq = ph.magic_gq; a.magic_s = ph.magic_ls;
+
+    const int begin = me * groups, end = begin + groups;          // in n-ths of a group
+    const int group0 = begin / N;
+    for (int g = group0; g * N < end; ++g) {
+        const int from = max(begin - g * N, 0), to = min(end - g * N, N);
+        const WindowItem it = window_item<WINDOW_ROWS>(ph, g, lane, GQ);
+        const int r0 = it.qs * GQ + it.rg * WINDOW_ROWS, rend = min(it.qe * GQ, r0 + WINDOW_ROWS);
+        const bool whole = from == 0 && to == N;
+        const size_t pbase = ((size_t)hkv * 2 * N + 2 * me + (g == group0 ? 0 : 1)) * WINDOW_ROWS;
+        const HW_GLOBAL int* btw = ph.block_table + (size_t)it.w * ph.max_blocks;
+
+        auto run = [&](auto rbx) {
+            constexpr int RBX = decltype(rbx)::value;
+            constexpr int wrows = 16 * RBX;
+            const int w0 = r0 + rw * wrows;              // the wave's first row
+            // the rows' positions: lane l rows l and 64 + l of the group (behind the last row, that row again)
+            const int at0 = ph.loc[fast_div(min(r0 + lane, rend - 1), ph.magic_gq)];
+            const int at1 = ph.loc[fast_div(min(r0 + 64 + lane, rend - 1), ph.magic_gq)];
+            u32x4 qreg[RBX * G::KJ];
+#pragma unroll
+            for (int rb = 0; rb < RBX; ++rb) {
+                const HW_GLOBAL char* qp = ph.q + map_row(a, min(w0 + rb * 16 + n, rend - 1), hkv, GQ).qrow * G::KROW;
+#pragma unroll
+                for (int j = 0; j < G::KJ; ++j) qreg[rb * G::KJ + j] = *reinterpret_cast<const HW_GLOBAL u32x4*>(qp + (4 * j + q) * 16);
+            }
+            auto lim_of = [&](int at) { return max(0, at < cap ? at + 1 : cap); };
+            auto lo_of = [&](int at) { return max(0, at < 0 ? 0 : at - args.window + 1); };
+            const int lim0 = lim_of(at0), lim1 = lim_of(at1), lo0 = lo_of(at0), lo1 = lo_of(at1);
+            const int high = wave_max(max(lo0 < lim0 ? lim0 : 0, lo1 < lim1 ? lim1 : 0));
+            const int low = -wave_max(max(lo0 < lim0 ? -lo0 : -0x7fffffff, lo1 < lim1 ? -lo1 : -0x7fffffff));
+            const int sink_end = min(args.sinks, wave_max(max(lim0, lim1)));
+            const bool alike = __ballot(at0 != __builtin_amdgcn_readfirstlane(at0) || at1 != __builtin_amdgcn_readfirstlane(at0)) == 0;
+            const int all_from = wave_max(max(lo0, lo1)), all_to = -wave_max(max(-lim0, -lim1));
+            Band<RBX> band;
+#pragma unroll
+            for (int rb = 0; rb < RBX; ++rb) {
+                const int rr = rw * wrows + rb * 16;
+                const int at = __shfl(rr < 64 ? at0 : at1, (rr & 63) + n, 64);
+                band.lim[rb] = lim_of(at);
+                band.lo[rb] = lo_of(at);
+                band.snk[rb] = min(args.sinks, band.lim[rb]);
+            }
+            // Tiles: of the sinks; of the windows, those that some row may not see all of (at the lower end, at the upper end), then those
+            // that every row sees completely.
+            const int sink_tiles = (sink_end + TILE - 1) / TILE;
+            const int first = high > 0 ? max(low / TILE, sink_tiles) : 0, last = high > 0 ? max((high + TILE - 1) / TILE, first) : 0;
+            const int full0 = min(max((all_from + TILE - 1) / TILE, first), last), full1 = min(max(all_to / TILE, full0), last);
+            const int n_low = full0 - first, n_part = sink_tiles + n_low + last - full1, tiles = n_part + full1 - full0;
+            auto tile_at = [&](int k) {
+                const int up = k - sink_tiles - n_low;                // number among those of the upper end
+                const int t = k < sink_tiles ? k : up < 0 ? first + k - sink_tiles : full1 + up;
+                return k < n_part ? t : full0 + k - n_part;
+            };
+            const int k0 = tiles * from / N, k1 = tiles * to / N;
+
+            WaveState<RBX, G::NOC> st;
+#pragma unroll
+            for (int rb = 0; rb < RBX; ++rb) {
+                st.m[rb] = NEG_BIG;
+                st.l[rb] = 0.f;
+#pragma unroll
+                for (int c = 0; c < G::NOC; ++c) st.o[rb][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+            st.fresh = true;
+            const bool live = w0 < rend;                              // the wave has rows
+
+            __syncthreads();                                          // everybody is done with the ring (the group before)
+            if (k0 < k1) {                                            // uniform over the workgroup
+                // the table entries of step s: lanes 0..31 those of its first tile's tokens, 32..63 of its second's
+                auto request_entries = [&](int s, int slot) {
+                    const int t = tile_at(k0 + s * PAR + (PAR - 1) * (lane >> 5));
+                    const int tok = min(t * TILE + (lane & 31), cap - 1);
+                    lds_transfer_flat<true, true>(__builtin_amdgcn_readfirstlane(my_entries + slot * 256), reinterpret_cast<unsigned long long>(btw + fast_div(tok, ph.magic_bs)));
+                };
+                // Source addresses of this wave's transfers of step s.  Tokens that no row sees are replaced by one of the tile that some row
+                // sees; what a tile that does not exist reads is not used.
+                auto addresses = [&](unsigned long long* src, int s, int slot) {
+#pragma unroll
+                    for (int pp = 0; pp < PAR; ++pp) {
+                        const int t0 = tile_at(k0 + s * PAR + pp) * TILE;
+                        const int stop = t0 + TILE > low && high > 0 ? high : sink_end;
+                        const int star = min(max(stop - 1 - t0, 0), TILE - 1);
+#pragma unroll
+                        for (int j = 0; j < NP; ++j) {
+                            const int raw = t0 + trow[j];
+                            const int tr = raw < sink_end || (raw >= low && raw < high) ? trow[j] : star;
+                            const int tok = min(t0 + tr, cap - 1);
+                            const int bi = fast_div(tok, ph.magic_bs);
+                            const int blk = min(max(entries[wv][slot][pp * 32 + tr], 0), ph.num_blocks - 1);
+                            const int rid = (blk * ph.Hkv + hkv) * ph.block_size + (tok - bi * ph.block_size);
+#pragma unroll
+                            for (int im = 0; im < NI; ++im) src[(pp * NP + j) * NI + im] = image[im] + (unsigned long long)(unsigned)rid * G::KROW + chunk[im][j];
+                        }
+                    }
+                };
+                auto request = [&](int step_slot, const unsigned long long* src) {
+#pragma unroll
+                    for (int pp = 0; pp < PAR; ++pp)
+#pragma unroll
+                        for (int j = 0; j < NP; ++j)
+#pragma unroll
+                            for (int im = 0; im < NI; ++im)
+                                lds_transfer_flat<true>(__builtin_amdgcn_readfirstlane(my_image[im] + (step_slot * PAR + pp) * SLOT + j * 1024), src[(pp * NP + j) * NI + im]);
+                };
+                // Step i requests the entries of step i + 2 DP + 1 and the tiles of step i + DP, in this order, and forms the addresses of
+                // step i + DP + 1 from the entries that step i - DP requested.  Steps -DP .. -1 here.
+#pragma unroll
+                for (int i = 0; i <= DP; ++i) request_entries(i, i);
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // (queries and positions as well)
+                unsigned long long src[TPS];
+#pragma unroll
+                for (int i = 0; i < DP; ++i) {
+                    addresses(src, i, i);
+                    request_entries(i + DP + 1, i + DP + 1);
+                    request(i, src);
+                }
+                addresses(src, DP, DP);
+                int sl = 0, es = 0, step = 0;                         // ring slots of this step's tiles and entries
+                auto arrive = [&]() {
+                    // this wave's transfers of the step have landed (loads complete in order; those of the DP - 1 steps since may be
+                    // in flight), then every wave's; and every wave has left the step before, whose slots are free
+                    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((DP - 1) * (TPS + 1)) : "memory");
+                    request_entries(step + 2 * DP + 1, es);
+                    request(sl == 0 ? NSTEP - 1 : sl - 1, src);
+                    int es1 = es + DP + 1;
+                    es1 = es1 >= ER ? es1 - ER : es1;
+                    addresses(src, step + DP + 1, es1);
+                };
+                auto next = [&]() {
+                    sl = sl + 1 == NSTEP ? 0 : sl + 1;
+                    es = es + 1 == ER ? 0 : es + 1;
+                    ++step;
+                };
+                // two loops with one instantiation of the tile arithmetic each; waves may change over one step apart
+                int k = k0 + par;
+#pragma unroll 1
+                for (; k - par < k1 && k < n_part; k += PAR) {
+                    arrive();
+                    if (live && k < k1) {
+                        const char* slot = ring + (sl * PAR + par) * SLOT;
+                        band_tile_lds<DT, D, RBX, true>(qreg, band, st, tile_at(k) * TILE, n, q, ph.sc, slot, slot + KBYTES, voff, !alike);
+                    }
+                    next();
+                }
+#pragma unroll 1
+                for (; k - par < k1; k += PAR) {
+                    arrive();
+                    if (live && k < k1) {
+                        const char* slot = ring + (sl * PAR + par) * SLOT;
+                        band_tile_lds<DT, D, RBX, false>(qreg, band, st, 0, n, q, ph.sc, slot, slot + KBYTES, voff, false);
+                    }
+                    next();
+                }
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // the requests behind the last tile, before the ring is used again
+            }
+
+            // The PAR waves that share their rows hold a sum each: block rb goes to wave rb % PAR of them through LDS and is added up there.
+            // Every wave then stores its blocks, staged through LDS so that they leave as whole rows.
+            __syncthreads();
+            float* const regions = reinterpret_cast<float*>(ring);
+            float* const mls = regions + NW * REGION;
+            if constexpr (PAR > 1) {
+#pragma unroll
+                for (int rb = 0; rb < RBX; ++rb) {
+                    const int owner = rw + (rb % PAR) * NRW;
+                    if (owner != wv) {
+#pragma unroll
+                        for (int c = 0; c < G::NOC; ++c) *reinterpret_cast<f32x4*>(regions + owner * REGION + (c * 64 + lane) * 4) = st.o[rb][c];
+                        *reinterpret_cast<f32x2*>(mls + (owner * 64 + lane) * 2) = f32x2{st.m[rb], st.l[rb]};
+                    }
+                }
+                __syncthreads();
+            }
+            float* stage = regions + wv * REGION;
+#pragma unroll
+            for (int rb = 0; rb < RBX; ++rb) {
+                if (rw + (rb % PAR) * NRW != wv) continue;            // uniform over the wave
+                if constexpr (PAR > 1) {
+                    const f32x2 oml = *reinterpret_cast<const f32x2*>(mls + (wv * 64 + lane) * 2);
+                    const float mnew = fmaxf(st.m[rb], oml.x);
+                    const float mine = fast_exp2(st.m[rb] - mnew), theirs = fast_exp2(oml.x - mnew);
+#pragma unroll
+                    for (int c = 0; c < G::NOC; ++c) {
+                        const f32x4 o2 = *reinterpret_cast<const f32x4*>(stage + (c * 64 + lane) * 4);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) st.o[rb][c][i] = st.o[rb][c][i] * mine + o2[i] * theirs;
+                    }
+                    st.l[rb] = st.l[rb] * mine + oml.y * theirs;
+                    st.m[rb] = mnew;
+                }
+                const float lsum = quarter_sum(st.l[rb]);
+                const float scale = !whole ? 1.0f : lsum > 0.f ? 1.0f / lsum : 0.f;
+                const int row0 = w0 + rb * 16;
+                if (q == 0 && row0 + n < rend) {
+                    if (!whole) *reinterpret_cast<HW_GLOBAL f32x2*>(ph.part_ml + (pbase + (row0 - r0) + n) * 2) = f32x2{st.m[rb], lsum};
+                    else if (args.lse != nullptr)
+                        args.lse[map_row(a, row0 + n, hkv, GQ).qrow] = lsum > 0.f ? (st.m[rb] + __builtin_amdgcn_logf(lsum)) * 0.69314718055994530942f : -__builtin_inff();
+                }
+#pragma unroll
+                for (int c = 0; c < G::NOC; ++c) *reinterpret_cast<f32x4*>(stage + n * OSTR + 16 * c + 4 * q) = st.o[rb][c] * scale;
+                const int nvalid = min(16, rend - row0);
+#pragma unroll
+                for (int ps = 0; ps < 16 * D / 256; ++ps) {
+                    const int idx = ps * 256 + lane * 4;
+                    const int rr = idx / D, e = idx % D;
+                    if (rr < nvalid) {
+                        const f32x4 x = *reinterpret_cast<const f32x4*>(stage + rr * OSTR + e);
+                        if (whole)
+                            *reinterpret_cast<u32x2*>(reinterpret_cast<store_t*>(args.out) + map_row(a, row0 + rr, hkv, GQ).qrow * D + e) =
+                                u32x2{Elem<DT>::pack2(x[0], x[1]), Elem<DT>::pack2(x[2], x[3])};
+                        else
+                            *reinterpret_cast<HW_GLOBAL f32x4*>(ph.part_o + (pbase + (row0 - r0)) * D + idx) = x;
+                    }
+                }
+            }
+        };
+        if (rend - r0 <= WINDOW_ROWS / 2) run(std::integral_constant<int, RB / 2>{});
+        else run(std::integral_constant<int, RB>{});
+    }
+
+    if (ph.cu_q != nullptr) {                    // zeros for query tokens that belong to no sequence
+        const int before = min(max(ph.cu_q[0], 0), T), after = min(max(ph.cu_q[ph.W], 0), T), rest = before + T - after;
+        for (int i = me; i < rest; i += N) {
+            const size_t orow = (size_t)(i < before ? i : after + i - before) * ph.Hq + hkv * GQ;
+            for (int x = tid; x < GQ * D; x += NT) reinterpret_cast<store_t*>(args.out)[orow * D + x] = 0;
+            if (args.lse != nullptr)
+                for (int x = tid; x < GQ; x += NT) args.lse[orow + x] = -__builtin_inff();
+        }
+    }
+}
+
+// The groups that lie across workgroups: workgroup j of the launch's (kv head, j, 8 rows) takes those rows of the group that workgroup j of
+// the attention kernel began and did not end.  32 lanes and more a row; parts in their order.
+template <class DT, int D>
+__global__ __launch_bounds__(256) void window_merge_kernel(const WindowHeader args) {
+    typedef typename Elem<DT>::store_t store_t;
+    constexpr int V4 = D / 4, ROWS = 256 / V4, UN = 8;
+    const PagedHeader& h = args.p;
+    const int tid = threadIdx.x, lane = tid & 63;
+    PagedDevHeader ph;
+    {
+        PagedHeaderBits hb;
+        paged_header_request(hb);
+        ph = paged_header_wait(hb);
+    }
+    const int N = h.nsplit, GQ = h.Hq / h.Hkv;
+    constexpr int BLOCKS = WINDOW_ROWS / ROWS;
+    const int rblk = blockIdx.x % BLOCKS, hj = blockIdx.x / BLOCKS;
+    const int hkv = hj / N, j = hj - hkv * N;
+    const int groups = window_groups(ph, lane, GQ);
+    const int end = (j + 1) * groups;
+    if (groups == 0 || end % N == 0) return;     // the last group ends here
+    const int g = end / N;
+    const int w0 = g * N / groups, w1 = ((g + 1) * N - 1) / groups;       // its workgroups
+    if (w0 != j) return;
+    const WindowItem it = window_item<WINDOW_ROWS>(ph, g, lane, GQ);
+    const int r0 = it.qs * GQ + it.rg * WINDOW_ROWS, rend = min(it.qe * GQ, r0 + WINDOW_ROWS);
+    const int rr = rblk * ROWS + tid / V4, e = tid % V4 * 4;
+    if (r0 + rr >= rend) return;
+    // (the slot of workgroup w: its first group's, or, for the one that begins the group in the middle of its stretch, the other)
+    auto row_of = [&](int w) { return ((size_t)hkv * 2 * N + 2 * w + (w * groups / N == g ? 0 : 1)) * WINDOW_ROWS + rr; };
+    float m = NEG_BIG, l = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int w = w0; w <= w1; w += UN) {
+        f32x4 o[UN];
+        f32x2 ml[UN];
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            const size_t row = row_of(min(w + u, w1));
+            o[u] = *reinterpret_cast<const f32x4*>(h.part_o + row * D + e);
+            ml[u] = *reinterpret_cast<const f32x2*>(h.part_ml + row * 2);
+            if (w + u > w1) {
+                ml[u] = f32x2{NEG_BIG, 0.f};
+                o[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+        }
+        float mb = m;
+#pragma unroll
+        for (int u = 0; u < UN; ++u) mb = fmaxf(mb, ml[u].x);
+        const float old = fast_exp2(m - mb);
+        acc *= old;
+        l *= old;
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            const float x = fast_exp2(ml[u].x - mb);
+            acc += o[u] * x;
+            l += ml[u].y * x;
+        }
+        m = mb;
+    }
+    const float inv = l > 0.f ? 1.0f / l : 0.f;
+    const int row = r0 + rr, ws = row / GQ, head = hkv * GQ + row - ws * GQ, w = ws / h.LS;
+    const size_t orow = ((size_t)w * h.Hq + head) * h.LS + (ws - w * h.LS);
+    *reinterpret_cast<u32x2*>(reinterpret_cast<store_t*>(args.out) + orow * D + e) =
+        u32x2{Elem<DT>::pack2(acc[0] * inv, acc[1] * inv), Elem<DT>::pack2(acc[2] * inv, acc[3] * inv)};
+    if (args.lse != nullptr && e == 0) args.lse[orow] = l > 0.f ? (m + __builtin_amdgcn_logf(l)) * 0.69314718055994530942f : -__builtin_inff();
+}
+
 // ------------------------------------------------------------------------------------------------
 // launchers
 // ------------------------------------------------------------------------------------------------
+template <class DT, int D, int NS, int NW, int PAR>
+static hipError_t launch_window_wide(const WindowHeader& wh, hipStream_t stream) {
+    hipLaunchKernelGGL((window_wide_kernel<DT, D, NS, NW, PAR>), dim3(wh.p.nwg), dim3(NW * 64), 0, stream, wh);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || wh.p.nsplit == 1) return e;
+    hipLaunchKernelGGL((window_merge_kernel<DT, D>), dim3(wh.p.nwg * (WINDOW_ROWS * D / 1024)), dim3(256), 0, stream, wh);
+    return hipGetLastError();
+}
+
 template <class DT, int D>
 static hipError_t launch_window_d(const WindowHeader& wh, int rb, hipStream_t stream) {
+    if constexpr (Elem<DT>::size == 2) {
+        if (rb == WIDE_ROW_BLOCKS) {
+            if constexpr (D == 256) return launch_window_wide<DT, D, 4, 4, 1>(wh, stream);
+            else return launch_window_wide<DT, D, 6, 8, 2>(wh, stream);
+        }
+    }
     if constexpr (Elem<DT>::size == 2 && D <= 128) {
         if (rb == 2) {
             hipLaunchKernelGGL((window_kernel<DT, D, 2>), dim3(wh.p.nwg), dim3(NTHREADS), 0, stream, wh);
