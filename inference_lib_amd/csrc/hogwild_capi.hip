@@ -365,7 +365,7 @@ int window_run(const hw_window_problem* p, void* stream_) {
     paged_header(&pp, plan, wh.p);
     wh.p.part_o = reinterpret_cast<float*>(p->workspace);
     const bool wide = plan.row_blocks == hw::WIDE_ROW_BLOCKS;
-    const size_t prows = wide ? (size_t)2 * plan.splits * 16 * hw::WIDE_ROW_BLOCKS : (size_t)plan.splits * plan.rows;
+    const size_t prows = wide ? (size_t)2 * plan.splits * (p->D == 256 ? hw::WINDOW_ROWS_256 : hw::WINDOW_ROWS) : (size_t)plan.splits * plan.rows;
     if (!direct) wh.p.part_ml = wh.p.part_o + (size_t)p->Hkv * prows * p->D;
     wh.p.flags = (plan.workgroups % 8 == 0 ? hw::PH_XCD_REMAP : 0) | (direct ? hw::PH_DIRECT : 0);
     wh.out = p->out;

@@ -7,7 +7,7 @@
 // sinks, and the union of the rows' windows.  Both are cut into tiles of 32 tokens at multiples of 32, numbered through (tile_at), and
 // tile k goes to wave k mod (4 * nsplit) of the workgroups that share the rows.
 //
-// Sequences with more rows (prompt chunks) go through window_wide_kernel: row groups of 128, whose waves share every tile through LDS.
+// Sequences with more rows (prompt chunks) go through window_wide_kernel: row groups of 256, whose waves share every tile through LDS.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -25,18 +25,54 @@ struct Band {
     __device__ __forceinline__ bool sees(int rb, int tok) const { return tok < snk[rb] || (tok >= lo[rb] && tok < lim[rb]); }
 };
 
-// Not 0 under SIGNS: one of the two 16-bit elements (the 32-bit one) of the word is infinite or NaN, its exponent all ones.
+// Infinite and NaN values.  A row's weight of a token that it does not see is 0, which times an infinite value would be NaN.  Tiles of which
+// rows see different tokens are therefore looked over, and where one holds such values the products take 0 in their place, and every
+// row that sees one gets it by itself: with ones in the place of the values and of the weights that are seen, a product is more than 0 where a
+// row sees a value of the kind.  NaN counts as both infinities, whose sum it is.
 template <class DT>
 struct Wild {
-    static constexpr u32 EXP = Elem<DT>::size == 4 ? 0x7f800000u : std::is_same<DT, F16>::value ? 0x7c007c00u : 0x7f807f80u;
-    static constexpr u32 ONE = Elem<DT>::size == 4 ? 0x00800000u : std::is_same<DT, F16>::value ? 0x04000400u : 0x00800080u;
-    static constexpr u32 SIGNS = Elem<DT>::size == 4 ? 0x80000000u : 0x80008000u;
-    static __device__ __forceinline__ u32 of(u32 x) { return (x & EXP) + ONE; }
+    static constexpr bool WIDE = Elem<DT>::size == 4;
+    static constexpr u32 EXP = WIDE ? 0x7f800000u : std::is_same<DT, F16>::value ? 0x7c00u : 0x7f80u;
+    static constexpr u32 ONE = WIDE ? 0x3f800000u : std::is_same<DT, F16>::value ? 0x3c00u : 0x3f80u;
+    static constexpr u32 SIGN = WIDE ? 0x80000000u : 0x8000u;
+    static constexpr u32 LOW = EXP & (0u - EXP);                // the exponent's lowest bit
+    static constexpr u32 TWO = WIDE ? 1u : 0x10001u;
+    // not 0 under the signs: an element's exponent is all ones
+    static __device__ __forceinline__ u32 signs(u32 x) { return (x & EXP * TWO) + LOW * TWO; }
+    static constexpr u32 SIGNS = SIGN * TWO;
+    // element by element: `clean` the finite ones, `pos` and `neg` ones where they are infinite in that direction or NaN
+    static __device__ __forceinline__ void split(u32 x, u32& clean, u32& pos, u32& neg) {
+        clean = pos = neg = 0;
+#pragma unroll
+        for (int h = 0; h < (WIDE ? 1 : 2); ++h) {
+            const u32 e = WIDE ? x : (x >> (16 * h)) & 0xffffu;
+            const bool wild = (e & EXP) == EXP, nan = wild && (e & (SIGN - 1) & ~EXP) != 0;
+            clean |= wild ? 0u : e << (16 * h);
+            pos |= wild && (nan || (e & SIGN) == 0) ? ONE << (16 * h) : 0u;
+            neg |= wild && (nan || (e & SIGN) != 0) ? ONE << (16 * h) : 0u;
+        }
+    }
+    // the ones of a lane's eight tokens that row block rb of the band sees, as MFMA operands (16-bit types)
+    template <int RB>
+    static __device__ __forceinline__ u32x4 seen(const Band<RB>& band, int rb, int t0, int q) {
+        u32x4 r;
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+            r[d] = (band.sees(rb, t0 + slot_token(q, 2 * d)) ? ONE : 0u) | (band.sees(rb, t0 + slot_token(q, 2 * d + 1)) ? ONE << 16 : 0u);
+        return r;
+    }
+    static __device__ __forceinline__ f32x4 add(f32x4 o, f32x4 pos, f32x4 neg) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            o[i] += pos[i] > 0.f ? __builtin_inff() : 0.f;
+            o[i] -= neg[i] > 0.f ? __builtin_inff() : 0.f;
+        }
+        return o;
+    }
 };
 
 // One 32-token tile against all rows of the wave: K in the staging slot, V in registers (see compute_tile, whose layouts these are).
-// A row's weight of a token that it does not see is 0, which times an infinite value would be NaN: where the tile holds one, the products
-// with V are taken row by row, from the values that the row sees.  mixed: the rows do not all see the same of its tokens.
+// mixed: the rows do not all see the same of its tokens.
 template <class DT, int D, int RB>
 __device__ __forceinline__ void band_tile(const TileRegs<DT, D, D>& t, const u32x4* qreg, const Band<RB>& band, WaveState<RB, D / 16>& st, int t0, int n, int q,
                                           float sc, const char* kstage, bool mixed) {
@@ -107,74 +143,76 @@ __device__ __forceinline__ void band_tile(const TileRegs<DT, D, D>& t, const u32
         st.l[rb] += psum;
     }
 
-    bool by_row = false;
+    bool wild = false;
     if (mixed) {                                                      // uniform over the wave
-        u32 wild = 0;
+        u32 any = 0;
 #pragma unroll
         for (int idx = 0; idx < 8; ++idx)
 #pragma unroll
-            for (int d = 0; d < G::VW; ++d) wild |= Wild<DT>::of(t.v[idx][d]);
-        by_row = __builtin_amdgcn_ballot_w64((wild & Wild<DT>::SIGNS) != 0) != 0;
+            for (int d = 0; d < G::VW; ++d) any |= Wild<DT>::signs(t.v[idx][d]);
+        wild = __builtin_amdgcn_ballot_w64((any & Wild<DT>::SIGNS) != 0) != 0;
     }
-
-    auto products = [&](const u32 (&v)[8][G::VW], auto&& add) {       // add(row block, accumulator, MFMA of them)
+    auto products = [&](auto wild_tag) {
+        constexpr bool WILD = decltype(wild_tag)::value;
         if constexpr (G::SZ == 2) {
-            u32x4 pp[RB];
+            u32x4 pp[RB], seen[RB];
 #pragma unroll
-            for (int rb = 0; rb < RB; ++rb)
+            for (int rb = 0; rb < RB; ++rb) {
                 pp[rb] = u32x4{Elem<DT>::pack2(p[rb][0], p[rb][1]), Elem<DT>::pack2(p[rb][2], p[rb][3]), Elem<DT>::pack2(p[rb][4], p[rb][5]),
                                Elem<DT>::pack2(p[rb][6], p[rb][7])};
+                if constexpr (WILD) seen[rb] = Wild<DT>::seen(band, rb, t0, q);
+            }
 #pragma unroll
-            for (int d = 0; d < G::VW; ++d) {
-                u32x4 lo, hi;
-                lo.x = __builtin_amdgcn_perm(v[1][d], v[0][d], 0x05040100u);
-                lo.y = __builtin_amdgcn_perm(v[3][d], v[2][d], 0x05040100u);
-                lo.z = __builtin_amdgcn_perm(v[5][d], v[4][d], 0x05040100u);
-                lo.w = __builtin_amdgcn_perm(v[7][d], v[6][d], 0x05040100u);
-                hi.x = __builtin_amdgcn_perm(v[1][d], v[0][d], 0x07060302u);
-                hi.y = __builtin_amdgcn_perm(v[3][d], v[2][d], 0x07060302u);
-                hi.z = __builtin_amdgcn_perm(v[5][d], v[4][d], 0x07060302u);
-                hi.w = __builtin_amdgcn_perm(v[7][d], v[6][d], 0x07060302u);
+            for (int c = 0; c < G::NOC; ++c) {
+                const int d = c / 2;                                  // dword d of a V row: the lane's elements for accumulators 2d and 2d + 1
+                const u32 pick = c % 2 == 0 ? 0x05040100u : 0x07060302u;
+                u32x4 v;
+                v.x = __builtin_amdgcn_perm(t.v[1][d], t.v[0][d], pick);
+                v.y = __builtin_amdgcn_perm(t.v[3][d], t.v[2][d], pick);
+                v.z = __builtin_amdgcn_perm(t.v[5][d], t.v[4][d], pick);
+                v.w = __builtin_amdgcn_perm(t.v[7][d], t.v[6][d], pick);
+                if constexpr (WILD) {
+                    u32x4 pos, neg;
 #pragma unroll
-                for (int rb = 0; rb < RB; ++rb) {
-                    add(rb, 2 * d, [&](f32x4 c) { return Elem<DT>::mfma(lo, pp[rb], c); });
-                    add(rb, 2 * d + 1, [&](f32x4 c) { return Elem<DT>::mfma(hi, pp[rb], c); });
+                    for (int i = 0; i < 4; ++i) {
+                        u32 a, b, e;
+                        Wild<DT>::split(v[i], a, b, e);
+                        v[i] = a;
+                        pos[i] = b;
+                        neg[i] = e;
+                    }
+                    const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int rb = 0; rb < RB; ++rb) st.o[rb][c] = Wild<DT>::add(st.o[rb][c], Elem<DT>::mfma(pos, seen[rb], z), Elem<DT>::mfma(neg, seen[rb], z));
                 }
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) st.o[rb][c] = Elem<DT>::mfma(v, pp[rb], st.o[rb][c]);
             }
         } else {
 #pragma unroll
             for (int c = 0; c < G::NOC; ++c)
 #pragma unroll
-                for (int rb = 0; rb < RB; ++rb)
-                    add(rb, c, [&](f32x4 x) {
+                for (int rb = 0; rb < RB; ++rb) {
+                    [[maybe_unused]] f32x4 pos = {0.f, 0.f, 0.f, 0.f}, neg = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                        for (int idx = 0; idx < 8; ++idx) x = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[idx][c]), p[rb][idx], x, 0, 0, 0);
-                        return x;
-                    });
+                    for (int idx = 0; idx < 8; ++idx) {
+                        u32 v = t.v[idx][c];
+                        if constexpr (WILD) {
+                            const float seen = band.sees(rb, t0 + slot_token(q, idx)) ? 1.0f : 0.f;
+                            u32 a, b, e;
+                            Wild<DT>::split(v, a, b, e);
+                            v = a;
+                            pos = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(b), seen, pos, 0, 0, 0);
+                            neg = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(e), seen, neg, 0, 0, 0);
+                        }
+                        st.o[rb][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v), p[rb][idx], st.o[rb][c], 0, 0, 0);
+                    }
+                    if constexpr (WILD) st.o[rb][c] = Wild<DT>::add(st.o[rb][c], pos, neg);
+                }
         }
     };
-    if (!by_row) {
-        products(t.v, [&](int rb, int c, auto&& mfma) { st.o[rb][c] = mfma(st.o[rb][c]); });
-        return;
-    }
-#pragma unroll 1
-    for (int i = 0; i < 16 * RB; ++i) {
-        Band<1> row;
-        row.lo[0] = __builtin_amdgcn_readlane(RB == 1 || i < 16 ? band.lo[0] : band.lo[RB - 1], i & 15);
-        row.lim[0] = __builtin_amdgcn_readlane(RB == 1 || i < 16 ? band.lim[0] : band.lim[RB - 1], i & 15);
-        row.snk[0] = __builtin_amdgcn_readlane(RB == 1 || i < 16 ? band.snk[0] : band.snk[RB - 1], i & 15);
-        u32 v[8][G::VW];
-#pragma unroll
-        for (int idx = 0; idx < 8; ++idx) {
-            const bool seen = row.sees(0, t0 + slot_token(q, idx));
-#pragma unroll
-            for (int d = 0; d < G::VW; ++d) v[idx][d] = seen ? t.v[idx][d] : 0u;
-        }
-        products(v, [&](int rb, int c, auto&& mfma) {
-            const f32x4 x = mfma(f32x4{0.f, 0.f, 0.f, 0.f});
-            if (rb * 16 + n == i) st.o[rb][c] += x;
-        });
-    }
+    if (wild) products(std::true_type{});
+    else products(std::false_type{});
 }
 
 // Which rows a work item stands for.  Packed queries: the row groups of ROWS rows are numbered through the sequences in order; an item behind
@@ -434,25 +472,70 @@ __global__ __launch_bounds__(NTHREADS, 1) void window_kernel(const WindowHeader 
 
 // ---- many rows -------------------------------------------------------------------------------------------------------------------
 //
-// Row groups of 128 rows of one sequence (a last one of fewer), numbered through the sequences, `groups` of them for every kv head.  The
-// `n` workgroups of a head share them out evenly, in the order of the rows: workgroup i takes the stretch [i groups / n, (i + 1) groups / n),
-// and a part of a group is that part of its tiles.  So every workgroup has the same to do where the groups see about the same (the bound of a
-// window), whatever their number, and a group is cut only where it lies across the end of a stretch.  A workgroup that sees a whole group
-// writes its result; parts leave partial sums in the workgroup's two slots (its first group's, and its last one's), which
-// window_merge_kernel adds up.
+// Row groups of ROWS rows of one sequence (a last one of fewer), numbered through the sequences, `all` of them for every kv head.  The n
+// workgroups of a head take q = all / n whole groups each, and share the rest of them out evenly, in the order of the rows: workgroup i takes
+// the stretch [i rest / n, (i + 1) rest / n) of them, and a part of a group is that part of its tiles.  So every workgroup has the same to do
+// where the groups see about the same (the bound of a window), whatever their number.  A workgroup that sees a whole group writes its
+// result; parts leave partial sums in the workgroup's two slots (its first group's, and its last one's), which window_merge_kernel adds
+// up.
 
-constexpr int WINDOW_ROWS = 128;
+constexpr int VMCNT_0 = 0x0f70;          // s_waitcnt: no vector memory operation outstanding, the other counters as they are
 
-__device__ __forceinline__ int window_groups(const PagedDevHeader& ph, int lane, int GQ) {
-    if (ph.cu_q == nullptr) return ph.W * ph.nrg;
-    const int T = ph.LW * ph.LS;
-    int n = 0;
-    for (int c = 0; c < ph.W; c += 64) {
-        const int idx = c + lane;
-        const int a0 = min(max(ph.cu_q[min(idx, ph.W)], 0), T), a1 = min(max(ph.cu_q[min(idx + 1, ph.W)], 0), T);
-        n += __builtin_amdgcn_readlane(wave_scan_inclusive(idx < ph.W ? (max(a1 - a0, 0) * GQ + WINDOW_ROWS - 1) / WINDOW_ROWS : 0), 63);
+struct Deal {
+    int all, whole, rest;                // row groups of a kv head; whole ones of a workgroup; what is shared out
+    // the first 64 sequences, one a lane: their query tokens, row groups, and the groups up to and with them
+    int qs, qe, count, upto;
+};
+__device__ __forceinline__ int bounded(int x, int T) { return min(max(x, 0), T); }        // a malformed array must not lead outside the buffers
+template <int ROWS>
+__device__ __forceinline__ Deal window_deal(const PagedDevHeader& ph, int n, int lane, int GQ) {
+    Deal d = {0, 0, 0, 0, 0, 0, 0};
+    if (ph.cu_q == nullptr) d.all = ph.W * ph.nrg;
+    else {
+        const int T = ph.LW * ph.LS;
+        for (int c = 0; c < ph.W; c += 64) {
+            const int idx = c + lane;
+            const int a0 = bounded(ph.cu_q[min(idx, ph.W)], T), a1 = bounded(ph.cu_q[min(idx + 1, ph.W)], T);
+            const int cnt = idx < ph.W ? (max(a1 - a0, 0) * GQ + ROWS - 1) / ROWS : 0;
+            const int inc = wave_scan_inclusive(cnt);
+            if (c == 0) {
+                d.qs = a0;
+                d.qe = a1;
+                d.count = cnt;
+                d.upto = inc;
+            }
+            d.all += __builtin_amdgcn_readlane(inc, 63);
+        }
     }
-    return n;
+    d.whole = d.all / n;
+    d.rest = d.all - d.whole * n;
+    // (almost a group each: whole ones to as many workgroups take about as long, and nothing is left to merge)
+    if (d.rest * 8 > n * 7) {
+        ++d.whole;
+        d.rest = 0;
+    }
+    return d;
+}
+// Row group g < all: sequence, number in it, query tokens.
+struct WindowGroup {
+    int w, rg, qs, qe;
+};
+template <int ROWS>
+__device__ __forceinline__ WindowGroup window_group(const PagedDevHeader& ph, const Deal& d, int g, int lane, int GQ) {
+    WindowGroup r;
+    if (ph.cu_q != nullptr && ph.W <= 64) {
+        r.w = __builtin_ctzll(__ballot(d.upto > g));
+        r.rg = g - __builtin_amdgcn_readlane(d.upto - d.count, r.w);
+        r.qs = __builtin_amdgcn_readlane(d.qs, r.w);
+        r.qe = __builtin_amdgcn_readlane(d.qe, r.w);
+    } else {
+        const WindowItem it = window_item<ROWS>(ph, g, lane, GQ);
+        r.w = it.w;
+        r.rg = it.rg;
+        r.qs = it.qs;
+        r.qe = it.qe;
+    }
+    return r;
 }
 
 // One 32-token tile, K and V images in LDS, against the wave's RB * 16 rows.  MASKED: some row may not see all of it.
@@ -492,10 +575,14 @@ __device__ __forceinline__ void band_tile_lds(const u32x4* qreg, const Band<RB>&
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
         float mx = NEG_BIG;
+        // (counted from the lane's first token: one subtraction and two comparisons a logit)
+        const int base = t0 + slot_token(q, 0);
+        [[maybe_unused]] const unsigned from = MASKED ? band.lo[rb] - base : 0, len = MASKED ? max(band.lim[rb] - band.lo[rb], 0) : 0;
+        [[maybe_unused]] const int sink = MASKED ? band.snk[rb] - base : 0;
 #pragma unroll
         for (int idx = 0; idx < 8; ++idx) {
             s[rb][idx] = sacc[rb][idx >> 2][idx & 3];
-            if constexpr (MASKED) s[rb][idx] = band.sees(rb, t0 + slot_token(q, idx)) ? s[rb][idx] : NEG_BIG;
+            if constexpr (MASKED) s[rb][idx] = (unsigned)slot_token(0, idx) - from < len || slot_token(0, idx) < sink ? s[rb][idx] : NEG_BIG;
             mx = fmaxf(mx, s[rb][idx]);
         }
         mxl[rb] = mx;
@@ -532,36 +619,31 @@ __device__ __forceinline__ void band_tile_lds(const u32x4* qreg, const Band<RB>&
         pp[rb] = u32x4{Elem<DT>::pack2(p[0], p[1]), Elem<DT>::pack2(p[2], p[3]), Elem<DT>::pack2(p[4], p[5]), Elem<DT>::pack2(p[6], p[7])};
     }
     if constexpr (MASKED) {
-        if (mixed) {                                                  // uniform over the wave (see band_tile)
-            u32 wild = 0;
+        if (mixed) {                                                  // uniform over the wave
+            u32 any = 0;
 #pragma unroll
             for (int c = 0; c < G::NOC; ++c)
 #pragma unroll
-                for (int d = 0; d < 4; ++d) wild |= Wild<DT>::of(vops[c][d]);
-            if (__builtin_amdgcn_ballot_w64((wild & Wild<DT>::SIGNS) != 0) != 0) {
-#pragma unroll 1
-                for (int i = 0; i < 16 * RB; ++i) {
-                    Band<1> row;
-                    row.lo[0] = __builtin_amdgcn_readlane(RB == 1 || i < 16 ? band.lo[0] : band.lo[RB - 1], i & 15);
-                    row.lim[0] = __builtin_amdgcn_readlane(RB == 1 || i < 16 ? band.lim[0] : band.lim[RB - 1], i & 15);
-                    row.snk[0] = __builtin_amdgcn_readlane(RB == 1 || i < 16 ? band.snk[0] : band.snk[RB - 1], i & 15);
-                    u32x4 seen;
+                for (int d = 0; d < 4; ++d) any |= Wild<DT>::signs(vops[c][d]);
+            if (__builtin_amdgcn_ballot_w64((any & Wild<DT>::SIGNS) != 0) != 0) {
+                u32x4 seen[RB];
 #pragma unroll
-                    for (int d = 0; d < 4; ++d)
-                        seen[d] = (row.sees(0, t0 + slot_token(q, 2 * d)) ? 0xffffu : 0u) | (row.sees(0, t0 + slot_token(q, 2 * d + 1)) ? 0xffff0000u : 0u);
+                for (int rb = 0; rb < RB; ++rb) seen[rb] = Wild<DT>::seen(band, rb, t0, q);
 #pragma unroll
-                    for (int c = 0; c < G::NOC; ++c) {                // (read again: held in registers through this loop they cost all others)
-                        const char* vp = vimg + voff[c];
-                        const u32x2 a0 = lds_read_tr16(vp), a1 = lds_read_tr16(vp + 16 * G::VROW);
-                        const u32x4 v = u32x4{a0.x, a0.y, a1.x, a1.y} & seen;
+                for (int c = 0; c < G::NOC; ++c) {
+                    u32x4 pos, neg;
 #pragma unroll
-                        for (int rb = 0; rb < RB; ++rb) {
-                            const f32x4 x = Elem<DT>::mfma(v, pp[rb], f32x4{0.f, 0.f, 0.f, 0.f});
-                            if (rb * 16 + n == i) st.o[rb][c] += x;
-                        }
+                    for (int i = 0; i < 4; ++i) {
+                        u32 x, y, z;
+                        Wild<DT>::split(vops[c][i], x, y, z);
+                        vops[c][i] = x;
+                        pos[i] = y;
+                        neg[i] = z;
                     }
+                    const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int rb = 0; rb < RB; ++rb) st.o[rb][c] = Wild<DT>::add(st.o[rb][c], Elem<DT>::mfma(pos, seen[rb], z), Elem<DT>::mfma(neg, seen[rb], z));
                 }
-                return;
             }
         }
     }
@@ -571,61 +653,47 @@ __device__ __forceinline__ void band_tile_lds(const u32x4* qreg, const Band<RB>&
         for (int rb = 0; rb < RB; ++rb) st.o[rb][c] = Elem<DT>::mfma(vops[c], pp[rb], st.o[rb][c]);
 }
 
-// NW waves; NW / PAR of them differ in their rows, and the PAR waves that share their rows take the tiles of a step in turn and add up
-// their sums at the end.  A tile comes into LDS once per workgroup, into a ring of NS slots in steps of PAR tiles with one barrier each (see
-// paged_wide_kernel, whose ring this is).  The sequence's table entries come the same way: every wave brings those of the 32 tokens of the
-// tiles of a step into a small ring of its own, one transfer a step, DP steps before it forms the addresses.  (A window may lie anywhere
-// in a table of any length.)
-template <class DT, int D, int NS, int NW, int PAR>
+// NW waves of 32 rows each, which all take every tile of the group.  A tile comes into LDS once per workgroup, into a ring of NS slots in steps
+// of TS tiles with one barrier each: a wave waits for its own transfers of the step, all waves meet, the step is complete, and the slots of
+// the step before are free for the request behind the barrier.  The sequence's table entries come the same way: every wave brings those of
+// the 32 tokens of the tiles of a step into a small ring of its own, one transfer a step, DP steps before it forms the addresses.  (A window
+// may lie anywhere in a table of any length.)
+template <class DT, int D, int NS, int NW, int TS>
 __global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHeader args) {
     typedef Geo<DT, D, D> G;
     typedef typename Elem<DT>::store_t store_t;
-    constexpr int NT = NW * 64;
-    constexpr int NRW = NW / PAR;                // waves that differ in their rows
-    constexpr int RB = WINDOW_ROWS / 16 / NRW;   // 16-row blocks of a wave when the group has more than 64 rows
-    constexpr int NSTEP = NS / PAR, DP = NSTEP - 1;
+    constexpr int NT = NW * 64, ROWS = NW * 32;
+    constexpr int NSTEP = NS / TS, DP = NSTEP - 1;
     constexpr int KBYTES = G::KSTAGE, VBYTES = TILE * G::VROW, SLOT = KBYTES + VBYTES;
     constexpr int TPW = SLOT / 1024 / NW;        // 1 KB transfers of a wave per tile
-    constexpr int TPS = PAR * TPW;
+    constexpr int TPS = TS * TPW;
     constexpr int RPL = 64 / G::CPR;
     constexpr int ER = 2 * DP + 1;               // steps of table entries in a wave's ring
-    static_assert(G::SZ == 2 && KBYTES == VBYTES && TPW >= 1 && NS % PAR == 0 && DP >= 1 && (PAR == 1 || PAR == 2) && RB == 2, "16-bit types, 32 rows a wave");
-    constexpr int OSTR = D + 4, REGION = 16 * OSTR;        // floats of a wave at the end: 16 rows, or as many accumulators
-    static_assert(G::NOC * 64 * 4 <= REGION && (NW * REGION + NW * 64 * 2) * 4 <= NS * SLOT, "the blocks of all waves fit into the ring");
+    static_assert(G::SZ == 2 && KBYTES == VBYTES && TPW >= 1 && NS % TS == 0 && DP >= 1 && (TS == 1 || TS == 2), "16-bit types");
+    constexpr int OSTR = D + 4;                  // floats of a row on its way out
+    static_assert(NW * 16 * OSTR * 4 <= NS * SLOT, "16 rows of every wave fit into the ring");
     __shared__ int entries[NW][ER][64];
     __shared__ __attribute__((aligned(16))) char ring[NS * SLOT];
 
-    const int tid = threadIdx.x, lane = tid & 63;
+    const int tid = threadIdx.x;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int rw = wv % NRW, par = wv / NRW;
-    const int n = lane & 15, q = lane >> 4;
 
     PagedHeaderBits hb;
     paged_header_request(hb);
-    // this wave's transfers of a tile (see paged_wide_kernel): with an even number the same rows of both images
+    // this wave's transfers of a tile: with an even number of them the same rows of both images (one look-up serves both), otherwise the first
+    // half of the waves brings K, the second half V
     constexpr bool BOTH = TPW % 2 == 0;
     constexpr int NI = BOTH ? 2 : 1, NP = TPW / NI;
     static_assert((KBYTES / 1024) % NP == 0 && NW * NP * NI * 1024 == SLOT, "the waves' pieces tile both images");
     const bool k_wave = BOTH || wv < NW / 2;
     const int piece0 = (BOTH ? wv : (k_wave ? wv : wv - NW / 2)) * NP;
-    const int lrow = lane / G::CPR, lslot = lane % G::CPR;
-    unsigned chunk[NI][NP];
-    int trow[NP];
-#pragma unroll
-    for (int j = 0; j < NP; ++j) {
-        const int row = (piece0 + j) * RPL + lrow;
-        const int key = G::CPR >= 16 ? (row & 15) : ((row >> 1) & (G::CPR - 1));
-        const unsigned kchunk = (unsigned)((lslot ^ key) << 4), vchunk = (unsigned)((lslot ^ (2 * vimg_segment_key<G::VROW>(row))) << 4);
-        trow[j] = row;
-        chunk[0][j] = k_wave ? kchunk : vchunk;
-        if constexpr (BOTH) chunk[1][j] = vchunk;
-    }
     unsigned my_image[NI];
     my_image[0] = lds_address(ring) + (k_wave ? 0 : KBYTES) + piece0 * 1024;
     if constexpr (BOTH) my_image[1] = my_image[0] + KBYTES;
     const unsigned my_entries = __builtin_amdgcn_readfirstlane(lds_address(entries) + wv * ER * 256);
-    unsigned voff[G::NOC];
-    vtr_lane_offsets<G::VROW>(voff, lane);
+    // The two waves of a SIMD would go through a tile in step, both at the matrix unit, then both at the exponentials.  With one ahead of
+    // the other at every issue they drift apart, and one's products run beside the other's exponentials.
+    if (wv >= NW / 2) __builtin_amdgcn_s_setprio(1);
     const PagedDevHeader ph = paged_header_wait(hb);
 
     int bid = blockIdx.x;                        // kv head * nsplit + workgroup of the head; consecutive ids share an XCD
@@ -635,7 +703,7 @@ __global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHea
     const int GQ = ph.Hq / ph.Hkv;
     const int T = ph.LW * ph.LS;
     const int cap = ph.block_size * ph.max_blocks;
-    const int groups = window_groups(ph, lane, GQ);
+    const Deal deal = window_deal<ROWS>(ph, N, tid & 63, GQ);
     unsigned long long image[NI];
     image[0] = reinterpret_cast<unsigned long long>(k_wave ? ph.kcache : ph.vcache);
     if constexpr (BOTH) image[1] = reinterpret_cast<unsigned long long>(ph.vcache);
@@ -644,23 +712,33 @@ __global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHea
     a.Hq = ph.Hq; a.S = ph.LS;
     a.magic_gq = ph.magic_gq; a.magic_s = ph.magic_ls;
 
-    const int begin = me * groups, end = begin + groups;          // in n-ths of a group
-    const int group0 = begin / N;
-    for (int g = group0; g * N < end; ++g) {
-        const int from = max(begin - g * N, 0), to = min(end - g * N, N);
-        const WindowItem it = window_item<WINDOW_ROWS>(ph, g, lane, GQ);
-        const int r0 = it.qs * GQ + it.rg * WINDOW_ROWS, rend = min(it.qe * GQ, r0 + WINDOW_ROWS);
+    const int begin = me * deal.rest, end = begin + deal.rest;    // in n-ths of a group
+    const int part0 = begin / N, parts = deal.rest > 0 ? (end + N - 1) / N - part0 : 0;
+    for (int item = 0; item < deal.whole + parts; ++item) {
+        const bool whole_one = item < deal.whole;
+        const int cut = part0 + item - deal.whole;               // a part: of this one of the groups that are shared out
+        const int g = whole_one ? me * deal.whole + item : N * deal.whole + cut;
+        if (g >= deal.all) break;                                 // (the last workgroups, where almost a group each was left)
+        const int from = whole_one ? 0 : max(begin - cut * N, 0), to = whole_one ? N : min(end - cut * N, N);
+        const WindowGroup it = window_group<ROWS>(ph, deal, g, tid & 63, GQ);
+        const int r0 = it.qs * GQ + it.rg * ROWS, rend = min(it.qe * GQ, r0 + ROWS);
         const bool whole = from == 0 && to == N;
-        const size_t pbase = ((size_t)hkv * 2 * N + 2 * me + (g == group0 ? 0 : 1)) * WINDOW_ROWS;
+        const size_t pbase = ((size_t)hkv * 2 * N + 2 * me + (cut == part0 ? 0 : 1)) * ROWS;
         const HW_GLOBAL int* btw = ph.block_table + (size_t)it.w * ph.max_blocks;
 
         auto run = [&](auto rbx) {
             constexpr int RBX = decltype(rbx)::value;
-            constexpr int wrows = 16 * RBX;
-            const int w0 = r0 + rw * wrows;              // the wave's first row
-            // the rows' positions: lane l rows l and 64 + l of the group (behind the last row, that row again)
-            const int at0 = ph.loc[fast_div(min(r0 + lane, rend - 1), ph.magic_gq)];
-            const int at1 = ph.loc[fast_div(min(r0 + 64 + lane, rend - 1), ph.magic_gq)];
+            const int w0 = r0 + wv * 16 * RBX;           // the wave's first row
+            // (the lane as the compiler cannot see through it: what follows from it is formed here, per group, and does not stay in
+            // registers through the tile loops of the other form, which have none to spare)
+            int lane = tid & 63;
+            asm volatile("" : "+v"(lane));
+            const int n = lane & 15, q = lane >> 4;
+            // the rows' positions (behind the last row, that row again): lane l rows l, 64 + l, ... of the group, and l % (16 RBX) of the wave
+            int at[ROWS / 64];
+#pragma unroll
+            for (int i = 0; i < ROWS / 64; ++i) at[i] = ph.loc[fast_div(min(r0 + 64 * i + lane, rend - 1), ph.magic_gq)];
+            const int at_own = ph.loc[fast_div(min(w0 + (lane & (16 * RBX - 1)), rend - 1), ph.magic_gq)];
             u32x4 qreg[RBX * G::KJ];
 #pragma unroll
             for (int rb = 0; rb < RBX; ++rb) {
@@ -668,33 +746,59 @@ __global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHea
 #pragma unroll
                 for (int j = 0; j < G::KJ; ++j) qreg[rb * G::KJ + j] = *reinterpret_cast<const HW_GLOBAL u32x4*>(qp + (4 * j + q) * 16);
             }
-            auto lim_of = [&](int at) { return max(0, at < cap ? at + 1 : cap); };
-            auto lo_of = [&](int at) { return max(0, at < 0 ? 0 : at - args.window + 1); };
-            const int lim0 = lim_of(at0), lim1 = lim_of(at1), lo0 = lo_of(at0), lo1 = lo_of(at1);
-            const int high = wave_max(max(lo0 < lim0 ? lim0 : 0, lo1 < lim1 ? lim1 : 0));
-            const int low = -wave_max(max(lo0 < lim0 ? -lo0 : -0x7fffffff, lo1 < lim1 ? -lo1 : -0x7fffffff));
-            const int sink_end = min(args.sinks, wave_max(max(lim0, lim1)));
-            const bool alike = __ballot(at0 != __builtin_amdgcn_readfirstlane(at0) || at1 != __builtin_amdgcn_readfirstlane(at0)) == 0;
-            const int all_from = wave_max(max(lo0, lo1)), all_to = -wave_max(max(-lim0, -lim1));
+            const int lrow = lane / G::CPR, lslot = lane % G::CPR;
+            unsigned chunk[NI][NP];                      // byte offset of the lane's 16 bytes in its row, by image and piece
+            int trow[NP];                                // the tile row it belongs to
+#pragma unroll
+            for (int j = 0; j < NP; ++j) {
+                const int row = (piece0 + j) * RPL + lrow;
+                const int key = G::CPR >= 16 ? (row & 15) : ((row >> 1) & (G::CPR - 1));
+                const unsigned kchunk = (unsigned)((lslot ^ key) << 4), vchunk = (unsigned)((lslot ^ (2 * vimg_segment_key<G::VROW>(row))) << 4);
+                trow[j] = row;
+                chunk[0][j] = k_wave ? kchunk : vchunk;
+                if constexpr (BOTH) chunk[1][j] = vchunk;
+            }
+            unsigned voff[G::NOC];
+            vtr_lane_offsets<G::VROW>(voff, lane);
+            auto lim_of = [&](int x) { return max(0, x < cap ? x + 1 : cap); };
+            auto lo_of = [&](int x) { return max(0, x < 0 ? 0 : x - args.window + 1); };
+            int top = 0, bottom = -0x7fffffff, most = 0, above = 0, least = -0x7fffffff;
+            bool other = false;                          // not all rows of the group are at one position
+#pragma unroll
+            for (int i = 0; i < ROWS / 64; ++i) {
+                const int lim = lim_of(at[i]), lo = lo_of(at[i]);
+                const bool any = lo < lim;               // the row's window holds something
+                top = max(top, any ? lim : 0);
+                bottom = max(bottom, any ? -lo : -0x7fffffff);
+                most = max(most, lim);
+                above = max(above, lo);
+                least = max(least, -lim);
+                other = other || at[i] != __builtin_amdgcn_readfirstlane(at[0]);
+            }
+            const bool alike = __ballot(other) == 0;
+            const int high = wave_max(top), low = -wave_max(bottom);                   // the windows of the group lie in [low, high)
+            const int sink_end = min(args.sinks, wave_max(most));
+            const int all_from = wave_max(above), all_to = -wave_max(least);           // what every row's window holds
+            // the same of the wave's own rows
+            const int own_high = wave_max(lo_of(at_own) < lim_of(at_own) ? lim_of(at_own) : 0), own_low = -wave_max(lo_of(at_own) < lim_of(at_own) ? -lo_of(at_own) : -0x7fffffff);
+            const int own_from = wave_max(lo_of(at_own)), own_to = -wave_max(-lim_of(at_own)), own_sinks = min(args.sinks, wave_max(lim_of(at_own)));
             Band<RBX> band;
 #pragma unroll
             for (int rb = 0; rb < RBX; ++rb) {
-                const int rr = rw * wrows + rb * 16;
-                const int at = __shfl(rr < 64 ? at0 : at1, (rr & 63) + n, 64);
-                band.lim[rb] = lim_of(at);
-                band.lo[rb] = lo_of(at);
+                const int x = RBX == 1 ? at_own : __shfl(at_own, rb * 16 + n, 64);
+                band.lim[rb] = lim_of(x);
+                band.lo[rb] = lo_of(x);
                 band.snk[rb] = min(args.sinks, band.lim[rb]);
             }
-            // Tiles: of the sinks; of the windows, those that some row may not see all of (at the lower end, at the upper end), then those
-            // that every row sees completely.
+            // Tiles: of the sinks, then of the windows; of them every row sees those numbered full0 .. full1 - 1 completely, which are taken last.
             const int sink_tiles = (sink_end + TILE - 1) / TILE;
-            const int first = high > 0 ? max(low / TILE, sink_tiles) : 0, last = high > 0 ? max((high + TILE - 1) / TILE, first) : 0;
-            const int full0 = min(max((all_from + TILE - 1) / TILE, first), last), full1 = min(max(all_to / TILE, full0), last);
-            const int n_low = full0 - first, n_part = sink_tiles + n_low + last - full1, tiles = n_part + full1 - full0;
+            const int first = high > 0 ? max(low / TILE, sink_tiles) : 0, tiles = sink_tiles + (high > 0 ? max((high + TILE - 1) / TILE - first, 0) : 0);
+            const int jump = first - sink_tiles;
+            const int full0 = min(max((all_from + TILE - 1) / TILE - jump, sink_tiles), tiles), full1 = min(max(all_to / TILE - jump, full0), tiles);
+            const int part = tiles - (full1 - full0);
             auto tile_at = [&](int k) {
-                const int up = k - sink_tiles - n_low;                // number among those of the upper end
-                const int t = k < sink_tiles ? k : up < 0 ? first + k - sink_tiles : full1 + up;
-                return k < n_part ? t : full0 + k - n_part;
+                const int x = k + (k >= full0 ? full1 - full0 : 0) - (k >= part ? tiles - full0 : 0);
+                return x + (x >= sink_tiles ? jump : 0);
             };
             const int k0 = tiles * from / N, k1 = tiles * to / N;
 
@@ -707,31 +811,31 @@ __global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHea
                 for (int c = 0; c < G::NOC; ++c) st.o[rb][c] = f32x4{0.f, 0.f, 0.f, 0.f};
             }
             st.fresh = true;
-            const bool live = w0 < rend;                              // the wave has rows
 
-            __syncthreads();                                          // everybody is done with the ring (the group before)
             if (k0 < k1) {                                            // uniform over the workgroup
                 // the table entries of step s: lanes 0..31 those of its first tile's tokens, 32..63 of its second's
                 auto request_entries = [&](int s, int slot) {
-                    const int t = tile_at(k0 + s * PAR + (PAR - 1) * (lane >> 5));
+                    const int t = tile_at(k0 + s * TS + (TS - 1) * (lane >> 5));
                     const int tok = min(t * TILE + (lane & 31), cap - 1);
                     lds_transfer_flat<true, true>(__builtin_amdgcn_readfirstlane(my_entries + slot * 256), reinterpret_cast<unsigned long long>(btw + fast_div(tok, ph.magic_bs)));
                 };
                 // Source addresses of this wave's transfers of step s.  Tokens that no row sees are replaced by one of the tile that some row
-                // sees; what a tile that does not exist reads is not used.
+                // sees; what a tile that does not exist reads is not used.  (Without branches: they would cut the tile loops into pieces.)
                 auto addresses = [&](unsigned long long* src, int s, int slot) {
+                    const int* ent = &entries[wv][slot][0];
 #pragma unroll
-                    for (int pp = 0; pp < PAR; ++pp) {
-                        const int t0 = tile_at(k0 + s * PAR + pp) * TILE;
-                        const int stop = t0 + TILE > low && high > 0 ? high : sink_end;
-                        const int star = min(max(stop - 1 - t0, 0), TILE - 1);
+                    for (int pp = 0; pp < TS; ++pp) {
+                        const int t0 = tile_at(k0 + s * TS + pp) * TILE;
+                        const bool windows = t0 + TILE > low && high > 0;             // (uniform)
+                        const int lowest = windows ? low : sink_end - 1, highest = windows ? high - 1 : sink_end - 1;
 #pragma unroll
                         for (int j = 0; j < NP; ++j) {
                             const int raw = t0 + trow[j];
-                            const int tr = raw < sink_end || (raw >= low && raw < high) ? trow[j] : star;
+                            const int moved = min(max(min(max(raw, lowest), highest) - t0, 0), TILE - 1);
+                            const int tr = raw < sink_end ? trow[j] : moved;
                             const int tok = min(t0 + tr, cap - 1);
                             const int bi = fast_div(tok, ph.magic_bs);
-                            const int blk = min(max(entries[wv][slot][pp * 32 + tr], 0), ph.num_blocks - 1);
+                            const int blk = min(max(ent[pp * 32 + tr], 0), ph.num_blocks - 1);
                             const int rid = (blk * ph.Hkv + hkv) * ph.block_size + (tok - bi * ph.block_size);
 #pragma unroll
                             for (int im = 0; im < NI; ++im) src[(pp * NP + j) * NI + im] = image[im] + (unsigned long long)(unsigned)rid * G::KROW + chunk[im][j];
@@ -740,19 +844,23 @@ __global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHea
                 };
                 auto request = [&](int step_slot, const unsigned long long* src) {
 #pragma unroll
-                    for (int pp = 0; pp < PAR; ++pp)
+                    for (int pp = 0; pp < TS; ++pp)
 #pragma unroll
                         for (int j = 0; j < NP; ++j)
 #pragma unroll
                             for (int im = 0; im < NI; ++im)
-                                lds_transfer_flat<true>(__builtin_amdgcn_readfirstlane(my_image[im] + (step_slot * PAR + pp) * SLOT + j * 1024), src[(pp * NP + j) * NI + im]);
+                                lds_transfer_flat<true>(__builtin_amdgcn_readfirstlane(my_image[im] + (step_slot * TS + pp) * SLOT + j * 1024), src[(pp * NP + j) * NI + im]);
                 };
                 // Step i requests the entries of step i + 2 DP + 1 and the tiles of step i + DP, in this order, and forms the addresses of
                 // step i + DP + 1 from the entries that step i - DP requested.  Steps -DP .. -1 here.
 #pragma unroll
                 for (int i = 0; i <= DP; ++i) request_entries(i, i);
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // (queries and positions as well)
+                // (queries and positions as well; stated so that the compiler sees it: it would place its own wait for the queries where they
+                // are used, inside the tile loops, and there it would also wait for the tiles in flight)
+                __builtin_amdgcn_s_waitcnt(VMCNT_0);
+                asm volatile("" ::: "memory");
                 unsigned long long src[TPS];
+                __syncthreads();                                      // everybody is done with the ring (the group before)
 #pragma unroll
                 for (int i = 0; i < DP; ++i) {
                     addresses(src, i, i);
@@ -776,63 +884,59 @@ __global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHea
                     es = es + 1 == ER ? 0 : es + 1;
                     ++step;
                 };
-                // two loops with one instantiation of the tile arithmetic each; waves may change over one step apart
-                int k = k0 + par;
-#pragma unroll 1
-                for (; k - par < k1 && k < n_part; k += PAR) {
+                // One instantiation of the arithmetic for tiles that some row may not see all of and one for the others, in loops of their
+                // own (a step with both kinds, and a last one of one tile, are the first loop's).
+                const bool live = w0 < rend;                          // (a wave without rows only takes part in the barriers)
+                int k = k0;
+                auto partly = [&]() {
                     arrive();
-                    if (live && k < k1) {
-                        const char* slot = ring + (sl * PAR + par) * SLOT;
-                        band_tile_lds<DT, D, RBX, true>(qreg, band, st, tile_at(k) * TILE, n, q, ph.sc, slot, slot + KBYTES, voff, !alike);
+                    if (live) {
+#pragma unroll 1
+                        for (int pp = 0; pp < TS; ++pp) {
+                            const int t0 = tile_at(k + pp) * TILE;
+                            // (nothing of the tile is seen by the wave)
+                            if (k + pp >= k1 || !(t0 < own_sinks || (t0 < own_high && t0 + TILE > own_low))) continue;
+                            const char* slot = ring + (sl * TS + pp) * SLOT;
+                            band_tile_lds<DT, D, RBX, true>(qreg, band, st, t0, n, q, ph.sc, slot, slot + KBYTES, voff,
+                                                            !alike && !(t0 >= own_from && t0 + TILE <= own_to));
+                        }
                     }
                     next();
-                }
+                    k += TS;
+                };
 #pragma unroll 1
-                for (; k - par < k1; k += PAR) {
-                    arrive();
-                    if (live && k < k1) {
-                        const char* slot = ring + (sl * PAR + par) * SLOT;
+                while (k < k1 && k < part) partly();
+                if (live) {
+#pragma unroll 1
+                    for (; k + TS <= k1; k += TS) {
+                        arrive();
+#pragma unroll 1
+                        for (int pp = 0; pp < TS; ++pp) {
+                            const char* slot = ring + (sl * TS + pp) * SLOT;
+                            band_tile_lds<DT, D, RBX, false>(qreg, band, st, 0, n, q, ph.sc, slot, slot + KBYTES, voff, false);
+                        }
+                        next();
+                    }
+                    if (k < k1) {
+                        arrive();
+                        const char* slot = ring + sl * TS * SLOT;
                         band_tile_lds<DT, D, RBX, false>(qreg, band, st, 0, n, q, ph.sc, slot, slot + KBYTES, voff, false);
                     }
-                    next();
+                } else {
+#pragma unroll 1
+                    for (; k < k1; k += TS) {
+                        arrive();
+                        next();
+                    }
                 }
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // the requests behind the last tile, before the ring is used again
             }
 
-            // The PAR waves that share their rows hold a sum each: block rb goes to wave rb % PAR of them through LDS and is added up there.
-            // Every wave then stores its blocks, staged through LDS so that they leave as whole rows.
+            // every wave stores its rows, staged through LDS so that they leave whole
             __syncthreads();
-            float* const regions = reinterpret_cast<float*>(ring);
-            float* const mls = regions + NW * REGION;
-            if constexpr (PAR > 1) {
-#pragma unroll
-                for (int rb = 0; rb < RBX; ++rb) {
-                    const int owner = rw + (rb % PAR) * NRW;
-                    if (owner != wv) {
-#pragma unroll
-                        for (int c = 0; c < G::NOC; ++c) *reinterpret_cast<f32x4*>(regions + owner * REGION + (c * 64 + lane) * 4) = st.o[rb][c];
-                        *reinterpret_cast<f32x2*>(mls + (owner * 64 + lane) * 2) = f32x2{st.m[rb], st.l[rb]};
-                    }
-                }
-                __syncthreads();
-            }
-            float* stage = regions + wv * REGION;
+            float* stage = reinterpret_cast<float*>(ring) + wv * 16 * OSTR;
 #pragma unroll
             for (int rb = 0; rb < RBX; ++rb) {
-                if (rw + (rb % PAR) * NRW != wv) continue;            // uniform over the wave
-                if constexpr (PAR > 1) {
-                    const f32x2 oml = *reinterpret_cast<const f32x2*>(mls + (wv * 64 + lane) * 2);
-                    const float mnew = fmaxf(st.m[rb], oml.x);
-                    const float mine = fast_exp2(st.m[rb] - mnew), theirs = fast_exp2(oml.x - mnew);
-#pragma unroll
-                    for (int c = 0; c < G::NOC; ++c) {
-                        const f32x4 o2 = *reinterpret_cast<const f32x4*>(stage + (c * 64 + lane) * 4);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) st.o[rb][c][i] = st.o[rb][c][i] * mine + o2[i] * theirs;
-                    }
-                    st.l[rb] = st.l[rb] * mine + oml.y * theirs;
-                    st.m[rb] = mnew;
-                }
                 const float lsum = quarter_sum(st.l[rb]);
                 const float scale = !whole ? 1.0f : lsum > 0.f ? 1.0f / lsum : 0.f;
                 const int row0 = w0 + rb * 16;
@@ -859,12 +963,12 @@ __global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHea
                 }
             }
         };
-        if (rend - r0 <= WINDOW_ROWS / 2) run(std::integral_constant<int, RB / 2>{});
-        else run(std::integral_constant<int, RB>{});
+        if (rend - r0 <= ROWS / 2) run(std::integral_constant<int, 1>{});
+        else run(std::integral_constant<int, 2>{});
     }
 
     if (ph.cu_q != nullptr) {                    // zeros for query tokens that belong to no sequence
-        const int before = min(max(ph.cu_q[0], 0), T), after = min(max(ph.cu_q[ph.W], 0), T), rest = before + T - after;
+        const int before = bounded(ph.cu_q[0], T), after = bounded(ph.cu_q[ph.W], T), rest = before + T - after;
         for (int i = me; i < rest; i += N) {
             const size_t orow = (size_t)(i < before ? i : after + i - before) * ph.Hq + hkv * GQ;
             for (int x = tid; x < GQ * D; x += NT) reinterpret_cast<store_t*>(args.out)[orow * D + x] = 0;
@@ -874,47 +978,43 @@ __global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHea
     }
 }
 
-// The groups that lie across workgroups: workgroup j of the launch's (kv head, j, 8 rows) takes those rows of the group that workgroup j of
-// the attention kernel began and did not end.  32 lanes and more a row; parts in their order.
-template <class DT, int D>
-__global__ __launch_bounds__(256) void window_merge_kernel(const WindowHeader args) {
+// The groups that lie across workgroups: workgroup (kv head, cut, block of rows) of the launch takes those rows of group `cut` of the ones
+// that were shared out.  D / 4 lanes a row; parts in their order.  A kv head's partial sums are read on the XCD that wrote them.
+template <class DT, int D, int ROWS>
+__global__ __launch_bounds__(256) void window_merge_kernel(const WindowHeader args, int cuts) {
     typedef typename Elem<DT>::store_t store_t;
-    constexpr int V4 = D / 4, ROWS = 256 / V4, UN = 8;
-    const PagedHeader& h = args.p;
+    constexpr int V4 = D / 4, RPB = 256 / V4, BLOCKS = ROWS / RPB, UN = 8;
     const int tid = threadIdx.x, lane = tid & 63;
-    PagedDevHeader ph;
-    {
-        PagedHeaderBits hb;
-        paged_header_request(hb);
-        ph = paged_header_wait(hb);
-    }
-    const int N = h.nsplit, GQ = h.Hq / h.Hkv;
-    constexpr int BLOCKS = WINDOW_ROWS / ROWS;
-    const int rblk = blockIdx.x % BLOCKS, hj = blockIdx.x / BLOCKS;
-    const int hkv = hj / N, j = hj - hkv * N;
-    const int groups = window_groups(ph, lane, GQ);
-    const int end = (j + 1) * groups;
-    if (groups == 0 || end % N == 0) return;     // the last group ends here
-    const int g = end / N;
-    const int w0 = g * N / groups, w1 = ((g + 1) * N - 1) / groups;       // its workgroups
-    if (w0 != j) return;
-    const WindowItem it = window_item<WINDOW_ROWS>(ph, g, lane, GQ);
-    const int r0 = it.qs * GQ + it.rg * WINDOW_ROWS, rend = min(it.qe * GQ, r0 + WINDOW_ROWS);
-    const int rr = rblk * ROWS + tid / V4, e = tid % V4 * 4;
+    PagedHeaderBits hb;
+    paged_header_request(hb);
+    const PagedDevHeader ph = paged_header_wait(hb);
+    const int N = ph.nsplit, GQ = ph.Hq / ph.Hkv;
+    int bid = blockIdx.x;
+    if (ph.flags & PH_XCD_REMAP) bid = (bid & 7) * (gridDim.x >> 3) + (bid >> 3);
+    const int rblk = bid % BLOCKS, hc = bid / BLOCKS;
+    const int hkv = hc / cuts, cut = hc - hkv * cuts;
+    const Deal deal = window_deal<ROWS>(ph, N, lane, GQ);
+    const int rest = deal.rest;
+    if (cut >= rest) return;
+    const int first = cut * N / rest, last = ((cut + 1) * N - 1) / rest;       // its workgroups
+    if (first == last) return;                   // it saw the whole group
+    const WindowGroup it = window_group<ROWS>(ph, deal, N * deal.whole + cut, lane, GQ);
+    const int r0 = it.qs * GQ + it.rg * ROWS, rend = min(it.qe * GQ, r0 + ROWS);
+    const int rr = rblk * RPB + tid / V4, e = tid % V4 * 4;
     if (r0 + rr >= rend) return;
     // (the slot of workgroup w: its first group's, or, for the one that begins the group in the middle of its stretch, the other)
-    auto row_of = [&](int w) { return ((size_t)hkv * 2 * N + 2 * w + (w * groups / N == g ? 0 : 1)) * WINDOW_ROWS + rr; };
+    auto row_of = [&](int w) { return ((size_t)hkv * 2 * N + 2 * w + (w * rest / N == cut ? 0 : 1)) * ROWS + rr; };
     float m = NEG_BIG, l = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int w = w0; w <= w1; w += UN) {
+    for (int w = first; w <= last; w += UN) {
         f32x4 o[UN];
         f32x2 ml[UN];
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
-            const size_t row = row_of(min(w + u, w1));
-            o[u] = *reinterpret_cast<const f32x4*>(h.part_o + row * D + e);
-            ml[u] = *reinterpret_cast<const f32x2*>(h.part_ml + row * 2);
-            if (w + u > w1) {
+            const size_t row = row_of(min(w + u, last));
+            o[u] = *reinterpret_cast<const HW_GLOBAL f32x4*>(ph.part_o + row * D + e);
+            ml[u] = *reinterpret_cast<const HW_GLOBAL f32x2*>(ph.part_ml + row * 2);
+            if (w + u > last) {
                 ml[u] = f32x2{NEG_BIG, 0.f};
                 o[u] = f32x4{0.f, 0.f, 0.f, 0.f};
             }
@@ -934,8 +1034,10 @@ __global__ __launch_bounds__(256) void window_merge_kernel(const WindowHeader ar
         m = mb;
     }
     const float inv = l > 0.f ? 1.0f / l : 0.f;
-    const int row = r0 + rr, ws = row / GQ, head = hkv * GQ + row - ws * GQ, w = ws / h.LS;
-    const size_t orow = ((size_t)w * h.Hq + head) * h.LS + (ws - w * h.LS);
+    DevHeader a;
+    a.Hq = ph.Hq; a.S = ph.LS;
+    a.magic_gq = ph.magic_gq; a.magic_s = ph.magic_ls;
+    const size_t orow = map_row(a, r0 + rr, hkv, GQ).qrow;
     *reinterpret_cast<u32x2*>(reinterpret_cast<store_t*>(args.out) + orow * D + e) =
         u32x2{Elem<DT>::pack2(acc[0] * inv, acc[1] * inv), Elem<DT>::pack2(acc[2] * inv, acc[3] * inv)};
     if (args.lse != nullptr && e == 0) args.lse[orow] = l > 0.f ? (m + __builtin_amdgcn_logf(l)) * 0.69314718055994530942f : -__builtin_inff();
@@ -944,12 +1046,14 @@ __global__ __launch_bounds__(256) void window_merge_kernel(const WindowHeader ar
 // ------------------------------------------------------------------------------------------------
 // launchers
 // ------------------------------------------------------------------------------------------------
-template <class DT, int D, int NS, int NW, int PAR>
+template <class DT, int D, int NS, int NW, int TS>
 static hipError_t launch_window_wide(const WindowHeader& wh, hipStream_t stream) {
-    hipLaunchKernelGGL((window_wide_kernel<DT, D, NS, NW, PAR>), dim3(wh.p.nwg), dim3(NW * 64), 0, stream, wh);
+    static_assert(NW * 32 == (D == 256 ? WINDOW_ROWS_256 : WINDOW_ROWS), "the planner's row groups");
+    hipLaunchKernelGGL((window_wide_kernel<DT, D, NS, NW, TS>), dim3(wh.p.nwg), dim3(NW * 64), 0, stream, wh);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || wh.p.nsplit == 1) return e;
-    hipLaunchKernelGGL((window_merge_kernel<DT, D>), dim3(wh.p.nwg * (WINDOW_ROWS * D / 1024)), dim3(256), 0, stream, wh);
+    const int cuts = wh.p.nitems < wh.p.nsplit ? wh.p.nitems : wh.p.nsplit - 1;       // groups that are shared out, at most
+    hipLaunchKernelGGL((window_merge_kernel<DT, D, NW * 32>), dim3(wh.p.Hkv * cuts * (NW * 32 * D / 1024)), dim3(256), 0, stream, wh, cuts);
     return hipGetLastError();
 }
 
