@@ -423,8 +423,8 @@ typedef struct hw_window_problem {
     void* workspace;           /* hw_window_workspace_bytes() bytes, 16-byte aligned (NULL if those are 0) */
     size_t workspace_bytes;
     int32_t splits;            /* 0 = automatic; otherwise workgroups per (kv head, row group), or, with row_blocks = 8, per kv head */
-    int32_t row_blocks;        /* 0 = automatic; 1 or 2 = 16-row MFMA blocks per workgroup; 8 = row groups of 256 rows (128 at D == 256) whose waves
-                                  share every K/V tile (16-bit types; the automatic choice beyond 32 query rows per sequence and kv head, in the mean) */
+    int32_t row_blocks;        /* 0 = automatic; 1 or 2 = 16-row MFMA blocks per workgroup; 8 = row groups of up to 256 rows (128 at D == 256) whose
+                                  waves share every K/V tile (16-bit types; the automatic choice beyond 32 query rows per sequence and kv head, in the mean) */
 } hw_window_problem;
 
 int hw_window_validate(const hw_window_problem* p);

@@ -372,6 +372,7 @@ int window_run(const hw_window_problem* p, void* stream_) {
     wh.lse = p->lse;
     wh.window = p->window;
     wh.sinks = p->sinks;
+    wh.rows = wide ? window_rows(p, cus) : 0;
     const hipError_t e = hw::launch_window_attention(wh, p->dtype, p->D, plan.row_blocks, stream);
     if (e != hipSuccess || direct || wide) return (int)e;      // (128-row groups: merged by the launcher)
     hw::MergeArgs ma;

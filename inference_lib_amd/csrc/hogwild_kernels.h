@@ -196,6 +196,7 @@ struct alignas(64) WindowHeader {
     void* out;             // written with PH_DIRECT, and where query tokens belong to no sequence
     float* lse;            // or null
     int window, sinks;
+    int rows;              // of a row group (128-row workgroups and wider)
 };
 hipError_t launch_window_attention(const WindowHeader& wh, int dtype, int D, int rb, hipStream_t stream);
 

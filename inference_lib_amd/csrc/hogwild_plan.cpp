@@ -832,6 +832,19 @@ int window_validate(const hw_window_problem* p) {
     return HW_OK;
 }
 
+// Rows of a row group of the many-rows kernel.  The most of them take in every tile for the most rows; but groups that do not go round the
+// workgroups of a kv head are cut along their tiles, which costs a second opening, and partial sums of 4 bytes that are written and read.
+// Where there are enough rows for it (half a full group for every workgroup) their number is chosen so that the groups go round.
+int window_rows(const hw_window_problem* p, int num_cus) {
+    const int most = p->D == 256 ? hw::WINDOW_ROWS_256 : hw::WINDOW_ROWS;
+    const long long rows = (p->cu_seqlens_q != nullptr ? p->total_q : (long long)p->W * p->S) * (p->Hq / p->Hkv);
+    const long long wgs = p->splits > 0 ? p->splits : std::max(num_cus / p->Hkv, 1);
+    const long long rounds = (rows + wgs * most - 1) / (wgs * most);
+    if (rounds == 0) return most;
+    const long long even = (((rows + wgs * rounds - 1) / (wgs * rounds)) + 15) / 16 * 16;
+    return even >= most / 2 ? (int)even : most;
+}
+
 int window_plan(const hw_window_problem* p, int num_cus, hw_paged_plan* plan) {
     if (plan == nullptr) return HW_ERR_NULL;
     if (num_cus < 1) return HW_ERR_SHAPE;
@@ -845,7 +858,7 @@ int window_plan(const hw_window_problem* p, int num_cus, hw_paged_plan* plan) {
     plan->row_blocks = p->row_blocks != 0 ? p->row_blocks : p->dtype != HW_F32 && usual > 32 ? hw::WIDE_ROW_BLOCKS : two && usual > 16 ? 2 : 1;
     const bool wide = plan->row_blocks == hw::WIDE_ROW_BLOCKS && p->dtype != HW_F32;
     if (plan->row_blocks != 1 && !(plan->row_blocks == 2 && two) && !wide) return HW_ERR_UNSUPPORTED;
-    const int rows = !wide ? 16 * plan->row_blocks : p->D == 256 ? hw::WINDOW_ROWS_256 : hw::WINDOW_ROWS;
+    const int rows = wide ? window_rows(p, num_cus) : 16 * plan->row_blocks;
     // (packed: one more than there can be, which writes the zeros of tokens that belong to no sequence)
     plan->row_groups = varlen ? (plan->rows + rows - 1) / rows + p->W : p->W * ((p->S * gq + rows - 1) / rows);
     // The tiles that a row group usually sees, at most: sinks and a window that moves over its tokens.  Splits of two tiles a wave and more,
@@ -860,9 +873,9 @@ int window_plan(const hw_window_problem* p, int num_cus, hw_paged_plan* plan) {
         // tiles.  Two slots of partial sums each.
         if (splits == 0) splits = std::min((long long)std::max(num_cus / p->Hkv, 1), std::max(1ll, std::max(plan->row_groups, 1) * tiles / 8));
         plan->splits = (int)std::min(splits, (long long)HW_MAX_SPLITS);
-        if ((long long)plan->splits * p->Hkv * (rows * p->D / 1024) >= (1ll << 31)) return HW_ERR_SHAPE;
+        if ((long long)plan->splits * p->Hkv * (hw::WINDOW_ROWS * p->D / 1024) >= (1ll << 31)) return HW_ERR_SHAPE;
         plan->workgroups = plan->splits * p->Hkv;
-        if (plan->splits > 1) plan->workspace_bytes = (size_t)p->Hkv * 2 * plan->splits * rows * ((size_t)p->D + 2) * sizeof(float);
+        if (plan->splits > 1) plan->workspace_bytes = (size_t)p->Hkv * 2 * plan->splits * (p->D == 256 ? hw::WINDOW_ROWS_256 : hw::WINDOW_ROWS) * ((size_t)p->D + 2) * sizeof(float);
         return HW_OK;
     }
     if (splits == 0) splits = std::max(1ll, std::min((num_cus + groups - 1) / groups, tiles / (2 * hw::NWAVES)));

@@ -215,7 +215,7 @@ __device__ __forceinline__ void band_tile(const TileRegs<DT, D, D>& t, const u32
     else products(std::false_type{});
 }
 
-// Which rows a work item stands for.  Packed queries: the row groups of ROWS rows are numbered through the sequences in order; an item behind
+// Which rows a work item stands for.  Packed queries: the row groups of `rows` rows are numbered through the sequences in order; an item behind
 // the last of them is `spare`, of which there is one at least (the grid is sized for more row groups than there can be).
 struct WindowItem {
     int w, rg, qs, qe;       // sequence, row group in it, its query tokens
@@ -223,8 +223,7 @@ struct WindowItem {
     int spare, spares;       // not found: the how manieth of how many
     int first, end;          // and the query tokens that belong to sequences
 };
-template <int ROWS>
-__device__ __forceinline__ WindowItem window_item(const PagedDevHeader& ph, int item, int lane, int GQ) {
+__device__ __forceinline__ WindowItem window_item(const PagedDevHeader& ph, int rows, int item, int lane, int GQ) {
     WindowItem it = {0, 0, 0, 0, false, 0, 1, 0, 0};
     const int T = ph.LW * ph.LS;
     if (ph.cu_q == nullptr) {
@@ -240,7 +239,7 @@ __device__ __forceinline__ WindowItem window_item(const PagedDevHeader& ph, int 
     for (int c = 0; c < ph.W && !it.found; c += 64) {
         const int idx = c + lane;
         const int a0 = bound(ph.cu_q[min(idx, ph.W)]), a1 = bound(ph.cu_q[min(idx + 1, ph.W)]);
-        const int cnt = idx < ph.W ? (max(a1 - a0, 0) * GQ + ROWS - 1) / ROWS : 0;
+        const int cnt = idx < ph.W ? (max(a1 - a0, 0) * GQ + rows - 1) / rows : 0;
         const int inc = wave_scan_inclusive(cnt);
         const int total = __builtin_amdgcn_readlane(inc, 63);
         if (item < base + total) {
@@ -315,7 +314,7 @@ __global__ __launch_bounds__(NTHREADS, 1) void window_kernel(const WindowHeader 
     const int T = ph.LW * ph.LS;
     const int cap = ph.block_size * ph.max_blocks;
 
-    const WindowItem it = window_item<ROWS>(ph, item, lane, GQ);
+    const WindowItem it = window_item(ph, ROWS, item, lane, GQ);
     if (!it.found) {                        // uniform over the workgroup: zeros for query tokens that belong to no sequence
         const int before = it.first, rest = before + T - it.end;
         for (int i = it.spare; i < rest; i += it.spares) {
@@ -472,7 +471,7 @@ __global__ __launch_bounds__(NTHREADS, 1) void window_kernel(const WindowHeader 
 
 // ---- many rows -------------------------------------------------------------------------------------------------------------------
 //
-// Row groups of ROWS rows of one sequence (a last one of fewer), numbered through the sequences, `all` of them for every kv head.  The n
+// Row groups of `rows` rows of one sequence (a last one of fewer), numbered through the sequences, `all` of them for every kv head.  The n
 // workgroups of a head take q = all / n whole groups each, and share the rest of them out evenly, in the order of the rows: workgroup i takes
 // the stretch [i rest / n, (i + 1) rest / n) of them, and a part of a group is that part of its tiles.  So every workgroup has the same to do
 // where the groups see about the same (the bound of a window), whatever their number.  A workgroup that sees a whole group writes its
@@ -487,8 +486,7 @@ struct Deal {
     int qs, qe, count, upto;
 };
 __device__ __forceinline__ int bounded(int x, int T) { return min(max(x, 0), T); }        // a malformed array must not lead outside the buffers
-template <int ROWS>
-__device__ __forceinline__ Deal window_deal(const PagedDevHeader& ph, int n, int lane, int GQ) {
+__device__ __forceinline__ Deal window_deal(const PagedDevHeader& ph, int rows, int n, int lane, int GQ) {
     Deal d = {0, 0, 0, 0, 0, 0, 0};
     if (ph.cu_q == nullptr) d.all = ph.W * ph.nrg;
     else {
@@ -496,7 +494,7 @@ __device__ __forceinline__ Deal window_deal(const PagedDevHeader& ph, int n, int
         for (int c = 0; c < ph.W; c += 64) {
             const int idx = c + lane;
             const int a0 = bounded(ph.cu_q[min(idx, ph.W)], T), a1 = bounded(ph.cu_q[min(idx + 1, ph.W)], T);
-            const int cnt = idx < ph.W ? (max(a1 - a0, 0) * GQ + ROWS - 1) / ROWS : 0;
+            const int cnt = idx < ph.W ? (max(a1 - a0, 0) * GQ + rows - 1) / rows : 0;
             const int inc = wave_scan_inclusive(cnt);
             if (c == 0) {
                 d.qs = a0;
@@ -520,8 +518,7 @@ __device__ __forceinline__ Deal window_deal(const PagedDevHeader& ph, int n, int
 struct WindowGroup {
     int w, rg, qs, qe;
 };
-template <int ROWS>
-__device__ __forceinline__ WindowGroup window_group(const PagedDevHeader& ph, const Deal& d, int g, int lane, int GQ) {
+__device__ __forceinline__ WindowGroup window_group(const PagedDevHeader& ph, const Deal& d, int rows, int g, int lane, int GQ) {
     WindowGroup r;
     if (ph.cu_q != nullptr && ph.W <= 64) {
         r.w = __builtin_ctzll(__ballot(d.upto > g));
@@ -529,7 +526,7 @@ __device__ __forceinline__ WindowGroup window_group(const PagedDevHeader& ph, co
         r.qs = __builtin_amdgcn_readlane(d.qs, r.w);
         r.qe = __builtin_amdgcn_readlane(d.qe, r.w);
     } else {
-        const WindowItem it = window_item<ROWS>(ph, g, lane, GQ);
+        const WindowItem it = window_item(ph, rows, g, lane, GQ);
         r.w = it.w;
         r.rg = it.rg;
         r.qs = it.qs;
@@ -653,7 +650,7 @@ __device__ __forceinline__ void band_tile_lds(const u32x4* qreg, const Band<RB>&
         for (int rb = 0; rb < RB; ++rb) st.o[rb][c] = Elem<DT>::mfma(vops[c], pp[rb], st.o[rb][c]);
 }
 
-// NW waves of 32 rows each, which all take every tile of the group.  A tile comes into LDS once per workgroup, into a ring of NS slots in steps
+// NW waves of up to 32 rows each, two 16-row blocks NW blocks apart, which all take every tile of the group.  A tile comes into LDS once per workgroup, into a ring of NS slots in steps
 // of TS tiles with one barrier each: a wave waits for its own transfers of the step, all waves meet, the step is complete, and the slots of
 // the step before are free for the request behind the barrier.  The sequence's table entries come the same way: every wave brings those of
 // the 32 tokens of the tiles of a step into a small ring of its own, one transfer a step, DP steps before it forms the addresses.  (A window
@@ -662,7 +659,7 @@ template <class DT, int D, int NS, int NW, int TS>
 __global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHeader args) {
     typedef Geo<DT, D, D> G;
     typedef typename Elem<DT>::store_t store_t;
-    constexpr int NT = NW * 64, ROWS = NW * 32;
+    constexpr int NT = NW * 64, ROWS = NW * 32;  // (rows of a group, at most)
     constexpr int NSTEP = NS / TS, DP = NSTEP - 1;
     constexpr int KBYTES = G::KSTAGE, VBYTES = TILE * G::VROW, SLOT = KBYTES + VBYTES;
     constexpr int TPW = SLOT / 1024 / NW;        // 1 KB transfers of a wave per tile
@@ -691,9 +688,6 @@ __global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHea
     my_image[0] = lds_address(ring) + (k_wave ? 0 : KBYTES) + piece0 * 1024;
     if constexpr (BOTH) my_image[1] = my_image[0] + KBYTES;
     const unsigned my_entries = __builtin_amdgcn_readfirstlane(lds_address(entries) + wv * ER * 256);
-    // The two waves of a SIMD would go through a tile in step, both at the matrix unit, then both at the exponentials.  With one ahead of
-    // the other at every issue they drift apart, and one's products run beside the other's exponentials.
-    if (wv >= NW / 2) __builtin_amdgcn_s_setprio(1);
     const PagedDevHeader ph = paged_header_wait(hb);
 
     int bid = blockIdx.x;                        // kv head * nsplit + workgroup of the head; consecutive ids share an XCD
@@ -703,7 +697,8 @@ __global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHea
     const int GQ = ph.Hq / ph.Hkv;
     const int T = ph.LW * ph.LS;
     const int cap = ph.block_size * ph.max_blocks;
-    const Deal deal = window_deal<ROWS>(ph, N, tid & 63, GQ);
+    const int rows = args.rows;
+    const Deal deal = window_deal(ph, rows, N, tid & 63, GQ);
     unsigned long long image[NI];
     image[0] = reinterpret_cast<unsigned long long>(k_wave ? ph.kcache : ph.vcache);
     if constexpr (BOTH) image[1] = reinterpret_cast<unsigned long long>(ph.vcache);
@@ -720,29 +715,30 @@ __global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHea
         const int g = whole_one ? me * deal.whole + item : N * deal.whole + cut;
         if (g >= deal.all) break;                                 // (the last workgroups, where almost a group each was left)
         const int from = whole_one ? 0 : max(begin - cut * N, 0), to = whole_one ? N : min(end - cut * N, N);
-        const WindowGroup it = window_group<ROWS>(ph, deal, g, tid & 63, GQ);
-        const int r0 = it.qs * GQ + it.rg * ROWS, rend = min(it.qe * GQ, r0 + ROWS);
+        const WindowGroup it = window_group(ph, deal, rows, g, tid & 63, GQ);
+        const int r0 = it.qs * GQ + it.rg * rows, rend = min(it.qe * GQ, r0 + rows);
         const bool whole = from == 0 && to == N;
         const size_t pbase = ((size_t)hkv * 2 * N + 2 * me + (cut == part0 ? 0 : 1)) * ROWS;
         const HW_GLOBAL int* btw = ph.block_table + (size_t)it.w * ph.max_blocks;
 
         auto run = [&](auto rbx) {
             constexpr int RBX = decltype(rbx)::value;
-            const int w0 = r0 + wv * 16 * RBX;           // the wave's first row
+            const int w0 = r0 + wv * 16;                 // the wave's first row; row block rb begins at w0 + rb * BLOCK
+            constexpr int BLOCK = NW * 16;
             // (the lane as the compiler cannot see through it: what follows from it is formed here, per group, and does not stay in
             // registers through the tile loops of the other form, which have none to spare)
             int lane = tid & 63;
             asm volatile("" : "+v"(lane));
             const int n = lane & 15, q = lane >> 4;
-            // the rows' positions (behind the last row, that row again): lane l rows l, 64 + l, ... of the group, and l % (16 RBX) of the wave
+            // the rows' positions (behind the last row, that row again): lane l rows l, 64 + l, ... of the group, and one of the wave's
             int at[ROWS / 64];
 #pragma unroll
             for (int i = 0; i < ROWS / 64; ++i) at[i] = ph.loc[fast_div(min(r0 + 64 * i + lane, rend - 1), ph.magic_gq)];
-            const int at_own = ph.loc[fast_div(min(w0 + (lane & (16 * RBX - 1)), rend - 1), ph.magic_gq)];
+            const int at_own = ph.loc[fast_div(min(w0 + n + (RBX == 1 ? 0 : (q & 1) * BLOCK), rend - 1), ph.magic_gq)];
             u32x4 qreg[RBX * G::KJ];
 #pragma unroll
             for (int rb = 0; rb < RBX; ++rb) {
-                const HW_GLOBAL char* qp = ph.q + map_row(a, min(w0 + rb * 16 + n, rend - 1), hkv, GQ).qrow * G::KROW;
+                const HW_GLOBAL char* qp = ph.q + map_row(a, min(w0 + rb * BLOCK + n, rend - 1), hkv, GQ).qrow * G::KROW;
 #pragma unroll
                 for (int j = 0; j < G::KJ; ++j) qreg[rb * G::KJ + j] = *reinterpret_cast<const HW_GLOBAL u32x4*>(qp + (4 * j + q) * 16);
             }
@@ -939,7 +935,7 @@ __global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHea
             for (int rb = 0; rb < RBX; ++rb) {
                 const float lsum = quarter_sum(st.l[rb]);
                 const float scale = !whole ? 1.0f : lsum > 0.f ? 1.0f / lsum : 0.f;
-                const int row0 = w0 + rb * 16;
+                const int row0 = w0 + rb * BLOCK;
                 if (q == 0 && row0 + n < rend) {
                     if (!whole) *reinterpret_cast<HW_GLOBAL f32x2*>(ph.part_ml + (pbase + (row0 - r0) + n) * 2) = f32x2{st.m[rb], lsum};
                     else if (args.lse != nullptr)
@@ -963,8 +959,9 @@ __global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHea
                 }
             }
         };
-        if (rend - r0 <= ROWS / 2) run(std::integral_constant<int, 1>{});
-        else run(std::integral_constant<int, 2>{});
+        // (the waves of a workgroup may be in different ones: what they meet at are barriers, as many in both)
+        if (r0 + wv * 16 + NW * 16 < rend) run(std::integral_constant<int, 2>{});
+        else run(std::integral_constant<int, 1>{});
     }
 
     if (ph.cu_q != nullptr) {                    // zeros for query tokens that belong to no sequence
@@ -983,7 +980,7 @@ __global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHea
 template <class DT, int D, int ROWS>
 __global__ __launch_bounds__(256) void window_merge_kernel(const WindowHeader args, int cuts) {
     typedef typename Elem<DT>::store_t store_t;
-    constexpr int V4 = D / 4, RPB = 256 / V4, BLOCKS = ROWS / RPB, UN = 8;
+    constexpr int V4 = D / 4, RPB = 256 / V4, BLOCKS = ROWS / RPB, UN = 4;
     const int tid = threadIdx.x, lane = tid & 63;
     PagedHeaderBits hb;
     paged_header_request(hb);
@@ -993,13 +990,14 @@ __global__ __launch_bounds__(256) void window_merge_kernel(const WindowHeader ar
     if (ph.flags & PH_XCD_REMAP) bid = (bid & 7) * (gridDim.x >> 3) + (bid >> 3);
     const int rblk = bid % BLOCKS, hc = bid / BLOCKS;
     const int hkv = hc / cuts, cut = hc - hkv * cuts;
-    const Deal deal = window_deal<ROWS>(ph, N, lane, GQ);
+    const int rows = args.rows;
+    const Deal deal = window_deal(ph, rows, N, lane, GQ);
     const int rest = deal.rest;
     if (cut >= rest) return;
     const int first = cut * N / rest, last = ((cut + 1) * N - 1) / rest;       // its workgroups
     if (first == last) return;                   // it saw the whole group
-    const WindowGroup it = window_group<ROWS>(ph, deal, N * deal.whole + cut, lane, GQ);
-    const int r0 = it.qs * GQ + it.rg * ROWS, rend = min(it.qe * GQ, r0 + ROWS);
+    const WindowGroup it = window_group(ph, deal, rows, N * deal.whole + cut, lane, GQ);
+    const int r0 = it.qs * GQ + it.rg * rows, rend = min(it.qe * GQ, r0 + rows);
     const int rr = rblk * RPB + tid / V4, e = tid % V4 * 4;
     if (r0 + rr >= rend) return;
     // (the slot of workgroup w: its first group's, or, for the one that begins the group in the middle of its stretch, the other)
