@@ -980,7 +980,7 @@ __global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHea
 template <class DT, int D, int ROWS>
 __global__ __launch_bounds__(256) void window_merge_kernel(const WindowHeader args, int cuts) {
     typedef typename Elem<DT>::store_t store_t;
-    constexpr int V4 = D / 4, RPB = 256 / V4, BLOCKS = ROWS / RPB, UN = 4;
+    constexpr int V4 = D / 4, RPB = 256 / V4, PER = 2, BLOCKS = ROWS / (RPB * PER), UN = 4;     // PER rows a thread
     const int tid = threadIdx.x, lane = tid & 63;
     PagedHeaderBits hb;
     paged_header_request(hb);
@@ -998,47 +998,62 @@ __global__ __launch_bounds__(256) void window_merge_kernel(const WindowHeader ar
     if (first == last) return;                   // it saw the whole group
     const WindowGroup it = window_group(ph, deal, rows, N * deal.whole + cut, lane, GQ);
     const int r0 = it.qs * GQ + it.rg * rows, rend = min(it.qe * GQ, r0 + rows);
-    const int rr = rblk * RPB + tid / V4, e = tid % V4 * 4;
+    const int rr = rblk * RPB * PER + tid / V4, e = tid % V4 * 4;
     if (r0 + rr >= rend) return;
     // (the slot of workgroup w: its first group's, or, for the one that begins the group in the middle of its stretch, the other)
-    auto row_of = [&](int w) { return ((size_t)hkv * 2 * N + 2 * w + (w * rest / N == cut ? 0 : 1)) * ROWS + rr; };
-    float m = NEG_BIG, l = 0.f;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int w = first; w <= last; w += UN) {
-        f32x4 o[UN];
-        f32x2 ml[UN];
+    auto row_of = [&](int w, int i) { return ((size_t)hkv * 2 * N + 2 * w + (w * rest / N == cut ? 0 : 1)) * ROWS + min(rr + i * RPB, rend - 1 - r0); };
+    float m[PER], l[PER];
+    f32x4 acc[PER];
 #pragma unroll
-        for (int u = 0; u < UN; ++u) {
-            const size_t row = row_of(min(w + u, last));
-            o[u] = *reinterpret_cast<const HW_GLOBAL f32x4*>(ph.part_o + row * D + e);
-            ml[u] = *reinterpret_cast<const HW_GLOBAL f32x2*>(ph.part_ml + row * 2);
-            if (w + u > last) {
-                ml[u] = f32x2{NEG_BIG, 0.f};
-                o[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-            }
-        }
-        float mb = m;
-#pragma unroll
-        for (int u = 0; u < UN; ++u) mb = fmaxf(mb, ml[u].x);
-        const float old = fast_exp2(m - mb);
-        acc *= old;
-        l *= old;
-#pragma unroll
-        for (int u = 0; u < UN; ++u) {
-            const float x = fast_exp2(ml[u].x - mb);
-            acc += o[u] * x;
-            l += ml[u].y * x;
-        }
-        m = mb;
+    for (int i = 0; i < PER; ++i) {
+        m[i] = NEG_BIG;
+        l[i] = 0.f;
+        acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    const float inv = l > 0.f ? 1.0f / l : 0.f;
+    for (int w = first; w <= last; w += UN) {
+        f32x4 o[PER][UN];
+        f32x2 ml[PER][UN];
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+#pragma unroll
+            for (int u = 0; u < UN; ++u) {
+                const size_t row = row_of(min(w + u, last), i);
+                o[i][u] = *reinterpret_cast<const HW_GLOBAL f32x4*>(ph.part_o + row * D + e);
+                ml[i][u] = *reinterpret_cast<const HW_GLOBAL f32x2*>(ph.part_ml + row * 2);
+                if (w + u > last) {
+                    ml[i][u] = f32x2{NEG_BIG, 0.f};
+                    o[i][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+                }
+            }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            float mb = m[i];
+#pragma unroll
+            for (int u = 0; u < UN; ++u) mb = fmaxf(mb, ml[i][u].x);
+            const float old = fast_exp2(m[i] - mb);
+            acc[i] *= old;
+            l[i] *= old;
+#pragma unroll
+            for (int u = 0; u < UN; ++u) {
+                const float x = fast_exp2(ml[i][u].x - mb);
+                acc[i] += o[i][u] * x;
+                l[i] += ml[i][u].y * x;
+            }
+            m[i] = mb;
+        }
+    }
     DevHeader a;
     a.Hq = ph.Hq; a.S = ph.LS;
     a.magic_gq = ph.magic_gq; a.magic_s = ph.magic_ls;
-    const size_t orow = map_row(a, r0 + rr, hkv, GQ).qrow;
-    *reinterpret_cast<u32x2*>(reinterpret_cast<store_t*>(args.out) + orow * D + e) =
-        u32x2{Elem<DT>::pack2(acc[0] * inv, acc[1] * inv), Elem<DT>::pack2(acc[2] * inv, acc[3] * inv)};
-    if (args.lse != nullptr && e == 0) args.lse[orow] = l > 0.f ? (m + __builtin_amdgcn_logf(l)) * 0.69314718055994530942f : -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        if (r0 + rr + i * RPB >= rend) break;
+        const float inv = l[i] > 0.f ? 1.0f / l[i] : 0.f;
+        const size_t orow = map_row(a, r0 + rr + i * RPB, hkv, GQ).qrow;
+        *reinterpret_cast<u32x2*>(reinterpret_cast<store_t*>(args.out) + orow * D + e) =
+            u32x2{Elem<DT>::pack2(acc[i][0] * inv, acc[i][1] * inv), Elem<DT>::pack2(acc[i][2] * inv, acc[i][3] * inv)};
+        if (args.lse != nullptr && e == 0) args.lse[orow] = l[i] > 0.f ? (m[i] + __builtin_amdgcn_logf(l[i])) * 0.69314718055994530942f : -__builtin_inff();
+    }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -1050,8 +1065,9 @@ static hipError_t launch_window_wide(const WindowHeader& wh, hipStream_t stream)
     hipLaunchKernelGGL((window_wide_kernel<DT, D, NS, NW, TS>), dim3(wh.p.nwg), dim3(NW * 64), 0, stream, wh);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || wh.p.nsplit == 1) return e;
-    const int cuts = wh.p.nitems < wh.p.nsplit ? wh.p.nitems : wh.p.nsplit - 1;       // groups that are shared out, at most
-    hipLaunchKernelGGL((window_merge_kernel<DT, D, NW * 32>), dim3(wh.p.Hkv * cuts * (NW * 32 * D / 1024)), dim3(256), 0, stream, wh, cuts);
+    const int most = wh.p.nsplit * 7 / 8, cuts = wh.p.nitems < most ? wh.p.nitems : most;     // groups that are shared out, at most (window_deal)
+    if (cuts == 0 || (wh.p.cu_q == nullptr && wh.p.nitems % wh.p.nsplit == 0)) return e;
+    hipLaunchKernelGGL((window_merge_kernel<DT, D, NW * 32>), dim3(wh.p.Hkv * cuts * (NW * 32 * D / 2048)), dim3(256), 0, stream, wh, cuts);
     return hipGetLastError();
 }
 
