@@ -472,25 +472,27 @@ __global__ __launch_bounds__(NTHREADS, 1) void window_kernel(const WindowHeader 
 // ---- many rows -------------------------------------------------------------------------------------------------------------------
 //
 // Row groups of `rows` rows of one sequence (a last one of fewer), numbered through the sequences, `all` of them for every kv head.  The n
-// workgroups of a head take q = all / n whole groups each, and share the rest of them out evenly, in the order of the rows: workgroup i takes
-// the stretch [i rest / n, (i + 1) rest / n) of them, and a part of a group is that part of its tiles.  So every workgroup has the same to do
-// where the groups see about the same (the bound of a window), whatever their number.  A workgroup that sees a whole group writes its
-// result; parts leave partial sums in the workgroup's two slots (its first group's, and its last one's), which window_merge_kernel adds
-// up.
+// workgroups of a head take q = all / n whole groups each, and share the rest of them out.  Many of them (more than a third of n) evenly, in
+// the order of the rows: workgroup i takes the stretch [i rest / n, (i + 1) rest / n), and a part of a group is that part of its tiles.  Few
+// of them have workgroups to themselves, as many as their tiles and rows ask for, since a second opening in a workgroup costs as much as ten
+// tiles and more.  A workgroup that sees a whole group writes its result; parts leave partial sums in the workgroup's two slots (its first
+// group's, and its last one's), which window_merge_kernel adds up.
 
 constexpr int VMCNT_0 = 0x0f70;          // s_waitcnt: no vector memory operation outstanding, the other counters as they are
 
 struct Deal {
     int all, whole, rest;                // row groups of a kv head; whole ones of a workgroup; what is shared out
+    bool apart;                          // the latter have workgroups to themselves
     // the first 64 sequences, one a lane: their query tokens, row groups, and the groups up to and with them
     int qs, qe, count, upto;
+    int first, parts;                    // apart: lane g, the workgroups of the g-th of the groups shared out
 };
 __device__ __forceinline__ int bounded(int x, int T) { return min(max(x, 0), T); }        // a malformed array must not lead outside the buffers
-__device__ __forceinline__ Deal window_deal(const PagedDevHeader& ph, int rows, int n, int lane, int GQ) {
-    Deal d = {0, 0, 0, 0, 0, 0, 0};
+__device__ __forceinline__ Deal window_deal(const WindowHeader& args, const PagedDevHeader& ph, int n, int lane, int GQ) {
+    Deal d = {0, 0, 0, false, 0, 0, 0, 0, 0, 0};
+    const int rows = args.rows, T = ph.LW * ph.LS;
     if (ph.cu_q == nullptr) d.all = ph.W * ph.nrg;
     else {
-        const int T = ph.LW * ph.LS;
         for (int c = 0; c < ph.W; c += 64) {
             const int idx = c + lane;
             const int a0 = bounded(ph.cu_q[min(idx, ph.W)], T), a1 = bounded(ph.cu_q[min(idx + 1, ph.W)], T);
@@ -512,6 +514,40 @@ __device__ __forceinline__ Deal window_deal(const PagedDevHeader& ph, int rows, 
         ++d.whole;
         d.rest = 0;
     }
+    if (d.rest == 0 || d.rest * 3 > n || d.rest > 64) return d;
+    d.apart = true;
+    int cost = 1;                                        // lane g: what the g-th of them costs
+    if (ph.cu_q == nullptr || ph.W <= 64) {
+        const int g = d.whole * n + min(lane, d.rest - 1);
+        int qs, qe, rg;
+        if (ph.cu_q == nullptr) {
+            const int w = fast_div(g, ph.magic_nrg);
+            qs = w * ph.LS;
+            qe = qs + ph.LS;
+            rg = g - w * ph.nrg;
+        } else {
+            int w = 0;                                   // the first sequence with more groups up to and with it
+#pragma unroll
+            for (int step = 32; step > 0; step >>= 1) w += __shfl(d.upto, w + step - 1, 64) <= g ? step : 0;
+            qs = __shfl(d.qs, w, 64);
+            qe = __shfl(d.qe, w, 64);
+            rg = g - __shfl(d.upto - d.count, w, 64);
+        }
+        const int here = min((qe - qs) * GQ - rg * rows, rows);
+        // the tiles that its last row sees, about; a tile of up to eight row blocks takes as long as it needs to come in, each further pair a sixth
+        // of that more; and an opening
+        const int at = min(ph.loc[min(max(qs + (rg * rows + here - 1) / GQ, 0), T - 1)], ph.block_size * ph.max_blocks - 1);
+        const int seen = at < 0 ? 0 : at < args.window ? at : args.window + min(args.sinks, at - args.window);
+        cost = (seen / TILE + 10) * max(6, 3 + (here + 31) / 32 * 3 / 4);
+    }
+    const int mine = lane < d.rest ? cost : 0;
+    const int sum = __builtin_amdgcn_readlane(wave_scan_inclusive(mine), 63);
+    // one workgroup each, the others in proportion (rounded down), and what is left over one more to the first ones
+    const float share = (float)(n - d.rest) * __builtin_amdgcn_rcpf((float)sum) * 0.99999f;
+    d.parts = lane < d.rest ? 1 + (int)((float)mine * share) : 0;
+    const int left = n - __builtin_amdgcn_readlane(wave_scan_inclusive(d.parts), 63);
+    if (lane < min(left, d.rest)) ++d.parts;
+    d.first = wave_scan_inclusive(d.parts) - d.parts;
     return d;
 }
 // Row group g < all: sequence, number in it, query tokens.
@@ -698,7 +734,7 @@ __global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHea
     const int T = ph.LW * ph.LS;
     const int cap = ph.block_size * ph.max_blocks;
     const int rows = args.rows;
-    const Deal deal = window_deal(ph, rows, N, tid & 63, GQ);
+    const Deal deal = window_deal(args, ph, N, tid & 63, GQ);
     unsigned long long image[NI];
     image[0] = reinterpret_cast<unsigned long long>(k_wave ? ph.kcache : ph.vcache);
     if constexpr (BOTH) image[1] = reinterpret_cast<unsigned long long>(ph.vcache);
@@ -707,17 +743,25 @@ __global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHea
     a.Hq = ph.Hq; a.S = ph.LS;
     a.magic_gq = ph.magic_gq; a.magic_s = ph.magic_ls;
 
-    const int begin = me * deal.rest, end = begin + deal.rest;    // in n-ths of a group
-    const int part0 = begin / N, parts = deal.rest > 0 ? (end + N - 1) / N - part0 : 0;
+    int begin = me * deal.rest, end = begin + deal.rest, den = N;                     // the stretch, in den-ths of a group
+    int part0 = begin / N, parts = deal.rest > 0 ? (end + N - 1) / N - part0 : 0;     // its groups
+    if (deal.apart) {
+        const unsigned long long owner = __ballot((tid & 63) < deal.rest && me >= deal.first && me < deal.first + deal.parts);
+        parts = owner != 0 ? 1 : 0;
+        part0 = owner != 0 ? __builtin_ctzll(owner) : 0;
+        den = max(__builtin_amdgcn_readlane(deal.parts, part0), 1);
+        begin = part0 * den + me - __builtin_amdgcn_readlane(deal.first, part0);
+        end = begin + 1;
+    }
     for (int item = 0; item < deal.whole + parts; ++item) {
         const bool whole_one = item < deal.whole;
         const int cut = part0 + item - deal.whole;               // a part: of this one of the groups that are shared out
         const int g = whole_one ? me * deal.whole + item : N * deal.whole + cut;
         if (g >= deal.all) break;                                 // (the last workgroups, where almost a group each was left)
-        const int from = whole_one ? 0 : max(begin - cut * N, 0), to = whole_one ? N : min(end - cut * N, N);
+        const int from = whole_one ? 0 : max(begin - cut * den, 0), to = whole_one ? den : min(end - cut * den, den);
         const WindowGroup it = window_group(ph, deal, rows, g, tid & 63, GQ);
         const int r0 = it.qs * GQ + it.rg * rows, rend = min(it.qe * GQ, r0 + rows);
-        const bool whole = from == 0 && to == N;
+        const bool whole = from == 0 && to == den;
         const size_t pbase = ((size_t)hkv * 2 * N + 2 * me + (cut == part0 ? 0 : 1)) * ROWS;
         const HW_GLOBAL int* btw = ph.block_table + (size_t)it.w * ph.max_blocks;
 
@@ -796,7 +840,7 @@ __global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHea
                 const int x = k + (k >= full0 ? full1 - full0 : 0) - (k >= part ? tiles - full0 : 0);
                 return x + (x >= sink_tiles ? jump : 0);
             };
-            const int k0 = tiles * from / N, k1 = tiles * to / N;
+            const int k0 = tiles * from / den, k1 = tiles * to / den;
 
             WaveState<RBX, G::NOC> st;
 #pragma unroll
@@ -991,17 +1035,21 @@ __global__ __launch_bounds__(256) void window_merge_kernel(const WindowHeader ar
     const int rblk = bid % BLOCKS, hc = bid / BLOCKS;
     const int hkv = hc / cuts, cut = hc - hkv * cuts;
     const int rows = args.rows;
-    const Deal deal = window_deal(ph, rows, N, lane, GQ);
+    const Deal deal = window_deal(args, ph, N, lane, GQ);
     const int rest = deal.rest;
     if (cut >= rest) return;
-    const int first = cut * N / rest, last = ((cut + 1) * N - 1) / rest;       // its workgroups
+    int first = cut * N / rest, last = ((cut + 1) * N - 1) / rest;             // its workgroups
+    if (deal.apart) {
+        first = __builtin_amdgcn_readlane(deal.first, cut);
+        last = first + __builtin_amdgcn_readlane(deal.parts, cut) - 1;
+    }
     if (first == last) return;                   // it saw the whole group
     const WindowGroup it = window_group(ph, deal, rows, N * deal.whole + cut, lane, GQ);
     const int r0 = it.qs * GQ + it.rg * rows, rend = min(it.qe * GQ, r0 + rows);
     const int rr = rblk * RPB * PER + tid / V4, e = tid % V4 * 4;
     if (r0 + rr >= rend) return;
     // (the slot of workgroup w: its first group's, or, for the one that begins the group in the middle of its stretch, the other)
-    auto row_of = [&](int w, int i) { return ((size_t)hkv * 2 * N + 2 * w + (w * rest / N == cut ? 0 : 1)) * ROWS + min(rr + i * RPB, rend - 1 - r0); };
+    auto row_of = [&](int w, int i) { return ((size_t)hkv * 2 * N + 2 * w + (deal.apart || w * rest / N == cut ? 0 : 1)) * ROWS + min(rr + i * RPB, rend - 1 - r0); };
     float m[PER], l[PER];
     f32x4 acc[PER];
 #pragma unroll
