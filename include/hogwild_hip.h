@@ -460,7 +460,7 @@ int hw_packed_slots(const hw_packed_batch* b, void* stream);
 
 /* Rows key_states / value_states [total, Hkv, D] (element strides for the first two dimensions, a contiguous last one) to the rows
    `slots` of the caches [num_blocks, Hkv, block_size, D].  Rows whose slot is no row of the caches are left out; no slot is named
-   twice. */
+   twice.  Hkv * (E + Ev) <= 2^16. */
 typedef struct hw_copy_slots {
     int32_t dtype;
     int32_t total, Hkv, E, Ev;
@@ -499,7 +499,7 @@ typedef struct hw_verify {
     int32_t* seq_lengths;          /* [W] or NULL */
     void* tokens;                  /* [W, K + 1] */
     int32_t* accepted;             /* [W] */
-    void* workspace;               /* hw_verify_workspace_bytes() bytes, 16-byte aligned */
+    void* workspace;               /* hw_verify_workspace_bytes() bytes, 16-byte aligned (NULL if those are 0) */
     size_t workspace_bytes;
 } hw_verify;
 int hw_verify_workspace_bytes(const hw_verify* v, size_t* bytes);

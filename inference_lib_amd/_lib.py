@@ -826,8 +826,8 @@ def verify_drafts(drafts: torch.Tensor, target_probs: torch.Tensor, uniforms: to
     with torch.cuda.device(device):
         n = C.c_size_t(0)
         check(lib.hw_verify_workspace_bytes(C.byref(v), C.byref(n)), "hw_verify_workspace_bytes")
-        ws = torch.empty(n.value, dtype=torch.uint8, device=device)
-        v.workspace, v.workspace_bytes = ws.data_ptr(), n.value
+        ws = torch.empty(n.value, dtype=torch.uint8, device=device) if n.value else None
+        v.workspace, v.workspace_bytes = ptr(ws), n.value
         check(lib.hw_verify_drafts(C.byref(v), C.c_void_p(torch.cuda.current_stream(device).cuda_stream)), "hw_verify_drafts")
     return tokens, accepted
 

@@ -759,9 +759,12 @@ std::tuple<at::Tensor, at::Tensor> verify_drafts(const at::Tensor& drafts, const
     c10::hip::HIPGuardMasqueradingAsCUDA guard(device);
     size_t bytes = 0;
     check_status(hw_verify_workspace_bytes(&v, &bytes), "hw_verify_workspace_bytes");
-    const at::Tensor workspace = at::empty({(int64_t)bytes}, uniforms.options().dtype(at::kByte));
-    v.workspace = workspace.data_ptr();
-    v.workspace_bytes = bytes;
+    at::Tensor workspace;
+    if (bytes > 0) {
+        workspace = at::empty({(int64_t)bytes}, uniforms.options().dtype(at::kByte));
+        v.workspace = workspace.data_ptr();
+        v.workspace_bytes = bytes;
+    }
     check_status(hw_verify_drafts(&v, stream_of(target_probs)), "hw_verify_drafts");
     return {tokens, accepted};
 }

@@ -764,6 +764,26 @@ struct PagedDevHeader {
 static_assert(sizeof(PagedDevHeader) == 160, "40 dwords of PagedHeader are fetched");
 static_assert(offsetof(PagedHeader, pad) == 160, "PagedDevHeader mirrors the used part of PagedHeader");
 
+// SMALL: below 4 GB the K cache is reached through one buffer descriptor, and its transfers are buffer loads.  A transfer by 64-bit address
+// is a flat-encoded instruction with an LDS operand, for which the compiler waits until nothing is outstanding: it emptied the
+// look-ahead at every tile (vmcnt(0) in front of each request, where 16 and 17 operations may be in flight).  Four sequences of 12 528
+// tokens, append and attention 41.2 -> 39.3 us (6.0 TB/s in the attention), 2500 to 3600 tokens 18.2 -> 17.1, five of 296 to 10 543 22.3 -> 20.4;
+// bit-identical.
+struct CacheView {
+    __amdgpu_buffer_rsrc_t k;
+};
+__device__ __forceinline__ CacheView make_cache_view(const PagedDevHeader& ph, int krow) {
+    CacheView v;
+    v.k = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(reinterpret_cast<unsigned long long>(ph.kcache)), 0,
+                                            (int)((unsigned)ph.num_blocks * (unsigned)ph.Hkv * (unsigned)ph.block_size * (unsigned)krow), 0x00020000);
+    return v;
+}
+
+template <int AUX>
+__device__ __forceinline__ void cache_transfer(const CacheView& v, char* lds, unsigned offset) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(v.k, HW_LDS_PTR(lds), 16, offset, 0, 0, AUX);
+}
+
 // n / d for n < 2^20, d < 2^12 with the host-computed multiplier ceil(2^32 / d) mod 2^32: one multiply-high instead
 // of the ~25-instruction integer division sequence.  d == 1 gives the multiplier 0, which stands for "n itself".
 // Without a branch on purpose: the multiplier is uniform, a branch on it cuts the code around every division into basic

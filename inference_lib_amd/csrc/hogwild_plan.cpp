@@ -878,7 +878,7 @@ int window_plan(const hw_window_problem* p, int num_cus, hw_paged_plan* plan) {
         if (plan->splits > 1) plan->workspace_bytes = (size_t)p->Hkv * 2 * plan->splits * (p->D == 256 ? hw::WINDOW_ROWS_256 : hw::WINDOW_ROWS) * ((size_t)p->D + 2) * sizeof(float);
         return HW_OK;
     }
-    if (splits == 0) splits = std::max(1ll, std::min((num_cus + groups - 1) / groups, tiles / (2 * hw::NWAVES)));
+    if (splits == 0) splits = std::max(1ll, std::min((num_cus + groups - 1) / groups, (tiles + 2 * hw::NWAVES - 1) / (2 * hw::NWAVES)));
     splits = std::min(splits, (long long)HW_MAX_SPLITS);
     plan->splits = (int)splits;
     const long long wgs = groups * splits;

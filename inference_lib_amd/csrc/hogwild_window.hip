@@ -261,7 +261,8 @@ __device__ __forceinline__ WindowItem window_item(const PagedDevHeader& ph, int 
     return it;
 }
 
-template <class DT, int D, int RB>
+// SMALL: the K cache is reached through one buffer descriptor (see make_cache_view).
+template <class DT, int D, int RB, bool SMALL>
 __global__ __launch_bounds__(NTHREADS, 1) void window_kernel(const WindowHeader args) {
     typedef Geo<DT, D, D> G;
     typedef typename Elem<DT>::store_t store_t;
@@ -304,6 +305,8 @@ __global__ __launch_bounds__(NTHREADS, 1) void window_kernel(const WindowHeader 
     st.fresh = true;
     const PagedDevHeader ph = paged_header_wait(hb);
     const bool direct = (ph.flags & PH_DIRECT) != 0;
+    [[maybe_unused]] CacheView all;              // the whole K cache
+    if constexpr (SMALL) all = make_cache_view(ph, G::KROW);
 
     // logical workgroup id = ((kv head * nitems) + item) * nsplit + split; consecutive ids share an XCD
     int bid = blockIdx.x;
@@ -405,8 +408,12 @@ __global__ __launch_bounds__(NTHREADS, 1) void window_kernel(const WindowHeader 
 #pragma unroll
         for (int i = 0; i < G::KL; ++i) {
             const int r = __shfl(rid, i * RPL + lrow, 64);
-            const HW_GLOBAL char* src = ph.kcache + (unsigned long long)(unsigned)r * G::KROW + k_chunk(i);
-            __builtin_amdgcn_global_load_lds(src, HW_LDS_PTR(kslot + i * 1024), 16, 0, HW_KV_AUX);
+            if constexpr (SMALL) {
+                cache_transfer<HW_KV_AUX>(all, kslot + i * 1024, (unsigned)r * G::KROW + k_chunk(i));
+            } else {
+                const HW_GLOBAL char* src = ph.kcache + (unsigned long long)(unsigned)r * G::KROW + k_chunk(i);
+                __builtin_amdgcn_global_load_lds(src, HW_LDS_PTR(kslot + i * 1024), 16, 0, HW_KV_AUX);
+            }
         }
         asm volatile("" ::: "memory");
 #pragma unroll
@@ -1129,12 +1136,14 @@ static hipError_t launch_window_d(const WindowHeader& wh, int rb, hipStream_t st
     }
     if constexpr (Elem<DT>::size == 2 && D <= 128) {
         if (rb == 2) {
-            hipLaunchKernelGGL((window_kernel<DT, D, 2>), dim3(wh.p.nwg), dim3(NTHREADS), 0, stream, wh);
+            if (wh.p.flags & PH_SMALL) hipLaunchKernelGGL((window_kernel<DT, D, 2, true>), dim3(wh.p.nwg), dim3(NTHREADS), 0, stream, wh);
+            else hipLaunchKernelGGL((window_kernel<DT, D, 2, false>), dim3(wh.p.nwg), dim3(NTHREADS), 0, stream, wh);
             return hipGetLastError();
         }
     }
     if (rb != 1) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((window_kernel<DT, D, 1>), dim3(wh.p.nwg), dim3(NTHREADS), 0, stream, wh);
+    if (wh.p.flags & PH_SMALL) hipLaunchKernelGGL((window_kernel<DT, D, 1, true>), dim3(wh.p.nwg), dim3(NTHREADS), 0, stream, wh);
+    else hipLaunchKernelGGL((window_kernel<DT, D, 1, false>), dim3(wh.p.nwg), dim3(NTHREADS), 0, stream, wh);
     return hipGetLastError();
 }
 
