@@ -740,23 +740,23 @@ def window_plan(*, W: int, Hq: int, Hkv: int, D: int, block_size: int, max_block
     return out
 
 
-def packed_slots(block_table: torch.Tensor, positions: torch.Tensor, n_new: torch.Tensor, total: int, block_size: int, num_blocks: int):
-    """(cu_seqlens [W + 1], locations [total], slots [total]) of a packed batch, int32."""
+def packed_slots(block_table: torch.Tensor, positions: torch.Tensor, n_new: torch.Tensor, cu_seqlens: torch.Tensor, locations: torch.Tensor,
+                 slots: torch.Tensor, block_size: int, num_blocks: int) -> None:
+    """cu_seqlens [W + 1], locations [total] and slots [total] of a packed batch, int32."""
     if block_table.dim() != 2 or block_table.numel() == 0 or tuple(positions.shape) != (block_table.size(0),) or positions.shape != n_new.shape:
         raise ValueError("block_table must be [W, max_blocks], positions and n_new [W]")
-    for t in (block_table, positions, n_new):
+    W, total, block_size, num_blocks = block_table.size(0), locations.numel(), int(block_size), int(num_blocks)
+    if tuple(cu_seqlens.shape) != (W + 1,) or tuple(locations.shape) != (total,) or slots.shape != locations.shape:
+        raise ValueError("cu_seqlens must be [W + 1], locations and slots [total]")
+    for t in (block_table, positions, n_new, cu_seqlens, locations, slots):
         if t.dtype != torch.int32 or not t.is_contiguous() or t.device != block_table.device:
-            raise ValueError("block_table, positions and n_new must be contiguous int32 on one device")
-    total, block_size, num_blocks = int(total), int(block_size), int(num_blocks)
-    if not 0 <= total < 1 << 28 or not 1 <= block_size < 1 << 31 or not 1 <= num_blocks < 1 << 31:
-        raise ValueError("total must be 0 .. 2^28 - 1, block_size and num_blocks positive")
-    W = block_table.size(0)
-    cu, loc, slots = (torch.empty(n, dtype=torch.int32, device=block_table.device) for n in (W + 1, total, total))
+            raise ValueError("the tables of a packed batch must be contiguous int32 on one device")
+    if total >= 1 << 28 or not 1 <= block_size < 1 << 31 or not 1 <= num_blocks < 1 << 31:
+        raise ValueError("total must be below 2^28, block_size and num_blocks positive")
     b = HwPackedBatch(W, block_table.size(1), num_blocks, block_size, total, block_table.data_ptr(), positions.data_ptr(), n_new.data_ptr(),
-                      cu.data_ptr(), loc.data_ptr(), slots.data_ptr())
+                      cu_seqlens.data_ptr(), locations.data_ptr(), slots.data_ptr())
     with torch.cuda.device(block_table.device):
         check(lib.hw_packed_slots(C.byref(b), C.c_void_p(torch.cuda.current_stream(block_table.device).cuda_stream)), "hw_packed_slots")
-    return cu, loc, slots
 
 
 def copy_to_slots(key_states: torch.Tensor, value_states: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, slots: torch.Tensor) -> None:

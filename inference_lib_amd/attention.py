@@ -260,15 +260,21 @@ def hogwild_varlen_paged_sdpa_window(queries: torch.Tensor, locations: torch.Ten
     return _window_sdpa(queries, locations, key_cache, value_cache, block_table, cu_seqlens_q, scale, window, sinks, out, lse)
 
 
-def packed_slots(block_table: torch.Tensor, positions: torch.Tensor, n_new: torch.Tensor, total: int, block_size: int,
-                 num_blocks: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+def packed_slots(block_table: torch.Tensor, positions: torch.Tensor, n_new: torch.Tensor, total: int, block_size: int, num_blocks: int,
+                 out: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """A packed batch laid out on the device: the new tokens of all sequences one behind the other, n_new[w] (int32 [W]) of sequence w from
     positions[w] (int32 [W]) on, in `total` rows.  Returns cu_seqlens [W+1], where each sequence begins, and of every row its position and
     its row of the caches [total] each, all int32.  Both are -1 for tokens that have no place (behind the last sequence or the block table,
-    on no page); what goes beyond `total` rows is cut off."""
+    on no page); what goes beyond `total` rows is cut off.  `out`: the three tensors to write into."""
+    if out is None:
+        out = tuple(torch.empty(n, dtype=torch.int32, device=block_table.device) for n in (block_table.size(0) + 1, int(total), int(total)))
+    elif out[1].numel() != int(total):
+        raise ValueError("out must be (cu_seqlens [W + 1], locations [total], slots [total])")
     if HAVE_TORCH_OPS:
-        return torch.ops.libhogatt.packed_slots(block_table, positions, n_new, total, block_size, num_blocks)
-    return _lib.packed_slots(block_table, positions, n_new, total, block_size, num_blocks)
+        torch.ops.libhogatt.packed_slots(block_table, positions, n_new, *out, block_size, num_blocks)
+    else:
+        _lib.packed_slots(block_table, positions, n_new, *out, block_size, num_blocks)
+    return out
 
 
 def copy_to_slots(key_states: torch.Tensor, value_states: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,

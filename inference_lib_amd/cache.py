@@ -21,7 +21,7 @@ Everything numeric runs in the HIP library; there is no torch fallback.
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Any, Dict, List, Optional, Sequence
+from typing import Any, Dict, List, Optional, Sequence, Tuple
 
 import torch
 
@@ -409,6 +409,16 @@ class PagedCache:
         cache.fork(parents)                              # sequence w goes on as sequence parents[w]; pages are shared until they are written
         cache.free(finished); cache.compact()            # pages in use to the front of the pool
 
+    With `window` the attention is that of hogwild_paged_sdpa_window: the last `window` positions and the first `sinks` (16 and 32 bits), and
+    trim() gives back the pages that no later token sees.  Steps in which sequences bring different numbers of tokens need not be padded:
+
+        cache.reserve_packed(n_new, total)               # n_new int32 [max_seqs]; the batch's rows, total of them
+        for layer in ...:
+            cache.update_packed(k, v, layer)             # [total, Hkv, D] (16 and 32 bits)
+            out = cache.attend_packed(q, layer, scale)   # [total, Hq, D]
+        tokens, accepted = cache.verify(drafts, target_probs, uniforms)      # a step of one token and its drafts: which of them stand
+        cache.trim()
+
     A sequence that `reserve` has nothing for (the pool or its row of the table is full, or it asked for no tokens) is left out of the
     step: its states are not written, its output is 0 and its length stays; `granted()` says which ones took part.  Tokens behind those
     that a sequence asked for get 0 too; no other sequence sees their states.  A sequence has at most max_blocks pages: by default as many as
@@ -420,7 +430,12 @@ class PagedCache:
     MAX_POSITIONS, MAX_BLOCK_SIZE = 1 << 20, 1 << 12         # of hw_paged_sdpa and hw_paged_sdpa_q4
 
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, num_blocks: int, max_seqs: int, *, block_size: int = 16,
-                 max_blocks: Optional[int] = None, bits: int = 16, dtype=torch.bfloat16, device="cuda"):
+                 max_blocks: Optional[int] = None, bits: int = 16, dtype=torch.bfloat16, device="cuda", window: Optional[int] = None, sinks: int = 0):
+        if window is None and sinks != 0:
+            raise ValueError("sinks are tokens that stay visible outside of a window: there is none")
+        if window is not None and (int(window) < 1 or int(sinks) < 0 or bits == 4):
+            raise ValueError("window must be positive and sinks not negative, and a window needs a cache in 16 or 32 bits")
+        self.window, self.sinks = None if window is None else int(window), int(sinks)
         if bits not in (4, 16, 32) or (bits != 4 and torch.empty((), dtype=dtype).element_size() * 8 != bits):
             raise ValueError(f"bits must be 4, or the size of {dtype}")
         self.bits, self.block_size, self.dtype = bits, int(block_size), dtype
@@ -444,6 +459,8 @@ class PagedCache:
         self.used = torch.zeros(1, **ints)
         self._longest = torch.full((1,), max_blocks * self.block_size, **ints)
         self._made: Dict[tuple, torch.Tensor] = {}       # locations, by capture and number of tokens
+        self._layouts: Dict[int, tuple] = {}             # (cu_seqlens, locations, slots) of packed batches, by their rows, the last one used last
+        self._in_graphs = set()                          # rows of those that a graph writes or reads
         self._replayed = False                           # whether a graph holds a reserve
 
     @property
@@ -482,8 +499,64 @@ class PagedCache:
         append(key_states, value_states, self.keys[layer_idx], self.values[layer_idx], self.block_table, self.positions)
 
     def attend(self, queries: torch.Tensor, layer_idx: int, scale: float) -> torch.Tensor:
+        if self.window is not None:
+            return _ops.hogwild_paged_sdpa_window(queries, self._locations(queries.size(2))[0], self.keys[layer_idx], self.values[layer_idx],
+                                                  self.block_table, scale, self.window, self.sinks)
         sdpa = _ops.hogwild_paged_sdpa_q4 if self.bits == 4 else _ops.hogwild_paged_sdpa
         return sdpa(queries.unsqueeze(0), self._locations(queries.size(2)), self._longest, self.keys[layer_idx], self.values[layer_idx], self.block_table, scale)
+
+    KEPT_LAYOUTS = 8                                     # of batches that no graph holds
+
+    def reserve_packed(self, n_new: torch.Tensor, total: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Room for n_new[w] tokens of every sequence, which lie one behind the other in the batch's `total` rows.  Returns where each begins,
+        int32 [max_seqs + 1], and the rows' positions, int32 [total], -1 for those that take no part: rows behind the last sequence's, and
+        those of a sequence that the pool had nothing for.  update_packed and attend_packed go by the last batch of as many rows; its
+        layout is written over by the next one."""
+        if self.bits == 4:
+            raise ValueError("packed batches are for caches in 16 and 32 bits")
+        total = int(total)
+        if total < 0 or not isinstance(n_new, torch.Tensor):
+            raise ValueError("n_new: a tensor of one number per sequence; total: the rows of the batch")
+        positions = self.reserve(n_new)
+        out = _ops.packed_slots(self.block_table, positions, n_new, total, self.block_size, self.ref_counts.numel(), out=self._layouts.pop(total, None))
+        self._layouts[total] = out
+        self._hold(total)
+        loose = [rows for rows in self._layouts if rows not in self._in_graphs]
+        for rows in loose[: max(0, len(loose) - self.KEPT_LAYOUTS)]:
+            del self._layouts[rows]
+        return out[0], out[1]
+
+    def _hold(self, rows: int) -> None:
+        if self._capture() != 0:                         # the graph goes on using the tensors
+            self._in_graphs.add(rows)
+
+    def _layout(self, rows: int) -> tuple:
+        if rows not in self._layouts:
+            raise ValueError(f"reserve_packed was not called for a batch of {rows} rows")
+        self._hold(rows)
+        return self._layouts[rows]
+
+    def update_packed(self, key_states: torch.Tensor, value_states: torch.Tensor, layer_idx: int) -> None:
+        _ops.copy_to_slots(key_states, value_states, self.keys[layer_idx], self.values[layer_idx], self._layout(key_states.size(0))[2])
+
+    def attend_packed(self, queries: torch.Tensor, layer_idx: int, scale: float) -> torch.Tensor:
+        """[total, Hq, D]; 0 for rows that take no part."""
+        cu, locations, _ = self._layout(queries.size(0))
+        window = self.window if self.window is not None else (1 << 31) - 1
+        return _ops.hogwild_varlen_paged_sdpa_window(queries, locations, self.keys[layer_idx], self.values[layer_idx], self.block_table, cu, scale,
+                                                     window, self.sinks)
+
+    def verify(self, drafts: torch.Tensor, target_probs: torch.Tensor, uniforms: torch.Tensor, draft_probs: Optional[torch.Tensor] = None,
+               n_drafts: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Which drafts of the step stand, and the next tokens (attention.verify_drafts), after a reserve of 1 + n_drafts[w] tokens: the last
+        token of every sequence and its drafts.  What does not stand leaves the sequences; the next tokens are not in them yet."""
+        return _ops.verify_drafts(drafts, target_probs, uniforms, draft_probs, n_drafts, self.positions, self.seq_lengths)
+
+    def trim(self) -> None:
+        """The pages that no later token sees are given back.  (After verify: a length that is shortened later needs them again.)"""
+        if self.window is None:
+            raise ValueError("without a window every token is seen")
+        _ops.trim_blocks(self.block_table, self.seq_lengths, self.ref_counts, self.window, self.sinks, self.block_size)
 
     def fork(self, parents: torch.Tensor) -> None:
         _ops.fork_blocks(self.block_table, self.seq_lengths, self.ref_counts, parents, self.block_size)

@@ -654,30 +654,31 @@ void trim_blocks(at::Tensor& block_table, const at::Tensor& seq_lengths, at::Ten
     check_status(hw_trim_blocks(&u.p, (int)window, (int)sinks, stream_of(block_table)), "hw_trim_blocks");
 }
 
-// (cu_seqlens [W + 1], locations [total], slots [total])
-std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_slots(const at::Tensor& block_table, const at::Tensor& positions, const at::Tensor& n_new, int64_t total,
-                                                            int64_t block_size, int64_t num_blocks) {
+void packed_slots(const at::Tensor& block_table, const at::Tensor& positions, const at::Tensor& n_new, at::Tensor& cu_seqlens, at::Tensor& locations, at::Tensor& slots,
+                  int64_t block_size, int64_t num_blocks) {
     TORCH_CHECK(block_table.dim() == 2 && block_table.scalar_type() == at::kInt && block_table.is_contiguous() && block_table.numel() > 0,
                 "libhogatt: block_table must be contiguous int32 [W, max_blocks]");
     for (const at::Tensor* t : {&positions, &n_new})
         TORCH_CHECK(t->dim() == 1 && t->size(0) == block_table.size(0) && t->scalar_type() == at::kInt && t->is_contiguous() && t->device() == block_table.device(),
                     "libhogatt: positions and n_new must be contiguous int32 [W] on the table's device");
-    TORCH_CHECK(total >= 0 && total < (1ll << 28) && block_size >= 1 && block_size < (1ll << 31) && num_blocks >= 1 && num_blocks < (1ll << 31) &&
+    const int64_t W = block_table.size(0), total = locations.numel();
+    TORCH_CHECK(total < (1ll << 28) && block_size >= 1 && block_size < (1ll << 31) && num_blocks >= 1 && num_blocks < (1ll << 31) &&
                     block_table.size(0) < (1ll << 31) && block_table.size(1) < (1ll << 31),
-                "libhogatt: packed_slots: total must be 0 .. 2^28 - 1, block_size and num_blocks positive");
-    const int64_t W = block_table.size(0);
-    const at::Tensor cu = at::empty({W + 1}, positions.options()), loc = at::empty({total}, positions.options()), slots = at::empty({total}, positions.options());
+                "libhogatt: packed_slots: total must be below 2^28, block_size and num_blocks positive");
+    TORCH_CHECK(cu_seqlens.dim() == 1 && cu_seqlens.size(0) == W + 1 && locations.dim() == 1 && slots.dim() == 1 && slots.size(0) == total,
+                "libhogatt: cu_seqlens must be [W + 1], locations and slots [total]");
+    for (const at::Tensor* t : std::initializer_list<const at::Tensor*>{&cu_seqlens, &locations, &slots})
+        TORCH_CHECK(t->scalar_type() == at::kInt && t->is_contiguous() && t->device() == block_table.device(), "libhogatt: packed_slots writes contiguous int32 on the table's device");
     hw_packed_batch b{};
     b.W = (int32_t)W; b.max_blocks = (int32_t)block_table.size(1); b.num_blocks = (int32_t)num_blocks; b.block_size = (int32_t)block_size; b.total = (int32_t)total;
     b.block_table = block_table.const_data_ptr<int32_t>();
     b.positions = positions.const_data_ptr<int32_t>();
     b.n_new = n_new.const_data_ptr<int32_t>();
-    b.cu_seqlens = cu.data_ptr<int32_t>();
-    b.locations = loc.data_ptr<int32_t>();
+    b.cu_seqlens = cu_seqlens.data_ptr<int32_t>();
+    b.locations = locations.data_ptr<int32_t>();
     b.slots = slots.data_ptr<int32_t>();
     c10::hip::HIPGuardMasqueradingAsCUDA guard(block_table.device());
     check_status(hw_packed_slots(&b, stream_of(block_table)), "hw_packed_slots");
-    return {cu, loc, slots};
 }
 
 void copy_to_slots(const at::Tensor& key_states, const at::Tensor& value_states, at::Tensor& key_cache, at::Tensor& value_cache, const at::Tensor& slots) {
@@ -988,7 +989,8 @@ TORCH_LIBRARY(libhogatt, m) {
     m.def("window_paged_sdpa(Tensor(a!) output, Tensor(b!)? lse, float scale, Tensor locations, Tensor queries, "
           "Tensor key_cache, Tensor value_cache, Tensor block_table, Tensor? cu_seqlens_q, int window, int sinks) -> ()", tags);
     m.def("trim_blocks(Tensor(a!) block_table, Tensor seq_lengths, Tensor(b!) ref_counts, int window, int sinks, int block_size) -> ()", tags);
-    m.def("packed_slots(Tensor block_table, Tensor positions, Tensor n_new, int total, int block_size, int num_blocks) -> (Tensor, Tensor, Tensor)", tags);
+    m.def("packed_slots(Tensor block_table, Tensor positions, Tensor n_new, Tensor(a!) cu_seqlens, Tensor(b!) locations, Tensor(c!) slots, "
+          "int block_size, int num_blocks) -> ()", tags);
     m.def("copy_to_slots(Tensor key_states, Tensor value_states, Tensor(a!) key_cache, Tensor(b!) value_cache, Tensor slots) -> ()", tags);
     m.def("verify_drafts(Tensor drafts, Tensor target_probs, Tensor uniforms, Tensor? draft_probs, Tensor? n_drafts, Tensor? positions, "
           "Tensor(a!)? seq_lengths) -> (Tensor, Tensor)", tags);

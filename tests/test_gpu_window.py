@@ -238,3 +238,37 @@ def test_no_query_tokens():
     q = torch.zeros((0, 4, 64), dtype=torch.float16, device=DEV)
     out = ops().hogwild_varlen_paged_sdpa_window(q, torch.zeros(0, dtype=torch.int32, device=DEV), kc, kc, t, torch.zeros(3, dtype=torch.int32, device=DEV), 1.0, 5)
     assert out.shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("dtype,heads", [("bf16", (8, 2, 64)), ("f16", (5, 1, 128)), ("bf16", (2, 2, 256)), ("f32", (4, 2, 64))], ids=str)
+@pytest.mark.parametrize("W", [5, 64, 65, 130])
+def test_many_sequences_of_all_lengths(dtype, heads, W):
+    """More sequences than a wave has lanes, some without tokens; workgroups shared out in every way."""
+    g = torch.Generator().manual_seed(W)
+    positions = []
+    for w in range(W):
+        s = [0, 1, 1, 2, 7, 40][int(torch.randint(0, 6, (1,), generator=g))]
+        n = s + int(torch.randint(0, 300, (1,), generator=g))
+        positions.append(list(range(n - s, n)))
+    b = Batch(dtype, *heads, positions, 90, 5, 16, seed=W)
+    b.check(b.packed(behind=2))
+    if dtype != "f32":
+        for splits in (1, 3, 30, 256):
+            b.check(b.packed(splits, 8, behind=9), f"128-row groups, {splits}")
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_random_batches(seed):
+    import random
+    rng = random.Random(seed)
+    Hq, Hkv, D = rng.choice(HEADS)
+    dtype = rng.choice(["f16", "bf16", "f32"]) if D < 256 else "bf16"
+    positions = []
+    for _ in range(rng.randint(1, 9)):
+        s = rng.choice([0, 1, 1, 3, 33, 100, 170])
+        n = s + rng.choice([0, 1, 31, 700, 1500])
+        positions.append(list(range(n - s, n)))
+    if not any(positions):
+        positions[0] = [12]
+    b = Batch(dtype, Hq, Hkv, D, positions, rng.choice([1, 31, 32, 33, 200, 1000]), rng.choice([0, 0, 1, 32, 77]), rng.choice([1, 8, 16, 17, 64]), seed=seed)
+    b.check(b.packed(splits=rng.choice([0, 0, 1, 4, 9]), before=rng.choice([0, 3]), behind=rng.choice([0, 1, 300])))
