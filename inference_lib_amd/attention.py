@@ -267,11 +267,13 @@ def packed_slots(block_table: torch.Tensor, positions: torch.Tensor, n_new: torc
     its row of the caches [total] each, all int32.  Both are -1 for tokens that have no place (behind the last sequence or the block table,
     on no page); what goes beyond `total` rows is cut off.  `out`: the three tensors to write into."""
     if out is None:
+        if HAVE_TORCH_OPS:
+            return torch.ops.libhogatt.packed_slots(block_table, positions, n_new, total, block_size, num_blocks)
         out = tuple(torch.empty(n, dtype=torch.int32, device=block_table.device) for n in (block_table.size(0) + 1, int(total), int(total)))
     elif out[1].numel() != int(total):
         raise ValueError("out must be (cu_seqlens [W + 1], locations [total], slots [total])")
     if HAVE_TORCH_OPS:
-        torch.ops.libhogatt.packed_slots(block_table, positions, n_new, *out, block_size, num_blocks)
+        torch.ops.libhogatt.packed_slots_out(block_table, positions, n_new, *out, block_size, num_blocks)
     else:
         _lib.packed_slots(block_table, positions, n_new, *out, block_size, num_blocks)
     return out

@@ -654,8 +654,8 @@ void trim_blocks(at::Tensor& block_table, const at::Tensor& seq_lengths, at::Ten
     check_status(hw_trim_blocks(&u.p, (int)window, (int)sinks, stream_of(block_table)), "hw_trim_blocks");
 }
 
-void packed_slots(const at::Tensor& block_table, const at::Tensor& positions, const at::Tensor& n_new, at::Tensor& cu_seqlens, at::Tensor& locations, at::Tensor& slots,
-                  int64_t block_size, int64_t num_blocks) {
+void packed_slots_out(const at::Tensor& block_table, const at::Tensor& positions, const at::Tensor& n_new, at::Tensor& cu_seqlens, at::Tensor& locations,
+                      at::Tensor& slots, int64_t block_size, int64_t num_blocks) {
     TORCH_CHECK(block_table.dim() == 2 && block_table.scalar_type() == at::kInt && block_table.is_contiguous() && block_table.numel() > 0,
                 "libhogatt: block_table must be contiguous int32 [W, max_blocks]");
     for (const at::Tensor* t : {&positions, &n_new})
@@ -681,6 +681,15 @@ void packed_slots(const at::Tensor& block_table, const at::Tensor& positions, co
     check_status(hw_packed_slots(&b, stream_of(block_table)), "hw_packed_slots");
 }
 
+// (cu_seqlens [W + 1], locations [total], slots [total])
+std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_slots(const at::Tensor& block_table, const at::Tensor& positions, const at::Tensor& n_new, int64_t total,
+                                                            int64_t block_size, int64_t num_blocks) {
+    TORCH_CHECK(block_table.dim() == 2 && block_table.scalar_type() == at::kInt && total >= 0, "libhogatt: block_table must be contiguous int32 [W, max_blocks], total not negative");
+    at::Tensor cu = at::empty({block_table.size(0) + 1}, block_table.options()), loc = at::empty({total}, block_table.options()), slots = at::empty({total}, block_table.options());
+    packed_slots_out(block_table, positions, n_new, cu, loc, slots, block_size, num_blocks);
+    return {cu, loc, slots};
+}
+
 void copy_to_slots(const at::Tensor& key_states, const at::Tensor& value_states, at::Tensor& key_cache, at::Tensor& value_cache, const at::Tensor& slots) {
     TORCH_CHECK(key_states.dim() == 3 && value_states.dim() == 3 && key_states.size(0) == value_states.size(0) && key_states.size(1) == value_states.size(1),
                 "libhogatt: key_states / value_states must be [total, Hkv, D]");
@@ -693,6 +702,7 @@ void copy_to_slots(const at::Tensor& key_states, const at::Tensor& value_states,
     TORCH_CHECK(slots.dim() == 1 && slots.size(0) == key_states.size(0) && slots.scalar_type() == at::kInt && slots.is_contiguous(), "libhogatt: slots must be contiguous int32 [total]");
     for (const at::Tensor* t : std::initializer_list<const at::Tensor*>{&key_states, &value_states, &value_cache, &slots})
         TORCH_CHECK(t->device() == key_cache.device(), "libhogatt: all tensors must live on the caches' device");
+    TORCH_CHECK(key_states.size(0) < (1ll << 31), "libhogatt: copy_to_slots: too many rows");
     const at::Tensor ks = (key_states.size(2) > 1 && key_states.stride(2) != 1) ? key_states.contiguous() : key_states;
     const at::Tensor vs = (value_states.size(2) > 1 && value_states.stride(2) != 1) ? value_states.contiguous() : value_states;
     hw_copy_slots c{};
@@ -989,7 +999,8 @@ TORCH_LIBRARY(libhogatt, m) {
     m.def("window_paged_sdpa(Tensor(a!) output, Tensor(b!)? lse, float scale, Tensor locations, Tensor queries, "
           "Tensor key_cache, Tensor value_cache, Tensor block_table, Tensor? cu_seqlens_q, int window, int sinks) -> ()", tags);
     m.def("trim_blocks(Tensor(a!) block_table, Tensor seq_lengths, Tensor(b!) ref_counts, int window, int sinks, int block_size) -> ()", tags);
-    m.def("packed_slots(Tensor block_table, Tensor positions, Tensor n_new, Tensor(a!) cu_seqlens, Tensor(b!) locations, Tensor(c!) slots, "
+    m.def("packed_slots(Tensor block_table, Tensor positions, Tensor n_new, int total, int block_size, int num_blocks) -> (Tensor, Tensor, Tensor)", tags);
+    m.def("packed_slots_out(Tensor block_table, Tensor positions, Tensor n_new, Tensor(a!) cu_seqlens, Tensor(b!) locations, Tensor(c!) slots, "
           "int block_size, int num_blocks) -> ()", tags);
     m.def("copy_to_slots(Tensor key_states, Tensor value_states, Tensor(a!) key_cache, Tensor(b!) value_cache, Tensor slots) -> ()", tags);
     m.def("verify_drafts(Tensor drafts, Tensor target_probs, Tensor uniforms, Tensor? draft_probs, Tensor? n_drafts, Tensor? positions, "
@@ -1030,6 +1041,7 @@ TORCH_LIBRARY_IMPL(libhogatt, CUDA, m) {
     m.impl("window_paged_sdpa", window_paged_sdpa);
     m.impl("trim_blocks", trim_blocks);
     m.impl("packed_slots", packed_slots);
+    m.impl("packed_slots_out", packed_slots_out);
     m.impl("copy_to_slots", copy_to_slots);
     m.impl("verify_drafts", verify_drafts);
     m.impl("merge_segments", merge_segments);

@@ -808,7 +808,7 @@ __global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHea
             unsigned voff[G::NOC];
             vtr_lane_offsets<G::VROW>(voff, lane);
             auto lim_of = [&](int x) { return max(0, x < cap ? x + 1 : cap); };
-            auto lo_of = [&](int x) { return max(0, x < 0 ? 0 : x - args.window + 1); };
+            auto lo_of = [&](int x) { return min(max(0, x < 0 ? 0 : x - args.window + 1), cap); };       // (so that it can be rounded up to tiles)
             int top = 0, bottom = -0x7fffffff, most = 0, above = 0, least = -0x7fffffff;
             bool other = false;                          // not all rows of the group are at one position
 #pragma unroll

@@ -192,6 +192,18 @@ def test_longest_table_and_far_pages():
         assert torch.equal(a, c)
 
 
+@pytest.mark.parametrize("heads", [(8, 2, 64), (7, 1, 128), (2, 2, 256)], ids=str)
+def test_positions_behind_the_table(heads):
+    """Up to the last one that there is: of the table's tokens they see what their window and the sinks leave."""
+    top = (1 << 31) - 1
+    positions = [[top, 90, 97, top - 9] * 12, [80, top - 31, 100, 131, 143, 144, 159, 160, 161, 5000] * 6, [top] * 50]
+    for sinks in (0, 20):
+        b = Batch("bf16", *heads, positions, 40, sinks, 16, seed=sinks, max_blocks=9)
+        b.check(b.packed(), "packed")
+        b.check(b.packed(splits=1, row_blocks=1), "16-row groups")
+        b.check(b.packed(splits=2, row_blocks=8), "many rows")
+
+
 def test_window_over_everything_is_the_attention_without():
     """A window as long as the sequences: the same visible keys as hogwild_paged_sdpa's."""
     g = torch.Generator().manual_seed(1)
