@@ -236,7 +236,7 @@ def _window_sdpa(queries, locations, key_cache, value_cache, block_table, cu_seq
     if out is None:
         out = torch.empty_like(queries)
     if HAVE_TORCH_OPS:
-        torch.ops.libhogatt.window_paged_sdpa(out, lse, scale, locations, queries, key_cache, value_cache, block_table, cu_seqlens_q, window, sinks)
+        torch.ops.libhogatt.window_paged_sdpa.default(out, lse, scale, locations, queries, key_cache, value_cache, block_table, cu_seqlens_q, window, sinks)
         return out
     _lib.WindowProblem(q=queries, locations=locations, key_cache=key_cache, value_cache=value_cache, block_table=block_table, scale=scale,
                        window=window, sinks=sinks, out=out, cu_seqlens_q=cu_seqlens_q, lse=lse).run()
@@ -268,12 +268,12 @@ def packed_slots(block_table: torch.Tensor, positions: torch.Tensor, n_new: torc
     on no page); what goes beyond `total` rows is cut off.  `out`: the three tensors to write into."""
     if out is None:
         if HAVE_TORCH_OPS:
-            return torch.ops.libhogatt.packed_slots(block_table, positions, n_new, total, block_size, num_blocks)
+            return torch.ops.libhogatt.packed_slots.default(block_table, positions, n_new, total, block_size, num_blocks)
         out = tuple(torch.empty(n, dtype=torch.int32, device=block_table.device) for n in (block_table.size(0) + 1, int(total), int(total)))
     elif out[1].numel() != int(total):
         raise ValueError("out must be (cu_seqlens [W + 1], locations [total], slots [total])")
     if HAVE_TORCH_OPS:
-        torch.ops.libhogatt.packed_slots_out(block_table, positions, n_new, *out, block_size, num_blocks)
+        torch.ops.libhogatt.packed_slots_out.default(block_table, positions, n_new, *out, block_size, num_blocks)
     else:
         _lib.packed_slots(block_table, positions, n_new, *out, block_size, num_blocks)
     return out
@@ -284,7 +284,7 @@ def copy_to_slots(key_states: torch.Tensor, value_states: torch.Tensor, key_cach
     """New K/V rows [total,Hkv,D] of a packed batch to the rows `slots` (int32 [total], from packed_slots) of the paged caches; those at -1
     are left out.  No slot is named twice."""
     if HAVE_TORCH_OPS:
-        torch.ops.libhogatt.copy_to_slots(key_states, value_states, key_cache, value_cache, slots)
+        torch.ops.libhogatt.copy_to_slots.default(key_states, value_states, key_cache, value_cache, slots)
         return
     _lib.copy_to_slots(key_states, value_states, key_cache, value_cache, slots)
 
@@ -300,7 +300,7 @@ def verify_drafts(drafts: torch.Tensor, target_probs: torch.Tensor, uniforms: to
     seq_lengths (int32 [W]; as reserve_blocks left them for a step of 1 + n_drafts tokens) the lengths are shortened in place to the
     token before the drafts and the accepted ones.  Rounding and special values: see hw_verify_drafts."""
     if HAVE_TORCH_OPS:
-        return torch.ops.libhogatt.verify_drafts(drafts, target_probs, uniforms, draft_probs, n_drafts, positions, seq_lengths)
+        return torch.ops.libhogatt.verify_drafts.default(drafts, target_probs, uniforms, draft_probs, n_drafts, positions, seq_lengths)
     return _lib.verify_drafts(drafts, target_probs, uniforms, draft_probs, n_drafts, positions, seq_lengths)
 
 
@@ -329,7 +329,7 @@ def trim_blocks(block_table: torch.Tensor, seq_lengths: torch.Tensor, ref_counts
     """Pages of which no token from position seq_lengths[w] on sees anything (behind the sinks, before the window) are given back.  A
     length that is shortened afterwards brings back a window whose pages are gone: verify drafts first."""
     if HAVE_TORCH_OPS:
-        torch.ops.libhogatt.trim_blocks(block_table, seq_lengths, ref_counts, window, sinks, block_size)
+        torch.ops.libhogatt.trim_blocks.default(block_table, seq_lengths, ref_counts, window, sinks, block_size)
         return
     _lib.trim_blocks(block_table, seq_lengths, ref_counts, window, sinks, block_size)
 

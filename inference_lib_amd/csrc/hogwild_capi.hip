@@ -374,6 +374,8 @@ int window_run(const hw_window_problem* p, void* stream_) {
     wh.window = p->window;
     wh.sinks = p->sinks;
     wh.rows = wide ? window_rows(p, cus) : 0;
+    wh.most_cuts = wide ? window_most_cuts(plan) : 0;
+    wh.cuts = wide && !direct ? reinterpret_cast<int*>(wh.p.part_ml + (size_t)p->Hkv * prows * 2) : nullptr;
     const hipError_t e = hw::launch_window_attention(wh, p->dtype, p->D, plan.row_blocks, stream);
     if (e != hipSuccess || direct || wide) return (int)e;      // (128-row groups: merged by the launcher)
     hw::MergeArgs ma;
@@ -433,7 +435,7 @@ int verify_check(const hw_verify* v) {
 bool verify_in_one(const hw_verify* v) { return v->V <= 4 * hw::VERIFY_CHUNK; }
 
 size_t verify_bytes(const hw_verify* v) {
-    return verify_in_one(v) ? 0 : (size_t)v->W * ((v->V + hw::VERIFY_CHUNK - 1) / hw::VERIFY_CHUNK) * 2 * sizeof(double);
+    return verify_in_one(v) ? 0 : (size_t)v->W * ((v->V + hw::VERIFY_CHUNK - 1) / hw::VERIFY_CHUNK * 2 * sizeof(double) + sizeof(hw::VerifyRow));
 }
 
 int verify_run(const hw_verify* v, void* stream) {
@@ -453,6 +455,7 @@ int verify_run(const hw_verify* v, void* stream) {
     a.sums = one ? nullptr : reinterpret_cast<double*>(v->workspace);
     a.W = v->W; a.K = v->K; a.V = v->V;
     a.chunks = (v->V + hw::VERIFY_CHUNK - 1) / hw::VERIFY_CHUNK;
+    a.rows = one ? nullptr : reinterpret_cast<hw::VerifyRow*>(a.sums + (size_t)v->W * a.chunks * 2);
     return (int)hw::launch_verify(a, v->dtype, v->token_bytes == 8, reinterpret_cast<hipStream_t>(stream));
 }
 

@@ -197,6 +197,9 @@ struct alignas(64) WindowHeader {
     float* lse;            // or null
     int window, sinks;
     int rows;              // of a row group (128-row workgroups and wider)
+    int most_cuts;         // row groups that are shared out, at most (window_most_cuts)
+    int* cuts;             // [Hkv][1 + most_cuts][4]: their number and whether they have workgroups to themselves; of each the first and the
+                           // last workgroup, the first row and the row behind the last
 };
 hipError_t launch_window_attention(const WindowHeader& wh, int dtype, int D, int rb, hipStream_t stream);
 
@@ -223,6 +226,10 @@ struct CopySlotsArgs {
 };
 hipError_t launch_copy_to_slots(const CopySlotsArgs& a, int dtype, hipStream_t stream);
 
+struct VerifyRow {
+    int n, accepted;           // drafts, and how many of them are accepted
+    long long draft;           // the first one that is not (accepted < n), a token or not
+};
 struct VerifyArgs {
     const void* drafts;        // [W, K]
     const void* target;        // [W, K + 1, V]
@@ -236,6 +243,7 @@ struct VerifyArgs {
     int* accepted;             // [W]
     double* sums;              // [W][chunks][2]: of the weights left over and of the target's probabilities; null: one launch, up to
                                // VERIFY_MOST_CHUNKS chunks
+    VerifyRow* rows;           // [W], with sums
     int W, K, V, chunks;
 };
 constexpr int VERIFY_CHUNK = 4096;      // probabilities that a group of 256 threads adds up at a time

@@ -845,6 +845,10 @@ int window_rows(const hw_window_problem* p, int num_cus) {
     return even >= most / 2 ? (int)even : most;
 }
 
+// The row groups of a kv head that its workgroups share out, at most: fewer than there are workgroups (all but an eighth of them; the
+// kernel gives more than that whole ones).
+int window_most_cuts(const hw_paged_plan& plan) { return std::min(plan.row_groups, plan.splits * 7 / 8); }
+
 int window_plan(const hw_window_problem* p, int num_cus, hw_paged_plan* plan) {
     if (plan == nullptr) return HW_ERR_NULL;
     if (num_cus < 1) return HW_ERR_SHAPE;
@@ -875,7 +879,9 @@ int window_plan(const hw_window_problem* p, int num_cus, hw_paged_plan* plan) {
         plan->splits = (int)std::min(splits, (long long)HW_MAX_SPLITS);
         if ((long long)plan->splits * p->Hkv * (hw::WINDOW_ROWS * p->D / 1024) >= (1ll << 31)) return HW_ERR_SHAPE;
         plan->workgroups = plan->splits * p->Hkv;
-        if (plan->splits > 1) plan->workspace_bytes = (size_t)p->Hkv * 2 * plan->splits * (p->D == 256 ? hw::WINDOW_ROWS_256 : hw::WINDOW_ROWS) * ((size_t)p->D + 2) * sizeof(float);
+        if (plan->splits > 1)
+            plan->workspace_bytes = (size_t)p->Hkv * (2 * plan->splits * (p->D == 256 ? hw::WINDOW_ROWS_256 : hw::WINDOW_ROWS) * ((size_t)p->D + 2) * sizeof(float) +
+                                                      (1 + window_most_cuts(*plan)) * 4 * sizeof(int32_t));
         return HW_OK;
     }
     if (splits == 0) splits = std::max(1ll, std::min((num_cus + groups - 1) / groups, (tiles + 2 * hw::NWAVES - 1) / (2 * hw::NWAVES)));

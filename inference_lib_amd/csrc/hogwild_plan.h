@@ -92,6 +92,7 @@ int paged_q4_shares_save(const hw_paged_problem* p, const hw_paged_plan& plan, i
 int window_validate(const hw_window_problem* p);
 int window_plan(const hw_window_problem* p, int num_cus, hw_paged_plan* plan);
 int window_rows(const hw_window_problem* p, int num_cus);      // rows of a group of the many-rows kernel (row_blocks = 8)
+int window_most_cuts(const hw_paged_plan& plan);               // row groups that its workgroups share out, at most
 // Whether the tiles of a paged launch are to stay in the L2 (hogwild_plan.cpp).
 bool paged_keep_in_l2(const hw_paged_problem* p, const hw_paged_plan& plan);
 

@@ -130,10 +130,6 @@ __device__ __forceinline__ float prob_at(const void* base, long long i) {
 // What a probability counts in a sum: negative, infinite and NaN ones nothing.
 __device__ __forceinline__ double weight_of(double x) { return x > 0.0 && x < __builtin_inf() ? x : 0.0; }
 
-struct VerifyRow {
-    int n, accepted;
-    long long draft;         // the first draft that is not accepted (accepted < n), a token or not
-};
 // Which drafts of sequence w are accepted, by every thread for itself: lane i of a wave looks at draft 64 c + i.
 template <class DT, class TOK>
 __device__ __forceinline__ VerifyRow verify_row(const VerifyArgs& a, int w, int lane) {
@@ -238,8 +234,8 @@ __device__ __forceinline__ double lane_value(double v, int lane) {          // (
     return __longlong_as_double((unsigned long long)(u32)__builtin_amdgcn_readlane((u32)(x >> 32), lane) << 32 | (u32)__builtin_amdgcn_readlane((u32)x, lane));
 }
 
-// Sums of the chunks (SUMS) and the token (DRAW).  In two launches the sums lie in `sums`, the first with a workgroup to a chunk, the second with
-// one to a sequence; in one, a workgroup of GROUPS groups of 256 threads does all of a sequence, with the sums in LDS.
+// Sums of the chunks (SUMS) and the token (DRAW).  In two launches the sums lie in `sums` and the accepted drafts in `rows`, the first with a
+// workgroup to a chunk, the second with one to a sequence; in one, a workgroup of GROUPS groups of 256 threads does all of a sequence, with the sums in LDS.
 template <class DT, class TOK, int GROUPS, bool SUMS, bool DRAW>
 __global__ __launch_bounds__(VERIFY_THREADS * GROUPS) void verify_kernel(const VerifyArgs a) {
     constexpr bool BOTH = SUMS && DRAW;
@@ -249,7 +245,11 @@ __global__ __launch_bounds__(VERIFY_THREADS * GROUPS) void verify_kernel(const V
     __shared__ int found[VERIFY_WAVES], last_one[VERIFY_WAVES];
     const int lane = threadIdx.x & 63, t = threadIdx.x % VERIFY_THREADS, grp = threadIdx.x / VERIFY_THREADS, wv = t >> 6;
     const int w = DRAW ? blockIdx.x : blockIdx.x / a.chunks;
-    const VerifyRow r = verify_row<DT, TOK>(a, w, lane);
+    VerifyRow r;
+    if constexpr (SUMS) r = verify_row<DT, TOK>(a, w, lane);
+    else r = a.rows[w];
+    if constexpr (!DRAW)
+        if (threadIdx.x == 0 && blockIdx.x == w * a.chunks) a.rows[w] = r;
     double* const sums = BOTH ? lds_sums : a.sums + (size_t)w * a.chunks * 2;
 
     if constexpr (SUMS) {

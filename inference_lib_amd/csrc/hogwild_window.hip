@@ -494,6 +494,10 @@ struct Deal {
     int qs, qe, count, upto;
     int first, parts;                    // apart: lane g, the workgroups of the g-th of the groups shared out
 };
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ HW_GLOBAL i32x4* cuts_of(const WindowHeader& args, int hkv) {
+    return reinterpret_cast<HW_GLOBAL i32x4*>(reinterpret_cast<unsigned long long>(args.cuts)) + (size_t)hkv * (args.most_cuts + 1);
+}
 __device__ __forceinline__ int bounded(int x, int T) { return min(max(x, 0), T); }        // a malformed array must not lead outside the buffers
 __device__ __forceinline__ Deal window_deal(const WindowHeader& args, const PagedDevHeader& ph, int n, int lane, int GQ) {
     Deal d = {0, 0, 0, false, 0, 0, 0, 0, 0, 0};
@@ -760,6 +764,9 @@ __global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHea
         begin = part0 * den + me - __builtin_amdgcn_readlane(deal.first, part0);
         end = begin + 1;
     }
+    // word for window_merge_kernel: how many groups are shared out and how
+    HW_GLOBAL i32x4* const cuts = cuts_of(args, hkv);
+    if (N > 1 && me == 0 && tid == 0) cuts[0] = i32x4{deal.rest, deal.apart ? 1 : 0, 0, 0};
     for (int item = 0; item < deal.whole + parts; ++item) {
         const bool whole_one = item < deal.whole;
         const int cut = part0 + item - deal.whole;               // a part: of this one of the groups that are shared out
@@ -769,6 +776,8 @@ __global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHea
         const WindowGroup it = window_group(ph, deal, rows, g, tid & 63, GQ);
         const int r0 = it.qs * GQ + it.rg * rows, rend = min(it.qe * GQ, r0 + rows);
         const bool whole = from == 0 && to == den;
+        if (!whole_one && from == 0 && tid == 0 && cut < args.most_cuts)        // which workgroups have it, and its rows
+            cuts[cut + 1] = i32x4{me, deal.apart ? me + den - 1 : ((cut + 1) * N - 1) / deal.rest, r0, rend};
         const size_t pbase = ((size_t)hkv * 2 * N + 2 * me + (cut == part0 ? 0 : 1)) * ROWS;
         const HW_GLOBAL int* btw = ph.block_table + (size_t)it.w * ph.max_blocks;
 
@@ -1026,88 +1035,86 @@ __global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHea
     }
 }
 
-// The groups that lie across workgroups: workgroup (kv head, cut, block of rows) of the launch takes those rows of group `cut` of the ones
-// that were shared out.  D / 4 lanes a row; parts in their order.  A kv head's partial sums are read on the XCD that wrote them.
-template <class DT, int D, int ROWS>
-__global__ __launch_bounds__(256) void window_merge_kernel(const WindowHeader args, int cuts) {
+// The groups that lie across workgroups, as the attention kernel left word of them (WindowCut): a workgroup takes PER rows a thread, D / 4
+// lanes a row, of one of them at a time; parts in their order.  A kv head's partial sums are read on the XCD that wrote them.
+template <class DT, int D, int PER, int UN>
+__global__ __launch_bounds__(256) void window_merge_kernel(const WindowHeader args) {
     typedef typename Elem<DT>::store_t store_t;
-    constexpr int V4 = D / 4, RPB = 256 / V4, PER = 2, BLOCKS = ROWS / (RPB * PER), UN = 4;     // PER rows a thread
-    const int tid = threadIdx.x, lane = tid & 63;
+    constexpr int V4 = D / 4, RPB = 256 / V4, MOST = D == 256 ? WINDOW_ROWS_256 : WINDOW_ROWS;
+    const int tid = threadIdx.x;
     PagedHeaderBits hb;
     paged_header_request(hb);
     const PagedDevHeader ph = paged_header_wait(hb);
     const int N = ph.nsplit, GQ = ph.Hq / ph.Hkv;
-    int bid = blockIdx.x;
-    if (ph.flags & PH_XCD_REMAP) bid = (bid & 7) * (gridDim.x >> 3) + (bid >> 3);
-    const int rblk = bid % BLOCKS, hc = bid / BLOCKS;
-    const int hkv = hc / cuts, cut = hc - hkv * cuts;
-    const int rows = args.rows;
-    const Deal deal = window_deal(args, ph, N, lane, GQ);
-    const int rest = deal.rest;
-    if (cut >= rest) return;
-    int first = cut * N / rest, last = ((cut + 1) * N - 1) / rest;             // its workgroups
-    if (deal.apart) {
-        first = __builtin_amdgcn_readlane(deal.first, cut);
-        last = first + __builtin_amdgcn_readlane(deal.parts, cut) - 1;
-    }
-    if (first == last) return;                   // it saw the whole group
-    const WindowGroup it = window_group(ph, deal, rows, N * deal.whole + cut, lane, GQ);
-    const int r0 = it.qs * GQ + it.rg * rows, rend = min(it.qe * GQ, r0 + rows);
-    const int rr = rblk * RPB * PER + tid / V4, e = tid % V4 * 4;
-    if (r0 + rr >= rend) return;
-    // (the slot of workgroup w: its first group's, or, for the one that begins the group in the middle of its stretch, the other)
-    auto row_of = [&](int w, int i) { return ((size_t)hkv * 2 * N + 2 * w + (deal.apart || w * rest / N == cut ? 0 : 1)) * ROWS + min(rr + i * RPB, rend - 1 - r0); };
-    float m[PER], l[PER];
-    f32x4 acc[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        m[i] = NEG_BIG;
-        l[i] = 0.f;
-        acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-    for (int w = first; w <= last; w += UN) {
-        f32x4 o[PER][UN];
-        f32x2 ml[PER][UN];
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-#pragma unroll
-            for (int u = 0; u < UN; ++u) {
-                const size_t row = row_of(min(w + u, last), i);
-                o[i][u] = *reinterpret_cast<const HW_GLOBAL f32x4*>(ph.part_o + row * D + e);
-                ml[i][u] = *reinterpret_cast<const HW_GLOBAL f32x2*>(ph.part_ml + row * 2);
-                if (w + u > last) {
-                    ml[i][u] = f32x2{NEG_BIG, 0.f};
-                    o[i][u] = f32x4{0.f, 0.f, 0.f, 0.f};
-                }
-            }
+    const int homes = ph.flags & PH_XCD_REMAP && ph.Hkv % 8 == 0 ? 8 : 1, heads = ph.Hkv / homes;      // (kv heads of an XCD)
+    const int blocks = (args.rows + RPB * PER - 1) / (RPB * PER);
+    const int home = blockIdx.x % homes, step = gridDim.x / homes;
+    const HW_GLOBAL i32x4* const cuts = cuts_of(args, 0);
+    // (cuts first, then kv heads, then rows: where to begin does not depend on how many cuts there are)
+    for (int x = blockIdx.x / homes; x < args.most_cuts * heads * blocks; x += step) {
+        const int cut = x / (heads * blocks), hr = x - cut * heads * blocks;
+        const int hkv = home * heads + hr / blocks, rblk = hr % blocks;
+        const HW_GLOBAL i32x4* const mine = cuts + (size_t)hkv * (args.most_cuts + 1);
+        const i32x4 all = mine[0], c = mine[cut + 1];
+        const int rest = all.x;
+        if (cut >= rest) return;
+        const int first = c.x, last = c.y, r0 = c.z, rend = c.w;
+        const int rr = rblk * RPB * PER + tid / V4, e = tid % V4 * 4;
+        if (first == last || r0 + rr >= rend) continue;              // (one that saw the whole group has written the result)
+        // (the slot of workgroup w: its first group's, or, for the one that begins the group in the middle of its stretch, the other)
+        auto row_of = [&](int w, int k) { return ((size_t)hkv * 2 * N + 2 * w + (all.y != 0 || w * rest / N == cut ? 0 : 1)) * MOST + min(rr + k * RPB, rend - 1 - r0); };
+        float m[PER], l[PER];
+        f32x4 acc[PER];
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            float mb = m[i];
-#pragma unroll
-            for (int u = 0; u < UN; ++u) mb = fmaxf(mb, ml[i][u].x);
-            const float old = fast_exp2(m[i] - mb);
-            acc[i] *= old;
-            l[i] *= old;
-#pragma unroll
-            for (int u = 0; u < UN; ++u) {
-                const float x = fast_exp2(ml[i][u].x - mb);
-                acc[i] += o[i][u] * x;
-                l[i] += ml[i][u].y * x;
-            }
-            m[i] = mb;
+            m[i] = NEG_BIG;
+            l[i] = 0.f;
+            acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
-    }
-    DevHeader a;
-    a.Hq = ph.Hq; a.S = ph.LS;
-    a.magic_gq = ph.magic_gq; a.magic_s = ph.magic_ls;
+        for (int w = first; w <= last; w += UN) {
+            f32x4 o[PER][UN];
+            f32x2 ml[PER][UN];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        if (r0 + rr + i * RPB >= rend) break;
-        const float inv = l[i] > 0.f ? 1.0f / l[i] : 0.f;
-        const size_t orow = map_row(a, r0 + rr + i * RPB, hkv, GQ).qrow;
-        *reinterpret_cast<u32x2*>(reinterpret_cast<store_t*>(args.out) + orow * D + e) =
-            u32x2{Elem<DT>::pack2(acc[i][0] * inv, acc[i][1] * inv), Elem<DT>::pack2(acc[i][2] * inv, acc[i][3] * inv)};
-        if (args.lse != nullptr && e == 0) args.lse[orow] = l[i] > 0.f ? (m[i] + __builtin_amdgcn_logf(l[i])) * 0.69314718055994530942f : -__builtin_inff();
+            for (int i = 0; i < PER; ++i)
+#pragma unroll
+                for (int u = 0; u < UN; ++u) {
+                    const size_t row = row_of(min(w + u, last), i);
+                    o[i][u] = *reinterpret_cast<const HW_GLOBAL f32x4*>(ph.part_o + row * D + e);
+                    ml[i][u] = *reinterpret_cast<const HW_GLOBAL f32x2*>(ph.part_ml + row * 2);
+                    if (w + u > last) {
+                        ml[i][u] = f32x2{NEG_BIG, 0.f};
+                        o[i][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    }
+                }
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                float mb = m[i];
+#pragma unroll
+                for (int u = 0; u < UN; ++u) mb = fmaxf(mb, ml[i][u].x);
+                const float old = fast_exp2(m[i] - mb);
+                acc[i] *= old;
+                l[i] *= old;
+#pragma unroll
+                for (int u = 0; u < UN; ++u) {
+                    const float x = fast_exp2(ml[i][u].x - mb);
+                    acc[i] += o[i][u] * x;
+                    l[i] += ml[i][u].y * x;
+                }
+                m[i] = mb;
+            }
+        }
+        DevHeader a;
+        a.Hq = ph.Hq; a.S = ph.LS;
+        a.magic_gq = ph.magic_gq; a.magic_s = ph.magic_ls;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            if (r0 + rr + i * RPB >= rend) break;
+            const float inv = l[i] > 0.f ? 1.0f / l[i] : 0.f;
+            const size_t orow = map_row(a, r0 + rr + i * RPB, hkv, GQ).qrow;
+            *reinterpret_cast<u32x2*>(reinterpret_cast<store_t*>(args.out) + orow * D + e) =
+                u32x2{Elem<DT>::pack2(acc[i][0] * inv, acc[i][1] * inv), Elem<DT>::pack2(acc[i][2] * inv, acc[i][3] * inv)};
+            if (args.lse != nullptr && e == 0) args.lse[orow] = l[i] > 0.f ? (m[i] + __builtin_amdgcn_logf(l[i])) * 0.69314718055994530942f : -__builtin_inff();
+        }
     }
 }
 
@@ -1120,9 +1127,10 @@ static hipError_t launch_window_wide(const WindowHeader& wh, hipStream_t stream)
     hipLaunchKernelGGL((window_wide_kernel<DT, D, NS, NW, TS>), dim3(wh.p.nwg), dim3(NW * 64), 0, stream, wh);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || wh.p.nsplit == 1) return e;
-    const int most = wh.p.nsplit * 7 / 8, cuts = wh.p.nitems < most ? wh.p.nitems : most;     // groups that are shared out, at most (window_deal)
-    if (cuts == 0 || (wh.p.cu_q == nullptr && wh.p.nitems % wh.p.nsplit == 0)) return e;
-    hipLaunchKernelGGL((window_merge_kernel<DT, D, NW * 32>), dim3(wh.p.Hkv * cuts * (NW * 32 * D / 2048)), dim3(256), 0, stream, wh, cuts);
+    if (wh.most_cuts == 0 || (wh.p.cu_q == nullptr && wh.p.nitems % wh.p.nsplit == 0)) return e;
+    constexpr int PER = 2, UN = 4, RPB = 1024 / D;
+    const int all = wh.p.Hkv * wh.most_cuts * ((wh.rows + RPB * PER - 1) / (RPB * PER));
+    hipLaunchKernelGGL((window_merge_kernel<DT, D, PER, UN>), dim3(all < 1024 ? all : 1024), dim3(256), 0, stream, wh);
     return hipGetLastError();
 }
 
