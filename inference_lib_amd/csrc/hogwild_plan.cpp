@@ -865,8 +865,7 @@ int window_plan(const hw_window_problem* p, int num_cus, hw_paged_plan* plan) {
     const int rows = wide ? window_rows(p, num_cus) : 16 * plan->row_blocks;
     // (packed: one more than there can be, which writes the zeros of tokens that belong to no sequence)
     plan->row_groups = varlen ? (plan->rows + rows - 1) / rows + p->W : p->W * ((p->S * gq + rows - 1) / rows);
-    // The tiles that a row group usually sees, at most: sinks and a window that moves over its tokens.  Splits of two tiles a wave and more,
-    // as far as there are CUs.
+    // The tiles that a row group usually sees, at most: sinks and a window that moves over its tokens.
     const long long cap = ((long long)p->block_size * p->max_blocks + hw::TILE - 1) / hw::TILE;
     const long long seen = (std::min((long long)p->sinks, 1ll << 20) + hw::TILE - 1) / hw::TILE + (std::min((long long)p->window, 1ll << 20) + rows / gq) / hw::TILE + 2;
     const long long tiles = std::min(cap, seen);
@@ -884,7 +883,12 @@ int window_plan(const hw_window_problem* p, int num_cus, hw_paged_plan* plan) {
                                                       (1 + window_most_cuts(*plan)) * 4 * sizeof(int32_t));
         return HW_OK;
     }
-    if (splits == 0) splits = std::max(1ll, std::min((num_cus + groups - 1) / groups, (tiles + 2 * hw::NWAVES - 1) / (2 * hw::NWAVES)));
+    // As many workgroups as have a CU each (160 groups of 128 channels behind 1024 tokens on 256 CUs: 1, 2 and 3 splits 18.9, 21.6 and 18.9 us; of
+    // 256 channels 33.8, 45 and 37.9; 80 groups: 3 and 4 splits 12.7 and 14.8), down to one tile for a wave (a sequence of 512 tokens: one
+    // tile, two, four 9.1, 9.6, 11.2; of 256 channels 12.1, 12.9, 15.5).  A few tiles are one workgroup's, which spares the merge: three a wave where
+    // they are short (256 tokens: 8.7 against 9.0), two otherwise (128 tokens in float32 8.2 against 9.4; 256: 10.5 against 9.5).
+    const long long lone = (p->dtype != HW_F32 && p->D <= 128 ? 3 : 2) * hw::NWAVES;
+    if (splits == 0) splits = tiles <= lone ? 1 : std::max(1ll, std::min(num_cus / groups, (tiles + hw::NWAVES - 1) / hw::NWAVES));
     splits = std::min(splits, (long long)HW_MAX_SPLITS);
     plan->splits = (int)splits;
     const long long wgs = groups * splits;

@@ -545,19 +545,25 @@ __device__ __forceinline__ Deal window_deal(const WindowHeader& args, const Page
             rg = g - __shfl(d.upto - d.count, w, 64);
         }
         const int here = min((qe - qs) * GQ - rg * rows, rows);
-        // the tiles that its last row sees, about; a tile of up to eight row blocks takes as long as it needs to come in, each further pair a sixth
-        // of that more; and an opening
+        // the tiles that its last row sees, about, in fifths of a microsecond a step of two: with up to four row blocks as long as it needs to come
+        // in, with four to a SIMD eleven; and an opening
         const int at = min(ph.loc[min(max(qs + (rg * rows + here - 1) / GQ, 0), T - 1)], ph.block_size * ph.max_blocks - 1);
         const int seen = at < 0 ? 0 : at < args.window ? at : args.window + min(args.sinks, at - args.window);
-        cost = (seen / TILE + 10) * max(6, 3 + (here + 31) / 32 * 3 / 4);
+        cost = (seen / TILE + 11) * max(6, 3 + (here + 63) / 64 * 2);
     }
-    const int mine = lane < d.rest ? cost : 0;
-    const int sum = __builtin_amdgcn_readlane(wave_scan_inclusive(mine), 63);
-    // one workgroup each, the others in proportion (rounded down), and what is left over one more to the first ones
-    const float share = (float)(n - d.rest) * __builtin_amdgcn_rcpf((float)sum) * 0.99999f;
-    d.parts = lane < d.rest ? 1 + (int)((float)mine * share) : 0;
-    const int left = n - __builtin_amdgcn_readlane(wave_scan_inclusive(d.parts), 63);
-    if (lane < min(left, d.rest)) ++d.parts;
+    // The least time t in which they are done with n workgroups, ceil(cost / t) for each: between the sum over n and over n - rest, where they
+    // are enough in any case (n - rest is 2/3 n and more; the thousandth is for the roundings).
+    const float mine = lane < d.rest ? (float)cost : 0.f;
+    auto parts_in = [&](float t) { return (int)__builtin_ceilf(mine * __builtin_amdgcn_rcpf(t)); };
+    const float sum = (float)__builtin_amdgcn_readlane(wave_scan_inclusive(lane < d.rest ? cost : 0), 63);
+    float no = sum * __builtin_amdgcn_rcpf((float)n), yes = sum * __builtin_amdgcn_rcpf((float)(n - d.rest)) * 1.001f;
+#pragma unroll 1
+    for (int i = 0; i < 6; ++i) {
+        const float t = 0.5f * (no + yes);
+        if (__builtin_amdgcn_readlane(wave_scan_inclusive(parts_in(t)), 63) <= n) yes = t;
+        else no = t;
+    }
+    d.parts = parts_in(yes);
     d.first = wave_scan_inclusive(d.parts) - d.parts;
     return d;
 }
@@ -664,12 +670,12 @@ __device__ __forceinline__ void band_tile_lds(const u32x4* qreg, const Band<RB>&
     }
     if constexpr (MASKED) {
         if (mixed) {                                                  // uniform over the wave
-            u32 any = 0;
+            // (nothing times them all: NaN where one is infinite or NaN; the matrix unit has time for it here, 32 registers looked at have not)
+            f32x4 any[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-            for (int c = 0; c < G::NOC; ++c)
-#pragma unroll
-                for (int d = 0; d < 4; ++d) any |= Wild<DT>::signs(vops[c][d]);
-            if (__builtin_amdgcn_ballot_w64((any & Wild<DT>::SIGNS) != 0) != 0) {
+            for (int c = 0; c < G::NOC; ++c) any[c & 1] = Elem<DT>::mfma(vops[c], u32x4{0, 0, 0, 0}, any[c & 1]);
+            const float sum = (any[0][0] + any[0][1] + any[0][2] + any[0][3]) + (any[1][0] + any[1][1] + any[1][2] + any[1][3]);
+            if (__builtin_amdgcn_ballot_w64(sum != 0.f) != 0) {
                 u32x4 seen[RB];
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb) seen[rb] = Wild<DT>::seen(band, rb, t0, q);
@@ -856,7 +862,10 @@ __global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHea
                 const int x = k + (k >= full0 ? full1 - full0 : 0) - (k >= part ? tiles - full0 : 0);
                 return x + (x >= sink_tiles ? jump : 0);
             };
-            const int k0 = tiles * from / den, k1 = tiles * to / den;
+            // (a tile that is not seen completely takes half as long again as another)
+            const int weight = 2 * tiles + part;
+            auto tile_of = [&](int x) { return x <= 3 * part ? x / 3 : part + (x - 3 * part) / 2; };
+            const int k0 = tile_of(weight * from / den), k1 = tile_of(weight * to / den);
 
             WaveState<RBX, G::NOC> st;
 #pragma unroll
