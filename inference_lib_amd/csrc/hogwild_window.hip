@@ -7,6 +7,11 @@
 // sinks, and the union of the rows' windows.  Both are cut into tiles of 32 tokens at multiples of 32, numbered through (tile_at), and
 // tile k goes to wave k mod (4 * nsplit) of the workgroups that share the rows.
 //
+// Bound by what is loaded: 16 sequences that see 4096 tokens of 40/8 heads of 128 channels take 47 us a layer, 269 MB at 5.7 TB/s.  Smaller steps
+// show the chain in front of the loads (positions, table entries, first tiles) and the merge, 8 to 9 us together: 5 ragged sequences that see up to
+// 1088 tokens of 256 channels, 36 MB, 15.5 us; 4 sequences of 4 tokens that see 2048, 34 MB, 16.3; the least step 6 (one workgroup a group, no merge).
+// Two row blocks share what is loaded: 4 tokens at 64/8 heads 16.7 us a layer with them, 17 and more with one.
+//
 // Sequences with more rows (prompt chunks) go through window_wide_kernel: row groups of 256, whose waves share every tile through LDS.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -479,11 +484,18 @@ __global__ __launch_bounds__(NTHREADS, 1) void window_kernel(const WindowHeader 
 // ---- many rows -------------------------------------------------------------------------------------------------------------------
 //
 // Row groups of `rows` rows of one sequence (a last one of fewer), numbered through the sequences, `all` of them for every kv head.  The n
-// workgroups of a head take q = all / n whole groups each, and share the rest of them out.  Many of them (more than a third of n) evenly, in
+// workgroups of a head take q = all / n whole groups each, every n-th one (so that a prompt among sequences that decode falls to many: 60 of
+// those and 512 tokens 261 -> 251 us, the prompt in front 230), and share the rest of them out.  Many of them (more than a third of n) evenly, in
 // the order of the rows: workgroup i takes the stretch [i rest / n, (i + 1) rest / n), and a part of a group is that part of its tiles.  Few
-// of them have workgroups to themselves, as many as their tiles and rows ask for, since a second opening in a workgroup costs as much as ten
-// tiles and more.  A workgroup that sees a whole group writes its result; parts leave partial sums in the workgroup's two slots (its first
-// group's, and its last one's), which window_merge_kernel adds up.
+// of them have workgroups to themselves, as many as their tiles and rows ask for (1, 8, 32 and 64 tokens behind 4096 at 40/8 heads: 48 -> 37 us),
+// since a second opening in a workgroup costs as much as eleven tiles.  A workgroup that sees a whole group writes its result; parts leave partial
+// sums in the workgroup's two slots (its first group's, and its last one's), which window_merge_kernel adds up.
+//
+// What bounds it (128 channels, 256 CUs at 2.0 GHz): a step of two tiles takes 2.2 us with 256 rows (0.95 PFLOP/s), 1.8 with 160, 1.2 with 64
+// and fewer (the loads: 27 GB/s a CU).  Matrix products, exponentials with the rest of the softmax, and LDS reads are a microsecond each of
+// the 2.2; leaving any one out saves a tenth, taking the logits a tile ahead 1 %.  Around the steps 6 us before the first one (row positions,
+// table entries, tiles: a chain of loads), 1 to 3 of results or partial sums, 4 to 7 of the merge.  1024 tokens on 5120 that see 2048, 40/8 heads: 66 us
+// a layer, 0.65 PFLOP/s.
 
 constexpr int VMCNT_0 = 0x0f70;          // s_waitcnt: no vector memory operation outstanding, the other counters as they are
 
@@ -776,7 +788,7 @@ __global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHea
     for (int item = 0; item < deal.whole + parts; ++item) {
         const bool whole_one = item < deal.whole;
         const int cut = part0 + item - deal.whole;               // a part: of this one of the groups that are shared out
-        const int g = whole_one ? me * deal.whole + item : N * deal.whole + cut;
+        const int g = whole_one ? item * N + me : N * deal.whole + cut;
         if (g >= deal.all) break;                                 // (the last workgroups, where almost a group each was left)
         const int from = whole_one ? 0 : max(begin - cut * den, 0), to = whole_one ? den : min(end - cut * den, den);
         const WindowGroup it = window_group(ph, deal, rows, g, tid & 63, GQ);
