@@ -859,16 +859,21 @@ int window_plan(const hw_window_problem* p, int num_cus, hw_paged_plan* plan) {
     plan->rows = tokens * gq;
     const bool two = p->dtype != HW_F32 && p->D <= 128;        // two row blocks: what the registers hold
     const int usual = varlen ? (plan->rows + p->W - 1) / p->W : p->S * gq;      // rows of a sequence, in the mean
-    plan->row_blocks = p->row_blocks != 0 ? p->row_blocks : p->dtype != HW_F32 && usual > 32 ? hw::WIDE_ROW_BLOCKS : two && usual > 16 ? 2 : 1;
+    // The tiles that a row group of r rows usually sees, at most: sinks and a window that moves over its tokens.
+    auto tiles_of = [&](int r) {
+        const long long cap = ((long long)p->block_size * p->max_blocks + hw::TILE - 1) / hw::TILE;
+        const long long seen = (std::min((long long)p->sinks, 1ll << 20) + hw::TILE - 1) / hw::TILE + (std::min((long long)p->window, 1ll << 20) + r / gq) / hw::TILE + 2;
+        return std::min(cap, seen);
+    };
+    // (17 to 32 rows of a sequence in one workgroup rather than two where the tiles are many: 4, 16 and 40 sequences that see 2048 tokens 14.8, 29.5 and
+    // 80 us against 14.8, 31 and 84, 4096 19.5, 49 and 146 against 20.4, 55 and 167, 1024 12.1, 20 and 47 against 12.0, 18.5 and 45)
+    plan->row_blocks = p->row_blocks != 0 ? p->row_blocks : p->dtype != HW_F32 && usual > 32 ? hw::WIDE_ROW_BLOCKS : two && usual > 16 && tiles_of(32) > 48 ? 2 : 1;
     const bool wide = plan->row_blocks == hw::WIDE_ROW_BLOCKS && p->dtype != HW_F32;
     if (plan->row_blocks != 1 && !(plan->row_blocks == 2 && two) && !wide) return HW_ERR_UNSUPPORTED;
     const int rows = wide ? window_rows(p, num_cus) : 16 * plan->row_blocks;
     // (packed: one more than there can be, which writes the zeros of tokens that belong to no sequence)
     plan->row_groups = varlen ? (plan->rows + rows - 1) / rows + p->W : p->W * ((p->S * gq + rows - 1) / rows);
-    // The tiles that a row group usually sees, at most: sinks and a window that moves over its tokens.
-    const long long cap = ((long long)p->block_size * p->max_blocks + hw::TILE - 1) / hw::TILE;
-    const long long seen = (std::min((long long)p->sinks, 1ll << 20) + hw::TILE - 1) / hw::TILE + (std::min((long long)p->window, 1ll << 20) + rows / gq) / hw::TILE + 2;
-    const long long tiles = std::min(cap, seen);
+    const long long tiles = tiles_of(rows);
     const long long groups = (long long)std::max(plan->row_groups, 1) * p->Hkv;
     long long splits = p->splits;
     if (wide) {
@@ -883,12 +888,16 @@ int window_plan(const hw_window_problem* p, int num_cus, hw_paged_plan* plan) {
                                                       (1 + window_most_cuts(*plan)) * 4 * sizeof(int32_t));
         return HW_OK;
     }
-    // As many workgroups as have a CU each (160 groups of 128 channels behind 1024 tokens on 256 CUs: 1, 2 and 3 splits 18.9, 21.6 and 18.9 us; of
+    // As many workgroups as have a CU each, going by sequences of the mean length (160 groups of 128 channels behind 1024 tokens on 256 CUs: 1, 2 and 3 splits 18.9, 21.6 and 18.9 us; of
     // 256 channels 33.8, 45 and 37.9; 80 groups: 3 and 4 splits 12.7 and 14.8), down to one tile for a wave (a sequence of 512 tokens: one
     // tile, two, four 9.1, 9.6, 11.2; of 256 channels 12.1, 12.9, 15.5).  A few tiles are one workgroup's, which spares the merge: three a wave where
-    // they are short (256 tokens: 8.7 against 9.0), two otherwise (128 tokens in float32 8.2 against 9.4; 256: 10.5 against 9.5).
+    // they are short (256 tokens: 8.7 against 9.0), two otherwise (128 tokens in float32 8.2 against 9.4; 256: 10.5 against 9.5).  A workgroup of 64
+    // channels in 16 bits does not keep a CU's loads busy: two of them where there are less than three splits otherwise (96 and 160 groups
+    // behind 4096 tokens 23.9 -> 20.9 and 51.9 -> 35.6 us; 48 groups 5 splits already: not better).
     const long long lone = (p->dtype != HW_F32 && p->D <= 128 ? 3 : 2) * hw::NWAVES;
-    if (splits == 0) splits = tiles <= lone ? 1 : std::max(1ll, std::min(num_cus / groups, (tiles + hw::NWAVES - 1) / hw::NWAVES));
+    const long long likely = std::max(1ll, std::min(groups, (long long)p->W * ((usual + rows - 1) / rows) * p->Hkv));
+    const long long room = p->dtype != HW_F32 && p->D == 64 && num_cus / likely < 3 ? 2ll * num_cus : num_cus;
+    if (splits == 0) splits = tiles <= lone ? 1 : std::max(1ll, std::min(room / likely, (tiles + hw::NWAVES - 1) / hw::NWAVES));
     splits = std::min(splits, (long long)HW_MAX_SPLITS);
     plan->splits = (int)splits;
     const long long wgs = groups * splits;

@@ -10,7 +10,7 @@
 // Bound by what is loaded: 16 sequences that see 4096 tokens of 40/8 heads of 128 channels take 47 us a layer, 269 MB at 5.7 TB/s.  Smaller steps
 // show the chain in front of the loads (positions, table entries, first tiles) and the merge, 8 to 9 us together: 5 ragged sequences that see up to
 // 1088 tokens of 256 channels, 36 MB, 15.5 us; 4 sequences of 4 tokens that see 2048, 34 MB, 16.3; the least step 6 (one workgroup a group, no merge).
-// Two row blocks share what is loaded: 4 tokens at 64/8 heads 16.7 us a layer with them, 17 and more with one.
+// Two row blocks share what is loaded, which pays where the tiles are many (see window_plan).
 //
 // Sequences with more rows (prompt chunks) go through window_wide_kernel: row groups of 256, whose waves share every tile through LDS.
 #include <hip/hip_runtime.h>
