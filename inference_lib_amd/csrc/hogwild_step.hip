@@ -78,7 +78,7 @@ __global__ __launch_bounds__(SLOTS_THREADS) void packed_slots_kernel(const Packe
 
 // One wave to a token: its row of the caches is found once, and its pieces of VEC bytes, keys then values, head by head, are dealt to the lanes,
 // four of a lane in flight.  What is written streams past the caches, as attention reads it from there once in a step.  Bound by the
-// writes: 8143 tokens of 8 heads of 128 channels in 16 bits, 67 MB read and written, 13 us (5.1 TB/s).
+// writes: 8172 tokens of 8 heads of 128 channels in 16 bits, 67 MB read and written, 13 us (5.1 TB/s).
 template <int VEC>
 __global__ __launch_bounds__(256) void copy_to_slots_kernel(const CopySlotsArgs a, int sz, unsigned magic_k, unsigned magic_v) {
     typedef typename std::conditional<VEC == 16, u32x4, typename std::conditional<VEC == 4, u32, unsigned short>::type>::type piece_t;

@@ -284,3 +284,14 @@ def test_random_batches(seed):
         positions[0] = [12]
     b = Batch(dtype, Hq, Hkv, D, positions, rng.choice([1, 31, 32, 33, 200, 1000]), rng.choice([0, 0, 1, 32, 77]), rng.choice([1, 8, 16, 17, 64]), seed=seed)
     b.check(b.packed(splits=rng.choice([0, 0, 1, 4, 9]), before=rng.choice([0, 3]), behind=rng.choice([0, 1, 300])))
+
+
+@pytest.mark.parametrize("heads", [(16, 8, 128), (8, 8, 64), (32, 16, 64), (16, 8, 256)], ids=str)
+@pytest.mark.parametrize("splits", [0, 2, 7, 32])
+def test_row_groups_shared_out(heads, splits):
+    """Few groups with workgroups to themselves, many in stretches, whole ones beside them, and kv heads that stay on their part of the card."""
+    for seed, (new, behind) in enumerate([([1, 8, 32, 64], 500), ([130, 3, 270], 40), ([600], 100), ([40] * 12, 7), ([1] * 30 + [200], 300)]):
+        b = Batch("bf16", *heads, [list(range(behind + 11 * w, behind + 11 * w + s)) for w, s in enumerate(new)], 200, 4, 16, seed=seed)
+        b.check(b.packed(splits, 8, behind=5), f"{new}")
+    b = Batch("f16", *heads, [list(range(n, n + 150)) for n in (0, 31, 400)], 200, 4, 16, seed=9)
+    b.check(b.fixed(splits, 8), "fixed")
