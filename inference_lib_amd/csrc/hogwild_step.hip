@@ -287,8 +287,14 @@ __global__ __launch_bounds__(VERIFY_THREADS * GROUPS) void verify_kernel(const V
     }
     if constexpr (DRAW) {
         // The chunk in which the running sum passes u times the whole: lane = chunk, 64 at a time; every wave for itself.
-        double total[2] = {0.0, 0.0};
-        for (int c0 = 0; c0 < a.chunks; c0 += 64) {
+        double total[2], mine64[2], run64[2];            // (of the first 64, which are all of them up to 262 144 tokens)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            mine64[k] = lane < a.chunks ? sums[2 * lane + k] : 0.0;
+            run64[k] = wave_scan(mine64[k]);
+            total[k] = lane_value(run64[k], 63);
+        }
+        for (int c0 = 64; c0 < a.chunks; c0 += 64) {
             const int c = c0 + lane;
 #pragma unroll
             for (int k = 0; k < 2; ++k) total[k] += lane_value(wave_scan(c < a.chunks ? sums[2 * c + k] : 0.0), 63);
@@ -299,7 +305,8 @@ __global__ __launch_bounds__(VERIFY_THREADS * GROUPS) void verify_kernel(const V
         double base = 0.0, before = 0.0;
         for (int c0 = 0; c0 < a.chunks; c0 += 64) {
             const int c = c0 + lane;
-            const double mine = c < a.chunks ? sums[2 * c + which] : 0.0, run = wave_scan(mine);
+            const double mine = c0 == 0 ? (which == 0 ? mine64[0] : mine64[1]) : c < a.chunks ? sums[2 * c + which] : 0.0;
+            const double run = c0 == 0 ? (which == 0 ? run64[0] : run64[1]) : wave_scan(mine);
             const unsigned long long over = __ballot(mine > 0.0 && base + run > aim), some = __ballot(mine > 0.0);
             if (chunk < 0 && over != 0) {
                 const int l = __builtin_ctzll(over);

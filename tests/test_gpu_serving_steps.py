@@ -160,6 +160,45 @@ def test_verify_weights_at_the_end_of_chunks():
         assert tokens.tolist() == [[token]] and accepted.tolist() == [0], u
 
 
+def test_verify_more_chunks_than_a_wave_has_lanes():
+    """600 001 tokens: the chunks are looked through 64 at a time.  From the target's weights, and from what a draft leaves of them."""
+    V = 600001
+    at = [5, 262143, 262144, 262145, 524287, 524288, V - 1]
+    p = torch.zeros((1, 2, V))
+    p[:, :, at] = torch.tensor([0.125, 0.125, 0.25, 0.125, 0.125, 0.125, 0.125])
+    q = torch.zeros((1, 1, V))
+    q[0, 0, 262144] = 1.0
+    none = torch.zeros((1, 0), dtype=torch.int64)
+    for u, token in [(0.0, 5), (0.1249, 5), (0.125, 262143), (0.25, 262144), (0.4999, 262144), (0.5, 262145), (0.625, 524287), (0.75, 524288), (0.875, V - 1), (1.0, V - 1)]:
+        tokens, _ = verify(none, p[:, :1], torch.tensor([[u]]))
+        assert tokens.tolist() == [[token]], u
+        for draft_probs in (q, None):                             # rejected (0.25 < 0.5): 0.75 of the weights are left
+            tokens, accepted = verify(torch.tensor([[262144]]), p, torch.tensor([[0.5, u]]), draft_probs)
+            left = [x for x in at if x != 262144]
+            assert accepted.tolist() == [0] and tokens.tolist() == [[left[min(int(u * 6), 5)], -1]], u
+
+
+@pytest.mark.parametrize("V", [9000, 40000])
+def test_verify_twice_at_once(V):
+    """Calls on two streams, and a captured one whose replays lie between eager ones: sums and accepted drafts are each call's own."""
+    cases = [[x.to(DEV) for x in draft_case(7, 3, V, "f32", s, False)] for s in (1, 2)]
+    want = [ops().verify_drafts(*c) for c in cases]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept = ops().verify_drafts(*cases[1])
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(5):
+        got = []
+        for c, stream in zip(cases, streams):
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                got.append(ops().verify_drafts(*c))
+        graph.replay()
+        torch.cuda.synchronize()
+        for g, w in zip(got + [kept], want + [want[1]]):
+            assert torch.equal(g[0], w[0]) and torch.equal(g[1], w[1])
+
+
 def test_verify_shortens_lengths_and_reads_views():
     """Strided probabilities; lengths as a reserve leaves them, those of sequences that got nothing too."""
     drafts, target, u, q = draft_case(12, 4, 300, "f32", 3, False)
