@@ -295,3 +295,43 @@ def test_row_groups_shared_out(heads, splits):
         b.check(b.packed(splits, 8, behind=5), f"{new}")
     b = Batch("f16", *heads, [list(range(n, n + 150)) for n in (0, 31, 400)], 200, 4, 16, seed=9)
     b.check(b.fixed(splits, 8), "fixed")
+
+
+@pytest.mark.parametrize("dtype,heads", [(torch.bfloat16, (16, 8, 128)), (torch.float16, (8, 2, 64)), (torch.bfloat16, (4, 1, 256))], ids=str)
+def test_packed_and_replayed_beside_eager_calls(dtype, heads):
+    """A packed step of row groups that are shared out, in two graphs: replayed with other sequences, lengths and positions, between eager
+    calls on another stream."""
+    Hq, Hkv, D = heads
+    g = torch.Generator().manual_seed(3)
+    W, total, block, n = 6, 300, 16, 60
+    kc, vc = (torch.randn((W * n, Hkv, block, D), generator=g).to(dtype).to(DEV) for _ in range(2))
+    table = torch.randperm(W * n, generator=g).int().view(W, n).to(DEV)
+    q = torch.randn((total, Hq, D), generator=g).to(dtype).to(DEV)
+    cu, loc = torch.zeros(W + 1, dtype=torch.int32, device=DEV), torch.zeros(total, dtype=torch.int32, device=DEV)
+
+    def lay_out(news):
+        cu.copy_(torch.tensor([sum(news[:w]) for w in range(W + 1)]))
+        at = sum([list(range(100 * w + 50, 100 * w + 50 + s)) for w, s in enumerate(news)], [])
+        loc.copy_(torch.tensor(at + [-1] * (total - len(at))))
+
+    run = lambda: ops().hogwild_varlen_paged_sdpa_window(q, loc, kc, vc, table, cu, 0.1, 200, 3)         # noqa: E731
+    lay_out([50] * W)
+    run()
+    graphs, outs = [], []
+    for _ in range(2):
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(run())
+        graphs.append(graph)
+    for news in ([1, 0, 240, 2, 3, 4], [0] * W, [300, 0, 0, 0, 0, 0], [17, 80, 33, 1, 90, 60], [1] * W):
+        lay_out(news)
+        other = torch.cuda.Stream()
+        other.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(other):
+            eager = run()
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], eager) and torch.equal(outs[1], eager), news
+        assert (eager[sum(news):] == 0).all() and (sum(news) == 0 or (eager[: sum(news)] != 0).any(-1).all())
