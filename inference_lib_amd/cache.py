@@ -410,7 +410,8 @@ class PagedCache:
         cache.free(finished); cache.compact()            # pages in use to the front of the pool
 
     With `window` the attention is that of hogwild_paged_sdpa_window: the last `window` positions and the first `sinks` (16 and 32 bits), and
-    trim() gives back the pages that no later token sees.  Steps in which sequences bring different numbers of tokens need not be padded:
+    trim() gives back the pages that no later token sees (positions count on from a sequence's beginning all the same: max_blocks is for all of
+    them, of which only those in the window hold a page).  Steps in which sequences bring different numbers of tokens need not be padded:
 
         cache.reserve_packed(n_new, total)               # n_new int32 [max_seqs]; the batch's rows, total of them
         for layer in ...:

@@ -145,6 +145,30 @@ def test_serving_steps(dtype, window, sinks, graphs):
             h.check(0, w, q[w], lengths[w], out[w].transpose(0, 1), scale, far, sinks)
 
 
+def test_a_small_pool_holds_long_sequences():
+    """With a window the pool need only hold what is seen: sequences of many times its size, single tokens and chunks."""
+    from inference_lib_amd.cache import PagedCache
+    window, sinks, block, n = 40, 3, 16, 2
+    cache = PagedCache(1, HKV, D, 14, n, block_size=block, dtype=torch.float16, device=DEV, window=window, sinks=sinks, max_blocks=64)
+    h = Histories(n, torch.float16, 11)
+    for step in range(40):
+        new = [1 + step % 3, 30 if step % 2 else 17]
+        total = sum(new)
+        n_new = torch.tensor(new, dtype=torch.int32, device=DEV)
+        q, kv = [h.rand(s, HQ, D) for s in new], [h.rand(s, 2, HKV, D) for s in new]
+        first = [h.length(w) for w in range(n)]
+        cache.reserve_packed(n_new, total)
+        assert cache.granted().all(), step
+        cache.update_packed(torch.cat(kv)[:, 0].to(DEV), torch.cat(kv)[:, 1].to(DEV), 0)      # (views)
+        out = cache.attend_packed(torch.cat(q).to(DEV), 0, 0.2).cpu()
+        for w in range(n):
+            h.kv[w][0] = torch.cat([h.kv[w][0], kv[w]])
+            if step % 5 == 0 or step > 36:
+                h.check(0, w, q[w], first[w], out[sum(new[:w]): sum(new[: w + 1])], 0.2, window, sinks)
+        cache.trim()
+    assert max(h.length(w) for w in range(n)) > 4 * 14 * block
+
+
 def test_a_full_pool_leaves_sequences_out():
     """Sequences that the pool has nothing for: their rows are not written and give 0, the others go on; layouts of batches that no graph
     holds are kept for some sizes only."""
