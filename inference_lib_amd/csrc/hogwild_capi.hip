@@ -377,7 +377,7 @@ int window_run(const hw_window_problem* p, void* stream_) {
     wh.most_cuts = wide ? window_most_cuts(plan) : 0;
     wh.cuts = wide && !direct ? reinterpret_cast<int*>(wh.p.part_ml + (size_t)p->Hkv * prows * 2) : nullptr;
     const hipError_t e = hw::launch_window_attention(wh, p->dtype, p->D, plan.row_blocks, stream);
-    if (e != hipSuccess || direct || wide) return (int)e;      // (128-row groups: merged by the launcher)
+    if (e != hipSuccess || direct || wide) return (int)e;      // (many rows: merged by the launcher)
     hw::MergeArgs ma;
     std::memset(&ma, 0, sizeof(ma));
     ma.part_o = wh.p.part_o;
