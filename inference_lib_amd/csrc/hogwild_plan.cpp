@@ -865,8 +865,8 @@ int window_plan(const hw_window_problem* p, int num_cus, hw_paged_plan* plan) {
         const long long seen = (std::min((long long)p->sinks, 1ll << 20) + hw::TILE - 1) / hw::TILE + (std::min((long long)p->window, 1ll << 20) + r / gq) / hw::TILE + 2;
         return std::min(cap, seen);
     };
-    // (17 to 32 rows of a sequence in one workgroup rather than two where the tiles are many: 4, 16 and 40 sequences that see 2048 tokens 14.8, 29.5 and
-    // 80 us against 14.8, 31 and 84, 4096 19.5, 49 and 146 against 20.4, 55 and 167, 1024 12.1, 20 and 47 against 12.0, 18.5 and 45)
+    // (17 to 32 rows of a sequence in one workgroup rather than two where the tiles are many: 4, 16 and 40 sequences that see 4096 tokens 18.5, 48.6 and
+    // 145 us against 19.7, 54.7 and 167, 2048 13.9, 28.5 and 78 against 14.0, 30.4 and 83, 1024 11.6, 18.9 and 45.1 against 11.2, 18.0 and 43.5)
     plan->row_blocks = p->row_blocks != 0 ? p->row_blocks : p->dtype != HW_F32 && usual > 32 ? hw::WIDE_ROW_BLOCKS : two && usual > 16 && tiles_of(32) > 48 ? 2 : 1;
     const bool wide = plan->row_blocks == hw::WIDE_ROW_BLOCKS && p->dtype != HW_F32;
     if (plan->row_blocks != 1 && !(plan->row_blocks == 2 && two) && !wide) return HW_ERR_UNSUPPORTED;
@@ -888,12 +888,13 @@ int window_plan(const hw_window_problem* p, int num_cus, hw_paged_plan* plan) {
                                                       (1 + window_most_cuts(*plan)) * 4 * sizeof(int32_t));
         return HW_OK;
     }
-    // As many workgroups as have a CU each, going by sequences of the mean length (160 groups of 128 channels behind 1024 tokens on 256 CUs: 1, 2 and 3 splits 18.9, 21.6 and 18.9 us; of
-    // 256 channels 33.8, 45 and 37.9; 80 groups: 3 and 4 splits 12.7 and 14.8), down to one tile for a wave (a sequence of 512 tokens: one
-    // tile, two, four 9.1, 9.6, 11.2; of 256 channels 12.1, 12.9, 15.5).  A few tiles are one workgroup's, which spares the merge: three a wave where
-    // they are short (256 tokens: 8.7 against 9.0), two otherwise (128 tokens in float32 8.2 against 9.4; 256: 10.5 against 9.5).  A workgroup of 64
-    // channels in 16 bits does not keep a CU's loads busy: two of them where there are less than three splits otherwise (96 and 160 groups
-    // behind 4096 tokens 23.9 -> 20.9 and 51.9 -> 35.6 us; 48 groups 5 splits already: not better).
+    // As many workgroups as have a CU each, going by sequences of the mean length (160 groups of 128 channels that see 1024 tokens on 256 CUs: 1, 2 and 3
+    // splits 18.0, 20.6 and 17.8 us; of 256 channels 32.2, 41.7 and 34.2; 80 groups: 3 and 4 splits 11.5 and 13.4), down to one tile for a wave (a
+    // sequence that sees 512: one tile, two, three 7.8, 8.9, 10.2; of 256 channels 9.7, 11.8, 13.7).  A few tiles are one workgroup's, which
+    // spares the merge: three a wave where they are short (256 tokens of 64 channels 6.6 against 7.2 us, of 128 7.8 against 7.6 for one sequence
+    // and 8.0 against 9.2 for 160 groups), two otherwise (128 tokens in float32 7.5 against 8.2, 256 9.5 against 8.2).  A workgroup of 64 channels in
+    // 16 bits does not keep a CU's loads busy: two of them where there are less than three splits otherwise (96 and 160 groups that see 4096 tokens
+    // 23.2 -> 19.9 and 51 -> 34.6 us; 48 groups with 5 splits already: not better).
     const long long lone = (p->dtype != HW_F32 && p->D <= 128 ? 3 : 2) * hw::NWAVES;
     const long long likely = std::max(1ll, std::min(groups, (long long)p->W * ((usual + rows - 1) / rows) * p->Hkv));
     const long long room = p->dtype != HW_F32 && p->D == 64 && num_cus / likely < 3 ? 2ll * num_cus : num_cus;

@@ -117,8 +117,8 @@ __global__ __launch_bounds__(256) void copy_to_slots_kernel(const CopySlotsArgs 
 // Probabilities are added up in chunks of VERIFY_CHUNK, by groups of 256 threads: 16 bytes in a row to a thread, two or four rows of the group to a
 // chunk.  A thread's in their order, then the threads' of a row by a scan over the wave, then the waves and rows.  A chunk's sum and its
 // running sum are the same additions wherever they are worked out, so a token is found where the sums say that it is, and it is the same in
-// every call.  Bound by the two rows of probabilities that are read: 64 sequences, 128 000 in float32, 65.5 MB, 13.4 us (4.9 TB/s) and 7 for the
-// draw, a chain of loads (sums, a chunk's probabilities) between scans.  One sequence of 32 000: 6.2 and 4.8 (5.2 where the draw looks for the
+// every call.  Bound by the two rows of probabilities that are read: 64 sequences, 128 000 in float32, 65.5 MB, 13.4 us (4.9 TB/s) and 6.5 for the
+// draw, a chain of loads (sums, a chunk's probabilities) between scans.  One sequence of 32 000: 6.2 and 4.6 (5.2 where the draw looks for the
 // accepted drafts again).
 constexpr int VERIFY_THREADS = 256, VERIFY_WAVES = VERIFY_THREADS / 64;
 template <class DT>

@@ -7,9 +7,9 @@
 // sinks, and the union of the rows' windows.  Both are cut into tiles of 32 tokens at multiples of 32, numbered through (tile_at), and
 // tile k goes to wave k mod (4 * nsplit) of the workgroups that share the rows.
 //
-// Bound by what is loaded: 16 sequences that see 4096 tokens of 40/8 heads of 128 channels take 47 us a layer, 269 MB at 5.7 TB/s.  Smaller steps
-// show the chain in front of the loads (positions, table entries, first tiles) and the merge, 8 to 9 us together: 5 ragged sequences that see up to
-// 1088 tokens of 256 channels, 36 MB, 15.5 us; 4 sequences of 4 tokens that see 2048, 34 MB, 16.3; the least step 6 (one workgroup a group, no merge).
+// Bound by what is loaded: 16 sequences that see 4096 tokens of 40/8 heads of 128 channels take 46 us a layer, 269 MB at 5.8 TB/s.  Smaller steps
+// show the chain in front of the loads (positions, table entries, first tiles: 3 us) and the merge, 8 us together: 5 ragged sequences that see up to
+// 1088 tokens of 256 channels, 36 MB, 15 us; 4 sequences of 4 tokens that see 2048, 34 MB, 15.4; the least step 5 (one workgroup a group, no merge).
 // Two row blocks share what is loaded, which pays where the tiles are many (see window_plan).
 //
 // Sequences with more rows (prompt chunks) go through window_wide_kernel: row groups of 256, whose waves share every tile through LDS.
