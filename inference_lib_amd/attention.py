@@ -232,6 +232,8 @@ def hogwild_varlen_paged_sdpa_q4(queries: torch.Tensor, locations: torch.Tensor,
 # ---- paged caches with a sliding window, packed batches, drafted tokens (no counterpart in the reference) ----------------------------
 
 def _window_sdpa(queries, locations, key_cache, value_cache, block_table, cu_seqlens_q, scale, window, sinks, out, lse):
+    if out is None and lse is None and HAVE_TORCH_OPS:
+        return torch.ops.libhogatt.window_paged_attention.default(scale, locations, queries, key_cache, value_cache, block_table, cu_seqlens_q, window, sinks)
     queries = queries.contiguous()
     if out is None:
         out = torch.empty_like(queries)

@@ -646,6 +646,15 @@ void window_paged_sdpa(at::Tensor& out, const std::optional<at::Tensor>& lse, do
     else check_status(hw_window_paged_sdpa(&p, stream_of(out)), "hw_window_paged_sdpa");
 }
 
+// The same with an output of its own (a step of small sequences takes as long as its call).
+at::Tensor window_paged_attention(double scale, const at::Tensor& locations, const at::Tensor& queries, const at::Tensor& key_cache, const at::Tensor& value_cache,
+                                  const at::Tensor& block_table, const std::optional<at::Tensor>& cu_seqlens_q, int64_t window, int64_t sinks) {
+    const at::Tensor q = queries.contiguous();
+    at::Tensor out = at::empty(q.sizes(), q.options());
+    window_paged_sdpa(out, std::nullopt, scale, locations, q, key_cache, value_cache, block_table, cu_seqlens_q, window, sinks);
+    return out;
+}
+
 void trim_blocks(at::Tensor& block_table, const at::Tensor& seq_lengths, at::Tensor& ref_counts, int64_t window, int64_t sinks, int64_t block_size) {
     TORCH_CHECK(window >= 1 && window < (1ll << 31) && sinks >= 0 && sinks < (1ll << 31), "libhogatt: window must be positive and sinks not negative, got ", window, " and ", sinks);
     Pool u;
@@ -998,6 +1007,8 @@ TORCH_LIBRARY(libhogatt, m) {
     // additions: paged attention with a sliding window and sinks, packed batches, drafted tokens
     m.def("window_paged_sdpa(Tensor(a!) output, Tensor(b!)? lse, float scale, Tensor locations, Tensor queries, "
           "Tensor key_cache, Tensor value_cache, Tensor block_table, Tensor? cu_seqlens_q, int window, int sinks) -> ()", tags);
+    m.def("window_paged_attention(float scale, Tensor locations, Tensor queries, Tensor key_cache, Tensor value_cache, Tensor block_table, "
+          "Tensor? cu_seqlens_q, int window, int sinks) -> Tensor", tags);
     m.def("trim_blocks(Tensor(a!) block_table, Tensor seq_lengths, Tensor(b!) ref_counts, int window, int sinks, int block_size) -> ()", tags);
     m.def("packed_slots(Tensor block_table, Tensor positions, Tensor n_new, int total, int block_size, int num_blocks) -> (Tensor, Tensor, Tensor)", tags);
     m.def("packed_slots_out(Tensor block_table, Tensor positions, Tensor n_new, Tensor(a!) cu_seqlens, Tensor(b!) locations, Tensor(c!) slots, "
@@ -1039,6 +1050,7 @@ TORCH_LIBRARY_IMPL(libhogatt, CUDA, m) {
     m.impl("compact_blocks", compact_blocks);
     m.impl("copy_blocks", copy_blocks);
     m.impl("window_paged_sdpa", window_paged_sdpa);
+    m.impl("window_paged_attention", window_paged_attention);
     m.impl("trim_blocks", trim_blocks);
     m.impl("packed_slots", packed_slots);
     m.impl("packed_slots_out", packed_slots_out);
