@@ -28,7 +28,8 @@
  *                            python/hogwild/attention.py:84-90, :313-318, :148-158; and merge_caches, :251-257
  *   hw_copy_to_blocks_q4, hw_read_blocks_q4, hw_paged_sdpa_q4, hw_varlen_paged_sdpa_q4 ... no counterpart: the paged operators with
  *                            caches in 4 bits
- *   hw_fork_blocks, hw_free_blocks, hw_reserve_blocks, hw_compact_blocks, hw_copy_pages ... no counterpart: the pages of paged caches
+ *   hw_fork_blocks, hw_free_blocks, hw_reserve_blocks, hw_reserve_step, hw_compact_blocks, hw_copy_pages ... no counterpart: the pages of
+ *                            paged caches
  *   hw_window_paged_sdpa, hw_window_varlen_paged_sdpa, hw_trim_blocks ... no counterpart: the paged operators with a sliding window
  *   hw_packed_slots, hw_copy_to_slots, hw_verify_drafts ... no counterpart: packed batches and drafted tokens of serving steps
  *   hw_build_inputs_dev, hw_advance_lengths, hw_problem.len_dev, hw_append.len_dev ... no counterpart: the same steps
@@ -382,6 +383,8 @@ int hw_free_blocks(const hw_pool* p, const uint8_t* finished, void* stream);
  * block_size * max_blocks, which the appends leave out, and its length stays.  positions are not seq_lengths (HW_ERR_SHAPE).
  */
 int hw_reserve_blocks(const hw_pool* p, const int32_t* n_new, int32_t* positions, void* stream);
+/* The same; taken[w] (device int32 [W], written, no part of the other tables: HW_ERR_SHAPE) = n_new[w] for a sequence that got its pages, otherwise 0. */
+int hw_reserve_step(const hw_pool* p, const int32_t* n_new, int32_t* positions, int32_t* taken, void* stream);
 
 /* The pages that sequences name (ref_counts > 0) become the first ones of the pool: those behind as many places as there are of them
    move, in ascending order, to the free pages before.  used[0] (device int32) = how many there are. */
@@ -482,8 +485,10 @@ int hw_copy_to_slots(const hw_copy_slots* c, void* stream);
  * p[w][n] behind the last one: the first token whose running sum exceeds uniforms[w][K] times the sum of all (for numbers in [0, 1); from
  * 1 on the last token with a weight).  Sums in float64; negative, infinite and NaN weights count as 0; -1 where there is no weight.
  * tokens[w] = the accepted drafts, the next token, -1 behind.  A draft that is no token (outside 0 .. V - 1) is not accepted, and q of
- * a certain one is 0 then.  With seq_lengths, a sequence whose step began at positions[w] keeps its token before the drafts and the accepted
- * ones: seq_lengths[w] = min(seq_lengths[w], positions[w] + 1 + accepted[w]).
+ * a certain one is 0 then.  With seq_lengths, a sequence loses the drafts that do not stand: its step brought n_new[w] tokens from positions[w]
+ * on (1 + n without n_new), the drafts behind the others, and all but its n - accepted[w] last ones stay, one at least:
+ * seq_lengths[w] = min(seq_lengths[w], positions[w] + min(n_new[w], max(n_new[w] - n, 1) + accepted[w])).  Positions behind the lengths
+ * (hw_reserve_blocks gives them to sequences that took no part) shorten nothing.
  */
 typedef struct hw_verify {
     int32_t dtype;                 /* of the probabilities */
@@ -501,6 +506,7 @@ typedef struct hw_verify {
     int32_t* accepted;             /* [W] */
     void* workspace;               /* hw_verify_workspace_bytes() bytes, 16-byte aligned (NULL if those are 0) */
     size_t workspace_bytes;
+    const int32_t* n_new;          /* [W] or NULL, with seq_lengths */
 } hw_verify;
 int hw_verify_workspace_bytes(const hw_verify* v, size_t* bytes);
 int hw_verify_drafts(const hw_verify* v, void* stream);

@@ -34,7 +34,7 @@ EXPORTS = [
     "hw_paged_sdpa_q4", "hw_varlen_paged_sdpa_q4",
     "hw_window_validate", "hw_window_plan_debug", "hw_window_workspace_bytes", "hw_window_paged_sdpa", "hw_window_varlen_paged_sdpa",
     "hw_trim_blocks", "hw_packed_slots", "hw_copy_to_slots", "hw_verify_workspace_bytes", "hw_verify_drafts",
-    "hw_pool_workspace_bytes", "hw_fork_blocks", "hw_free_blocks", "hw_reserve_blocks", "hw_compact_blocks", "hw_copy_pages",
+    "hw_pool_workspace_bytes", "hw_fork_blocks", "hw_free_blocks", "hw_reserve_blocks", "hw_reserve_step", "hw_compact_blocks", "hw_copy_pages",
 ]
 
 
@@ -141,6 +141,7 @@ class HwVerify(C.Structure):
         ("uniforms", C.c_void_p), ("n_drafts", C.c_void_p), ("positions", C.c_void_p), ("seq_lengths", C.c_void_p),
         ("tokens", C.c_void_p), ("accepted", C.c_void_p),
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("n_new", C.c_void_p),
     ]
 
 
@@ -235,6 +236,7 @@ def _load() -> C.CDLL:
     lib.hw_fork_blocks.argtypes = [C.POINTER(HwPool), C.c_void_p, C.c_void_p]
     lib.hw_free_blocks.argtypes = [C.POINTER(HwPool), C.c_void_p, C.c_void_p]
     lib.hw_reserve_blocks.argtypes = [C.POINTER(HwPool), C.c_void_p, C.c_void_p, C.c_void_p]
+    lib.hw_reserve_step.argtypes = [C.POINTER(HwPool), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]
     lib.hw_compact_blocks.argtypes = [C.POINTER(HwPool), C.c_void_p, C.c_void_p]
     lib.hw_copy_pages.argtypes = [C.POINTER(C.c_void_p), C.POINTER(C.c_size_t), C.c_int, C.c_int, C.POINTER(C.c_int32), C.POINTER(C.c_int32), C.c_int, C.c_void_p]
     return lib
@@ -786,7 +788,8 @@ def copy_to_slots(key_states: torch.Tensor, value_states: torch.Tensor, key_cach
 
 
 def verify_drafts(drafts: torch.Tensor, target_probs: torch.Tensor, uniforms: torch.Tensor, draft_probs: Optional[torch.Tensor] = None,
-                  n_drafts: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None, seq_lengths: Optional[torch.Tensor] = None):
+                  n_drafts: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None, seq_lengths: Optional[torch.Tensor] = None,
+                  n_new: Optional[torch.Tensor] = None):
     """(tokens [W, K + 1], accepted int32 [W]) of drafts [W, K]; see hw_verify."""
     if drafts.dim() != 2 or drafts.dtype not in (torch.int32, torch.int64) or not drafts.is_contiguous():
         raise ValueError("drafts must be contiguous int64 or int32 [W, K]")
@@ -802,11 +805,13 @@ def verify_drafts(drafts: torch.Tensor, target_probs: torch.Tensor, uniforms: to
         raise ValueError("draft_probs must be [W, K, V] in the dtype of target_probs")
     if (positions is None) != (seq_lengths is None):
         raise ValueError("positions and seq_lengths go together")
-    for t in (n_drafts, positions, seq_lengths):
+    if n_new is not None and seq_lengths is None:
+        raise ValueError("n_new goes with positions and seq_lengths")
+    for t in (n_drafts, positions, seq_lengths, n_new):
         if t is not None and (tuple(t.shape) != (W,) or t.dtype != torch.int32 or not t.is_contiguous()):
-            raise ValueError("n_drafts, positions and seq_lengths must be contiguous int32 [W]")
+            raise ValueError("n_drafts, positions, seq_lengths and n_new must be contiguous int32 [W]")
     device = target_probs.device
-    if any(t is not None and t.device != device for t in (drafts, uniforms, draft_probs, n_drafts, positions, seq_lengths)):
+    if any(t is not None and t.device != device for t in (drafts, uniforms, draft_probs, n_drafts, positions, seq_lengths, n_new)):
         raise ValueError("all tensors must live on one device")
     if V > 1 and target_probs.stride(2) != 1:
         target_probs = target_probs.contiguous()
@@ -822,6 +827,7 @@ def verify_drafts(drafts: torch.Tensor, target_probs: torch.Tensor, uniforms: to
     if draft_probs is not None:
         v.dp_w, v.dp_k = draft_probs.stride(0), draft_probs.stride(1)
     v.uniforms, v.n_drafts, v.positions, v.seq_lengths = uniforms.data_ptr(), ptr(n_drafts), ptr(positions), ptr(seq_lengths)
+    v.n_new = ptr(n_new)
     v.tokens, v.accepted = tokens.data_ptr(), accepted.data_ptr()
     with torch.cuda.device(device):
         n = C.c_size_t(0)
@@ -903,10 +909,14 @@ def trim_blocks(block_table, seq_lengths, ref_counts, window: int, sinks: int, b
 
 def reserve_blocks(block_table, seq_lengths, ref_counts, n_new, positions, caches, block_size: int) -> None:
     pool = _Pool(block_table, seq_lengths, ref_counts, block_size, caches)
-    if tuple(n_new.shape) != (block_table.size(0),) or tuple(positions.shape) != (block_table.size(0),):
-        raise ValueError("n_new and positions must be [W]")
+    W = block_table.size(0)
+    if tuple(n_new.shape) != (W,) or tuple(positions.shape) not in ((W,), (2, W)):
+        raise ValueError("n_new must be [W], positions [W] or [2, W]")
     pool.check_ints(n_new, positions)
-    pool.run(lib.hw_reserve_blocks, n_new.data_ptr(), positions.data_ptr(), workspace=True)
+    if positions.dim() == 2:
+        pool.run(lib.hw_reserve_step, n_new.data_ptr(), positions.data_ptr(), positions[1].data_ptr(), workspace=True)
+    else:
+        pool.run(lib.hw_reserve_blocks, n_new.data_ptr(), positions.data_ptr(), workspace=True)
 
 
 def compact_blocks(block_table, ref_counts, caches, used) -> None:

@@ -293,17 +293,17 @@ def copy_to_slots(key_states: torch.Tensor, value_states: torch.Tensor, key_cach
 
 def verify_drafts(drafts: torch.Tensor, target_probs: torch.Tensor, uniforms: torch.Tensor, draft_probs: Optional[torch.Tensor] = None,
                   n_drafts: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
-                  seq_lengths: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+                  seq_lengths: Optional[torch.Tensor] = None, n_new: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Which drafted tokens [W,K] (int64 or int32) stand, and the token behind them: drafts are accepted one after the other while
     uniforms[w,i] * q < p, p = target_probs[w,i,x] and q = draft_probs[w,i,x] (1 without draft_probs); the next token is drawn with
     uniforms[w,K] from what is left of the target's probabilities at the first draft that is not accepted, max(p - q, 0), or from the
     target's behind the last one.  n_drafts (int32 [W]): how many drafts a sequence has, K by default.  Returns tokens [W,K+1], the
     accepted drafts, the next token and -1 behind it, and accepted, int32 [W].  uniforms: float32 [W,K+1], in [0,1).  With positions and
-    seq_lengths (int32 [W]; as reserve_blocks left them for a step of 1 + n_drafts tokens) the lengths are shortened in place to the
-    token before the drafts and the accepted ones.  Rounding and special values: see hw_verify_drafts."""
+    seq_lengths (int32 [W]; as reserve_blocks left them) the lengths are shortened in place by the drafts that do not stand.  n_new (int32
+    [W]): how many tokens the step brought, the drafts behind the others; 1 + n_drafts by default.  Rounding and special values: see hw_verify_drafts."""
     if HAVE_TORCH_OPS:
-        return torch.ops.libhogatt.verify_drafts.default(drafts, target_probs, uniforms, draft_probs, n_drafts, positions, seq_lengths)
-    return _lib.verify_drafts(drafts, target_probs, uniforms, draft_probs, n_drafts, positions, seq_lengths)
+        return torch.ops.libhogatt.verify_drafts.default(drafts, target_probs, uniforms, draft_probs, n_drafts, positions, seq_lengths, n_new)
+    return _lib.verify_drafts(drafts, target_probs, uniforms, draft_probs, n_drafts, positions, seq_lengths, n_new)
 
 
 # ---- the pages of paged caches (no counterpart in the reference) --------------------------------------------------------------------
@@ -340,7 +340,8 @@ def reserve_blocks(block_table: torch.Tensor, seq_lengths: torch.Tensor, ref_cou
                    caches: Sequence[torch.Tensor], block_size: int, positions: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Pages for n_new[w] (int32 [W]) more tokens of every sequence: those its row lacks, a copy (in all `caches`) of a shared page that is
     about to be written, and a free one in the place of a shared page behind the sequence's tokens.  Returns positions [W], where the new tokens go (the lengths so far); a sequence that gets
-    nothing has block_size * max_blocks there, which the appends leave out, and keeps its length (see hw_reserve_blocks)."""
+    nothing has block_size * max_blocks there, which the appends leave out, and keeps its length (see hw_reserve_blocks).  `positions`: the tensor to
+    write into, or one [2, W], whose second row becomes the numbers of tokens that the sequences got."""
     if positions is None:
         positions = torch.empty_like(seq_lengths)
     if HAVE_TORCH_OPS:

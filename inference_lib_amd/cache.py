@@ -417,7 +417,7 @@ class PagedCache:
         for layer in ...:
             cache.update_packed(k, v, layer)             # [total, Hkv, D] (16 and 32 bits)
             out = cache.attend_packed(q, layer, scale)   # [total, Hq, D]
-        tokens, accepted = cache.verify(drafts, target_probs, uniforms)      # a step of one token and its drafts: which of them stand
+        tokens, accepted = cache.verify(drafts, target_probs, uniforms, n_drafts=n_drafts)      # which of the step's last n_drafts tokens stand
         cache.trim()
 
     A sequence that `reserve` has nothing for (the pool or its row of the table is full, or it asked for no tokens) is left out of the
@@ -456,7 +456,8 @@ class PagedCache:
         ints = dict(dtype=torch.int32, device=device)
         self.block_table = torch.full((max_seqs, max_blocks), -1, **ints)
         self.seq_lengths, self.ref_counts = torch.zeros(max_seqs, **ints), torch.zeros(num_blocks, **ints)
-        self.positions = torch.full((max_seqs,), max_blocks * self.block_size, **ints)
+        self._step = torch.tensor([[max_blocks * self.block_size], [0]], **ints).repeat(1, max_seqs)
+        self.positions, self._taken = self._step         # of the last reserve: where the new tokens stand, and how many a sequence got
         self.used = torch.zeros(1, **ints)
         self._longest = torch.full((1,), max_blocks * self.block_size, **ints)
         self._made: Dict[tuple, torch.Tensor] = {}       # locations, by capture and number of tokens
@@ -474,7 +475,8 @@ class PagedCache:
             n_new = torch.full_like(self.seq_lengths, int(n_new))
         self._made = {}
         self._replayed |= self._capture() != 0
-        return _ops.reserve_blocks(self.block_table, self.seq_lengths, self.ref_counts, n_new, self.caches, self.block_size, self.positions)
+        _ops.reserve_blocks(self.block_table, self.seq_lengths, self.ref_counts, n_new, self.caches, self.block_size, self._step)
+        return self.positions
 
     def _capture(self) -> int:
         return _lib.capture_id(self.positions.device) if self.positions.is_cuda else 0
@@ -549,9 +551,10 @@ class PagedCache:
 
     def verify(self, drafts: torch.Tensor, target_probs: torch.Tensor, uniforms: torch.Tensor, draft_probs: Optional[torch.Tensor] = None,
                n_drafts: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
-        """Which drafts of the step stand, and the next tokens (attention.verify_drafts), after a reserve of 1 + n_drafts[w] tokens: the last
-        token of every sequence and its drafts.  What does not stand leaves the sequences; the next tokens are not in them yet."""
-        return _ops.verify_drafts(drafts, target_probs, uniforms, draft_probs, n_drafts, self.positions, self.seq_lengths)
+        """Which drafts of the step stand, and the next tokens (attention.verify_drafts).  The drafts are the last n_drafts[w] (all K without
+        n_drafts) of the tokens that sequence w brought, behind one other at least: its last token, or, with n_drafts[w] = 0, any number of
+        them, a prompt or a chunk of one.  What does not stand leaves the sequences; the next tokens are not in them yet."""
+        return _ops.verify_drafts(drafts, target_probs, uniforms, draft_probs, n_drafts, self.positions, self.seq_lengths, self._taken)
 
     def trim(self) -> None:
         """The pages that no later token sees are given back.  (After verify: a length that is shortened later needs them again.)"""

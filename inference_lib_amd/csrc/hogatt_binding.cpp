@@ -536,17 +536,23 @@ void free_blocks(at::Tensor& block_table, at::Tensor& seq_lengths, at::Tensor& r
     check_status(hw_free_blocks(&u.p, reinterpret_cast<const uint8_t*>(finished.const_data_ptr()), stream_of(block_table)), "hw_free_blocks");
 }
 
+// positions [W], or [2, W] with the numbers of tokens taken behind them
 void reserve_blocks(at::Tensor& block_table, at::Tensor& seq_lengths, at::Tensor& ref_counts, const at::Tensor& n_new, at::Tensor& positions,
                     at::TensorList caches, int64_t block_size) {
     Pool u;
     pool_tables(u, block_table, &seq_lengths, ref_counts, block_size);
     pool_caches(u, caches, u.p.num_blocks, block_table.device());
+    const bool both = positions.dim() == 2 && positions.size(0) == 2;
+    TORCH_CHECK(n_new.dim() == 1 && n_new.size(0) == u.p.W && (both || positions.dim() == 1) && positions.size(-1) == u.p.W,
+                "libhogatt: n_new must be [W], positions [W] or [2, W]");
     for (const at::Tensor* t : std::initializer_list<const at::Tensor*>{&n_new, &positions})
-        TORCH_CHECK(t->dim() == 1 && t->size(0) == u.p.W && t->scalar_type() == at::kInt && t->is_contiguous() && t->device() == block_table.device(),
-                    "libhogatt: n_new and positions must be contiguous int32 [W] on the table's device");
+        TORCH_CHECK(t->scalar_type() == at::kInt && t->is_contiguous() && t->device() == block_table.device(),
+                    "libhogatt: n_new and positions must be contiguous int32 on the table's device");
     c10::hip::HIPGuardMasqueradingAsCUDA guard(block_table.device());
     pool_workspace(u, block_table);
-    check_status(hw_reserve_blocks(&u.p, n_new.const_data_ptr<int32_t>(), positions.data_ptr<int32_t>(), stream_of(block_table)), "hw_reserve_blocks");
+    int32_t* const at = positions.data_ptr<int32_t>();
+    if (both) check_status(hw_reserve_step(&u.p, n_new.const_data_ptr<int32_t>(), at, at + u.p.W, stream_of(block_table)), "hw_reserve_step");
+    else check_status(hw_reserve_blocks(&u.p, n_new.const_data_ptr<int32_t>(), at, stream_of(block_table)), "hw_reserve_blocks");
 }
 
 void compact_blocks(at::Tensor& block_table, at::Tensor& ref_counts, at::TensorList caches, at::Tensor& used) {
@@ -729,7 +735,8 @@ void copy_to_slots(const at::Tensor& key_states, const at::Tensor& value_states,
 // (tokens [W, K + 1] in the drafts' type, accepted int32 [W]); seq_lengths, where given, are shortened in place
 std::tuple<at::Tensor, at::Tensor> verify_drafts(const at::Tensor& drafts, const at::Tensor& target_probs, const at::Tensor& uniforms,
                                                  const std::optional<at::Tensor>& draft_probs, const std::optional<at::Tensor>& n_drafts,
-                                                 const std::optional<at::Tensor>& positions, const std::optional<at::Tensor>& seq_lengths) {
+                                                 const std::optional<at::Tensor>& positions, const std::optional<at::Tensor>& seq_lengths,
+                                                 const std::optional<at::Tensor>& n_new) {
     TORCH_CHECK(drafts.dim() == 2 && (drafts.scalar_type() == at::kLong || drafts.scalar_type() == at::kInt) && drafts.is_contiguous(),
                 "libhogatt: drafts must be contiguous int64 or int32 [W, K]");
     const int64_t W = drafts.size(0), K = drafts.size(1);
@@ -768,6 +775,11 @@ std::tuple<at::Tensor, at::Tensor> verify_drafts(const at::Tensor& drafts, const
         counts(seq_lengths, "seq_lengths");
         v.positions = positions->const_data_ptr<int32_t>();
         v.seq_lengths = seq_lengths->data_ptr<int32_t>();
+    }
+    TORCH_CHECK(!n_new.has_value() || seq_lengths.has_value(), "libhogatt: n_new goes with positions and seq_lengths");
+    if (n_new.has_value()) {
+        counts(n_new, "n_new");
+        v.n_new = n_new->const_data_ptr<int32_t>();
     }
     const at::Tensor tokens = at::empty({W, K + 1}, drafts.options()), accepted = at::empty({W}, uniforms.options().dtype(at::kInt));
     v.drafts = drafts.const_data_ptr();
@@ -1015,7 +1027,7 @@ TORCH_LIBRARY(libhogatt, m) {
           "int block_size, int num_blocks) -> ()", tags);
     m.def("copy_to_slots(Tensor key_states, Tensor value_states, Tensor(a!) key_cache, Tensor(b!) value_cache, Tensor slots) -> ()", tags);
     m.def("verify_drafts(Tensor drafts, Tensor target_probs, Tensor uniforms, Tensor? draft_probs, Tensor? n_drafts, Tensor? positions, "
-          "Tensor(a!)? seq_lengths) -> (Tensor, Tensor)", tags);
+          "Tensor(a!)? seq_lengths, Tensor? n_new=None) -> (Tensor, Tensor)", tags);
     // addition: merge_caches (python/hogwild/attention.py:251-257) for all layers of a segment
     m.def("merge_segments(Tensor(a!)[] k_dst, Tensor(b!)[] v_dst, int[] dst_len, Tensor[] k_src, Tensor[] v_src, int[] n, Tensor inv_freq, "
           "float scaling, int position, ScalarType table_dtype, int mode) -> bool", tags);

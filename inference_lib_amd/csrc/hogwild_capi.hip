@@ -450,7 +450,7 @@ int verify_run(const hw_verify* v, void* stream) {
     hw::VerifyArgs a;
     a.drafts = v->drafts; a.target = v->target; a.draft_probs = v->draft_probs;
     a.tp_w = v->tp_w; a.tp_k = v->tp_k; a.dp_w = v->dp_w; a.dp_k = v->dp_k;
-    a.uniforms = v->uniforms; a.n_drafts = v->n_drafts; a.positions = v->positions; a.lengths = v->seq_lengths;
+    a.uniforms = v->uniforms; a.n_drafts = v->n_drafts; a.positions = v->positions; a.lengths = v->seq_lengths; a.n_new = v->n_new;
     a.tokens = v->tokens; a.accepted = v->accepted;
     a.sums = one ? nullptr : reinterpret_cast<double*>(v->workspace);
     a.W = v->W; a.K = v->K; a.V = v->V;
@@ -571,18 +571,22 @@ int fork_run(const hw_pool* p, const void* who, bool free_rows, void* stream) {
     return (int)hw::launch_fork(a, who, free_rows, reinterpret_cast<hipStream_t>(stream));
 }
 
-int reserve_run(const hw_pool* p, const int32_t* n_new, int32_t* positions, void* stream_) {
+int reserve_run(const hw_pool* p, const int32_t* n_new, int32_t* positions, int32_t* taken, void* stream_) {
     hw::PoolArgs a;
     const int st = pool_args(p, true, true, &a);
     if (st != HW_OK) return st;
     if (n_new == nullptr || positions == nullptr) return HW_ERR_NULL;
     if (p->workspace == nullptr || p->workspace_bytes < pool_bytes(p)) return HW_ERR_WORKSPACE;
     // (the lengths grow: in their place the positions would be lost)
-    const uintptr_t at = reinterpret_cast<uintptr_t>(positions), len = reinterpret_cast<uintptr_t>(p->seq_lengths), bytes = (uintptr_t)p->W * sizeof(int32_t);
-    if (at < len + bytes && len < at + bytes) return HW_ERR_SHAPE;
+    auto apart = [&](const int32_t* x, const int32_t* y) {
+        const uintptr_t a0 = reinterpret_cast<uintptr_t>(x), b0 = reinterpret_cast<uintptr_t>(y), bytes = (uintptr_t)p->W * sizeof(int32_t);
+        return a0 >= b0 + bytes || b0 >= a0 + bytes;
+    };
+    if (!apart(positions, p->seq_lengths)) return HW_ERR_SHAPE;
+    if (taken != nullptr && !(apart(taken, p->seq_lengths) && apart(taken, positions) && apart(taken, n_new))) return HW_ERR_SHAPE;
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     int* ws = reinterpret_cast<int*>(p->workspace);
-    const hipError_t e = hw::launch_reserve(a, n_new, positions, ws, stream);
+    const hipError_t e = hw::launch_reserve(a, n_new, positions, taken, ws, stream);
     if (e != hipSuccess) return (int)e;
     hw::PageCopyArgs c;
     std::memset(&c, 0, sizeof(c));
@@ -1035,7 +1039,11 @@ int hw_fork_blocks(const hw_pool* p, const int32_t* parents, void* stream) { ret
 
 int hw_free_blocks(const hw_pool* p, const uint8_t* finished, void* stream) { return fork_run(p, finished, true, stream); }
 
-int hw_reserve_blocks(const hw_pool* p, const int32_t* n_new, int32_t* positions, void* stream) { return reserve_run(p, n_new, positions, stream); }
+int hw_reserve_blocks(const hw_pool* p, const int32_t* n_new, int32_t* positions, void* stream) { return reserve_run(p, n_new, positions, nullptr, stream); }
+
+int hw_reserve_step(const hw_pool* p, const int32_t* n_new, int32_t* positions, int32_t* taken, void* stream) {
+    return taken == nullptr ? (int)HW_ERR_NULL : reserve_run(p, n_new, positions, taken, stream);
+}
 
 int hw_compact_blocks(const hw_pool* p, int32_t* used, void* stream) { return compact_run(p, used, stream); }
 

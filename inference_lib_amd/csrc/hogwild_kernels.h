@@ -183,7 +183,7 @@ struct PageCopyArgs {
 };
 static_assert(sizeof(PageCopyArgs) <= 4096, "kernel arguments");
 hipError_t launch_fork(const PoolArgs& a, const void* who, bool free_rows, hipStream_t stream);
-hipError_t launch_reserve(const PoolArgs& a, const int* n_new, int* positions, int* ws, hipStream_t stream);
+hipError_t launch_reserve(const PoolArgs& a, const int* n_new, int* positions, int* taken, int* ws, hipStream_t stream);      // taken: or null
 hipError_t launch_compact(const PoolArgs& a, int* used, int* ws, hipStream_t stream);
 hipError_t launch_copy_pages(const PageCopyArgs& a, int most_pairs, hipStream_t stream);
 
@@ -239,6 +239,7 @@ struct VerifyArgs {
     const int* n_drafts;       // [W] or null
     const int* positions;      // [W]
     int* lengths;              // [W] or null
+    const int* n_new;          // [W] or null
     void* tokens;              // [W, K + 1]
     int* accepted;             // [W]
     double* sums;              // [W][chunks][2]: of the weights left over and of the target's probabilities; null: one launch, up to

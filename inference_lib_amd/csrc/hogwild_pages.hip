@@ -101,12 +101,13 @@ __device__ __forceinline__ int wave_base(int mine, int* lds, int wv, int lane, i
 // shortened), and neither do those behind the last new token, which the row gives up as far as others name them.  The pages that
 // the rows want, row by row and in a row by position, get the free pages in ascending order; the first row whose wants go beyond the free
 // pages gets none, and neither do the rows behind it that want any or keep a shared page.  positions[w] = where the new tokens go, or, for
-// a row that gets nothing or asks for nothing, a position behind the table (which the appends leave out).  Sixteen lanes to a row.
+// a row that gets nothing or asks for nothing, a position behind the table (which the appends leave out); taken[w] = how many, 0 for such a
+// row.  Sixteen lanes to a row.
 // Bound by latency: 6.1 us (with the copy launch behind it, in a graph) for 64 rows in a pool of 1024 pages, 43 of 131 072, whose counts it
 // reads whole; that pages without tokens are looked for is 0.2 us of it, where a row names some 0.6.
 // A count is lowered at once where nothing depends on it any more; where a row wants a page only because others name its own, after
 // all wants are served, by the pages that then stand in the list of the free ones.
-__global__ __launch_bounds__(POOL_THREADS) void reserve_kernel(const PoolArgs a, const int* n_new, int* positions, int* ws) {
+__global__ __launch_bounds__(POOL_THREADS) void reserve_kernel(const PoolArgs a, const int* n_new, int* positions, int* taken, int* ws) {
     __shared__ int page[POOL_MAX_ROWS];      // the shared page that row w is about to write, or -1
     __shared__ int need[POOL_MAX_ROWS];      // pages wanted; then the wants of all rows up to this one
     __shared__ int behind[POOL_MAX_ROWS];    // pages behind the last new token that the row gives up
@@ -242,6 +243,7 @@ __global__ __launch_bounds__(POOL_THREADS) void reserve_kernel(const PoolArgs a,
     auto finish = [&](int w, const Row& r, bool granted) {
         if (l16 == 0) {
             positions[w] = granted ? r.len : cap;
+            if (taken != nullptr) taken[w] = granted ? r.nn : 0;
             if (granted) a.lengths[w] = r.len + r.nn;
         }
     };
@@ -427,8 +429,8 @@ hipError_t launch_fork(const PoolArgs& a, const void* who, bool free_rows, hipSt
     return hipGetLastError();
 }
 
-hipError_t launch_reserve(const PoolArgs& a, const int* n_new, int* positions, int* ws, hipStream_t stream) {
-    hipLaunchKernelGGL(reserve_kernel, dim3(1), dim3(POOL_THREADS), 0, stream, a, n_new, positions, ws);
+hipError_t launch_reserve(const PoolArgs& a, const int* n_new, int* positions, int* taken, int* ws, hipStream_t stream) {
+    hipLaunchKernelGGL(reserve_kernel, dim3(1), dim3(POOL_THREADS), 0, stream, a, n_new, positions, taken, ws);
     return hipGetLastError();
 }
 

@@ -380,7 +380,11 @@ __global__ __launch_bounds__(VERIFY_THREADS * GROUPS) void verify_kernel(const V
         for (int i = threadIdx.x; i <= a.K; i += VERIFY_THREADS * GROUPS) tokens[i] = i < r.accepted ? drafts[i] : (TOK)(i == r.accepted ? token : -1);
         if (threadIdx.x == 0) {
             a.accepted[w] = r.accepted;
-            if (a.lengths != nullptr) a.lengths[w] = (int)min((long long)a.lengths[w], (long long)a.positions[w] + 1 + r.accepted);
+            if (a.lengths != nullptr) {
+                // (the drafts are the last of the step's tokens, behind one other at least)
+                const long long brought = a.n_new != nullptr ? max(a.n_new[w], 0) : 1 + r.n, kept = min(brought, max(brought - r.n, 1ll) + r.accepted);
+                a.lengths[w] = (int)min((long long)a.lengths[w], (long long)a.positions[w] + kept);
+            }
         }
     }
 }

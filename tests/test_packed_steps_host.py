@@ -1,0 +1,36 @@
+"""Refusals of packed steps and their verification that need no GPU."""
+import ctypes as C
+
+import pytest
+import torch
+
+from inference_lib_amd import _lib
+
+
+def ints(*s):
+    return torch.zeros(s, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("bad", [dict(n_new=ints(2)), dict(n_new=ints(2), positions=ints(2)), dict(n_new=ints(3), positions=ints(2), seq_lengths=ints(2)),
+                                 dict(n_new=ints(2).long(), positions=ints(2), seq_lengths=ints(2)), dict(n_new=ints(4)[::2], positions=ints(2), seq_lengths=ints(2))])
+def test_numbers_of_new_tokens_go_with_the_lengths(bad):
+    with pytest.raises(ValueError):
+        _lib.verify_drafts(torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 4, 9), torch.zeros(2, 4), **bad)
+
+
+@pytest.mark.parametrize("taken,status", [(None, -1), (4096, -3), (4112 - 4, -3), (8192 + 12, -3), (16384 - 12, -3)])
+def test_numbers_taken_lie_apart(taken, status):
+    """Not in the new tokens' numbers, the positions or the lengths, nor across them."""
+    p = _lib.HwPool()
+    p.W, p.max_blocks, p.num_blocks, p.block_size = 4, 3, 8, 16
+    p.block_table, p.seq_lengths, p.ref_counts = 65536, 8192, 32768
+    n = C.c_size_t(0)
+    assert _lib.lib.hw_pool_workspace_bytes(C.byref(p), C.byref(n)) == 0
+    p.workspace, p.workspace_bytes = 1 << 20, n.value
+    assert _lib.lib.hw_reserve_step(C.byref(p), 4096, 16384, taken, None) == status
+
+
+@pytest.mark.parametrize("positions", [ints(3), ints(3, 2), ints(1, 2), ints(2, 3), ints(2, 2).long(), ints(2, 4)[:, ::2]])
+def test_reserve_refuses_other_positions(positions):
+    with pytest.raises(ValueError):
+        _lib.reserve_blocks(ints(2, 5), ints(2), ints(9), ints(2), positions, [], 16)
