@@ -383,8 +383,10 @@ int hw_free_blocks(const hw_pool* p, const uint8_t* finished, void* stream);
  * block_size * max_blocks, which the appends leave out, and its length stays.  positions are not seq_lengths (HW_ERR_SHAPE).
  */
 int hw_reserve_blocks(const hw_pool* p, const int32_t* n_new, int32_t* positions, void* stream);
-/* The same; taken[w] (device int32 [W], written, no part of the other tables: HW_ERR_SHAPE) = n_new[w] for a sequence that got its pages, otherwise 0. */
-int hw_reserve_step(const hw_pool* p, const int32_t* n_new, int32_t* positions, int32_t* taken, void* stream);
+/* The same; taken[w] (device int32 [W], written, no part of the other tables: HW_ERR_SHAPE) = n_new[w] for a sequence that got its pages, otherwise 0.
+   With total >= 0 (below 2^28) the new tokens lie one behind the other in the `total` rows of a packed batch (hw_packed_slots): the first
+   sequence whose tokens end behind them, and those behind it, get nothing. */
+int hw_reserve_step(const hw_pool* p, const int32_t* n_new, int32_t total, int32_t* positions, int32_t* taken, void* stream);
 
 /* The pages that sequences name (ref_counts > 0) become the first ones of the pool: those behind as many places as there are of them
    move, in ascending order, to the free pages before.  used[0] (device int32) = how many there are. */

@@ -236,7 +236,7 @@ def _load() -> C.CDLL:
     lib.hw_fork_blocks.argtypes = [C.POINTER(HwPool), C.c_void_p, C.c_void_p]
     lib.hw_free_blocks.argtypes = [C.POINTER(HwPool), C.c_void_p, C.c_void_p]
     lib.hw_reserve_blocks.argtypes = [C.POINTER(HwPool), C.c_void_p, C.c_void_p, C.c_void_p]
-    lib.hw_reserve_step.argtypes = [C.POINTER(HwPool), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]
+    lib.hw_reserve_step.argtypes = [C.POINTER(HwPool), C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p]
     lib.hw_compact_blocks.argtypes = [C.POINTER(HwPool), C.c_void_p, C.c_void_p]
     lib.hw_copy_pages.argtypes = [C.POINTER(C.c_void_p), C.POINTER(C.c_size_t), C.c_int, C.c_int, C.POINTER(C.c_int32), C.POINTER(C.c_int32), C.c_int, C.c_void_p]
     return lib
@@ -907,14 +907,16 @@ def trim_blocks(block_table, seq_lengths, ref_counts, window: int, sinks: int, b
     _Pool(block_table, seq_lengths, ref_counts, block_size).run(lib.hw_trim_blocks, int(window), int(sinks))
 
 
-def reserve_blocks(block_table, seq_lengths, ref_counts, n_new, positions, caches, block_size: int) -> None:
+def reserve_blocks(block_table, seq_lengths, ref_counts, n_new, positions, caches, block_size: int, total: int = -1) -> None:
     pool = _Pool(block_table, seq_lengths, ref_counts, block_size, caches)
     W = block_table.size(0)
     if tuple(n_new.shape) != (W,) or tuple(positions.shape) not in ((W,), (2, W)):
         raise ValueError("n_new must be [W], positions [W] or [2, W]")
+    if total != -1 and not (positions.dim() == 2 and 0 <= int(total) < 1 << 28):
+        raise ValueError("the rows of a packed batch are below 2^28, and go with positions [2, W]")
     pool.check_ints(n_new, positions)
     if positions.dim() == 2:
-        pool.run(lib.hw_reserve_step, n_new.data_ptr(), positions.data_ptr(), positions[1].data_ptr(), workspace=True)
+        pool.run(lib.hw_reserve_step, n_new.data_ptr(), int(total), positions.data_ptr(), positions[1].data_ptr(), workspace=True)
     else:
         pool.run(lib.hw_reserve_blocks, n_new.data_ptr(), positions.data_ptr(), workspace=True)
 

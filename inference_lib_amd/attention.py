@@ -337,17 +337,18 @@ def trim_blocks(block_table: torch.Tensor, seq_lengths: torch.Tensor, ref_counts
 
 
 def reserve_blocks(block_table: torch.Tensor, seq_lengths: torch.Tensor, ref_counts: torch.Tensor, n_new: torch.Tensor,
-                   caches: Sequence[torch.Tensor], block_size: int, positions: Optional[torch.Tensor] = None) -> torch.Tensor:
+                   caches: Sequence[torch.Tensor], block_size: int, positions: Optional[torch.Tensor] = None, total: int = -1) -> torch.Tensor:
     """Pages for n_new[w] (int32 [W]) more tokens of every sequence: those its row lacks, a copy (in all `caches`) of a shared page that is
     about to be written, and a free one in the place of a shared page behind the sequence's tokens.  Returns positions [W], where the new tokens go (the lengths so far); a sequence that gets
     nothing has block_size * max_blocks there, which the appends leave out, and keeps its length (see hw_reserve_blocks).  `positions`: the tensor to
-    write into, or one [2, W], whose second row becomes the numbers of tokens that the sequences got."""
+    write into, or one [2, W], whose second row becomes the numbers of tokens that the sequences got.  `total` (with [2, W]): the rows of a packed
+    batch, in which the tokens lie one behind the other; the first sequence whose tokens do not fit, and those behind it, get nothing."""
     if positions is None:
         positions = torch.empty_like(seq_lengths)
     if HAVE_TORCH_OPS:
-        torch.ops.libhogatt.reserve_blocks(block_table, seq_lengths, ref_counts, n_new, positions, list(caches), block_size)
+        torch.ops.libhogatt.reserve_blocks(block_table, seq_lengths, ref_counts, n_new, positions, list(caches), block_size, total)
     else:
-        _lib.reserve_blocks(block_table, seq_lengths, ref_counts, n_new, positions, list(caches), block_size)
+        _lib.reserve_blocks(block_table, seq_lengths, ref_counts, n_new, positions, list(caches), block_size, total)
     return positions
 
 

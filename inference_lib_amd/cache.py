@@ -420,7 +420,7 @@ class PagedCache:
         tokens, accepted = cache.verify(drafts, target_probs, uniforms, n_drafts=n_drafts)      # which of the step's last n_drafts tokens stand
         cache.trim()
 
-    A sequence that `reserve` has nothing for (the pool or its row of the table is full, or it asked for no tokens) is left out of the
+    A sequence that `reserve` has nothing for (the pool, its row of the table or the packed batch is full, or it asked for no tokens) is left out of the
     step: its states are not written, its output is 0 and its length stays; `granted()` says which ones took part.  Tokens behind those
     that a sequence asked for get 0 too; no other sequence sees their states.  A sequence has at most max_blocks pages: by default as many as
     the pool, or as the attention takes (2^20 positions).
@@ -473,9 +473,12 @@ class PagedCache:
         """Positions [max_seqs] of the first new token of every sequence (see attention.reserve_blocks)."""
         if not isinstance(n_new, torch.Tensor):
             n_new = torch.full_like(self.seq_lengths, int(n_new))
+        return self._reserve(n_new)
+
+    def _reserve(self, n_new: torch.Tensor, *total) -> torch.Tensor:
         self._made = {}
         self._replayed |= self._capture() != 0
-        _ops.reserve_blocks(self.block_table, self.seq_lengths, self.ref_counts, n_new, self.caches, self.block_size, self._step)
+        _ops.reserve_blocks(self.block_table, self.seq_lengths, self.ref_counts, n_new, self.caches, self.block_size, self._step, *total)
         return self.positions
 
     def _capture(self) -> int:
@@ -513,14 +516,14 @@ class PagedCache:
     def reserve_packed(self, n_new: torch.Tensor, total: int) -> Tuple[torch.Tensor, torch.Tensor]:
         """Room for n_new[w] tokens of every sequence, which lie one behind the other in the batch's `total` rows.  Returns where each begins,
         int32 [max_seqs + 1], and the rows' positions, int32 [total], -1 for those that take no part: rows behind the last sequence's, and
-        those of a sequence that the pool had nothing for.  update_packed and attend_packed go by the last batch of as many rows; its
+        those of a sequence that the pool had nothing for or whose tokens do not all fit into the rows.  update_packed and attend_packed go by the last batch of as many rows; its
         layout is written over by the next one."""
         if self.bits == 4:
             raise ValueError("packed batches are for caches in 16 and 32 bits")
         total = int(total)
         if total < 0 or not isinstance(n_new, torch.Tensor):
             raise ValueError("n_new: a tensor of one number per sequence; total: the rows of the batch")
-        positions = self.reserve(n_new)
+        positions = self._reserve(n_new, total)
         out = _ops.packed_slots(self.block_table, positions, n_new, total, self.block_size, self.ref_counts.numel(), out=self._layouts.pop(total, None))
         self._layouts[total] = out
         self._hold(total)

@@ -536,22 +536,23 @@ void free_blocks(at::Tensor& block_table, at::Tensor& seq_lengths, at::Tensor& r
     check_status(hw_free_blocks(&u.p, reinterpret_cast<const uint8_t*>(finished.const_data_ptr()), stream_of(block_table)), "hw_free_blocks");
 }
 
-// positions [W], or [2, W] with the numbers of tokens taken behind them
+// positions [W], or [2, W] with the numbers of tokens taken behind them; total: the rows of a packed batch (with [2, W]), or -1
 void reserve_blocks(at::Tensor& block_table, at::Tensor& seq_lengths, at::Tensor& ref_counts, const at::Tensor& n_new, at::Tensor& positions,
-                    at::TensorList caches, int64_t block_size) {
+                    at::TensorList caches, int64_t block_size, int64_t total) {
     Pool u;
     pool_tables(u, block_table, &seq_lengths, ref_counts, block_size);
     pool_caches(u, caches, u.p.num_blocks, block_table.device());
     const bool both = positions.dim() == 2 && positions.size(0) == 2;
     TORCH_CHECK(n_new.dim() == 1 && n_new.size(0) == u.p.W && (both || positions.dim() == 1) && positions.size(-1) == u.p.W,
                 "libhogatt: n_new must be [W], positions [W] or [2, W]");
+    TORCH_CHECK(total == -1 || (both && total >= 0 && total < (1ll << 28)), "libhogatt: the rows of a packed batch are below 2^28, and go with positions [2, W]");
     for (const at::Tensor* t : std::initializer_list<const at::Tensor*>{&n_new, &positions})
         TORCH_CHECK(t->scalar_type() == at::kInt && t->is_contiguous() && t->device() == block_table.device(),
                     "libhogatt: n_new and positions must be contiguous int32 on the table's device");
     c10::hip::HIPGuardMasqueradingAsCUDA guard(block_table.device());
     pool_workspace(u, block_table);
     int32_t* const at = positions.data_ptr<int32_t>();
-    if (both) check_status(hw_reserve_step(&u.p, n_new.const_data_ptr<int32_t>(), at, at + u.p.W, stream_of(block_table)), "hw_reserve_step");
+    if (both) check_status(hw_reserve_step(&u.p, n_new.const_data_ptr<int32_t>(), (int32_t)total, at, at + u.p.W, stream_of(block_table)), "hw_reserve_step");
     else check_status(hw_reserve_blocks(&u.p, n_new.const_data_ptr<int32_t>(), at, stream_of(block_table)), "hw_reserve_blocks");
 }
 
@@ -1013,7 +1014,7 @@ TORCH_LIBRARY(libhogatt, m) {
     m.def("fork_blocks(Tensor(a!) block_table, Tensor(b!) seq_lengths, Tensor(c!) ref_counts, Tensor parents, int block_size) -> ()", tags);
     m.def("free_blocks(Tensor(a!) block_table, Tensor(b!) seq_lengths, Tensor(c!) ref_counts, Tensor finished) -> ()", tags);
     m.def("reserve_blocks(Tensor(a!) block_table, Tensor(b!) seq_lengths, Tensor(c!) ref_counts, Tensor n_new, Tensor(d!) positions, "
-          "Tensor(e!)[] caches, int block_size) -> ()", tags);
+          "Tensor(e!)[] caches, int block_size, int total=-1) -> ()", tags);
     m.def("compact_blocks(Tensor(a!) block_table, Tensor(b!) ref_counts, Tensor(c!)[] caches, Tensor(d!) used) -> ()", tags);
     m.def("copy_blocks(Tensor(a!)[] caches, int[] src, int[] dst) -> ()", tags);
     // additions: paged attention with a sliding window and sinks, packed batches, drafted tokens

@@ -571,11 +571,12 @@ int fork_run(const hw_pool* p, const void* who, bool free_rows, void* stream) {
     return (int)hw::launch_fork(a, who, free_rows, reinterpret_cast<hipStream_t>(stream));
 }
 
-int reserve_run(const hw_pool* p, const int32_t* n_new, int32_t* positions, int32_t* taken, void* stream_) {
+int reserve_run(const hw_pool* p, const int32_t* n_new, int32_t total, int32_t* positions, int32_t* taken, void* stream_) {
     hw::PoolArgs a;
     const int st = pool_args(p, true, true, &a);
     if (st != HW_OK) return st;
     if (n_new == nullptr || positions == nullptr) return HW_ERR_NULL;
+    if (total >= (1 << 28)) return HW_ERR_SHAPE;
     if (p->workspace == nullptr || p->workspace_bytes < pool_bytes(p)) return HW_ERR_WORKSPACE;
     // (the lengths grow: in their place the positions would be lost)
     auto apart = [&](const int32_t* x, const int32_t* y) {
@@ -586,7 +587,7 @@ int reserve_run(const hw_pool* p, const int32_t* n_new, int32_t* positions, int3
     if (taken != nullptr && !(apart(taken, p->seq_lengths) && apart(taken, positions) && apart(taken, n_new))) return HW_ERR_SHAPE;
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     int* ws = reinterpret_cast<int*>(p->workspace);
-    const hipError_t e = hw::launch_reserve(a, n_new, positions, taken, ws, stream);
+    const hipError_t e = hw::launch_reserve(a, n_new, total < 0 ? -1 : total, positions, taken, ws, stream);
     if (e != hipSuccess) return (int)e;
     hw::PageCopyArgs c;
     std::memset(&c, 0, sizeof(c));
@@ -1039,10 +1040,10 @@ int hw_fork_blocks(const hw_pool* p, const int32_t* parents, void* stream) { ret
 
 int hw_free_blocks(const hw_pool* p, const uint8_t* finished, void* stream) { return fork_run(p, finished, true, stream); }
 
-int hw_reserve_blocks(const hw_pool* p, const int32_t* n_new, int32_t* positions, void* stream) { return reserve_run(p, n_new, positions, nullptr, stream); }
+int hw_reserve_blocks(const hw_pool* p, const int32_t* n_new, int32_t* positions, void* stream) { return reserve_run(p, n_new, -1, positions, nullptr, stream); }
 
-int hw_reserve_step(const hw_pool* p, const int32_t* n_new, int32_t* positions, int32_t* taken, void* stream) {
-    return taken == nullptr ? (int)HW_ERR_NULL : reserve_run(p, n_new, positions, taken, stream);
+int hw_reserve_step(const hw_pool* p, const int32_t* n_new, int32_t total, int32_t* positions, int32_t* taken, void* stream) {
+    return taken == nullptr ? (int)HW_ERR_NULL : reserve_run(p, n_new, total, positions, taken, stream);
 }
 
 int hw_compact_blocks(const hw_pool* p, int32_t* used, void* stream) { return compact_run(p, used, stream); }

@@ -183,7 +183,7 @@ struct PageCopyArgs {
 };
 static_assert(sizeof(PageCopyArgs) <= 4096, "kernel arguments");
 hipError_t launch_fork(const PoolArgs& a, const void* who, bool free_rows, hipStream_t stream);
-hipError_t launch_reserve(const PoolArgs& a, const int* n_new, int* positions, int* taken, int* ws, hipStream_t stream);      // taken: or null
+hipError_t launch_reserve(const PoolArgs& a, const int* n_new, int total, int* positions, int* taken, int* ws, hipStream_t stream);      // total: or -1; taken: or null
 hipError_t launch_compact(const PoolArgs& a, int* used, int* ws, hipStream_t stream);
 hipError_t launch_copy_pages(const PageCopyArgs& a, int most_pairs, hipStream_t stream);
 

@@ -102,17 +102,20 @@ __device__ __forceinline__ int wave_base(int mine, int* lds, int wv, int lane, i
 // the rows want, row by row and in a row by position, get the free pages in ascending order; the first row whose wants go beyond the free
 // pages gets none, and neither do the rows behind it that want any or keep a shared page.  positions[w] = where the new tokens go, or, for
 // a row that gets nothing or asks for nothing, a position behind the table (which the appends leave out); taken[w] = how many, 0 for such a
-// row.  Sixteen lanes to a row.
+// row.  From the first row on whose new tokens, those of all rows one behind the other, end behind `total` (a packed batch; negative: none), no
+// row gets any.  Sixteen lanes to a row.
 // Bound by latency: 6.1 us (with the copy launch behind it, in a graph) for 64 rows in a pool of 1024 pages, 43 of 131 072, whose counts it
-// reads whole; that pages without tokens are looked for is 0.2 us of it, where a row names some 0.6.
+// reads whole; that pages without tokens are looked for is 0.2 us of it, where a row names some 0.6.  What fits into a batch's rows: 1.4.
 // A count is lowered at once where nothing depends on it any more; where a row wants a page only because others name its own, after
 // all wants are served, by the pages that then stand in the list of the free ones.
-__global__ __launch_bounds__(POOL_THREADS) void reserve_kernel(const PoolArgs a, const int* n_new, int* positions, int* taken, int* ws) {
+__global__ __launch_bounds__(POOL_THREADS) void reserve_kernel(const PoolArgs a, const int* n_new, int total_rows, int* positions, int* taken, int* ws) {
     __shared__ int page[POOL_MAX_ROWS];      // the shared page that row w is about to write, or -1
     __shared__ int need[POOL_MAX_ROWS];      // pages wanted; then the wants of all rows up to this one
     __shared__ int behind[POOL_MAX_ROWS];    // pages behind the last new token that the row gives up
     __shared__ int scan[POOL_WAVES];
     __shared__ int copies, spare;            // spare: some row gives up pages that hold no tokens of it
+    __shared__ int fits;                     // the rows before this one fit into the batch
+    constexpr int RPT = POOL_MAX_ROWS / POOL_THREADS;      // consecutive rows of a thread, where rows are added up
     int* const list = ws + POOL_WS_HEADER;
     int* const pairs = list + a.num_blocks;
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -124,8 +127,35 @@ __global__ __launch_bounds__(POOL_THREADS) void reserve_kernel(const PoolArgs a,
         for (int d = 1; d < 16; d <<= 1) v += __shfl_xor(v, d, 64);
         return v;
     };
-    if (tid == 0) copies = spare = 0;
+    if (tid == 0) {
+        copies = spare = 0;
+        fits = a.W;
+    }
     __syncthreads();
+    if (total_rows >= 0) {                   // (sums stop at total_rows + 1, below 2^29: associative, as those of packed_slots_kernel)
+        const int most = total_rows + 1;
+        auto add = [&](int sum, int w) { return w < a.W ? min(sum + min(max(n_new[w], 0), most), most) : sum; };
+        int sum = 0;
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) sum = add(sum, tid * RPT + i);
+        int inc = sum;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int v = __shfl_up(inc, d, 64);
+            if (lane >= d) inc = min(inc + v, most);
+        }
+        if (lane == 63) scan[wv] = inc;
+        __syncthreads();
+        int upto = __shfl_up(inc, 1, 64);
+        if (lane == 0) upto = 0;
+        for (int i = 0; i < wv; ++i) upto = min(upto + scan[i], most);
+        for (int i = 0; i < RPT && upto < most; ++i) {
+            upto = add(upto, tid * RPT + i);
+            if (upto == most) atomicMin(&fits, tid * RPT + i);
+        }
+        __syncthreads();
+    }
+    const int in_batch = fits;
     struct Row {
         int len, nn, first, last;
         bool grows;
@@ -134,7 +164,7 @@ __global__ __launch_bounds__(POOL_THREADS) void reserve_kernel(const PoolArgs a,
         Row r;
         r.len = a.lengths[w];
         r.nn = n_new[w];
-        r.grows = r.nn > 0 && r.len >= 0 && (long long)r.len + r.nn <= cap;
+        r.grows = r.nn > 0 && r.len >= 0 && (long long)r.len + r.nn <= cap && w < in_batch;
         r.first = r.grows ? r.len / a.block_size : 0;
         r.last = r.grows ? (r.len + r.nn - 1) / a.block_size : -1;
         return r;
@@ -186,8 +216,7 @@ __global__ __launch_bounds__(POOL_THREADS) void reserve_kernel(const PoolArgs a,
         if (l16 == 0 && before < a.refs[p0] - 1) need[w] = (need[w] + 1) | COPY;
     }
     __syncthreads();
-    // wants of all rows up to each: POOL_MAX_ROWS / POOL_THREADS rows a thread
-    constexpr int RPT = POOL_MAX_ROWS / POOL_THREADS;
+    // wants of all rows up to each
     int total = 0;
     long long moves = 0;                     // bit i: the thread's row i copies (kept outside of `need`, which becomes the prefix)
     {
@@ -429,8 +458,8 @@ hipError_t launch_fork(const PoolArgs& a, const void* who, bool free_rows, hipSt
     return hipGetLastError();
 }
 
-hipError_t launch_reserve(const PoolArgs& a, const int* n_new, int* positions, int* taken, int* ws, hipStream_t stream) {
-    hipLaunchKernelGGL(reserve_kernel, dim3(1), dim3(POOL_THREADS), 0, stream, a, n_new, positions, taken, ws);
+hipError_t launch_reserve(const PoolArgs& a, const int* n_new, int total, int* positions, int* taken, int* ws, hipStream_t stream) {
+    hipLaunchKernelGGL(reserve_kernel, dim3(1), dim3(POOL_THREADS), 0, stream, a, n_new, total, positions, taken, ws);
     return hipGetLastError();
 }
 

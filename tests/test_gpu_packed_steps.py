@@ -122,3 +122,89 @@ def test_lengths_lose_what_does_not_stand(V):
         assert torch.equal(tokens.cpu(), want_tokens) and torch.equal(accepted.cpu(), want) and got.tolist() == expect
     with pytest.raises(RuntimeError):
         attention.verify_drafts(*args, n_new=brought.to(DEV))
+
+
+@pytest.mark.parametrize("W", [1, 5, 64, 70, 1030, 4096])
+@pytest.mark.parametrize("big", [False, True])
+def test_what_does_not_fit_gets_nothing(W, big):
+    """The operator: a reserve for a batch of some rows is one in which the first sequence that does not fit, and those behind it, ask for nothing."""
+    import numpy as np
+    from inference_lib_amd import attention
+    from oracle import q4_oracle as Q
+    rng = np.random.default_rng(W)
+    block, n, P = 8, 6, 2 * W + 3
+    for step in range(8):
+        table, lengths, refs = np.full((W, n), -1, np.int32), np.zeros(W, np.int32), np.zeros(P, np.int32)
+        Q.reserve(table, lengths, refs, rng.integers(0, 2 * block, W), block)
+        ask = rng.choice([-4, 0, 1, 1, 5, 9], W).astype(np.int64)
+        if big:
+            ask[rng.integers(0, W, 2)] = 2 ** 31 - 1
+        upto = np.clip(ask, 0, None).cumsum()
+        total = int([0, min(int(upto[-1]), 2 ** 28 - 1), max(0, min(int(upto[-1]), 2 ** 28) - 1), 2 ** 28 - 1, upto[W // 2] % 2 ** 28, rng.integers(0, min(upto[-1], 9 * W) + 1), 1, upto[W // 3] % 2 ** 28][step])
+        t, l, r, at = ints(table), ints(lengths), ints(refs), torch.full((2, W), 77, dtype=torch.int32, device=DEV)
+        got = attention.reserve_blocks(t, l, r, ints(ask), [], block, positions=at, total=total)
+        asked = np.where(upto <= total, ask, 0)
+        want, _ = Q.reserve(table, lengths, refs, asked, block)
+        assert got is at and np.array_equal(at[0].cpu().numpy(), want), (step, total)
+        assert np.array_equal(at[1].cpu().numpy(), np.where(want < n * block, asked, 0)), (step, total)
+        for x, y in ((t, table), (l, lengths), (r, refs)):
+            assert np.array_equal(x.cpu().numpy(), y), (step, total)
+    for bad in (dict(total=3), dict(total=3, positions=ints([0] * W)), dict(total=-2, positions=at), dict(total=1 << 28, positions=at), dict(positions=ints([[0] * W]))):
+        with pytest.raises(RuntimeError):
+            attention.reserve_blocks(t, l, r, ints(ask), [], block, **bad)
+
+
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("window", [40, None])
+def test_more_new_tokens_than_rows(captured, window):
+    """A batch that is too small: sequences that do not fit are left out as by a full pool, nothing that was not written counts as held, and
+    what they asked for goes into a later step."""
+    from inference_lib_amd.cache import PagedCache
+    n, total, scale = 5, 40, 0.2
+    cache = PagedCache(1, HKV, D, 60, n, dtype=torch.bfloat16, device=DEV, max_blocks=12, window=window)
+    for c in cache.caches:
+        c.fill_(math.nan)                                         # what nobody wrote is nobody's to see
+    h = Histories(n, torch.bfloat16, 3)
+    n_new = ints([0] * n)
+    q, k, v = (torch.zeros((total, x, D), dtype=torch.bfloat16, device=DEV) for x in (HQ, HKV, HKV))
+
+    def step():
+        cu, at = cache.reserve_packed(n_new, total)
+        cache.update_packed(k, v, 0)
+        return cu, at, cache.attend_packed(q, 0, scale)
+
+    lengths, graph = [0] * n, None
+    for i, new in enumerate([[16, 20, 9, 0, 1], [0, 0, 9, 40, 1], [1, 1, 1, 39, 1], [2 ** 31 - 1, 1, 1, 1, 1], [8, 8, 8, 8, 8], [8, 8, 8, 8, 9], [41, 0, 0, 0, 0], [0, 40, 0, 0, 0]]):
+        n_new.copy_(torch.tensor(new))
+        taken, upto = [], 0
+        for s in new:
+            upto += s
+            taken.append(s if upto <= total else 0)
+        qs = [h.rand(s, HQ, D) for s in taken]
+        for x in (q, k, v):
+            x.fill_(math.nan)
+        row = 0
+        for w, s in enumerate(taken):
+            kv = h.rand(s, 2, HKV, D)
+            h.kv[w][0] = torch.cat([h.kv[w][0], kv])
+            q[row: row + s], k[row: row + s], v[row: row + s] = qs[w].to(DEV), kv[:, 0].to(DEV), kv[:, 1].to(DEV)
+            row += s
+        if not captured or i < 2:
+            cu, at, out = step()
+        else:
+            if graph is None:
+                graph = torch.cuda.CUDAGraph()
+                torch.cuda.synchronize()
+                with torch.cuda.graph(graph):
+                    cu, at, out = step()
+            graph.replay()
+        torch.cuda.synchronize()
+        assert cache.granted().tolist() == [s > 0 for s in taken] and cu.tolist() == [min(sum(new[:w]), total) for w in range(n + 1)], i
+        assert (at[row:] == -1).all() and (out[row:] == 0).all(), i
+        row = 0
+        for w, s in enumerate(taken):
+            assert at[row: row + s].tolist() == list(range(lengths[w], lengths[w] + s)), i
+            h.check(0, w, qs[w], lengths[w], out[row: row + s].cpu(), scale, window or 1 << 30, 0)
+            lengths[w], row = lengths[w] + s, row + s
+        assert cache.seq_lengths.tolist() == lengths, i
+        assert int((cache.block_table >= 0).sum()) == sum(-(-x // 16) for x in lengths), i
