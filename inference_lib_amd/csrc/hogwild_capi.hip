@@ -187,7 +187,7 @@ int run(const hw_problem* p, void* stream_, int fused, int stages = HW_STAGE_ATT
     ma.wgs_per_head = cp.slots;
     ma.xcd_local = (cp.groups == 1 && plan0.workgroups % 8 == 0 && p->Hkv % 8 == 0) ? 1 : 0;
     ma.row_tab = nullptr;
-    ma.pslots = ma.slot_rows = ma.guess = 0;
+    ma.pslots = ma.slot_rows = ma.guess = ma.wild = 0;
     ma.magic_rows = 0;
     if (stream_runs) {
         // (A row group with more pieces takes another batch of loads.  By the most pieces, one row group with five had all rows merged
@@ -288,6 +288,7 @@ int paged_run(const hw_paged_problem* p, void* stream_, int stages) {
     ma.pslots = planned ? plan.row_groups : shared ? plan.row_groups * plan.splits : 0;
     ma.slot_rows = shared ? plan.rows / p->W : 0;
     ma.guess = shared ? plan.splits : 0;
+    ma.wild = 0;
     ma.magic_rows = magic_of(shared ? ma.slot_rows : 1);
     if (planned) ma.wgs_per_head = 8;       // a row's slots are device data: the merge shape that suits a handful of them
     e = hw::launch_merge(ma, p->dtype, p->Ev, stream);
@@ -388,6 +389,7 @@ int window_run(const hw_window_problem* p, void* stream_) {
     ma.wgs_per_head = plan.splits;
     ma.xcd_local = (p->cu_seqlens_q == nullptr && plan.workgroups % 8 == 0 && p->Hkv % 8 == 0) ? 1 : 0;
     ma.magic_rows = magic_of(1);
+    ma.wild = 1;
     return (int)hw::launch_merge(ma, p->dtype, p->D, stream);
 }
 

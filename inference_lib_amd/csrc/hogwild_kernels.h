@@ -81,6 +81,7 @@ struct MergeArgs {
     int slot_rows;      // (with guess)
     int guess;          // > 0: slots of a row where every slot_rows rows have the same number, one behind the other; requested ahead of the table
     unsigned magic_rows;   // ceil(2^32 / slot_rows), for guess
+    int wild;           // infinite partial sums stay infinite (without guess)
 };
 
 hipError_t launch_attention(const KernelArgs& ka, int dtype, int E, int rb, int variant, hipStream_t stream);

@@ -30,10 +30,11 @@ struct Band {
     __device__ __forceinline__ bool sees(int rb, int tok) const { return tok < snk[rb] || (tok >= lo[rb] && tok < lim[rb]); }
 };
 
-// Infinite and NaN values.  A row's weight of a token that it does not see is 0, which times an infinite value would be NaN.  Tiles of which
-// rows see different tokens are therefore looked over, and where one holds such values the products take 0 in their place, and every
-// row that sees one gets it by itself: with ones in the place of the values and of the weights that are seen, a product is more than 0 where a
-// row sees a value of the kind.  NaN counts as both infinities, whose sum it is.
+// Infinite and NaN values.  A row's weight of a token that it does not see is 0, which times an infinite value would be NaN.  Tiles that some
+// row does not see all of are therefore looked over -- also where all rows see the same of them: a token that nobody sees has the values of one
+// that is seen (issue_tile) -- and where one holds such values the products take 0 in their place, and every row that sees one gets it by
+// itself: with ones in the place of the values and of the weights that are seen, a product is more than 0 where a row sees a value of the kind.  NaN counts as both infinities, whose sum it is.  (With rows at one position, single tokens, looking costs nothing that
+// shows; zeros in the place of the values that they do not see, without a look: two layers of 16 sequences 92.7 -> 93.5 us, of drafts 62.2 -> 63.4.)
 template <class DT>
 struct Wild {
     static constexpr bool WIDE = Elem<DT>::size == 4;
@@ -77,10 +78,10 @@ struct Wild {
 };
 
 // One 32-token tile against all rows of the wave: K in the staging slot, V in registers (see compute_tile, whose layouts these are).
-// mixed: the rows do not all see the same of its tokens.
+// edge: not every row sees all of its tokens.
 template <class DT, int D, int RB>
 __device__ __forceinline__ void band_tile(const TileRegs<DT, D, D>& t, const u32x4* qreg, const Band<RB>& band, WaveState<RB, D / 16>& st, int t0, int n, int q,
-                                          float sc, const char* kstage, bool mixed) {
+                                          float sc, const char* kstage, bool edge) {
     typedef Geo<DT, D, D> G;
     constexpr float LAZY_LOG2 = 8.0f;     // how far a row's maximum may exceed the reference of its exponentials before that follows
     float s[RB][8], mxl[RB];
@@ -149,7 +150,7 @@ __device__ __forceinline__ void band_tile(const TileRegs<DT, D, D>& t, const u32
     }
 
     bool wild = false;
-    if (mixed) {                                                      // uniform over the wave
+    if (edge) {                                                       // uniform over the wave
         u32 any = 0;
 #pragma unroll
         for (int idx = 0; idx < 8; ++idx)
@@ -382,7 +383,6 @@ __global__ __launch_bounds__(NTHREADS, 1) void window_kernel(const WindowHeader 
     const int high = wave_max(any ? lim1 : 0);
     const int low = -wave_max(any ? -lo1 : -0x7fffffff);
     const int sink_end = wave_max(snk1);
-    const bool alike = __ballot(at != __builtin_amdgcn_readfirstlane(at)) == 0;        // all rows at one position
     const int all_from = wave_max(lo1), all_to = -wave_max(-lim1);                     // what every row's window holds
     const int sink_tiles = (sink_end + TILE - 1) / TILE;
     const int first = high > 0 ? max(low / TILE, sink_tiles) : 0;                    // first tile of the window
@@ -394,7 +394,7 @@ __global__ __launch_bounds__(NTHREADS, 1) void window_kernel(const WindowHeader 
         const int tok = min(t * TILE + (lane & 31), cap - 1);
         return btw[fast_div(tok, ph.magic_bs)];
     };
-    auto mixed = [&](int t) { return !alike && !(t * TILE >= all_from && t * TILE + TILE <= all_to); };
+    auto edge = [&](int t) { return !(t * TILE >= all_from && t * TILE + TILE <= all_to); };
     // The loads of tile t, given its table entries: the same number of instructions whether or not the tile exists.  Tokens that no row
     // sees are replaced by one of the tile that some row does (there is one in every tile that exists), so that no byte of the cache
     // that is not seen is read; what a tile that does not exist reads is not used.
@@ -463,14 +463,14 @@ __global__ __launch_bounds__(NTHREADS, 1) void window_kernel(const WindowHeader 
             const int bt_n = bt_load(tile_at(k + 2 * NW));
             issue_tile(tr[1], kslots[1], bt_b, tile_at(k + NW));
             wait_k_landed<G, 1>();
-            band_tile<DT, D, RB>(tr[0], qreg, band, st, tile_at(k) * TILE, n, q, ph.sc, kslots[0], mixed(tile_at(k)));
+            band_tile<DT, D, RB>(tr[0], qreg, band, st, tile_at(k) * TILE, n, q, ph.sc, kslots[0], edge(tile_at(k)));
             bt_a = bt_n;
         }
         {
             const int bt_n = bt_load(tile_at(k + 3 * NW));
             issue_tile(tr[0], kslots[0], bt_a, tile_at(k + 2 * NW));
             wait_k_landed<G, 1>();
-            band_tile<DT, D, RB>(tr[1], qreg, band, st, tile_at(k + NW) * TILE, n, q, ph.sc, kslots[1], mixed(tile_at(k + NW)));
+            band_tile<DT, D, RB>(tr[1], qreg, band, st, tile_at(k + NW) * TILE, n, q, ph.sc, kslots[1], edge(tile_at(k + NW)));
             bt_b = bt_n;
         }
     }
@@ -480,10 +480,10 @@ __global__ __launch_bounds__(NTHREADS, 1) void window_kernel(const WindowHeader 
             issue_tile(tr[1], kslots[1], bt_b, tile_at(k + NW));
             wait_k_landed<G, 1>();
         } else wait_k_landed<G, 0>();
-        band_tile<DT, D, RB>(tr[0], qreg, band, st, tile_at(k) * TILE, n, q, ph.sc, kslots[0], mixed(tile_at(k)));
+        band_tile<DT, D, RB>(tr[0], qreg, band, st, tile_at(k) * TILE, n, q, ph.sc, kslots[0], edge(tile_at(k)));
         if (two) {
             wait_k_landed<G, 0>();
-            band_tile<DT, D, RB>(tr[1], qreg, band, st, tile_at(k + NW) * TILE, n, q, ph.sc, kslots[1], mixed(tile_at(k + NW)));
+            band_tile<DT, D, RB>(tr[1], qreg, band, st, tile_at(k + NW) * TILE, n, q, ph.sc, kslots[1], edge(tile_at(k + NW)));
         }
     }
 
@@ -618,7 +618,7 @@ __device__ __forceinline__ WindowGroup window_group(const PagedDevHeader& ph, co
 // One 32-token tile, K and V images in LDS, against the wave's RB * 16 rows.  MASKED: some row may not see all of it.
 template <class DT, int D, int RB, bool MASKED>
 __device__ __forceinline__ void band_tile_lds(const u32x4* qreg, const Band<RB>& band, WaveState<RB, D / 16>& st, int t0, int n, int q, float sc,
-                                              const char* kstage, const char* vimg, const unsigned* voff, bool mixed) {
+                                              const char* kstage, const char* vimg, const unsigned* voff, bool edge) {
     typedef Geo<DT, D, D> G;
     constexpr float LAZY_LOG2 = 8.0f;
     f32x4 sacc[RB][2];
@@ -696,7 +696,7 @@ __device__ __forceinline__ void band_tile_lds(const u32x4* qreg, const Band<RB>&
         pp[rb] = u32x4{Elem<DT>::pack2(p[0], p[1]), Elem<DT>::pack2(p[2], p[3]), Elem<DT>::pack2(p[4], p[5]), Elem<DT>::pack2(p[6], p[7])};
     }
     if constexpr (MASKED) {
-        if (mixed) {                                                  // uniform over the wave
+        if (edge) {                                                   // uniform over the wave
             // (nothing times them all: NaN where one is infinite or NaN; the matrix unit has time for it here, 32 registers looked at have not)
             f32x4 any[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
@@ -852,7 +852,6 @@ __global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHea
             auto lim_of = [&](int x) { return max(0, x < cap ? x + 1 : cap); };
             auto lo_of = [&](int x) { return min(max(0, x < 0 ? 0 : x - args.window + 1), cap); };       // (so that it can be rounded up to tiles)
             int top = 0, bottom = -0x7fffffff, most = 0, above = 0, least = -0x7fffffff;
-            bool other = false;                          // not all rows of the group are at one position
 #pragma unroll
             for (int i = 0; i < ROWS / 64; ++i) {
                 const int lim = lim_of(at[i]), lo = lo_of(at[i]);
@@ -862,9 +861,7 @@ __global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHea
                 most = max(most, lim);
                 above = max(above, lo);
                 least = max(least, -lim);
-                other = other || at[i] != __builtin_amdgcn_readfirstlane(at[0]);
             }
-            const bool alike = __ballot(other) == 0;
             const int high = wave_max(top), low = -wave_max(bottom);                   // the windows of the group lie in [low, high)
             const int sink_end = min(args.sinks, wave_max(most));
             const int all_from = wave_max(above), all_to = -wave_max(least);           // what every row's window holds
@@ -990,7 +987,7 @@ __global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHea
                             if (k + pp >= k1 || !(t0 < own_sinks || (t0 < own_high && t0 + TILE > own_low))) continue;
                             const char* slot = ring + (sl * TS + pp) * SLOT;
                             band_tile_lds<DT, D, RBX, true>(qreg, band, st, t0, n, q, ph.sc, slot, slot + KBYTES, voff,
-                                                            !alike && !(t0 >= own_from && t0 + TILE <= own_to));
+                                                            !(t0 >= own_from && t0 + TILE <= own_to));
                         }
                     }
                     next();
