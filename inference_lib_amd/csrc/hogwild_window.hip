@@ -23,6 +23,9 @@
 
 namespace hw {
 
+// The logit of a token that a row does not see: its weight is 0 whatever the scale (a finite one times the least scales is next to 0).
+constexpr float UNSEEN = -__builtin_inff();
+
 // The bounds of a lane's rows: row n of row block rb sees the tokens below snk[rb], and from lo[rb] to lim[rb] - 1.
 template <int RB>
 struct Band {
@@ -113,7 +116,7 @@ __device__ __forceinline__ void band_tile(const TileRegs<DT, D, D>& t, const u32
             float mx = NEG_BIG;
 #pragma unroll
             for (int idx = 0; idx < 8; ++idx) {
-                s[rb][idx] = band.sees(rb, t0 + slot_token(q, idx)) ? sacc[rb][idx >> 2][idx & 3] : NEG_BIG;
+                s[rb][idx] = band.sees(rb, t0 + slot_token(q, idx)) ? sacc[rb][idx >> 2][idx & 3] : UNSEEN;
                 mx = fmaxf(mx, s[rb][idx]);
             }
             mxl[rb] = mx;
@@ -659,7 +662,7 @@ __device__ __forceinline__ void band_tile_lds(const u32x4* qreg, const Band<RB>&
 #pragma unroll
         for (int idx = 0; idx < 8; ++idx) {
             s[rb][idx] = sacc[rb][idx >> 2][idx & 3];
-            if constexpr (MASKED) s[rb][idx] = (unsigned)slot_token(0, idx) - from < len || slot_token(0, idx) < sink ? s[rb][idx] : NEG_BIG;
+            if constexpr (MASKED) s[rb][idx] = (unsigned)slot_token(0, idx) - from < len || slot_token(0, idx) < sink ? s[rb][idx] : UNSEEN;
             mx = fmaxf(mx, s[rb][idx]);
         }
         mxl[rb] = mx;
