@@ -465,7 +465,7 @@ int hw_packed_slots(const hw_packed_batch* b, void* stream);
 
 /* Rows key_states / value_states [total, Hkv, D] (element strides for the first two dimensions, a contiguous last one) to the rows
    `slots` of the caches [num_blocks, Hkv, block_size, D].  Rows whose slot is no row of the caches are left out; no slot is named
-   twice.  Hkv * (E + Ev) <= 2^16. */
+   twice.  Hkv * (E + Ev) <= 2^16, total < 2^25. */
 typedef struct hw_copy_slots {
     int32_t dtype;
     int32_t total, Hkv, E, Ev;
@@ -491,6 +491,7 @@ int hw_copy_to_slots(const hw_copy_slots* c, void* stream);
  * on (1 + n without n_new), the drafts behind the others, and all but its n - accepted[w] last ones stay, one at least:
  * seq_lengths[w] = min(seq_lengths[w], positions[w] + min(n_new[w], max(n_new[w] - n, 1) + accepted[w])).  Positions behind the lengths
  * (hw_reserve_blocks gives them to sequences that took no part) shorten nothing.
+ * W < 2^22, W * ceil(V / 4096) < 2^24, K < 2^20, V < 2^30.
  */
 typedef struct hw_verify {
     int32_t dtype;                 /* of the probabilities */

@@ -411,7 +411,8 @@ int packed_slots_run(const hw_packed_batch* b, void* stream) {
 int copy_slots_run(const hw_copy_slots* c, void* stream) {
     if (c == nullptr) return HW_ERR_NULL;
     if (c->dtype != HW_F32 && c->dtype != HW_F16 && c->dtype != HW_BF16) return HW_ERR_DTYPE;
-    if (c->total < 0 || c->Hkv < 1 || c->E < 1 || c->Ev < 1 || c->block_size < 1 || c->num_blocks < 1) return HW_ERR_SHAPE;
+    // (a launch takes 2^32 - 1 threads at most, a token one wave; here and for drafts)
+    if (c->total < 0 || c->total >= (1 << 25) || c->Hkv < 1 || c->E < 1 || c->Ev < 1 || c->block_size < 1 || c->num_blocks < 1) return HW_ERR_SHAPE;
     if ((long long)c->num_blocks * c->Hkv * c->block_size >= (1ll << 31) || (long long)c->Hkv * ((long long)c->E + c->Ev) > (1ll << 16)) return HW_ERR_SHAPE;
     if (c->total == 0) return HW_OK;
     if (c->key_states == nullptr || c->value_states == nullptr || c->key_cache == nullptr || c->value_cache == nullptr || c->slots == nullptr) return HW_ERR_NULL;
@@ -427,7 +428,7 @@ int verify_check(const hw_verify* v) {
     if (v->dtype != HW_F32 && v->dtype != HW_F16 && v->dtype != HW_BF16) return HW_ERR_DTYPE;
     if (v->token_bytes != 4 && v->token_bytes != 8) return HW_ERR_DTYPE;
     if (v->W < 0 || v->K < 0 || v->V < 1 || v->K >= (1 << 20) || v->V >= (1 << 30)) return HW_ERR_SHAPE;
-    if ((long long)v->W * ((v->V + hw::VERIFY_CHUNK - 1) / hw::VERIFY_CHUNK) >= (1ll << 31)) return HW_ERR_SHAPE;
+    if (v->W >= (1 << 22) || (long long)v->W * ((v->V + hw::VERIFY_CHUNK - 1) / hw::VERIFY_CHUNK) >= (1ll << 24)) return HW_ERR_SHAPE;
     return HW_OK;
 }
 

@@ -50,3 +50,22 @@ def test_numbers_taken_lie_apart(taken, status):
 def test_reserve_refuses_other_positions(positions):
     with pytest.raises(ValueError):
         _lib.reserve_blocks(ints(2, 5), ints(2), ints(9), ints(2), positions, [], 16)
+
+
+def test_more_workgroups_than_a_launch_takes():
+    """Refused with a status of their own, before anything reaches the device."""
+    c = _lib.HwCopySlots()
+    c.dtype, c.Hkv, c.E, c.Ev, c.block_size, c.num_blocks = _lib.HW_F16, 1, 1, 1, 16, 4
+    c.key_states = c.value_states = c.key_cache = c.value_cache = c.slots = 4096
+    for total in (1 << 25, 1 << 26, (1 << 31) - 1):
+        c.total = total
+        assert _lib.lib.hw_copy_to_slots(C.byref(c), None) == -3
+    v, n = _lib.HwVerify(), C.c_size_t(0)
+    v.dtype, v.token_bytes, v.K = _lib.HW_F32, 8, 1
+    for W, V in [(1 << 22, 2), (1 << 20, 1 << 16), (1 << 12, 1 << 24), ((1 << 31) - 1, 4096)]:
+        v.W, v.V = W, V
+        assert _lib.lib.hw_verify_workspace_bytes(C.byref(v), C.byref(n)) == -3 and _lib.lib.hw_verify_drafts(C.byref(v), None) == -3
+    v.W, v.V = (1 << 22) - 1, 4096
+    assert _lib.lib.hw_verify_workspace_bytes(C.byref(v), C.byref(n)) == 0 and n.value == 0
+    v.W, v.V = (1 << 20) - 1, 1 << 16
+    assert _lib.lib.hw_verify_workspace_bytes(C.byref(v), C.byref(n)) == 0 and n.value > 0
