@@ -406,7 +406,8 @@ int hw_copy_pages(void* const* caches, const size_t* page_bytes, int n_caches, i
  * packed variable-length operator (cu_seqlens_q != NULL), hw_window_varlen_paged_sdpa:
  *   q [total_q, Hq, D], locations [total_q], cu_seqlens_q [W + 1] (device), out [total_q, Hq, D], lse [total_q, Hq]; query tokens
  *   before cu[0] and from cu[W] on belong to no sequence and get zeros (lse -inf)
- * What a query does not see reaches its result in no way, infinities and NaN included.  Limits: those of hw_paged_problem; window >= 1,
+ * What a query does not see reaches its result in no way, infinities and NaN included.  Logits, sums and partial sums are float32; the
+ * weights are rounded to the caches' type for their product with the values (float32: not).  Limits: those of hw_paged_problem; window >= 1,
  * sinks >= 0; D in {64, 128, 256}, float32 up to 128.
  */
 typedef struct hw_window_problem {

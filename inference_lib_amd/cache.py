@@ -560,7 +560,8 @@ class PagedCache:
         return _ops.verify_drafts(drafts, target_probs, uniforms, draft_probs, n_drafts, self.positions, self.seq_lengths, self._taken)
 
     def trim(self) -> None:
-        """The pages that no later token sees are given back.  (After verify: a length that is shortened later needs them again.)"""
+        """The pages that no later token sees are given back.  (Behind a step's layers, whose tokens see further back, and behind verify: a length
+        that is shortened later needs them again.)"""
         if self.window is None:
             raise ValueError("without a window every token is seen")
         _ops.trim_blocks(self.block_table, self.seq_lengths, self.ref_counts, self.window, self.sinks, self.block_size)

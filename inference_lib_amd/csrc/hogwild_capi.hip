@@ -435,7 +435,7 @@ int verify_check(const hw_verify* v) {
 // One launch, a workgroup of four groups of threads to a sequence, where they take a chunk each, or two with the sums of the chunks in
 // between: 16 000 tokens, 1 to 256 sequences, 9.7 to 17.1 us against 10.9 to 19.1, 32 000 11.8 to 25.9 against 10.1 to 27.4, 128 000 28 to 84 against
 // 10 to 75.
-bool verify_in_one(const hw_verify* v) { return v->V <= 4 * hw::VERIFY_CHUNK; }
+bool verify_in_one(const hw_verify* v) { return v->V <= hw::VERIFY_GROUPS * hw::VERIFY_CHUNK; }
 
 size_t verify_bytes(const hw_verify* v) {
     return verify_in_one(v) ? 0 : (size_t)v->W * ((v->V + hw::VERIFY_CHUNK - 1) / hw::VERIFY_CHUNK * 2 * sizeof(double) + sizeof(hw::VerifyRow));

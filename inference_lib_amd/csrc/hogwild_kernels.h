@@ -243,13 +243,12 @@ struct VerifyArgs {
     const int* n_new;          // [W] or null
     void* tokens;              // [W, K + 1]
     int* accepted;             // [W]
-    double* sums;              // [W][chunks][2]: of the weights left over and of the target's probabilities; null: one launch, up to
-                               // VERIFY_MOST_CHUNKS chunks
+    double* sums;              // [W][chunks][2]: of the weights left over and of the target's probabilities; null: one launch
     VerifyRow* rows;           // [W], with sums
     int W, K, V, chunks;
 };
 constexpr int VERIFY_CHUNK = 4096;      // probabilities that a group of 256 threads adds up at a time
-constexpr int VERIFY_MOST_CHUNKS = 64;
+constexpr int VERIFY_GROUPS = 4;        // groups of a workgroup that does all of a sequence in one launch, a chunk each: its vocabulary at most
 hipError_t launch_verify(const VerifyArgs& a, int dtype, bool wide_tokens, hipStream_t stream);
 
 // ---- caller-side steps: input builder and fused key rotation + append ----

@@ -19,7 +19,7 @@ constexpr int SLOTS_THREADS = 256;
 
 // Every workgroup adds up the numbers of new tokens for itself (W <= POOL_MAX_ROWS numbers, in LDS) and looks its tokens' sequences up there.
 // Sums stop at `total`: min(a + b, total) of numbers up to total is associative and stays below 2^31.  Bound by latency: counts, scan, table,
-// 2.4 us for 8 sequences of a token, 4.0 for 8192 rows of 32 sequences.
+// 2.4 us for 8 sequences of a token, 3.8 for 8192 rows of 32 sequences.
 __global__ __launch_bounds__(SLOTS_THREADS) void packed_slots_kernel(const PackedBatchArgs a) {
     __shared__ int end[POOL_MAX_ROWS];       // tokens up to and with sequence w
     __shared__ int wave_end[SLOTS_THREADS / 64];
@@ -117,9 +117,9 @@ __global__ __launch_bounds__(256) void copy_to_slots_kernel(const CopySlotsArgs 
 // Probabilities are added up in chunks of VERIFY_CHUNK, by groups of 256 threads: 16 bytes in a row to a thread, two or four rows of the group to a
 // chunk.  A thread's in their order, then the threads' of a row by a scan over the wave, then the waves and rows.  A chunk's sum and its
 // running sum are the same additions wherever they are worked out, so a token is found where the sums say that it is, and it is the same in
-// every call.  Bound by the two rows of probabilities that are read: 64 sequences, 128 000 in float32, 65.5 MB, 13.4 us (4.9 TB/s) and 6.5 for the
-// draw, a chain of loads (sums, a chunk's probabilities) between scans.  One sequence of 32 000: 6.2 and 4.6 (5.2 where the draw looks for the
-// accepted drafts again).
+// every call.  Bound by the two rows of probabilities that are read: 64 sequences, 128 000 in float32, 65.5 MB, 13.4 us (4.9 TB/s) and 6.4 for the
+// draw, a chain of loads (sums, a chunk's probabilities) between scans.  One sequence of 32 000: 6.0 and 4.8 (half a microsecond more where
+// the draw looks for the accepted drafts again).
 constexpr int VERIFY_THREADS = 256, VERIFY_WAVES = VERIFY_THREADS / 64;
 template <class DT>
 struct Chunks {
@@ -242,7 +242,7 @@ __device__ __forceinline__ double lane_value(double v, int lane) {          // (
 template <class DT, class TOK, int GROUPS, bool SUMS, bool DRAW>
 __global__ __launch_bounds__(VERIFY_THREADS * GROUPS) void verify_kernel(const VerifyArgs a) {
     constexpr bool BOTH = SUMS && DRAW;
-    __shared__ double lds_sums[BOTH ? 2 * VERIFY_MOST_CHUNKS : 1];
+    __shared__ double lds_sums[BOTH ? 2 * GROUPS : 1];
     constexpr int VEC = Chunks<DT>::VEC, ROWS = Chunks<DT>::ROWS;
     __shared__ double part[GROUPS][2][ROWS * VERIFY_WAVES];
     __shared__ int found[VERIFY_WAVES], last_one[VERIFY_WAVES];
@@ -418,7 +418,7 @@ hipError_t launch_copy_to_slots(const CopySlotsArgs& a, int dtype, hipStream_t s
 template <class DT, class TOK>
 static hipError_t launch_verify_dt(const VerifyArgs& a, hipStream_t stream) {
     if (a.sums == nullptr) {
-        hipLaunchKernelGGL((verify_kernel<DT, TOK, 4, true, true>), dim3(a.W), dim3(4 * VERIFY_THREADS), 0, stream, a);
+        hipLaunchKernelGGL((verify_kernel<DT, TOK, VERIFY_GROUPS, true, true>), dim3(a.W), dim3(VERIFY_GROUPS * VERIFY_THREADS), 0, stream, a);
         return hipGetLastError();
     }
     hipLaunchKernelGGL((verify_kernel<DT, TOK, 1, true, false>), dim3((unsigned)a.W * a.chunks), dim3(VERIFY_THREADS), 0, stream, a);

@@ -9,7 +9,8 @@
 //
 // Bound by what is loaded: 16 sequences that see 4096 tokens of 40/8 heads of 128 channels take 46 us a layer, 269 MB at 5.8 TB/s.  Smaller steps
 // show the chain in front of the loads (positions, table entries, first tiles: 3 us) and the merge, 8 us together: 5 ragged sequences that see up to
-// 1088 tokens of 256 channels, 36 MB, 15 us; 4 sequences of 4 tokens that see 2048, 34 MB, 15.4; the least step 5 (one workgroup a group, no merge).
+// 1088 tokens of 256 channels, 36 MB, 15 us a layer; 4 sequences of 4 tokens that see 2048, 34 MB, 15.5 (a quarter of a pass over four layers,
+// merges included); the least kernel 4.3 (one workgroup a group, no merge: one sequence that sees 64 tokens of 64 channels).
 // Two row blocks share what is loaded, which pays where the tiles are many (see window_plan).
 //
 // Sequences with more rows (prompt chunks) go through window_wide_kernel: row groups of 256, whose waves share every tile through LDS.
@@ -458,8 +459,8 @@ __global__ __launch_bounds__(NTHREADS, 1) void window_kernel(const WindowHeader 
             qreg[rb * G::KJ + j] = *reinterpret_cast<const u32x4*>(q_lds + (rb * 16 + n) * G::QSTR + (4 * j + q) * 16);
 
     // Two tiles in flight per wave: request the table entries two tiles ahead, then the next tile, then compute the current one.  The last one or
-    // two tiles are outside of the loop, where nothing is requested any more (4 tokens of 4 sequences that see 2048 14.8 -> 13.8 us, 5
-    // ragged ones at 256 channels 16.2 -> 15.1; a third tile in flight instead: 15.5).
+    // two tiles are outside of the loop, where nothing is requested any more (this kernel alone, traced: 4 tokens of 4 sequences that see 2048
+    // 15.0 -> 14.2 us, 5 ragged ones at 256 channels 14.2 -> 13.3; a third tile in flight instead: 5 % more than without).
     int k = gw;
     for (; k + 2 * NW < tiles; k += 2 * NW) {
         {
@@ -1071,7 +1072,7 @@ __global__ __launch_bounds__(NW * 64, 1) void window_wide_kernel(const WindowHea
     }
 }
 
-// The groups that lie across workgroups, as the attention kernel left word of them (WindowCut): a workgroup takes PER rows a thread, D / 4
+// The groups that lie across workgroups, as the attention kernel left word of them (cuts_of): a workgroup takes PER rows a thread, D / 4
 // lanes a row, of one of them at a time; parts in their order.  A kv head's partial sums are read on the XCD that wrote them.
 template <class DT, int D, int PER, int UN>
 __global__ __launch_bounds__(256) void window_merge_kernel(const WindowHeader args) {
