@@ -9,7 +9,7 @@ pytestmark = pytest.mark.gpu
 
 
 @pytest.mark.parametrize("dtype,heads", [("f32", (5, 5, 64)), ("f32", (4, 1, 128)), ("f16", (7, 1, 128)), ("bf16", (8, 2, 64)), ("bf16", (6, 1, 256))], ids=str)
-@pytest.mark.parametrize("scale", [2.0 ** -100, 2.0 ** -120, 2.0 ** -126])
+@pytest.mark.parametrize("scale", [2.0 ** -100, 2.0 ** -120, 2.0 ** -126, 2.0 ** -149])
 @pytest.mark.parametrize("splits,row_blocks", [(0, 0), (1, 1), (3, 1), (2, 2), (1, 8), (4, 8)])
 def test_least_scales(dtype, heads, scale, splits, row_blocks):
     """All logits are next to 0: a row's result is the mean of the values that it sees."""
